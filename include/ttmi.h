@@ -568,6 +568,70 @@ TTMI_API int ttmi_decoder_attention(const void* x, const void* gamma, const void
 TTMI_API int ttmi_decoder_feed_forward(const void* x, const void* gamma, const void* beta, float eps, const void* w1, const void* b1,
                                        const void* w2, const void* b2, void* out, void* exchange, int turn, int64_t rows, int64_t hidden,
                                        int64_t inner, int dtype, int workgroups, int patience, void* stream);
+/* ------------------------------------------------ a decoder's keys and values in pages -- */
+
+/* The keys and values of one decoder layer, [pages, kv_heads, page_size, head_dim] each, dense and 16-byte aligned.  A sequence's token i lies in
+ * slot i % page_size of the i / page_size-th of its pages, which may lie anywhere in the cache and in any order, and may belong to several
+ * sequences.  page_size is a power of two up to 4096; head_dim a multiple of 16 up to 256 (ttmi_paged_attention: 64 or 128).  No counterpart in the
+ * reference, whose layer cache is one dense tensor that every step copies (layers/multi_headed_attention.cpp:205-229). */
+typedef struct ttmi_paged_cache {
+  void* keys;
+  void* values;
+  int64_t pages;
+  int64_t kv_heads;
+  int64_t page_size;
+  int64_t head_dim;
+} ttmi_paged_cache;
+
+/* A batch of sequences and their new tokens.  All three arrays lie on the device and may change between replays of a recorded call.
+ *   table    [batch, table_pitch] the pages of each sequence, in order; entries past its last page are not read
+ *   starts   [batch + 1], never falling: the new tokens of sequence b are rows starts[b] to starts[b + 1] of the packed tensors (none, one or many);
+ *            rows from starts[batch] on are neither read nor written
+ *   lengths  [batch] keys of the sequence, those of its new tokens included: the i-th of n new tokens has position lengths[b] - n + i
+ * A page outside the cache, or a position outside the table, is an error that the kernels find (ttmi_check_async); they reach no memory outside
+ * the tensors then, and what they return for that sequence is unspecified. */
+typedef struct ttmi_paged_batch {
+  const int32_t* table;
+  int64_t table_pitch;
+  const int32_t* starts;
+  const int32_t* lengths;
+  int64_t batch;
+  int64_t tokens;         /* rows of the packed tensors */
+} ttmi_paged_batch;
+
+/* The new tokens' queries and keys turned by their positions, keys and values stored into their pages.
+ *   qkv [tokens, heads + 2 kv_heads, head_dim], rows qkv_pitch elements apart: queries, keys, values;  q_out [tokens, heads, head_dim], rows
+ *   q_pitch apart: the queries, turned; it may be qkv itself (same pitch), otherwise it must not overlap it.
+ *   The first rotary_dim (even, 0: none) elements of each head are turned: the pair number i by the angle position * inv_freq[i] (radians; inv_freq
+ *   DEVICE double[rotary_dim / 2]; angles are formed in 64 bits, any position keeps its place on the circle), times `amplitude`.  Pairs are elements
+ *   (2i, 2i + 1) where `interleaved`, else (i, i + rotary_dim / 2).  The rest of a head is copied.
+ * Two new tokens must not share a slot.  No counterpart in the reference. */
+TTMI_API int ttmi_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t q_pitch, int64_t heads,
+                                const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, const double* inv_freq,
+                                int64_t rotary_dim, int interleaved, float amplitude, int dtype, void* stream);
+
+/* Attention of the new tokens over their sequences' pages:
+ *   out[t, h, :] = sum_j p_j v_j, p = softmax over the keys j that token t sees of scale * q[t, h, :] . k_j
+ * `causal`: keys up to the token's own position, else all keys of its sequence; window > 0: of these only positions from its own - window + 1 on.
+ * A token that sees no key gets zeros.  q and out [tokens, heads, 64 or 128], rows q_pitch and out_pitch elements apart (a multiple of 16
+ * bytes); out must not overlap anything else; heads is a multiple of kv_heads, query head h reads key/value head h / (heads / kv_heads).
+ * max_tokens, max_length: the most new tokens and keys that a sequence has, or 0 if unknown.  They only choose how the work is cut; a
+ * call whose sequences have more is computed all the same.
+ * workspace: DEVICE memory of ttmi_paged_attention_workspace bytes (0: none is needed), 16-byte aligned, for this call alone while it runs.
+ * No counterpart in the reference (ttmi_attention_with_probs is its decoder's attention). */
+TTMI_API int ttmi_paged_attention_workspace(const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, int64_t heads, int64_t max_tokens,
+                                            int64_t max_length, int64_t window, int dtype, int64_t* bytes);
+TTMI_API int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_pitch, int64_t heads,
+                                  const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, int64_t max_tokens, int64_t max_length,
+                                  float scale, int causal, int64_t window, void* workspace, int64_t workspace_bytes, int dtype,
+                                  void* stream);
+
+/* Page destinations[i] becomes a copy of page sources[i], i < count, in `layers` caches that lie behind each other ([layers, pages, page_bytes]
+ * each of keys and values).  sources, destinations: HOST arrays.  A page must not be a destination twice, nor both a
+ * source and a destination; a source may be copied many times.  page_bytes a multiple of 16. */
+TTMI_API int ttmi_copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t page_bytes, const int32_t* sources,
+                             const int32_t* destinations, int64_t count, void* stream);
+
 /* *capturing = 1 while calls on the stream are recorded into a graph. */
 TTMI_API int ttmi_stream_capturing(void* stream, int* capturing);
 

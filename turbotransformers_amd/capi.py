@@ -34,6 +34,18 @@ class EpilogueArgs(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of ``ttmi_paged_cache``."""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("head_dim", ctypes.c_int64)]
+
+
+class PagedBatch(ctypes.Structure):
+    """Mirror of ``ttmi_paged_batch``."""
+    _fields_ = [("table", ctypes.c_void_p), ("table_pitch", ctypes.c_int64), ("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("batch", ctypes.c_int64), ("tokens", ctypes.c_int64)]
+
+
 _SCALARS = {
     "int": ctypes.c_int, "int64_t": ctypes.c_int64, "int32_t": ctypes.c_int32, "float": ctypes.c_float,
     "size_t": ctypes.c_size_t,

@@ -37,6 +37,7 @@ inline int launch_status(const char* what) { return check_hip(hipGetLastError(),
 
 int* async_error_flag();  // device-visible pinned int, 0 = ok, 1 = an embedding id out of range, or:
 constexpr int kRowsNeverCame = 2;
+constexpr int kPageOutOfRange = 3;
 
 // ---- kernel-selection switches ----------------------------------------------------------
 // Overrides of the launchers' own choices, for A/B timing and for tests of small and ragged shapes.  Each starts

@@ -237,6 +237,7 @@ int ttmi_check_async(void) {
     const int what = *flag;
     *flag = 0;
     if (what == kRowsNeverCame) return fail(TTMI_EDEVICE, "rows that a chain of steps waited for never came");
+    if (what == kPageOutOfRange) return fail(TTMI_EINDEX, "a page or a position of a paged cache is out of range");
     return fail(TTMI_EINDEX, "embedding id out of range");
   }
   return 0;

@@ -7,15 +7,18 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <algorithm>
 #include <cstring>
 #include <memory>
 
 #include "bert_model.h"
 #include "core/allocator.h"
 #include "core/device_context.h"
+#include "core/page_pool.h"
 #include "core/tensor.h"
 #include "layers/bert_layers.h"
 #include "layers/multi_headed_attention.h"
+#include "layers/paged.h"
 #include "layers/quantized_layers.h"
 #include "loaders/npz_load.h"
 #include "ttmi.h"
@@ -146,6 +149,68 @@ static py::object CallFeedForward(const FeedForward& self, const py::object& inp
   Tensor output(nullptr);
   self(*in.tensor, &output, is_trans_weight);
   return ToTorch(output);
+}
+
+// A Python argument of the operators over pages: a Tensor, or a torch tensor as it lies (its strides kept, nothing copied: the cache is written).
+struct ViewArg {
+  layers::TensorView view;
+  py::object capsule;  // keeps the alias until the call has been enqueued
+  ViewArg(const py::handle& obj, const char* what) {
+    if (py::isinstance<Tensor>(obj)) {
+      view = layers::TensorView(*obj.cast<Tensor*>());
+      return;
+    }
+    const TorchBridge& b = torch_bridge;
+    if (b.tensor_type == nullptr || PyObject_IsInstance(obj.ptr(), b.tensor_type) != 1) {
+      PyErr_Clear();
+      TT_THROW("%s: expected a tensor", what);
+    }
+    py::object t = py::reinterpret_borrow<py::object>(obj);
+    PyObject* c = PyObject_CallFunctionObjArgs(b.to_capsule, t.ptr(), nullptr);
+    if (c == nullptr) {  // (a tensor that requires gradients: asked only now, since such a question costs as much as the alias)
+      PyErr_Clear();
+      t = Owned(PyObject_CallMethodObjArgs(t.ptr(), b.detach, nullptr));
+      c = PyObject_CallFunctionObjArgs(b.to_capsule, t.ptr(), nullptr);
+    }
+    capsule = Owned(c);
+    auto* tensor = static_cast<DLManagedTensor*>(PyCapsule_GetPointer(capsule.ptr(), "dltensor"));
+    if (tensor == nullptr) throw py::error_already_set();
+    view = layers::TensorView(tensor->dl_tensor);
+  }
+};
+
+static void RotaryAppend(const py::object& qkv, const py::object& keys, const py::object& values, const py::object& table, const py::object& starts,
+                         const py::object& lengths, const py::object& inv_freq, bool interleaved, float amplitude, const py::object& q_out, int device,
+                         uintptr_t stream) {
+  const ViewArg in(qkv, "qkv"), k(keys, "keys"), v(values, "values"), t(table, "table"), s(starts, "starts"), l(lengths, "lengths"), out(q_out, "out");
+  std::unique_ptr<ViewArg> f;
+  if (!inv_freq.is_none()) f = std::make_unique<ViewArg>(inv_freq, "inv_freq");
+  layers::kernels::RotaryAppend(in.view, k.view, v.view, {t.view, s.view, l.view}, f ? &f->view : nullptr, interleaved, amplitude, out.view, device,
+                                reinterpret_cast<void*>(stream));
+}
+
+// `empty_bytes`: a Python function of a number of bytes that gives device memory of the caller's framework, whose allocator knows the stream (and
+// gives a call that is being recorded into a graph memory that stays the graph's).
+static void PagedAttention(const py::object& q, const py::object& keys, const py::object& values, const py::object& table, const py::object& starts,
+                           const py::object& lengths, const py::object& out, int64_t max_tokens, int64_t max_length, float scale, bool causal,
+                           int64_t window, const py::object& empty_bytes, int device, uintptr_t stream) {
+  const ViewArg in(q, "q"), k(keys, "keys"), v(values, "values"), t(table, "table"), s(starts, "starts"), l(lengths, "lengths"), o(out, "out");
+  std::unique_ptr<ViewArg> workspace;
+  py::object memory;
+  layers::kernels::PagedAttention(
+      in.view, k.view, v.view, {t.view, s.view, l.view}, o.view, max_tokens, max_length, scale, causal, window,
+      [&](int64_t bytes) -> void* {
+        memory = empty_bytes(bytes);
+        workspace = std::make_unique<ViewArg>(memory, "workspace");
+        return workspace->view.data;
+      },
+      device, reinterpret_cast<void*>(stream));
+}
+
+static void CopyPages(const py::object& keys, const py::object& values, const std::vector<int32_t>& sources, const std::vector<int32_t>& destinations,
+                      int device, uintptr_t stream) {
+  const ViewArg k(keys, "keys"), v(values, "values");
+  layers::kernels::CopyPages(k.view, v.view, sources, destinations, device, reinterpret_cast<void*>(stream));
 }
 
 template <typename T>
@@ -427,6 +492,41 @@ PYBIND11_MODULE(turbo_transformers_cxx, m) {
       current = target;
     }
   });
+
+  // The book of a cache in pages, and the operators over such a cache.  No counterpart in the reference.
+  py::class_<core::PagePool>(m, "PagePool")
+      .def(py::init<int64_t, int64_t>(), py::arg("pages"), py::arg("page_size"))
+      .def("add", &core::PagePool::Add)
+      .def("extend", &core::PagePool::Extend, py::arg("sequences"), py::arg("tokens"))
+      .def("fork", &core::PagePool::Fork, py::arg("sequence"))
+      .def("truncate", &core::PagePool::Truncate, py::arg("sequence"), py::arg("length"))
+      .def("free", &core::PagePool::Free, py::arg("sequence"))
+      .def("compact", &core::PagePool::Compact)
+      .def("length", &core::PagePool::Length, py::arg("sequence"))
+      .def("pages_of", &core::PagePool::Pages, py::arg("sequence"))
+      .def("references", &core::PagePool::References, py::arg("page"))
+      // rows of the given sequences' pages, filled up with page 0
+      .def("table",
+           [](const core::PagePool& pool, const std::vector<int64_t>& sequences, int64_t width) {
+             py::array_t<int32_t> out(std::vector<py::ssize_t>{(py::ssize_t)sequences.size(), (py::ssize_t)width});
+             int32_t* at = out.mutable_data();
+             for (int64_t s : sequences) {
+               const std::vector<int32_t>& pages = pool.Pages(s);
+               TT_ENFORCE((int64_t)pages.size() <= width, "sequence %ld has %ld pages, a row takes %ld", (long)s, (long)pages.size(), (long)width);
+               std::copy(pages.begin(), pages.end(), at);
+               std::fill(at + pages.size(), at + width, 0);
+               at += width;
+             }
+             return out;
+           },
+           py::arg("sequences"), py::arg("width"))
+      .def_property_readonly("free_pages", &core::PagePool::free_pages)
+      .def_property_readonly("pages", &core::PagePool::pages)
+      .def_property_readonly("page_size", &core::PagePool::page_size)
+      .def_property_readonly("sequences", &core::PagePool::sequences);
+  m.def("rotary_append", &RotaryAppend);
+  m.def("paged_attention", &PagedAttention);
+  m.def("copy_pages", &CopyPages);
 
   m.def("bind_torch", [](const py::object& tensor_type, const py::object& to_capsule, const py::object& from_capsule) {
     TorchBridge b;

@@ -8,6 +8,7 @@ from .qmodeling_bert import QBertIntermediate, QBertOutput, QBertAttention, QBer
 from .modules import MultiHeadedAttention, PositionwiseFeedForward, DistrillFFN
 from .modeling_roberta import RobertaModel
 from .modeling_distillbert import DistilBertModel
+from .paged import PagedCache, PagedBatch, rotary_append, paged_attention, copy_pages, rotary_frequencies
 from .return_type import ReturnType
 
 __all__ = [
@@ -16,4 +17,5 @@ __all__ = [
     'BertLayerSmartBatch', 'BertEncoderSmartBatch', 'BertModelNoPoolerSmartBatch', 'BertModelSmartBatch',
     'QBertIntermediate', 'QBertOutput', 'QBertAttention', 'QBertLayer', 'QBertEncoder', 'QBertModel',
     'MultiHeadedAttention', 'PositionwiseFeedForward', 'DistrillFFN', 'AlbertEmbeddings', 'AlbertAttention', 'AlbertLayer', 'AlbertLayerGroup', 'AlbertTransformer', 'AlbertModel', 'RobertaModel', 'DistilBertModel',
+    'PagedCache', 'PagedBatch', 'rotary_append', 'paged_attention', 'copy_pages', 'rotary_frequencies',
 ]
