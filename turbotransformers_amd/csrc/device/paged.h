@@ -37,7 +37,7 @@ inline int paged_view(const ttmi_paged_cache* cache, const ttmi_paged_batch* bat
                  "the cache's keys and values must be 16-byte aligned");
   }
   out->table = batch->table, out->starts = batch->starts, out->lengths = batch->lengths, out->error = async_error_flag();
-  out->table_pitch = batch->table_pitch;
+  out->table_pitch = cache->pages > 0 ? batch->table_pitch : 0;  // (without pages every key is one too many)
   out->batch = (int)batch->batch, out->tokens = (int)batch->tokens, out->pages = (int)cache->pages, out->kv_heads = (int)cache->kv_heads;
   out->page_shift = __builtin_ctzll((unsigned long long)cache->page_size), out->head_dim = (int)cache->head_dim;
   return 0;

@@ -1,65 +1,46 @@
 // Attention of new tokens over keys and values in pages: o = sum_j p_j v_j with p = softmax_j(scale q . k_j) over the keys that a token sees.
 // One pass over the keys: with the maximum m and the sum l of exp(s_j - m) so far, a tile of new scores moves m to m', scales what was summed by
-// exp(m - m') and adds its own exp(s_j - m') and exp(s_j - m') v_j.  All of it in fp32.
-#include "paged.h"
+// exp(m - m') and adds its own exp(s_j - m') and exp(s_j - m') v_j.  All of it in fp32; exp(x) as 2^(x log2 e).
+//
+// Two kernels share a batch by the rows (new tokens times query heads of a key/value head) of its sequences: up to 16 of them paged_few_rows.hip, more
+// paged_tiles.hip.  This file cuts the work: keys of a sequence into parts, where there are few rows and heads, whose results a small kernel joins.
+#include "paged_attention.h"
 
 namespace ttmi {
+namespace {
 
-// One wavefront per token and head: a lane per key for the scores, a lane per column for the sum over the values.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void paged_attention_kernel(const T* __restrict__ q, int64_t q_pitch, T* __restrict__ out, int64_t out_pitch, int group,
-                                                             const T* __restrict__ keys, const T* __restrict__ values, const PagedView view, float scale,
-                                                             int causal, int64_t window) {
-  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-  const int b = sequence_of(view, token);
-  if (b >= view.batch || token < view.starts[b]) return;
-  const int64_t held = view.table_pitch << view.page_shift;
-  const int length = (int)min((int64_t)view.lengths[b], held), position = view.lengths[b] - view.starts[b + 1] + token;
-  if (length < view.lengths[b] && lane == 0) page_error(view);
-  const int end = causal ? min(length, position + 1) : length;
-  const int begin = window > 0 ? (int)max((int64_t)0, (int64_t)position - window + 1) : 0;
-  __shared__ float q_lds[D], p_lds[64];
-  __shared__ int64_t row_lds[64];
-  for (int i = lane; i < D; i += 64) q_lds[i] = to_float(q[token * q_pitch + (int64_t)head * D + i]) * scale;
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, acc[D / 64] = {};
-  for (int j0 = begin; j0 < end; j0 += 64) {
-    const int j = j0 + lane;
-    float s = -INFINITY;
-    int64_t row = 0;
-    if (j < end) {
-      int page = view.table[(int64_t)b * view.table_pitch + (j >> view.page_shift)];
-      if ((unsigned)page >= (unsigned)view.pages) {
-        page_error(view);
-        page = 0;
-      }
-      row = ((((int64_t)page * view.kv_heads + head / group) << view.page_shift) + (j & ((1 << view.page_shift) - 1))) * D;
-      s = 0.f;
-      constexpr int W = 16 / (int)sizeof(T);
-      for (int i = 0; i < D; i += W) {
-        const Vec<T, W> k = load_vec<T, W>(keys + row + i);
-#pragma unroll
-        for (int e = 0; e < W; ++e) s += to_float(k.v[e]) * q_lds[i + e];
-      }
-    }
-    const float top = fmaxf(m, group_max<64>(s));
-    const float shrink = m == -INFINITY ? 0.f : expf(m - top), p = s == -INFINITY ? 0.f : expf(s - top);
-    l = l * shrink + group_sum<64>(p);
-    m = top;
-    p_lds[lane] = p, row_lds[lane] = row;
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) acc[c] *= shrink;
-    for (int i = 0; i < min(64, end - j0); ++i)
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) acc[c] += p_lds[i] * to_float(values[row_lds[i] + c * 64 + lane]);
-    __syncthreads();
-  }
-  const float inv = l > 0.f ? 1.0f / l : 0.f;
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) out[token * out_pitch + (int64_t)head * D + c * 64 + lane] = from_float<T>(acc[c] * inv);
+struct PagedPlan {
+  bool few, tiles;  // which kernels run; one alone takes all sequences
+  int few_chunk, few_splits, tile_chunk, tile_splits;
+  int64_t few_floats, tile_floats;  // of the workspace
+};
+
+void cut(int64_t units, int64_t wanted, int64_t least, int64_t reach, int64_t longest, int* chunk, int* splits) {
+  const int64_t parts = std::min(std::max<int64_t>(1, wanted / std::max<int64_t>(1, units)), std::max<int64_t>(1, ceil_div(reach, least)));
+  int64_t size = ceil_div(ceil_div(reach, parts), 64) * 64;
+  size = std::max(size, ceil_div(ceil_div(longest, 4096), 64) * 64);  // (at most 4096 parts)
+  *splits = parts > 1 ? (int)std::max<int64_t>(1, ceil_div(longest, size)) : 1;
+  *chunk = (int)std::min<int64_t>(size, INT32_MAX - 64);
 }
 
+PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, int64_t window) {
+  PagedPlan p;
+  const int64_t group = heads / view.kv_heads, tokens = view.tokens, batch = std::max(1, view.batch);
+  const int64_t held = view.table_pitch << view.page_shift;
+  const int64_t longest = std::max<int64_t>(1, max_length > 0 ? std::min(max_length, held) : held);
+  const int64_t most = max_tokens > 0 ? std::min(max_tokens, tokens) : tokens;
+  const int64_t reach = window > 0 ? std::min(longest, window + most) : longest;
+  p.tiles = most * group > kFewRows;
+  p.few = !p.tiles || tokens * group / batch < 512;
+  cut(batch * view.kv_heads, 2048, 128, reach, longest, &p.few_chunk, &p.few_splits);
+  cut(view.kv_heads * (tokens * group / 128 + std::min(batch, tokens)), 512, 256, reach, longest, &p.tile_chunk, &p.tile_splits);
+  const int64_t d = view.head_dim;
+  p.few_floats = p.few && p.few_splits > 1 ? batch * view.kv_heads * kFewRows * p.few_splits * (d + 2) : 0;
+  p.tile_floats = p.tiles && p.tile_splits > 1 ? tokens * heads * p.tile_splits * (d + 2) : 0;
+  return p;
+}
+
+}  // namespace
 }  // namespace ttmi
 
 using namespace ttmi;
@@ -71,15 +52,19 @@ int ttmi_paged_attention_workspace(const ttmi_paged_cache* cache, const ttmi_pag
   PagedView view;
   TTMI_REQUIRE(bytes != nullptr, "bytes is null");
   if (int rc = paged_view(cache, batch, heads, &view)) return rc;
+  TTMI_REQUIRE(window >= 0 && max_tokens >= 0 && max_length >= 0, "window, max_tokens and max_length must not be negative");
   *bytes = 0;
+  if (batch->tokens == 0 || batch->batch == 0) return 0;
+  const PagedPlan p = plan(view, heads, max_tokens, max_length, window);
+  *bytes = (p.few_floats + p.tile_floats) * 4;
   return 0;
 }
 
 int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_pitch, int64_t heads, const ttmi_paged_cache* cache,
                          const ttmi_paged_batch* batch, int64_t max_tokens, int64_t max_length, float scale, int causal, int64_t window,
                          void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
-  PagedView view;
-  if (int rc = paged_view(cache, batch, heads, &view)) return rc;
+  PagedArgs a;
+  if (int rc = paged_view(cache, batch, heads, &a.view)) return rc;
   const int64_t d = cache->head_dim;
   TTMI_REQUIRE(d == 64 || d == 128, "paged attention needs head_dim 64 or 128");
   TTMI_REQUIRE(q_pitch >= heads * d && out_pitch >= heads * d, "rows overlap: a pitch is too small");
@@ -89,16 +74,26 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   TTMI_REQUIRE(q != nullptr && out != nullptr, "q or out is null");
   TTMI_REQUIRE(rows_aligned(q, q_pitch, dtype) && rows_aligned(out, out_pitch, dtype), "rows of q and out must be 16-byte aligned");
-  TTMI_DISPATCH_FLOAT(dtype, T, {
-    const dim3 grid((unsigned)view.tokens, (unsigned)heads);
-    auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(64), 0, static_cast<hipStream_t>(stream), static_cast<const T*>(q), q_pitch, static_cast<T*>(out), out_pitch,
-                         (int)(heads / cache->kv_heads), static_cast<const T*>(cache->keys), static_cast<const T*>(cache->values), view, scale, causal, window);
-    };
-    if (d == 64) launch(paged_attention_kernel<T, 64>);
-    else launch(paged_attention_kernel<T, 128>);
-  });
-  return launch_status("paged_attention");
+  const PagedPlan p = plan(a.view, heads, max_tokens, max_length, window);
+  const int64_t bytes = (p.few_floats + p.tile_floats) * 4;
+  TTMI_REQUIRE(bytes == 0 || (workspace != nullptr && workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+               "the workspace is too small or not 16-byte aligned");
+  a.q = q, a.out = out, a.keys = cache->keys, a.values = cache->values, a.q_pitch = q_pitch, a.out_pitch = out_pitch;
+  a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads), a.causal = causal != 0;
+  a.window = (int)std::min<int64_t>(window, 1 << 30);  // (beyond every position)
+  a.scale_log2e = scale * 1.4426950408889634f;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p.tiles) {
+    a.every = !p.few, a.chunk = p.tile_chunk, a.splits = p.tile_splits;
+    a.partial = static_cast<float*>(workspace) + p.few_floats, a.partial_rows = batch->tokens * heads;
+    if (int rc = launch_tiles(a, dtype, d, s)) return rc;
+  }
+  if (p.few) {
+    a.every = !p.tiles, a.chunk = p.few_chunk, a.splits = p.few_splits;
+    a.partial = static_cast<float*>(workspace), a.partial_rows = batch->batch * cache->kv_heads * kFewRows;
+    if (int rc = launch_few_rows(a, dtype, d, s)) return rc;
+  }
+  return 0;
 }
 
 }  // extern "C"
