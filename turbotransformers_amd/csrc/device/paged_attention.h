@@ -18,13 +18,13 @@ struct PagedArgs {
   PagedView view;
   int heads, group, causal, window;  // window 0: none
   float scale_log2e;
-  // Keys are cut at multiples of `chunk` (a multiple of 64), counted from the first of the sequence, into at most `splits` parts (the grid); a sequence that has more
-  // keys than that takes longer parts.
-  int chunk, splits;
-  int every;  // the few-rows kernel takes sequences of any number of rows: the other one is not launched
-  // rows whose keys lie in several parts: their sums [row][part][d] and, behind all of them, maxima and sums of the probabilities [row][part][2]
-  float* partial;
-  int64_t partial_rows;
+  int every;  // this kernel takes all sequences: the other one is not launched
+  // Of the few-rows kernel.  splits: how many workgroups share the work, 0: one for each sequence and key/value head; waves: of a workgroup; few: the rows of a sequence
+  // that is its own (at most kFewRows).
+  // Of the other.  Keys are cut at multiples of `chunk` (a multiple of 64), counted from the first of the sequence, into at most `splits` parts (the grid); a sequence
+  // that has more keys than that takes longer parts.
+  int splits, waves, few, chunk;
+  float* partial;  // sums of rows whose keys are several workgroups' [..][d], behind them the maxima and sums of their probabilities [..][2]
 };
 
 struct Reach {
@@ -40,7 +40,7 @@ struct Sequence {
     if (r.begin >= r.end) r.begin = r.end = 0;
     return r;
   }
-  // keys of a part
+  // keys of a part (tiles)
   __device__ __forceinline__ int chunk(const PagedArgs& a) const {
     return a.splits <= 1 ? INT32_MAX : max(a.chunk, ((length + a.splits - 1) / a.splits + 63) & ~63);
   }
@@ -55,12 +55,12 @@ __device__ __forceinline__ Sequence sequence(const PagedArgs& a, int b) {
   return s;
 }
 
-// The pages that a wavefront is about to read, 64 of them a lane each, fetched when it comes to them.  (A page of 16 or more slots holds groups of 16 rows
-// whole, so the page of a group is one number for the wavefront; smaller pages are looked up row by row.)
+// The pages that a wavefront is about to read, 64 of them a lane each, and the 64 behind those, which are on their way.  (A page of 16 or more slots holds groups of
+// 16 rows whole, so the page of a group is one number for the wavefront; smaller pages are looked up row by row.)
 struct PageCursor {
   const int32_t* table;  // of the sequence
   int first, last;       // number of the first page held here; of the sequence's last one
-  int32_t entry;
+  int32_t entry, ahead;
 };
 __device__ __forceinline__ int32_t checked_page(const PagedView& view, int32_t page) {
   if ((unsigned)page < (unsigned)view.pages) return page;
@@ -68,15 +68,25 @@ __device__ __forceinline__ int32_t checked_page(const PagedView& view, int32_t p
   return 0;
 }
 __device__ __forceinline__ void fetch_pages(const PagedView& view, PageCursor& at, int page) {
+  const int lane = (int)(threadIdx.x % kWave);
   at.first = page;
-  at.entry = checked_page(view, at.table[min(page + (int)(threadIdx.x % kWave), at.last)]);
+  at.entry = checked_page(view, at.table[min(page + lane, at.last)]);
+  at.ahead = at.table[min(page + kWave + lane, at.last)];
+}
+__device__ __forceinline__ void next_pages(const PagedView& view, PageCursor& at) {
+  at.first += kWave;
+  at.entry = checked_page(view, at.ahead);
+  at.ahead = at.table[min(at.first + kWave + (int)(threadIdx.x % kWave), at.last)];
 }
 // Element of the cache at which the row of `key` begins; rows of a group of 16 follow each other.  For pages of 16 and more slots; key is uniform and a multiple
 // of 16.
 template <int D>
 __device__ __forceinline__ int64_t group_offset(const PagedView& view, PageCursor& at, int kv_head, int key) {
   const int page = min(key >> view.page_shift, at.last);
-  if (page - at.first >= kWave || page < at.first) fetch_pages(view, at, page);
+  if (page - at.first >= kWave) {
+    if (page - at.first < 2 * kWave) next_pages(view, at);
+    else fetch_pages(view, at, page);
+  }
   const int32_t entry = __builtin_amdgcn_readlane(at.entry, page - at.first);
   return ((((int64_t)entry * view.kv_heads + kv_head) << view.page_shift) + (key & ((1 << view.page_shift) - 1))) * D;
 }
@@ -122,6 +132,45 @@ __device__ __forceinline__ u32x2 read_transposed(const void* p) {
 #else
   return u32x2{};
 #endif
+}
+
+// o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over `parts` partial results of a row, the p-th of which is row at(p) of `partial` [.., D] and `ml` [.., 2];
+// 256 threads.
+template <typename T, int D, typename At>
+__device__ __forceinline__ void join_parts(const float* partial, const float* ml, int parts, At at, T* out) {
+  constexpr int kWide = 4, kThreads = D / kWide, kShares = 256 / kThreads;  // columns of a thread; threads of a part; parts at a time
+  const int d0 = threadIdx.x % kThreads * kWide, share = threadIdx.x / kThreads;
+  __shared__ float met[kShares][D + 2];
+  // (each share with the maximum of its own parts)
+  float best = -INFINITY;
+  for (int p = share; p < parts; p += kShares) best = fmaxf(best, ml[2 * at(p)]);
+  const float zero = best == -INFINITY ? 0.f : best;
+  float total = 0.f;
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = share; p < parts; p += kShares) {
+    const int64_t row = at(p);
+    const float weight = __builtin_amdgcn_exp2f(ml[2 * row] - zero);
+    total += ml[2 * row + 1] * weight;
+    sum += *reinterpret_cast<const floatx4*>(partial + row * D + d0) * weight;
+  }
+#pragma unroll
+  for (int c = 0; c < kWide; ++c) met[share][d0 + c] = sum[c];
+  if (d0 == 0) met[share][D] = best, met[share][D + 1] = total;
+  __syncthreads();
+  if ((int)threadIdx.x >= D) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kShares; ++i) top = fmaxf(top, met[i][D]);
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f, x = 0.f;
+#pragma unroll
+  for (int i = 0; i < kShares; ++i) {
+    const float weight = __builtin_amdgcn_exp2f(met[i][D] - base);
+    l += met[i][D + 1] * weight;
+    x += met[i][threadIdx.x] * weight;
+  }
+  out[threadIdx.x] = from_float<T>(l != 0.f ? x / l : 0.f);
 }
 
 int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream);

@@ -11,7 +11,7 @@ namespace {
 
 struct PagedPlan {
   bool few, tiles;  // which kernels run; one alone takes all sequences
-  int few_chunk, few_splits, tile_chunk, tile_splits;
+  int few_rows, few_splits, few_waves, tile_chunk, tile_splits;
   int64_t few_floats, tile_floats;  // of the workspace
 };
 
@@ -23,7 +23,12 @@ void cut(int64_t units, int64_t wanted, int64_t least, int64_t reach, int64_t lo
   *chunk = (int)std::min<int64_t>(size, INT32_MAX - 64);
 }
 
-PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, int64_t window) {
+// Few rows: up to so many bytes of keys and values of one sequence and head are one workgroup's.  A CU fetches about 50 GB/s, so these take 6 us, what sharing them out
+// and joining the parts costs besides their share.  us a call, one workgroup / shared: bf16, head_dim 128, 8 sequences of 255 keys (130 KB) 7.2 / 12.4, 500 10.6 / 13.5,
+// 1000 (512 KB) 15.6 / 15.9, 2000 25.2 / 22.6, 1 sequence of 1000 14.8 / 12.6; fp16, head_dim 64, 12 heads, 1 sequence of 1000 (256 KB) 9.7 / 12.1, 2000 14.4 / 12.1.
+constexpr int64_t kWholeBytes = 320 << 10;
+
+PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, int64_t window, int dtype) {
   PagedPlan p;
   const int64_t group = heads / view.kv_heads, tokens = view.tokens, batch = std::max(1, view.batch);
   const int64_t held = view.table_pitch << view.page_shift;
@@ -32,10 +37,12 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   const int64_t reach = window > 0 ? std::min(longest, window + most) : longest;
   p.tiles = most * group > kFewRows;
   p.few = !p.tiles || tokens * group / batch < 512;
-  cut(batch * view.kv_heads, 2048, 128, reach, longest, &p.few_chunk, &p.few_splits);
+  p.few_rows = p.tiles ? kFewRows : (int)(most * group);
+  p.few_splits = reach * 2 * view.head_dim * (int64_t)dtype_size(dtype) <= kWholeBytes ? 0 : 2 * compute_units();
+  p.few_waves = p.few_splits == 0 && batch * view.kv_heads < compute_units() ? 8 : 4;
   cut(view.kv_heads * (tokens * group / 128 + std::min(batch, tokens)), 512, 256, reach, longest, &p.tile_chunk, &p.tile_splits);
   const int64_t d = view.head_dim;
-  p.few_floats = p.few && p.few_splits > 1 ? batch * view.kv_heads * kFewRows * p.few_splits * (d + 2) : 0;
+  p.few_floats = p.few ? 2ll * p.few_splits * kFewRows * (d + 2) : 0;
   p.tile_floats = p.tiles && p.tile_splits > 1 ? tokens * heads * p.tile_splits * (d + 2) : 0;
   return p;
 }
@@ -55,7 +62,7 @@ int ttmi_paged_attention_workspace(const ttmi_paged_cache* cache, const ttmi_pag
   TTMI_REQUIRE(window >= 0 && max_tokens >= 0 && max_length >= 0, "window, max_tokens and max_length must not be negative");
   *bytes = 0;
   if (batch->tokens == 0 || batch->batch == 0) return 0;
-  const PagedPlan p = plan(view, heads, max_tokens, max_length, window);
+  const PagedPlan p = plan(view, heads, max_tokens, max_length, window, dtype);
   *bytes = (p.few_floats + p.tile_floats) * 4;
   return 0;
 }
@@ -74,7 +81,7 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   TTMI_REQUIRE(q != nullptr && out != nullptr, "q or out is null");
   TTMI_REQUIRE(rows_aligned(q, q_pitch, dtype) && rows_aligned(out, out_pitch, dtype), "rows of q and out must be 16-byte aligned");
-  const PagedPlan p = plan(a.view, heads, max_tokens, max_length, window);
+  const PagedPlan p = plan(a.view, heads, max_tokens, max_length, window, dtype);
   const int64_t bytes = (p.few_floats + p.tile_floats) * 4;
   TTMI_REQUIRE(bytes == 0 || (workspace != nullptr && workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                "the workspace is too small or not 16-byte aligned");
@@ -85,12 +92,12 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.tiles) {
     a.every = !p.few, a.chunk = p.tile_chunk, a.splits = p.tile_splits;
-    a.partial = static_cast<float*>(workspace) + p.few_floats, a.partial_rows = batch->tokens * heads;
+    a.partial = static_cast<float*>(workspace) + p.few_floats;
     if (int rc = launch_tiles(a, dtype, d, s)) return rc;
   }
   if (p.few) {
-    a.every = !p.tiles, a.chunk = p.few_chunk, a.splits = p.few_splits;
-    a.partial = static_cast<float*>(workspace), a.partial_rows = batch->batch * cache->kv_heads * kFewRows;
+    a.every = !p.tiles, a.few = p.few_rows, a.splits = p.few_splits, a.waves = p.few_waves;
+    a.partial = static_cast<float*>(workspace);
     if (int rc = launch_few_rows(a, dtype, d, s)) return rc;
   }
   return 0;

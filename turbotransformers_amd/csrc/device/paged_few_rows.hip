@@ -13,7 +13,7 @@
 namespace ttmi {
 namespace {
 
-template <typename T, int D>
+template <typename T, int D, int NW>
 struct FewRows {
   static constexpr int kKeys = sizeof(T) == 2 ? 32 : 16;        // of a tile
   static constexpr int kElems = 16 / (int)sizeof(T);            // of a 16-byte piece
@@ -24,8 +24,8 @@ struct FewRows {
   static constexpr int kTiles = D / 16;                         // of the output
   static constexpr int kValueBytes = kKeys * kRowBytes;         // of a wavefront, in LDS
   static constexpr int kPitch = D + 4;                          // floats of a row where the wavefronts meet
-  static constexpr int kMergeBytes = 4 * kFewRows * kPitch * 4;
-  static constexpr int kLds = 4 * kValueBytes > kMergeBytes ? 4 * kValueBytes : kMergeBytes;
+  static constexpr int kMergeBytes = NW * kFewRows * kPitch * 4;
+  static constexpr int kLds = NW * kValueBytes > kMergeBytes ? NW * kValueBytes : kMergeBytes;
 };
 
 // Place of a 16-byte piece in a row of a tile of values: the transposing reads take 32 bytes of each of sixteen rows at a time, plain ones 64 bytes of four rows
@@ -63,29 +63,108 @@ __device__ __forceinline__ float quarters_sum(float v) {
   return p.a + p.b;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void few_rows_kernel(const PagedArgs a) {
-  using S = FewRows<T, D>;
-  __shared__ __align__(16) char smem[S::kLds];
-  __shared__ float met[4][kFewRows][2];  // maximum and sum of each wavefront's rows
-  const PagedView& view = a.view;
-  const int kv_head = blockIdx.x % view.kv_heads, b = blockIdx.x / view.kv_heads, part = blockIdx.z;
+// The work is cut evenly over the workgroups whatever the sequences' lengths: a unit is a round, kRound keys of one sequence and key/value head, units are counted
+// sequence by sequence, head by head, and workgroup w of W takes those from w R / W to (w + 1) R / W.  So of the pairs of a sequence and a head that it meets only the first
+// and the last can be another's too; their partial results have a place each.
+constexpr int kRound = 128;
+// A pair has a unit more than rounds: what a workgroup waits for when it comes to one (its length, its pages, its first tile) is time that others have for theirs.
+// us, 64 sequences of 100 to 6000 keys (three draws, and all of 1450), without / with it / with two: 105 / 89 / 91, 87 / 75 / 77, 107 / 94 / 97, 104 / 95 / 98, 75 / 75 / 75.
+constexpr int kStart = 1;
+struct Walk {  // 64 sequences, a lane each
+  int base, rounds;       // number of the first; rounds of this lane's, for one head
+  int64_t before, upto;   // units of all sequences before these; of these up to this lane's, it included
+};
+__device__ __forceinline__ int rounds_of(const PagedArgs& a, int b) {
   const Sequence seq = sequence(a, b);
-  const int rows_all = seq.tokens * a.group;
-  if (rows_all <= 0 || (rows_all > kFewRows && !a.every)) return;
-  const bool whole = rows_all > kFewRows;  // (of these sequences the first part's workgroup takes everything)
-  if (whole && part != 0) return;
-  const int chunk = whole ? INT32_MAX : seq.chunk(a);
-  if (part == 0 && kv_head == 0 && threadIdx.x == 0 && view.lengths[b] > seq.length) page_error(view);
+  const int rows = seq.tokens * a.group;
+  if (rows <= 0) return 0;
+  if (rows > a.few) return a.every ? kStart + 1 : 0;  // (more rows than was said: not cut)
+  const Reach low = seq.reach(a, 0), high = seq.reach(a, seq.tokens - 1);
+  return kStart + max(1, (max(low.end, high.end) + kRound - 1) / kRound - low.begin / kRound);
+}
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ void walk_to(const PagedArgs& a, Walk& w, int base, int64_t before) {
+  const int lane = (int)(threadIdx.x % kWave);
+  w.base = base, w.before = before;
+  w.rounds = base + lane < a.view.batch ? rounds_of(a, base + lane) : 0;
+  w.upto = (int64_t)w.rounds * a.view.kv_heads;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int64_t below = __shfl_up((long long)w.upto, d, kWave);
+    if (lane >= d) w.upto += below;
+  }
+}
+// -> all units; w is at the first sequences
+__device__ __forceinline__ int64_t count_units(const PagedArgs& a, Walk& w) {
+  walk_to(a, w, 0, 0);
+  int64_t all = lane_of(w.upto, kWave - 1);
+  if (a.view.batch <= kWave) return all;
+  for (int base = kWave; base < a.view.batch; base += kWave) {
+    walk_to(a, w, base, all);
+    all += lane_of(w.upto, kWave - 1);
+  }
+  walk_to(a, w, 0, 0);
+  return all;
+}
+struct Place {
+  int b, kv_head, round, rounds;  // round: of this head's `rounds`
+};
+// w is at or before the unit's sequences
+__device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t unit) {
+  while (w.before + lane_of(w.upto, kWave - 1) <= unit) walk_to(a, w, w.base + kWave, w.before + lane_of(w.upto, kWave - 1));
+  const int64_t at = unit - w.before;
+  const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(w.upto > at)) - 1);
+  Place p;
+  p.b = w.base + found, p.rounds = __builtin_amdgcn_readlane(w.rounds, found);
+  const int rest = (int)(at - (lane_of(w.upto, found) - (int64_t)p.rounds * a.view.kv_heads));
+  p.kv_head = rest / p.rounds, p.round = rest - p.kv_head * p.rounds;
+  return p;
+}
+// Workgroups that share the work.  At least kFewest rounds each, so that a wavefront has more than its first tile's wait.
+constexpr int kFewest = 2;
+__device__ __forceinline__ int64_t sharers(const PagedArgs& a, int64_t units) { return max((int64_t)1, min((int64_t)a.splits, (units + kFewest - 1) / kFewest)); }
 
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedArgs a) {
+  using S = FewRows<T, D, NW>;
+  __shared__ __align__(16) char smem[S::kLds];
+  __shared__ float met[NW][kFewRows][2];
+  const PagedView& view = a.view;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 15, quarter = lane >> 4;
   const T* const q = static_cast<const T*>(a.q);
   const T* const keys = static_cast<const T*>(a.keys);
   const T* const values = static_cast<const T*>(a.values);
+  char* const tile = smem + wave * S::kValueBytes;
+
+  // splits 0: a workgroup for each pair
+  Walk walk;
+  int64_t unit = blockIdx.x, stop = unit + 1;
+  if (a.splits > 0) {
+    const int64_t units = count_units(a, walk), workgroups = sharers(a, units);
+    if (blockIdx.x >= workgroups) return;
+    unit = units * blockIdx.x / workgroups, stop = units * (blockIdx.x + 1) / workgroups;
+  }
+  while (unit < stop) {
+  Place place;
+  if (a.splits > 0) place = find_unit(a, walk, unit);
+  else place.b = (int)(unit / view.kv_heads), place.kv_head = (int)(unit % view.kv_heads), place.round = 0, place.rounds = INT32_MAX;
+  const int b = place.b, kv_head = place.kv_head;
+  const int64_t ends = a.splits > 0 ? min(stop, unit + place.rounds - place.round) : stop;
+  const int start = a.splits > 0 ? kStart : 0;  // (in a pair's first unit there is nothing to do)
+  const int round0 = max(0, place.round - start), round1 = place.round + (int)(a.splits > 0 ? ends - unit : INT32_MAX) - start;
+  const bool complete = round0 == 0 && round1 == place.rounds - start;
+  unit = ends;
+  if (round1 <= round0) continue;
+  const Sequence seq = sequence(a, b);
+  const int rows_all = seq.tokens * a.group;
+  if (rows_all <= 0 || (rows_all > a.few && !a.every)) return;  // (a workgroup of its own)
+  if (round0 == 0 && kv_head == 0 && tid == 0 && view.lengths[b] > seq.length) page_error(view);
   PageCursor cursor;
   cursor.table = view.table + (int64_t)b * view.table_pitch;
-  cursor.entry = 0;
-  char* const tile = smem + wave * S::kValueBytes;
+  cursor.first = 0, cursor.entry = 0, cursor.ahead = 0;
 
   for (int row0 = 0; row0 < rows_all; row0 += kFewRows) {
     const int rows = min(kFewRows, rows_all - row0);
@@ -94,8 +173,11 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const PagedArgs a) {
     const Reach mine = seq.reach(a, token), low = seq.reach(a, token0), high = seq.reach(a, token1);
     // Keys that some row sees, and those that all rows see: both ends rise with the position.  (A row without keys, before the first one, begins and ends at 0.)
     const int first = low.begin, end = max(low.end, high.end), sure_first = high.begin, sure_end = low.end;
-    const int lo = max(part * (int64_t)chunk, (int64_t)(first & ~(S::kKeys - 1))), hi = (int)min((part + 1) * (int64_t)chunk, (int64_t)end);
-    if (lo >= hi && part != 0) return;
+    int lo = first & ~(S::kKeys - 1), hi = end;
+    if (!complete) {
+      lo = max(lo, (first / kRound + round0) * kRound);
+      hi = min(hi, (first / kRound + round1) * kRound);
+    }
     cursor.last = max(0, (end - 1) >> view.page_shift);
 
     u32x4 qf[S::kSteps];
@@ -138,13 +220,14 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const PagedArgs a) {
       }
     };
 
+    constexpr int kStep = NW * S::kKeys;
     int key = lo + wave * S::kKeys;
     if (key < hi) {
       fetch_pages(view, cursor, min(key >> view.page_shift, cursor.last));
-      load_keys(key);
       load_values(key);
+      load_keys(key);
     }
-    for (; key < hi; key += 4 * S::kKeys) {
+    for (; key < hi; key += kStep) {
       const bool masked = key < sure_first || key + S::kKeys > sure_end || key + S::kKeys > hi;
       uint32_t wild = 0;
       if (masked) {  // keys that no row sees may hold anything: their values count as zeros, and one that only some rows see must not reach the others
@@ -166,7 +249,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const PagedArgs a) {
           *reinterpret_cast<u32x4*>(tile + r * S::kRowBytes + value_piece<T, D>(r, at % S::kRowBytes / 16) * 16) = wild ? finite_part<T>(vf[g][i]) : vf[g][i];
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the tile is this wavefront's alone: its LDS accesses are in order)
-      const int next = key + 4 * S::kKeys;
+      const int next = key + kStep;
       if (next < hi) load_values(next);
 
       floatx4 st[S::kGroups];
@@ -255,7 +338,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const PagedArgs a) {
       }
     }
 
-    // the four wavefronts meet
+    // the wavefronts meet
     sum = quarters_sum(sum);
     __syncthreads();
     float* const stage = reinterpret_cast<float*>(smem);
@@ -265,81 +348,63 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const PagedArgs a) {
     if (quarter == 0) met[wave][row][0] = top, met[wave][row][1] = sum;
     __syncthreads();
     {
-      constexpr int kWide = D / 16;  // columns of a thread
-      const int r = tid >> 4, d0 = (tid & 15) * kWide;
+      constexpr int kThreads = NW * 4, kWide = D / kThreads;  // of a row; columns of a thread
+      const int r = tid / kThreads, d0 = tid % kThreads * kWide;
       if (r < rows) {
         float best = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) best = fmaxf(best, met[w][r][0]);
+        for (int w = 0; w < NW; ++w) best = fmaxf(best, met[w][r][0]);
         const float zero = best == -INFINITY ? 0.f : best;
         float total = 0.f, o[kWide] = {};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
           const float weight = __builtin_amdgcn_exp2f(met[w][r][0] - zero);
           total += met[w][r][1] * weight;
 #pragma unroll
           for (int c = 0; c < kWide; ++c) o[c] += stage[(w * kFewRows + r) * S::kPitch + d0 + c] * weight;
         }
-        const int t = (row0 + r) / a.group, h = kv_head * a.group + row0 + r - t * a.group;
-        const Reach reach = seq.reach(a, t);
-        const int part0 = reach.begin / chunk, part1 = reach.end > 0 ? (reach.end - 1) / chunk : 0;
-        if (part0 == part1) {
-          if (part == part0) {
-            const float inv = total != 0.f ? 1.0f / total : 0.f;
-            T* to = static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D + d0;
-            Vec<T, kWide> x;
+        if (complete) {
+          const int t = (row0 + r) / a.group, h = kv_head * a.group + row0 + r - t * a.group;
+          const float inv = total != 0.f ? 1.0f / total : 0.f;
+          T* to = static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D + d0;
+          Vec<T, kWide> x;
 #pragma unroll
-            for (int c = 0; c < kWide; ++c) x.v[c] = from_float<T>(o[c] * inv);
-            store_vec<T, kWide>(to, x);
-          }
+          for (int c = 0; c < kWide; ++c) x.v[c] = from_float<T>(o[c] * inv);
+          store_vec<T, kWide>(to, x);
         } else {
-          const int64_t at = (((int64_t)b * view.kv_heads + kv_head) * kFewRows + r) * a.splits + part;
+          const int64_t at = (2 * (int64_t)blockIdx.x + (round0 == 0 ? 1 : 0)) * kFewRows + r;
+          float* const ml = a.partial + 2 * (int64_t)a.splits * kFewRows * D + at * 2;
 #pragma unroll
           for (int c = 0; c < kWide; ++c) a.partial[at * D + d0 + c] = o[c];
-          if (d0 == 0) {
-            float* ml = a.partial + a.partial_rows * a.splits * D + at * 2;
-            ml[0] = best, ml[1] = total;
-          }
+          if (d0 == 0) ml[0] = best, ml[1] = total;
         }
       }
     }
-    if (row0 + kFewRows < rows_all) __syncthreads();
+    if (row0 + kFewRows < rows_all || unit < stop) __syncthreads();
+  }
   }
 }
 
-// Rows whose keys lay in several parts: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.
+// Pairs that were several workgroups': o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over their partial results.  A workgroup per row of a pair.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a) {
-  constexpr int kWide = D / 16;
   const PagedView& view = a.view;
-  const int kv_head = blockIdx.x % view.kv_heads, b = blockIdx.x / view.kv_heads;
+  const int kv_head = blockIdx.x % view.kv_heads, b = blockIdx.x / view.kv_heads, r = blockIdx.y;
   const Sequence seq = sequence(a, b);
-  const int rows = seq.tokens * a.group, r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * kWide;
-  if (rows > kFewRows || r >= rows) return;
+  const int rows = seq.tokens * a.group;
+  if (rows > a.few || r >= rows) return;
+  Walk walk;
+  const int64_t units = count_units(a, walk), workgroups = sharers(a, units);
+  while (walk.base + kWave <= b) walk_to(a, walk, walk.base + kWave, walk.before + lane_of(walk.upto, kWave - 1));
+  const int lane = b - walk.base, rounds = __builtin_amdgcn_readlane(walk.rounds, lane);
+  const int64_t unit = walk.before + lane_of(walk.upto, lane) - (int64_t)rounds * (view.kv_heads - kv_head);
+  const int64_t first = ((unit + kStart + 1) * workgroups - 1) / units, last = ((unit + rounds) * workgroups - 1) / units;
+  if (first == last) return;
   const int t = r / a.group, h = kv_head * a.group + r - t * a.group;
-  const Reach reach = seq.reach(a, t);
-  const int chunk = seq.chunk(a), part0 = reach.begin / chunk, part1 = reach.end > 0 ? (reach.end - 1) / chunk : 0;
-  if (part0 == part1) return;
-  const int64_t at = (((int64_t)b * view.kv_heads + kv_head) * kFewRows + r) * a.splits;
-  const float* o = a.partial + at * D + d0;
-  const float* ml = a.partial + a.partial_rows * a.splits * D + at * 2;
-  float best = -INFINITY;
-  for (int p = part0; p <= part1; ++p) best = fmaxf(best, ml[2 * p]);
-  const float zero = best == -INFINITY ? 0.f : best;
-  float total = 0.f, sum[kWide] = {};
-#pragma unroll 4
-  for (int p = part0; p <= part1; ++p) {
-    const float weight = __builtin_amdgcn_exp2f(ml[2 * p] - zero);
-    total += ml[2 * p + 1] * weight;
-    const Vec<float, kWide> x = load_vec<float, kWide>(o + (int64_t)p * D);
-#pragma unroll
-    for (int c = 0; c < kWide; ++c) sum[c] += x.v[c] * weight;
-  }
-  const float inv = total != 0.f ? 1.0f / total : 0.f;
-  Vec<T, kWide> x;
-#pragma unroll
-  for (int c = 0; c < kWide; ++c) x.v[c] = from_float<T>(sum[c] * inv);
-  store_vec<T, kWide>(static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D + d0, x);
+  const float* ml = a.partial + 2 * (int64_t)a.splits * kFewRows * D;
+  join_parts<T, D>(
+      a.partial, ml, (int)(last - first) + 1, [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; },
+      static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D);
 }
 
 }  // namespace
@@ -348,11 +413,13 @@ int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t
   const unsigned pairs = (unsigned)((int64_t)a.view.batch * a.view.kv_heads);
   TTMI_DISPATCH_FLOAT(dtype, T, {
     auto launch = [&](auto kernel, auto join) {
-      hipLaunchKernelGGL(kernel, dim3(pairs, 1, (unsigned)a.splits), dim3(256), 0, stream, a);
-      if (a.splits > 1) hipLaunchKernelGGL(join, dim3(pairs), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL(kernel, dim3(a.splits > 0 ? (unsigned)a.splits : pairs), dim3(a.waves * 64), 0, stream, a);
+      if (a.splits > 0) hipLaunchKernelGGL(join, dim3(pairs, (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0, stream, a);
     };
-    if (head_dim == 64) launch(few_rows_kernel<T, 64>, join_few_rows_kernel<T, 64>);
-    else launch(few_rows_kernel<T, 128>, join_few_rows_kernel<T, 128>);
+    if (head_dim == 64 && a.waves == 4) launch(few_rows_kernel<T, 64, 4>, join_few_rows_kernel<T, 64>);
+    else if (head_dim == 64) launch(few_rows_kernel<T, 64, 8>, join_few_rows_kernel<T, 64>);
+    else if (a.waves == 4) launch(few_rows_kernel<T, 128, 4>, join_few_rows_kernel<T, 128>);
+    else launch(few_rows_kernel<T, 128, 8>, join_few_rows_kernel<T, 128>);
   });
   return launch_status("paged_attention");
 }

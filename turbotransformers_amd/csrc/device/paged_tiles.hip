@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   PageCursor cursor;
   cursor.table = view.table + (int64_t)b * view.table_pitch;
   cursor.last = max(0, (end - 1) >> view.page_shift);
-  cursor.entry = 0;
+  cursor.first = 0, cursor.entry = 0, cursor.ahead = 0;
   const bool small_pages = view.page_shift < 4;
   u32x4 kr[S::kPieces], vr[S::kPieces];
   // 16-byte pieces of a tile: thread by thread, 4 KB after 4 KB.  A wavefront's 1 KB lies in one group of 16 rows.
@@ -302,44 +302,26 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
     for (int g = 0; g < 4; ++g)
       *reinterpret_cast<floatx4*>(to + 32 * t + 8 * g) = floatx4{ot[t][4 * g], ot[t][4 * g + 1], ot[t][4 * g + 2], ot[t][4 * g + 3]};
   if (lhalf == 0) {
-    float* ml = a.partial + a.partial_rows * a.splits * D + at * 2;
+    float* ml = a.partial + (int64_t)view.tokens * a.heads * a.splits * D + at * 2;
     ml[0] = top, ml[1] = sum;
   }
 }
 
-// Rows whose keys lay in several parts: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.
+// Rows whose keys lay in several parts: a workgroup per row and head.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_tiles_kernel(const PagedArgs a) {
-  constexpr int kWide = D / 16;
   const PagedView& view = a.view;
-  const int row = blockIdx.x, b = sequence_of(view, row);
+  const int row = blockIdx.x, h = blockIdx.y, b = sequence_of(view, row);
   if (b >= view.batch) return;
   const Sequence seq = sequence(a, b);
-  const int h = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * kWide;
-  if (row < seq.start || (seq.tokens * a.group <= kFewRows && !a.every) || h >= a.heads) return;
+  if (row < seq.start || (seq.tokens * a.group <= kFewRows && !a.every)) return;
   const Reach reach = seq.reach(a, row - seq.start);
   const int chunk = seq.chunk(a), part0 = reach.begin / chunk, part1 = reach.end > 0 ? (reach.end - 1) / chunk : 0;
   if (part0 == part1) return;
-  const int64_t at = ((int64_t)row * a.heads + h) * a.splits;
-  const float* o = a.partial + at * D + d0;
-  const float* ml = a.partial + a.partial_rows * a.splits * D + at * 2;
-  float best = -INFINITY;
-  for (int p = part0; p <= part1; ++p) best = fmaxf(best, ml[2 * p]);
-  const float zero = best == -INFINITY ? 0.f : best;
-  float total = 0.f, sum[kWide] = {};
-#pragma unroll 4
-  for (int p = part0; p <= part1; ++p) {
-    const float weight = __builtin_amdgcn_exp2f(ml[2 * p] - zero);
-    total += ml[2 * p + 1] * weight;
-    const Vec<float, kWide> x = load_vec<float, kWide>(o + (int64_t)p * D);
-#pragma unroll
-    for (int c = 0; c < kWide; ++c) sum[c] += x.v[c] * weight;
-  }
-  const float inv = total != 0.f ? 1.0f / total : 0.f;
-  Vec<T, kWide> x;
-#pragma unroll
-  for (int c = 0; c < kWide; ++c) x.v[c] = from_float<T>(sum[c] * inv);
-  store_vec<T, kWide>(static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D + d0, x);
+  const int64_t at = ((int64_t)row * a.heads + h) * a.splits + part0;
+  join_parts<T, D>(
+      a.partial, a.partial + (int64_t)view.tokens * a.heads * a.splits * D, part1 - part0 + 1, [&](int p) { return at + p; },
+      static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D);
 }
 
 }  // namespace
@@ -350,7 +332,7 @@ int launch_tiles(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t st
   TTMI_DISPATCH_FLOAT(dtype, T, {
     auto launch = [&](auto kernel, auto join) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * a.view.kv_heads), 1, (unsigned)a.splits), dim3(256), 0, stream, a);
-      if (a.splits > 1) hipLaunchKernelGGL(join, dim3((unsigned)a.view.tokens, (unsigned)ceil_div(a.heads, 16)), dim3(256), 0, stream, a);
+      if (a.splits > 1) hipLaunchKernelGGL(join, dim3((unsigned)a.view.tokens, (unsigned)a.heads), dim3(256), 0, stream, a);
     };
     if (head_dim == 64) launch(tiles_kernel<T, 64>, join_tiles_kernel<T, 64>);
     else launch(tiles_kernel<T, 128>, join_tiles_kernel<T, 128>);

@@ -20,13 +20,14 @@ from .. import cxx
 __all__ = ['PagedCache', 'PagedBatch', 'rotary_append', 'paged_attention', 'copy_pages', 'rotary_frequencies']
 
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)  # absent from builds without a device
+_current_device, _is_initialized = torch.cuda.current_device, torch.cuda.is_initialized
 
 
 def _here():
     """The current device and stream; -1 where there is none (the operators then say what is wrong with their tensors)."""
-    if _raw_stream is None or not torch.cuda.is_available():
+    if _raw_stream is None or not _is_initialized():
         return -1, 0
-    device = torch.cuda.current_device()
+    device = _current_device()
     return device, _raw_stream(device)
 
 
@@ -63,7 +64,7 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     max_tokens, max_length: the most new tokens and keys of a sequence, where known: they choose how the work is cut, not what is computed.
     -> like q: `out` if given."""
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q)
     cxx.paged_attention(q, keys, values, table, starts, lengths, out, max_tokens, max_length, 0.0 if scale is None else scale, causal, window,
                         _empty_bytes, *_here())
     return out
