@@ -33,7 +33,7 @@ DEVICE_FLAGS = [
 # Per-file additions.  attention.hip: maxima over MFMA results would otherwise be preceded by one
 # canonicalising v_max per operand (signalling-NaN quieting), a tenth of the softmax's VALU work.
 # (Not attention_split.hip, which serves fp32 too and is bound by its waits: 1 x 387 tokens in fp16 6.6 us either way.)
-DEVICE_FILE_FLAGS = {"attention.hip": ["-fno-honor-nans"]}
+DEVICE_FILE_FLAGS = {name: ["-fno-honor-nans"] for name in ("attention.hip", "paged_tiles.hip", "paged_few_rows.hip")}
 for _name in ("gemm", "gemm_f16", "gemm_bf16", "gemm_f32", "gemm_i8"):
     DEVICE_FILE_FLAGS[_name + ".hip"] = ["-mllvm", "-pragma-unroll-threshold=65536"]
 

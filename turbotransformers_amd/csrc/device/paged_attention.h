@@ -55,41 +55,47 @@ __device__ __forceinline__ Sequence sequence(const PagedArgs& a, int b) {
   return s;
 }
 
-// The pages that a wavefront is about to read, 64 of them a lane each, and the 64 behind those, which are on their way.  (A page of 16 or more slots holds groups of
-// 16 rows whole, so the page of a group is one number for the wavefront; smaller pages are looked up row by row.)
+// The pages that a wavefront is about to read, 64 of them, a lane each: where their rows of one key/value head begin; and the numbers of the 64 behind those, which are on
+// their way.  A page of 16 or more slots holds groups of 16 rows whole, so where a group lies is one number for the wavefront (smaller pages are looked up row by row).
 struct PageCursor {
   const int32_t* table;  // of the sequence
   int first, last;       // number of the first page held here; of the sequence's last one
-  int32_t entry, ahead;
+  int32_t ahead;
+  int64_t at;            // bytes
 };
 __device__ __forceinline__ int32_t checked_page(const PagedView& view, int32_t page) {
   if ((unsigned)page < (unsigned)view.pages) return page;
   page_error(view);
   return 0;
 }
-__device__ __forceinline__ void fetch_pages(const PagedView& view, PageCursor& at, int page) {
-  const int lane = (int)(threadIdx.x % kWave);
-  at.first = page;
-  at.entry = checked_page(view, at.table[min(page + lane, at.last)]);
-  at.ahead = at.table[min(page + kWave + lane, at.last)];
+// Lanes past the sequence's last page hold that.
+template <int ROW_BYTES>
+__device__ __forceinline__ void hold_pages(const PagedView& view, PageCursor& c, int kv_head, int first, int32_t pages) {
+  c.first = first;
+  c.at = (((int64_t)checked_page(view, pages) * view.kv_heads + kv_head) << view.page_shift) * ROW_BYTES;
+  c.ahead = c.table[min(first + kWave + (int)(threadIdx.x % kWave), c.last)];
 }
-__device__ __forceinline__ void next_pages(const PagedView& view, PageCursor& at) {
-  at.first += kWave;
-  at.entry = checked_page(view, at.ahead);
-  at.ahead = at.table[min(at.first + kWave + (int)(threadIdx.x % kWave), at.last)];
+template <int ROW_BYTES>
+__device__ __forceinline__ void fetch_pages(const PagedView& view, PageCursor& c, int kv_head, int key) {
+  const int page = key >> view.page_shift;
+  hold_pages<ROW_BYTES>(view, c, kv_head, page, c.table[min(page + (int)(threadIdx.x % kWave), c.last)]);
 }
-// Element of the cache at which the row of `key` begins; rows of a group of 16 follow each other.  For pages of 16 and more slots; key is uniform and a multiple
-// of 16.
-template <int D>
-__device__ __forceinline__ int64_t group_offset(const PagedView& view, PageCursor& at, int kv_head, int key) {
-  const int page = min(key >> view.page_shift, at.last);
-  if (page - at.first >= kWave) {
-    if (page - at.first < 2 * kWave) next_pages(view, at);
-    else fetch_pages(view, at, page);
-  }
-  const int32_t entry = __builtin_amdgcn_readlane(at.entry, page - at.first);
-  return ((((int64_t)entry * view.kv_heads + kv_head) << view.page_shift) + (key & ((1 << view.page_shift) - 1))) * D;
+// Before the groups of a tile are asked for.  (The 64 pages that are held end where a tile ends: tiles and their steps are powers of two, and so are pages.)
+template <int ROW_BYTES>
+__device__ __forceinline__ void come_to(const PagedView& view, PageCursor& c, int kv_head, int key) {
+  const int past = (key >> view.page_shift) - c.first;
+  if (__builtin_expect(past < kWave, 1)) return;
+  if (past >= 2 * kWave) fetch_pages<ROW_BYTES>(view, c, kv_head, key);
+  else hold_pages<ROW_BYTES>(view, c, kv_head, c.first + kWave, c.ahead);
 }
+// Byte of the cache at which the row of `key`, uniform and a multiple of 16, begins; the rows of its group follow.
+template <int ROW_BYTES>
+__device__ __forceinline__ int64_t group_at(const PagedView& view, const PageCursor& c, int key) {
+  const int lane = (key >> view.page_shift) - c.first;
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)c.at, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(c.at >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo) + (key & ((1 << view.page_shift) - 1)) * ROW_BYTES;
+}
+// Element at which any row begins, looked up.
 template <int D>
 __device__ __forceinline__ int64_t row_offset(const PagedView& view, const PageCursor& at, int kv_head, int key) {
   const int32_t entry = checked_page(view, at.table[min(key >> view.page_shift, at.last)]);
@@ -122,6 +128,33 @@ __device__ __forceinline__ u32x4 finite_part(u32x4 x) {
     }
   }
   return x;
+}
+
+// (Both kernels are compiled as if there were no NaNs, which saves a canonicalising instruction for every operand of a maximum: what has to tell them asks for their bits.)
+template <typename T>
+__device__ __forceinline__ bool wild_value(T v) {
+  if constexpr (sizeof(T) == 4) return (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) == 0x7f800000u;
+  else {
+    constexpr uint16_t kExp = std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
+    return (__builtin_bit_cast(uint16_t, v) & kExp) == kExp;
+  }
+}
+// The reference point of a row's probabilities, in units of scale log2(e) score, a whole number: it moves only where a score lies more than this above it, so the sums are
+// seldom scaled, and then by powers of two.  Probabilities of up to 2^8 lose nothing: they are as exact in their type as those up to 1, and the division by their sum takes the factor back out.  (The
+// decision is the row's own: what is in the tile with it moves no bit of it.)
+constexpr float kSlack = 8.f;
+__device__ __forceinline__ float moved_reference(float top, float highest) { return highest > top + kSlack || top == -INFINITY ? fmaxf(__builtin_ceilf(highest), top) : top; }
+// Two packed probabilities times a power of two.
+template <typename T>
+__device__ __forceinline__ uint32_t scale_pair(uint32_t p, float by) {
+  float lo, hi;
+  if constexpr (std::is_same<T, f16>::value) {
+    const halfx2 x = __builtin_bit_cast(halfx2, p);
+    lo = (float)x[0], hi = (float)x[1];
+  } else {
+    lo = __builtin_bit_cast(float, p << 16), hi = __builtin_bit_cast(float, p & 0xffff0000u);
+  }
+  return pack2<T>(lo * by, hi * by);
 }
 
 // What this lane gets of a 4 x 16 block of 16-bit values in LDS that lies row by row: four lanes point at the 32 bytes of a row, lane i of the sixteen gets column i.

@@ -127,13 +127,14 @@ __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t 
 constexpr int kFewest = 2;
 __device__ __forceinline__ int64_t sharers(const PagedArgs& a, int64_t units) { return max((int64_t)1, min((int64_t)a.splits, (units + kFewest - 1) / kFewest)); }
 
-template <typename T, int D, int NW>
+// SMALL: pages of fewer than 16 slots
+template <typename T, int D, int NW, bool SMALL>
 __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedArgs a) {
   using S = FewRows<T, D, NW>;
   __shared__ __align__(16) char smem[S::kLds];
   __shared__ float met[NW][kFewRows][2];
   const PagedView& view = a.view;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 15, quarter = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = lane & 15, quarter = lane >> 4;
   const T* const q = static_cast<const T*>(a.q);
   const T* const keys = static_cast<const T*>(a.keys);
   const T* const values = static_cast<const T*>(a.values);
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
   if (round0 == 0 && kv_head == 0 && tid == 0 && view.lengths[b] > seq.length) page_error(view);
   PageCursor cursor;
   cursor.table = view.table + (int64_t)b * view.table_pitch;
-  cursor.first = 0, cursor.entry = 0, cursor.ahead = 0;
+  cursor.first = 0, cursor.ahead = 0, cursor.at = 0;
 
   for (int row0 = 0; row0 < rows_all; row0 += kFewRows) {
     const int rows = min(kFewRows, rows_all - row0);
@@ -192,22 +193,22 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
     float top = -INFINITY, sum = 0.f;  // of scale * log2(e) * score; the sum is this quarter's share
 
     u32x4 kf[S::kGroups][S::kSteps], vf[S::kGroups][S::kValuePieces];
-    const bool small_pages = view.page_shift < 4;
     auto load_keys = [&](int key) __attribute__((always_inline)) {
 #pragma unroll
       for (int g = 0; g < S::kGroups; ++g) {
         const T* p;
-        if (!small_pages) p = keys + group_offset<D>(view, cursor, kv_head, key + 16 * g) + row * D;
+        if constexpr (!SMALL) p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(keys) + group_at<S::kRowBytes>(view, cursor, key + 16 * g)) + row * D;
         else p = keys + row_offset<D>(view, cursor, kv_head, key + 16 * g + row);
 #pragma unroll
         for (int i = 0; i < S::kSteps; ++i) kf[g][i] = *reinterpret_cast<const u32x4*>(p + (quarter + 4 * i) * S::kElems);
       }
     };
-    auto load_values = [&](int key) __attribute__((always_inline)) {
+    auto load_values = [&](int key) __attribute__((always_inline)) {  // before the keys of the tile
+      if constexpr (!SMALL) come_to<S::kRowBytes>(view, cursor, kv_head, key);
 #pragma unroll
       for (int g = 0; g < S::kGroups; ++g) {
-        if (!small_pages) {
-          const T* p = values + group_offset<D>(view, cursor, kv_head, key + 16 * g) + lane * S::kElems;
+        if constexpr (!SMALL) {
+          const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(values) + group_at<S::kRowBytes>(view, cursor, key + 16 * g)) + lane * S::kElems;
 #pragma unroll
           for (int i = 0; i < S::kValuePieces; ++i) vf[g][i] = *reinterpret_cast<const u32x4*>(p + i * 64 * S::kElems);
         } else {
@@ -221,13 +222,8 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
     };
 
     constexpr int kStep = NW * S::kKeys;
-    int key = lo + wave * S::kKeys;
-    if (key < hi) {
-      fetch_pages(view, cursor, min(key >> view.page_shift, cursor.last));
-      load_values(key);
-      load_keys(key);
-    }
-    for (; key < hi; key += kStep) {
+    // One tile.  Whether another follows is known to the compiler: a load that may or may not have been sent would make it wait for all of them.
+    auto work_on = [&](int key, auto more) __attribute__((always_inline)) {
       const bool masked = key < sure_first || key + S::kKeys > sure_end || key + S::kKeys > hi;
       uint32_t wild = 0;
       if (masked) {  // keys that no row sees may hold anything: their values count as zeros, and one that only some rows see must not reach the others
@@ -249,8 +245,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
           *reinterpret_cast<u32x4*>(tile + r * S::kRowBytes + value_piece<T, D>(r, at % S::kRowBytes / 16) * 16) = wild ? finite_part<T>(vf[g][i]) : vf[g][i];
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the tile is this wavefront's alone: its LDS accesses are in order)
-      const int next = key + kStep;
-      if (next < hi) load_values(next);
+      if constexpr (decltype(more)::value) load_values(key + kStep);
 
       floatx4 st[S::kGroups];
 #pragma unroll
@@ -259,7 +254,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
 #pragma unroll
         for (int i = 0; i < S::kSteps; ++i) st[g] = mma16<T>(kf[g][i], qf[i], st[g]);
       }
-      if (next < hi) load_keys(next);
+      if constexpr (decltype(more)::value) load_keys(key + kStep);
       if (masked) {
 #pragma unroll
         for (int g = 0; g < S::kGroups; ++g)
@@ -274,7 +269,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
       for (int g = 0; g < S::kGroups; ++g)
 #pragma unroll
         for (int e = 0; e < 4; ++e) m = fmaxf(m, st[g][e]);
-      const float moved = fmaxf(top, quarters_max(m) * a.scale_log2e);
+      const float moved = moved_reference(top, quarters_max(m) * a.scale_log2e);
       const float zero = moved == -INFINITY ? 0.f : moved;  // (a row that has seen no key yet)
       const float shrink = __builtin_amdgcn_exp2f(top - zero);
       top = moved;
@@ -331,11 +326,19 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
           for (int t = 0; t < S::kTiles; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float x = to_float(v[16 * t + e]);
-              if (seen && !(fabsf(x) < INFINITY)) ot[t][e] += x;
+              const T x = v[16 * t + e];
+              if (seen && wild_value(x)) ot[t][e] += to_float(x);
             }
         }
       }
+    };
+    int key = lo + wave * S::kKeys;
+    if (key < hi) {
+      if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, key);
+      load_values(key);
+      load_keys(key);
+      for (; key + kStep < hi; key += kStep) work_on(key, std::true_type{});
+      work_on(key, std::false_type{});
     }
 
     // the wavefronts meet
@@ -416,10 +419,16 @@ int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t
       hipLaunchKernelGGL(kernel, dim3(a.splits > 0 ? (unsigned)a.splits : pairs), dim3(a.waves * 64), 0, stream, a);
       if (a.splits > 0) hipLaunchKernelGGL(join, dim3(pairs, (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0, stream, a);
     };
-    if (head_dim == 64 && a.waves == 4) launch(few_rows_kernel<T, 64, 4>, join_few_rows_kernel<T, 64>);
-    else if (head_dim == 64) launch(few_rows_kernel<T, 64, 8>, join_few_rows_kernel<T, 64>);
-    else if (a.waves == 4) launch(few_rows_kernel<T, 128, 4>, join_few_rows_kernel<T, 128>);
-    else launch(few_rows_kernel<T, 128, 8>, join_few_rows_kernel<T, 128>);
+    const bool small = a.view.page_shift < 4;
+    auto sized = [&](auto d) {
+      constexpr int D = decltype(d)::value;
+      if (small && a.waves == 4) launch(few_rows_kernel<T, D, 4, true>, join_few_rows_kernel<T, D>);
+      else if (small) launch(few_rows_kernel<T, D, 8, true>, join_few_rows_kernel<T, D>);
+      else if (a.waves == 4) launch(few_rows_kernel<T, D, 4, false>, join_few_rows_kernel<T, D>);
+      else launch(few_rows_kernel<T, D, 8, false>, join_few_rows_kernel<T, D>);
+    };
+    if (head_dim == 64) sized(std::integral_constant<int, 64>{});
+    else sized(std::integral_constant<int, 128>{});
   });
   return launch_status("paged_attention");
 }
