@@ -144,18 +144,6 @@ __device__ __forceinline__ bool wild_value(T v) {
 // decision is the row's own: what is in the tile with it moves no bit of it.)
 constexpr float kSlack = 8.f;
 __device__ __forceinline__ float moved_reference(float top, float highest) { return highest > top + kSlack || top == -INFINITY ? fmaxf(__builtin_ceilf(highest), top) : top; }
-// Two packed probabilities times a power of two.
-template <typename T>
-__device__ __forceinline__ uint32_t scale_pair(uint32_t p, float by) {
-  float lo, hi;
-  if constexpr (std::is_same<T, f16>::value) {
-    const halfx2 x = __builtin_bit_cast(halfx2, p);
-    lo = (float)x[0], hi = (float)x[1];
-  } else {
-    lo = __builtin_bit_cast(float, p << 16), hi = __builtin_bit_cast(float, p & 0xffff0000u);
-  }
-  return pack2<T>(lo * by, hi * by);
-}
 
 // What this lane gets of a 4 x 16 block of 16-bit values in LDS that lies row by row: four lanes point at the 32 bytes of a row, lane i of the sixteen gets column i.
 __device__ __forceinline__ u32x2 read_transposed(const void* p) {

@@ -36,7 +36,7 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   const int64_t most = max_tokens > 0 ? std::min(max_tokens, tokens) : tokens;
   const int64_t reach = window > 0 ? std::min(longest, window + most) : longest;
   p.tiles = most * group > kFewRows;
-  p.few = !p.tiles || tokens * group / batch < 512;
+  p.few = !p.tiles || tokens * group / batch < 64;
   p.few_rows = p.tiles ? kFewRows : (int)(most * group);
   p.few_splits = reach * 2 * view.head_dim * (int64_t)dtype_size(dtype) <= kWholeBytes ? 0 : 2 * compute_units();
   p.few_waves = p.few_splits == 0 && batch * view.kv_heads < compute_units() ? 8 : 4;
