@@ -23,7 +23,8 @@ struct PagedArgs {
   // that is its own (at most kFewRows).
   // Of the other.  Keys are cut at multiples of `chunk` (a multiple of 64), counted from the first of the sequence, into at most `splits` parts (the grid); a sequence
   // that has more keys than that takes longer parts.
-  int splits, waves, few, chunk;
+  // ordered: its workgroups begin with those that have the most keys.
+  int splits, waves, few, chunk, ordered;
   float* partial;  // sums of rows whose keys are several workgroups' [..][d], behind them the maxima and sums of their probabilities [..][2]
 };
 

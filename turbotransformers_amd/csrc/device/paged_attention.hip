@@ -36,11 +36,15 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   const int64_t most = max_tokens > 0 ? std::min(max_tokens, tokens) : tokens;
   const int64_t reach = window > 0 ? std::min(longest, window + most) : longest;
   p.tiles = most * group > kFewRows;
+  // One launch instead of two where sequences have many rows on average: the kernel for many rows takes those with few as well.  us, 40 sequences decoding and 3 chunks of
+  // 200 to 900 tokens (143 rows on average): two kernels 41.3, one 29.3.
   p.few = !p.tiles || tokens * group / batch < 64;
   p.few_rows = p.tiles ? kFewRows : (int)(most * group);
   p.few_splits = reach * 2 * view.head_dim * (int64_t)dtype_size(dtype) <= kWholeBytes ? 0 : 2 * compute_units();
   p.few_waves = p.few_splits == 0 && batch * view.kv_heads < compute_units() ? 8 : 4;
-  cut(view.kv_heads * (tokens * group / 128 + std::min(batch, tokens)), 512, 256, reach, longest, &p.tile_chunk, &p.tile_splits);
+  // Many rows: cut where two workgroups a CU are not reached, into parts of at least as many keys as take longer than their joining (fp32, whose matrix instructions take
+  // sixteen times as long: us for one prompt of 200 tokens, 12 heads of 64, parts of 256 / 64 at least 22.0 / 15.7; 16-bit types 9.8 / 11.7).
+  cut(view.kv_heads * (tokens * group / 128 + std::min(batch, tokens)), 512, dtype == TTMI_F32 ? 64 : 256, reach, longest, &p.tile_chunk, &p.tile_splits);
   const int64_t d = view.head_dim;
   p.few_floats = p.few ? 2ll * p.few_splits * kFewRows * (d + 2) : 0;
   p.tile_floats = p.tiles && p.tile_splits > 1 ? tokens * heads * p.tile_splits * (d + 2) : 0;

@@ -72,30 +72,41 @@ __device__ __forceinline__ void store_rows(const PagedArgs& a, const Sequence& s
   }
 }
 
-// The `want`-th block of rows of all sequences -> its sequence and number in it (false: there are fewer).  Every lane looks at a sequence.
+// The `want`-th block of rows of all sequences -> its sequence and number in it (false: there are fewer).  Every lane looks at a sequence of 64.
+// Where there are more workgroups than the chip takes at a time, those with the most keys come first: sequences by their keys (64 of them at a time), and in a sequence the
+// last rows, which have the most keys before them.
 __device__ __forceinline__ bool find_block(const PagedArgs& a, int want, int* b, int* block) {
   const int lane = (int)(threadIdx.x % kWave);
   for (int base = 0; base < a.view.batch; base += kWave) {
-    int blocks = 0;
+    int blocks = 0, reach = 0;
     if (base + lane < a.view.batch) {
-      const int rows = sequence(a, base + lane).tokens * a.group;
+      const Sequence seq = sequence(a, base + lane);
+      const int rows = seq.tokens * a.group;
       if (rows > kFewRows || a.every) blocks = (rows + kTileRows - 1) / kTileRows;
+      reach = a.window > 0 ? min(seq.length, a.window + seq.tokens) : seq.length;
     }
-    int upto = blocks;
+    int before = 0, all = 0;
+    if (!a.ordered) {
+      int upto = blocks;
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const int below = __shfl_up(upto, d, kWave);
-      if (lane >= d) upto += below;
+      for (int d = 1; d < kWave; d *= 2) {
+        const int below = __shfl_up(upto, d, kWave);
+        if (lane >= d) upto += below;
+      }
+      before = upto - blocks, all = __builtin_amdgcn_readlane(upto, kWave - 1);
+    } else for (uint64_t others = __ballot(blocks > 0); others != 0; others &= others - 1) {
+      const int j = __ffsll((unsigned long long)others) - 1;
+      const int their_blocks = __builtin_amdgcn_readlane(blocks, j), their_reach = __builtin_amdgcn_readlane(reach, j);
+      all += their_blocks;
+      if (their_reach > reach || (their_reach == reach && j < lane)) before += their_blocks;
     }
-    const uint64_t past = __ballot(upto > want);
-    if (past != 0) {
-      const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
+    if (want < all) {
+      const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(want >= before && want < before + blocks)) - 1);
       *b = base + found;
-      // the last rows have the most keys before them: they begin first
-      *block = __builtin_amdgcn_readlane(upto, found) - 1 - want;
+      *block = __builtin_amdgcn_readlane(before + blocks, found) - 1 - want;
       return true;
     }
-    want -= __builtin_amdgcn_readlane(upto, kWave - 1);
+    want -= all;
   }
   return false;
 }
@@ -310,19 +321,27 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
+static_assert(sizeof(T) == 2 || S::kSubs == 1, "32 keys");
 #pragma unroll
-        for (int u = 0; u < S::kSubs; ++u)
+        for (int e = 0; e < 16; ++e) {
+          st[0][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][e], a.scale_log2e, -zero));
+          sum += st[0][e];
+        }
+        auto read_value = [&](int n) __attribute__((always_inline)) {  // the operand of the n-th matrix instruction of Ot: kOut of them for each pair of keys
+          const int e = n / S::kOut, r = 8 * (e / 4) + 4 * lhalf + e % 4;
+          return *reinterpret_cast<const float*>(vt + r * S::kRowBytes + value_piece<T, D>(r, 8 * (n % S::kOut) + (lrow >> 2)) * 16 + (lrow & 3) * 4);
+        };
+        constexpr int kProducts = 16 * S::kOut;
+        float v[kAhead];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            st[u][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[u][e], a.scale_log2e, -zero));
-            sum += st[u][e];
-            const int r = 32 * u + 8 * (e / 4) + 4 * lhalf + e % 4;
+        for (int n = 0; n < kAhead; ++n) v[n] = read_value(n);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < S::kOut; ++t) {
-              const float v = *reinterpret_cast<const float*>(vt + r * S::kRowBytes + value_piece<T, D>(r, 8 * t + (lrow >> 2)) * 16 + (lrow & 3) * 4);
-              ot[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, st[u][e], ot[t], 0, 0, 0);
-            }
-          }
+        for (int n = 0; n < kProducts; ++n) {
+          ot[n % S::kOut] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[n % kAhead], st[0][n / S::kOut], ot[n % S::kOut], 0, 0, 0);
+          if (n + kAhead < kProducts) v[n % kAhead] = read_value(n + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
       if (__builtin_expect(partly_seen(key), 0) && wild) {  // an infinity or a NaN is what a sum with it is, whatever its weight
 #pragma unroll 1
@@ -356,21 +375,45 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   store_rows<T, D>(a, seq, token, head, part, mine.begin / chunk, mine.end > 0 ? (mine.end - 1) / chunk : 0, lhalf, ot, top, sum);
 }
 
-// Rows whose keys lay in several parts: a workgroup per row and head.
+// Rows whose keys lay in several parts: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A wavefront per row and head: four columns a lane, the parts shared by
+// the lanes that are left.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_tiles_kernel(const PagedArgs a) {
+  constexpr int kThreads = D / 4, kShares = kWave / kThreads;
   const PagedView& view = a.view;
-  const int row = blockIdx.x, h = blockIdx.y, b = sequence_of(view, row);
-  if (b >= view.batch) return;
+  const int row = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = sequence_of(view, row);
+  if (b >= view.batch || h >= a.heads) return;
   const Sequence seq = sequence(a, b);
   if (row < seq.start || (seq.tokens * a.group <= kFewRows && !a.every)) return;
   const Reach reach = seq.reach(a, row - seq.start);
   const int chunk = seq.chunk(a), part0 = reach.begin / chunk, part1 = reach.end > 0 ? (reach.end - 1) / chunk : 0;
   if (part0 == part1) return;
-  const int64_t at = ((int64_t)row * a.heads + h) * a.splits + part0;
-  join_parts<T, D>(
-      a.partial, a.partial + (int64_t)view.tokens * a.heads * a.splits * D, part1 - part0 + 1, [&](int p) { return at + p; },
-      static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D);
+  const int lane = threadIdx.x & 63, d0 = lane % kThreads * 4, share = lane / kThreads;
+  const int64_t at = ((int64_t)row * a.heads + h) * a.splits;
+  const float* const o = a.partial + at * D + d0;
+  const float* const ml = a.partial + (int64_t)view.tokens * a.heads * a.splits * D + at * 2;
+  float best = -INFINITY;
+  for (int p = part0; p <= part1; ++p) best = fmaxf(best, ml[2 * p]);
+  const float zero = best == -INFINITY ? 0.f : best;
+  float total = 0.f;
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int p = part0 + share; p <= part1; p += kShares) {
+    const float weight = __builtin_amdgcn_exp2f(ml[2 * p] - zero);
+    total += ml[2 * p + 1] * weight;
+    sum += *reinterpret_cast<const floatx4*>(o + (int64_t)p * D) * weight;
+  }
+#pragma unroll
+  for (int d = kThreads; d < kWave; d *= 2) {
+    total += __shfl_xor(total, d, kWave);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], d, kWave);
+  }
+  if (share != 0) return;
+  const float inv = total != 0.f ? 1.0f / total : 0.f;
+  Vec<T, 4> x;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) x.v[c] = from_float<T>(sum[c] * inv);
+  store_vec<T, 4>(static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D + d0, x);
 }
 
 }  // namespace
@@ -379,10 +422,12 @@ int launch_tiles(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t st
   // (at most so many blocks of rows: a part of one per sequence is a block of its own)
   const int64_t blocks = (int64_t)a.view.tokens * a.group / kTileRows + std::min(a.view.batch, a.view.tokens);
   const bool small = a.view.page_shift < 4;
+  PagedArgs args = a;
+  args.ordered = blocks * a.view.kv_heads * a.splits > 2 * compute_units();
   TTMI_DISPATCH_FLOAT(dtype, T, {
     auto launch = [&](auto kernel, auto join) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * a.view.kv_heads), 1, (unsigned)a.splits), dim3(256), 0, stream, a);
-      if (a.splits > 1) hipLaunchKernelGGL(join, dim3((unsigned)a.view.tokens, (unsigned)a.heads), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * a.view.kv_heads), 1, (unsigned)a.splits), dim3(256), 0, stream, args);
+      if (a.splits > 1) hipLaunchKernelGGL(join, dim3((unsigned)a.view.tokens, (unsigned)ceil_div(a.heads, 4)), dim3(256), 0, stream, a);
     };
     if (head_dim == 64 && small) launch(tiles_kernel<T, 64, true>, join_tiles_kernel<T, 64>);
     else if (head_dim == 64) launch(tiles_kernel<T, 64, false>, join_tiles_kernel<T, 64>);
