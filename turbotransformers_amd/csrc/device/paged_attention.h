@@ -195,6 +195,38 @@ __device__ __forceinline__ void join_parts(const float* partial, const float* ml
   out[threadIdx.x] = from_float<T>(l != 0.f ? x / l : 0.f);
 }
 
+// The same for one wavefront and few parts: four columns a lane, the parts shared by the lanes that are left.
+template <typename T, int D, typename At>
+__device__ __forceinline__ void join_parts_by_wavefront(const float* partial, const float* ml, int parts, At at, T* out) {
+  constexpr int kThreads = D / 4, kShares = kWave / kThreads;
+  const int lane = (int)(threadIdx.x % kWave), d0 = lane % kThreads * 4, share = lane / kThreads;
+  float best = -INFINITY;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) best = fmaxf(best, ml[2 * at(p)]);
+  const float zero = best == -INFINITY ? 0.f : best;
+  float total = 0.f;
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = share; p < parts; p += kShares) {
+    const int64_t row = at(p);
+    const float weight = __builtin_amdgcn_exp2f(ml[2 * row] - zero);
+    total += ml[2 * row + 1] * weight;
+    sum += *reinterpret_cast<const floatx4*>(partial + row * D + d0) * weight;
+  }
+#pragma unroll
+  for (int d = kThreads; d < kWave; d *= 2) {
+    total += __shfl_xor(total, d, kWave);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], d, kWave);
+  }
+  if (share != 0) return;
+  const float inv = total != 0.f ? 1.0f / total : 0.f;
+  Vec<T, 4> x;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) x.v[c] = from_float<T>(sum[c] * inv);
+  store_vec<T, 4>(out + d0, x);
+}
+
 int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream);
 int launch_tiles(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream);
 

@@ -388,14 +388,16 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
   }
 }
 
-// Pairs that were several workgroups': o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over their partial results.  A workgroup per row of a pair.
+// Pairs that were several workgroups': their rows' partial results are joined.  A workgroup per pair and row, or per pair where there are many of them: then a wavefront
+// takes a row, unless the pair had many parts.
+constexpr int kManyPairs = 64, kManyParts = 16;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a) {
   const PagedView& view = a.view;
-  const int kv_head = blockIdx.x % view.kv_heads, b = blockIdx.x / view.kv_heads, r = blockIdx.y;
+  const int kv_head = blockIdx.x % view.kv_heads, b = blockIdx.x / view.kv_heads;
   const Sequence seq = sequence(a, b);
   const int rows = seq.tokens * a.group;
-  if (rows > a.few || r >= rows) return;
+  if (rows > a.few || (int)blockIdx.y >= rows) return;
   Walk walk;
   const int64_t units = count_units(a, walk), workgroups = sharers(a, units);
   while (walk.base + kWave <= b) walk_to(a, walk, walk.base + kWave, walk.before + lane_of(walk.upto, kWave - 1));
@@ -403,11 +405,23 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a) {
   const int64_t unit = walk.before + lane_of(walk.upto, lane) - (int64_t)rounds * (view.kv_heads - kv_head);
   const int64_t first = ((unit + kStart + 1) * workgroups - 1) / units, last = ((unit + rounds) * workgroups - 1) / units;
   if (first == last) return;
-  const int t = r / a.group, h = kv_head * a.group + r - t * a.group;
-  const float* ml = a.partial + 2 * (int64_t)a.splits * kFewRows * D;
-  join_parts<T, D>(
-      a.partial, ml, (int)(last - first) + 1, [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; },
-      static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D);
+  const int parts = (int)(last - first) + 1;
+  const float* const ml = a.partial + 2 * (int64_t)a.splits * kFewRows * D;
+  auto place = [&](int r) {
+    const int t = r / a.group, h = kv_head * a.group + r - t * a.group;
+    return static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D;
+  };
+  if (gridDim.y == 1 && parts <= kManyParts) {
+    for (int r = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < rows; r += 4)
+      join_parts_by_wavefront<T, D>(
+          a.partial, ml, parts, [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
+    return;
+  }
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    join_parts<T, D>(
+        a.partial, ml, parts, [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
+    __syncthreads();
+  }
 }
 
 }  // namespace
@@ -417,7 +431,7 @@ int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t
   TTMI_DISPATCH_FLOAT(dtype, T, {
     auto launch = [&](auto kernel, auto join) {
       hipLaunchKernelGGL(kernel, dim3(a.splits > 0 ? (unsigned)a.splits : pairs), dim3(a.waves * 64), 0, stream, a);
-      if (a.splits > 0) hipLaunchKernelGGL(join, dim3(pairs, (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0, stream, a);
+      if (a.splits > 0) hipLaunchKernelGGL(join, dim3(pairs, pairs >= kManyPairs ? 1u : (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0, stream, a);
     };
     const bool small = a.view.page_shift < 4;
     auto sized = [&](auto d) {

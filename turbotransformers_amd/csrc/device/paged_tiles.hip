@@ -375,11 +375,9 @@ static_assert(sizeof(T) == 2 || S::kSubs == 1, "32 keys");
   store_rows<T, D>(a, seq, token, head, part, mine.begin / chunk, mine.end > 0 ? (mine.end - 1) / chunk : 0, lhalf, ot, top, sum);
 }
 
-// Rows whose keys lay in several parts: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A wavefront per row and head: four columns a lane, the parts shared by
-// the lanes that are left.
+// Rows whose keys lay in several parts: a wavefront per row and head.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_tiles_kernel(const PagedArgs a) {
-  constexpr int kThreads = D / 4, kShares = kWave / kThreads;
   const PagedView& view = a.view;
   const int row = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = sequence_of(view, row);
   if (b >= view.batch || h >= a.heads) return;
@@ -388,32 +386,10 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(const PagedArgs a) {
   const Reach reach = seq.reach(a, row - seq.start);
   const int chunk = seq.chunk(a), part0 = reach.begin / chunk, part1 = reach.end > 0 ? (reach.end - 1) / chunk : 0;
   if (part0 == part1) return;
-  const int lane = threadIdx.x & 63, d0 = lane % kThreads * 4, share = lane / kThreads;
-  const int64_t at = ((int64_t)row * a.heads + h) * a.splits;
-  const float* const o = a.partial + at * D + d0;
-  const float* const ml = a.partial + (int64_t)view.tokens * a.heads * a.splits * D + at * 2;
-  float best = -INFINITY;
-  for (int p = part0; p <= part1; ++p) best = fmaxf(best, ml[2 * p]);
-  const float zero = best == -INFINITY ? 0.f : best;
-  float total = 0.f;
-  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int p = part0 + share; p <= part1; p += kShares) {
-    const float weight = __builtin_amdgcn_exp2f(ml[2 * p] - zero);
-    total += ml[2 * p + 1] * weight;
-    sum += *reinterpret_cast<const floatx4*>(o + (int64_t)p * D) * weight;
-  }
-#pragma unroll
-  for (int d = kThreads; d < kWave; d *= 2) {
-    total += __shfl_xor(total, d, kWave);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], d, kWave);
-  }
-  if (share != 0) return;
-  const float inv = total != 0.f ? 1.0f / total : 0.f;
-  Vec<T, 4> x;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) x.v[c] = from_float<T>(sum[c] * inv);
-  store_vec<T, 4>(static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D + d0, x);
+  const int64_t at = ((int64_t)row * a.heads + h) * a.splits + part0;
+  join_parts_by_wavefront<T, D>(
+      a.partial, a.partial + (int64_t)view.tokens * a.heads * a.splits * D, part1 - part0 + 1, [&](int p) { return at + p; },
+      static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D);
 }
 
 }  // namespace

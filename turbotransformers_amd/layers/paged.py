@@ -45,10 +45,12 @@ def rotary_append(qkv: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     makes them), None: nothing turns.  interleaved: pairs are neighbours (2i, 2i + 1), else (i, i + len(inv_freq)).
     -> the queries [tokens, heads, head_dim]: `out` if given, which may be the queries' part of qkv itself."""
     if out is None:
-        heads = (qkv.shape[1] // keys.shape[3] if qkv.dim() == 2 else qkv.shape[1]) - 2 * keys.shape[1]
+        shape = qkv.shape
+        _, kv_heads, _, d = keys.shape
+        heads = (shape[1] // d if len(shape) == 2 else shape[1]) - 2 * kv_heads
         if heads < 1:
             raise ValueError("qkv has no room for queries beside the cache's heads")
-        out = qkv.new_empty((qkv.shape[0], heads, keys.shape[3]))
+        out = qkv.new_empty((shape[0], heads, d))
     cxx.rotary_append(qkv, keys, values, table, starts, lengths, inv_freq, interleaved, amplitude, out, *_here())
     return out
 
