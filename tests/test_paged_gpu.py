@@ -573,3 +573,17 @@ def test_c_interface():
     assert torch.equal(out, case.run_attention(max_tokens=1, max_length=5001))
     if n.value:
         assert call(n.value - 1) == -1
+
+
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("batch", [64, 65, 130, 400])
+def test_many_sequences(dt, batch):
+    """More sequences than a wavefront has lanes, long ones among short ones, some without new tokens: shared out evenly and joined, and in blocks of many rows."""
+    rng = random.Random(batch)
+    lengths = [rng.choice([1, 5, 40, 90, 700 if i % 9 == 0 else 130]) for i in range(batch)]
+    new = [0 if i % 7 == 3 else 1 for i in range(batch)]
+    check(dt, new, [n - m for n, m in zip(lengths, new)], 4, 2, 64, 16, spare_rows=1)
+    case = Case(dt, new, [n - m for n, m in zip(lengths, new)], 4, 2, 64, 16, seed=1)
+    case.check_attention(case.run_attention(max_length=5000))  # (long enough for sharing out)
+    new = [40 if i % 11 == 0 else m for i, m in enumerate(new)]
+    check(dt, new, lengths, 4, 2, 64, 16)

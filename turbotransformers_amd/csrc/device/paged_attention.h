@@ -144,7 +144,7 @@ __device__ __forceinline__ bool wild_value(T v) {
 // seldom scaled, and then by powers of two.  Probabilities of up to 2^8 lose nothing: they are as exact in their type as those up to 1, and the division by their sum takes the factor back out.  (The
 // decision is the row's own: what is in the tile with it moves no bit of it.)
 constexpr float kSlack = 8.f;
-__device__ __forceinline__ float moved_reference(float top, float highest) { return highest > top + kSlack || top == -INFINITY ? fmaxf(__builtin_ceilf(highest), top) : top; }
+__device__ __forceinline__ float moved_reference(float top, float highest) { return highest > top + kSlack || top == -INFINITY ? fmaxf(__builtin_floorf(highest), top) : top; }
 
 // What this lane gets of a 4 x 16 block of 16-bit values in LDS that lies row by row: four lanes point at the 32 bytes of a row, lane i of the sixteen gets column i.
 __device__ __forceinline__ u32x2 read_transposed(const void* p) {

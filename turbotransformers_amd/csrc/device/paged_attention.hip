@@ -81,6 +81,7 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
   TTMI_REQUIRE(q_pitch >= heads * d && out_pitch >= heads * d, "rows overlap: a pitch is too small");
   TTMI_REQUIRE(dtype == TTMI_F32 || dtype == TTMI_F16 || dtype == TTMI_BF16, "unsupported dtype");
   TTMI_REQUIRE(window >= 0 && max_tokens >= 0 && max_length >= 0, "window, max_tokens and max_length must not be negative");
+  TTMI_REQUIRE(batch->tokens * heads <= 1 << 30 && batch->batch * cache->kv_heads <= 1 << 30, "more rows or sequences than one launch takes");
   TTMI_REQUIRE(scale > 0.f && scale <= 3e38f, "scale must be positive and finite");
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   TTMI_REQUIRE(q != nullptr && out != nullptr, "q or out is null");

@@ -73,6 +73,7 @@ constexpr int kStart = 1;
 struct Walk {  // 64 sequences, a lane each
   int base, rounds;       // number of the first; rounds of this lane's, for one head
   int64_t before, upto;   // units of all sequences before these; of these up to this lane's, it included
+  int64_t groups;         // of batches of more than 64 sequences: units of this lane's 64th of them and of those before it
 };
 __device__ __forceinline__ int rounds_of(const PagedArgs& a, int b) {
   const Sequence seq = sequence(a, b);
@@ -86,35 +87,48 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane);
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
+__device__ __forceinline__ int64_t sum_up_to_lane(int64_t v) {
+  const int lane = (int)(threadIdx.x % kWave);
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int64_t below = __shfl_up((long long)v, d, kWave);
+    if (lane >= d) v += below;
+  }
+  return v;
+}
 __device__ __forceinline__ void walk_to(const PagedArgs& a, Walk& w, int base, int64_t before) {
   const int lane = (int)(threadIdx.x % kWave);
   w.base = base, w.before = before;
   w.rounds = base + lane < a.view.batch ? rounds_of(a, base + lane) : 0;
-  w.upto = (int64_t)w.rounds * a.view.kv_heads;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int64_t below = __shfl_up((long long)w.upto, d, kWave);
-    if (lane >= d) w.upto += below;
-  }
+  w.upto = sum_up_to_lane((int64_t)w.rounds * a.view.kv_heads);
 }
-// -> all units; w is at the first sequences
+__device__ __forceinline__ void walk_on(const PagedArgs& a, Walk& w) { walk_to(a, w, w.base + kWave, w.before + lane_of(w.upto, kWave - 1)); }
+__device__ __forceinline__ int group_size(const PagedArgs& a) { return (a.view.batch + kWave - 1) / kWave; }
+__device__ __forceinline__ void walk_to_group(const PagedArgs& a, Walk& w, int group) {
+  walk_to(a, w, group * group_size(a), group > 0 ? lane_of(w.groups, group - 1) : 0);
+}
+// -> all units
 __device__ __forceinline__ int64_t count_units(const PagedArgs& a, Walk& w) {
-  walk_to(a, w, 0, 0);
-  int64_t all = lane_of(w.upto, kWave - 1);
-  if (a.view.batch <= kWave) return all;
-  for (int base = kWave; base < a.view.batch; base += kWave) {
-    walk_to(a, w, base, all);
-    all += lane_of(w.upto, kWave - 1);
+  w.groups = 0;
+  if (a.view.batch <= kWave) {
+    walk_to(a, w, 0, 0);
+    return lane_of(w.upto, kWave - 1);
   }
-  walk_to(a, w, 0, 0);
-  return all;
+  const int size = group_size(a), first = (int)(threadIdx.x % kWave) * size;
+  int64_t mine = 0;
+#pragma unroll 4
+  for (int i = 0; i < size; ++i) mine += first + i < a.view.batch ? rounds_of(a, first + i) : 0;
+  w.groups = sum_up_to_lane(mine * a.view.kv_heads);
+  w.base = 0, w.rounds = 0, w.before = w.upto = 0;
+  return lane_of(w.groups, kWave - 1);
 }
 struct Place {
   int b, kv_head, round, rounds;  // round: of this head's `rounds`
 };
-// w is at or before the unit's sequences
 __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t unit) {
-  while (w.before + lane_of(w.upto, kWave - 1) <= unit) walk_to(a, w, w.base + kWave, w.before + lane_of(w.upto, kWave - 1));
+  if (a.view.batch > kWave && (unit < w.before || unit >= w.before + lane_of(w.upto, kWave - 1)))
+    walk_to_group(a, w, __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(w.groups > unit)) - 1));
+  while (w.before + lane_of(w.upto, kWave - 1) <= unit) walk_on(a, w);
   const int64_t at = unit - w.before;
   const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(w.upto > at)) - 1);
   Place p;
@@ -400,7 +414,8 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a) {
   if (rows > a.few || (int)blockIdx.y >= rows) return;
   Walk walk;
   const int64_t units = count_units(a, walk), workgroups = sharers(a, units);
-  while (walk.base + kWave <= b) walk_to(a, walk, walk.base + kWave, walk.before + lane_of(walk.upto, kWave - 1));
+  if (view.batch > kWave) walk_to_group(a, walk, b / group_size(a));
+  while (walk.base + kWave <= b) walk_on(a, walk);
   const int lane = b - walk.base, rounds = __builtin_amdgcn_readlane(walk.rounds, lane);
   const int64_t unit = walk.before + lane_of(walk.upto, lane) - (int64_t)rounds * (view.kv_heads - kv_head);
   const int64_t first = ((unit + kStart + 1) * workgroups - 1) / units, last = ((unit + rounds) * workgroups - 1) / units;
