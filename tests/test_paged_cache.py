@@ -158,7 +158,8 @@ def attend(ttmi, c, b, q=ADDRESS, q_pitch=256, out=2 * ADDRESS, out_pitch=256, h
 
 BAD_CACHE = [dict(page_size=0), dict(page_size=24), dict(page_size=8192), dict(head_dim=0), dict(head_dim=72), dict(head_dim=272), dict(kv_heads=0),
              dict(kv_heads=3), dict(pages=-1), dict(keys=None), dict(values=None), dict(keys=ADDRESS + 8), dict(values=ADDRESS + 2)]
-BAD_BATCH = [dict(table=None), dict(starts=None), dict(lengths=None), dict(batch=-1), dict(tokens=-1), dict(table_pitch=-1), dict(table_pitch=1 << 30)]
+BAD_BATCH = [dict(table=None), dict(starts=None), dict(lengths=None), dict(batch=-1), dict(tokens=-1), dict(table_pitch=-1), dict(table_pitch=1 << 30),
+             dict(table_pitch=(1 << 26) + 1), dict(tokens=1 << 23)]
 
 
 @pytest.fixture(scope="module")
@@ -197,6 +198,25 @@ def test_attention_refuses(lib):
     n = ctypes.c_int64(-7)
     assert lib.ttmi_paged_attention_workspace(ctypes.byref(cache(page_size=3)), ctypes.byref(batch()), 4, 0, 0, 0, capi.F16, ctypes.byref(n)) == -1
     assert lib.ttmi_paged_attention_workspace(ctypes.byref(cache()), ctypes.byref(batch()), 4, 0, 0, 0, capi.F16, None) == -1
+
+
+def test_launches_that_are_too_large_are_refused(lib):
+    """Before anything is started: more rows, or more sequences, than a launch has threads for."""
+    assert attend(lib, cache(kv_heads=1), batch(tokens=1 << 20), heads=1 << 10, q_pitch=1 << 16, out_pitch=1 << 16) == -1
+    assert attend(lib, cache(), batch(batch=1 << 22)) == -1
+    assert copy(lib, [0], [1], page_bytes=(1 << 36) + 16) == -1
+
+
+@pytest.mark.parametrize("dtype", [capi.F32, capi.F16])
+def test_workspace_does_not_grow_with_keys_that_a_window_hides(lib, dtype):
+    """What 300 tokens see of their last 500 keys, cut into parts: as much room with a table for 2^24 positions as with one for 2^12 (and some at all)."""
+    sizes = []
+    for pitch in (1 << 8, 1 << 20):
+        n = ctypes.c_int64(-7)
+        assert lib.ttmi_paged_attention_workspace(ctypes.byref(cache(pages=1 << 20)), ctypes.byref(batch(batch=1, tokens=300, table_pitch=pitch)), 4, 300, 0, 500,
+                                                  dtype, ctypes.byref(n)) == 0
+        sizes.append(n.value)
+    assert sizes[0] == sizes[1] and 0 < sizes[0] <= 300 * 4 * 66 * 4 * 20
 
 
 def copy(ttmi, sources, destinations, keys=ADDRESS, values=ADDRESS, layers=1, pages=8, page_bytes=64):

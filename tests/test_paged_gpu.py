@@ -161,6 +161,16 @@ def test_windows(dt, window, causal):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_windows_over_long_contexts_are_cut_and_joined(dt, causal):
+    """Few blocks of rows whose windows begin and end anywhere in the parts that their keys are cut into; more keys than was said; a window longer than some."""
+    for window, new, past in ((1000, [40], [5000]), (700, [130, 9, 20], [2999, 100, 4000]), (2000, [20], [1500])):
+        check(dt, new, past, 4, 2, 64, 16, causal=causal, window=window, spare_rows=1)
+    case = Case(dt, [90, 30], [3000, 17], 4, 2, 64, 16)
+    case.check_attention(case.run_attention(max_tokens=30, max_length=400, window=900, causal=causal), window=900, causal=causal)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 def test_all_keys_are_seen_without_causality(dt):
     check(dt, [1, 70, 3], [5, 30, 200], 4, 2, 64, 16, causal=False)
 
@@ -227,6 +237,43 @@ def test_rows_that_lie_apart(dt):
     got = tt.paged_attention(wide[:, 64:320], case.keys.cuda(), case.values.cuda(), *case.device_args(), out=result[:, 128:384])
     case.check_attention(got)
     assert (result[:, :128] == 7).all() and (result[:, 384:] == 7).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_what_is_not_finite_reaches_only_the_tokens_that_see_it(dt, bad):
+    """One value of a key of each of three sequences, one decoding, one with a few rows, one with many: rows whose windows and positions leave that key out
+    have what they would have without it, the others a NaN or an infinity in that column alone; and a query of it spoils its own rows only."""
+    new, past, window = [1, 5, 150], [300, 290, 200], 100
+    case = Case(dt, new, past, 4, 2, 64, 16)
+    clean = case.run_attention(window=window)
+    case.check_attention(clean, window=window)
+    hit = [[280, 0], [193, 260], [250, 149]]  # (seen by all or only by some of the new tokens, or behind the window)
+    kept = case.values.clone()
+    for which in range(2):
+        case.values.copy_(kept)
+        for b in range(3):
+            case.values[case.table[b, hit[b][which] // 16], 1, hit[b][which] % 16, 7] = bad
+        got = case.run_attention(window=window)
+        for b in range(3):
+            for i in range(new[b]):
+                row, position = int(case.starts[b]) + i, past[b] + i
+                sees = position - window < hit[b][which] <= position
+                spoiled = torch.zeros(4, 64, dtype=torch.bool)
+                spoiled[2:, 7] = sees
+                assert torch.equal(~torch.isfinite(got[row]).cpu(), spoiled), (which, b, i)
+                assert torch.equal(got[row].cpu()[~spoiled], clean[row].cpu()[~spoiled]), (which, b, i)
+    case.values.copy_(kept)
+    for row in (0, 3, 70):
+        case.q[row, 2, 5] = bad
+    got = case.run_attention(window=window)
+    for row in range(sum(new)):
+        spoiled = [row in (0, 3, 70) and h == 2 for h in range(4)]
+        for h in range(4):
+            if spoiled[h]:
+                assert torch.isnan(got[row, h]).all(), row
+            else:
+                assert torch.equal(got[row, h], clean[row, h]), (row, h)
 
 
 def test_result_does_not_depend_on_what_else_is_in_the_batch_or_runs_twice():
@@ -420,9 +467,25 @@ def test_python_refusals_with_device_tensors():
             attend(**bad)
     with pytest.raises(tt.cxx.EnforceNotMet, match="overlaps"):
         tt.paged_attention(q, k, v, table, starts, lengths, out=q)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(tt.cxx.EnforceNotMet, match="scale"):
+            tt.paged_attention(q, k, v, table, starts, lengths, scale=scale)
     qkv = torch.zeros(case.tokens, 8, 64, dtype=torch.float16, device="cuda")
     with pytest.raises(tt.cxx.EnforceNotMet, match="overlaps"):
         tt.rotary_append(qkv, k, v, table, starts, lengths, out=qkv[:, 1:5])
+    # memory that a kernel reads and another of its workgroups writes
+    inside = k.view(-1)[:q.numel()].view(q.shape)
+    for call in (lambda: tt.paged_attention(q, k, v, table, starts, lengths, out=inside), lambda: tt.rotary_append(qkv, k, v, table, starts, lengths, out=inside),
+                 lambda: tt.rotary_append(qkv, k, k, table, starts, lengths), lambda: tt.copy_pages(v, v, [0], [1]),
+                 lambda: tt.rotary_append(k.view(-1)[:qkv.numel()].view(qkv.shape), k, v, table, starts, lengths)):
+        with pytest.raises(tt.cxx.EnforceNotMet, match="overlap"):
+            call()
+    # tensors of another device than the current one
+    for call in (lambda: tt.cxx.paged_attention(q, k, v, table, starts, lengths, torch.empty_like(q), 0, 0, None, True, 0, None, 1, 0),
+                 lambda: tt.cxx.rotary_append(qkv, k, v, table, starts, lengths, None, False, 1.0, torch.empty_like(q), 1, 0),
+                 lambda: tt.cxx.copy_pages(k, v, [0], [1], 1, 0)):
+        with pytest.raises(tt.cxx.EnforceNotMet, match="the current device is 1"):
+            call()
     with pytest.raises(tt.cxx.EnforceNotMet):
         tt.rotary_append(qkv, k, v, table, starts, lengths, inv_freq=torch.ones(32, device="cuda"))
     with pytest.raises(tt.cxx.EnforceNotMet):

@@ -186,7 +186,7 @@ int ttmi_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t 
 int ttmi_copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t page_bytes, const int32_t* sources,
                     const int32_t* destinations, int64_t count, void* stream) {
   TTMI_REQUIRE(layers >= 0 && layers <= 32767 && pages >= 0 && pages <= INT32_MAX && count >= 0, "bad number of layers, pages or copies");
-  TTMI_REQUIRE(page_bytes >= 0 && page_bytes % 16 == 0 && page_bytes <= (1ll << 40), "page_bytes must be a multiple of 16");
+  TTMI_REQUIRE(page_bytes >= 0 && page_bytes % 16 == 0 && page_bytes <= (1ll << 36), "page_bytes must be a multiple of 16, at most 2^36");
   if (count == 0 || layers == 0 || page_bytes == 0) return 0;
   TTMI_REQUIRE(keys != nullptr && values != nullptr && sources != nullptr && destinations != nullptr, "keys, values, sources or destinations is null");
   TTMI_REQUIRE(((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15) == 0, "keys and values must be 16-byte aligned");

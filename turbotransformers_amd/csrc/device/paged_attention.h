@@ -21,8 +21,8 @@ struct PagedArgs {
   int every;  // this kernel takes all sequences: the other one is not launched
   // Of the few-rows kernel.  splits: how many workgroups share the work, 0: one for each sequence and key/value head; waves: of a workgroup; few: the rows of a sequence
   // that is its own (at most kFewRows).
-  // Of the other.  Keys are cut at multiples of `chunk` (a multiple of 64), counted from the first of the sequence, into at most `splits` parts (the grid); a sequence
-  // that has more keys than that takes longer parts.
+  // Of the other.  Keys are cut at multiples of `chunk` (a multiple of 64), counted from the first of the sequence, so that no row sees more than `splits` parts (the
+  // grid): a sequence that has more keys than was said takes longer ones.  Part p is in place p % splits.
   // ordered: its workgroups begin with those that have the most keys.
   int splits, waves, few, chunk, ordered;
   float* partial;  // sums of rows whose keys are several workgroups' [..][d], behind them the maxima and sums of their probabilities [..][2]
@@ -41,9 +41,11 @@ struct Sequence {
     if (r.begin >= r.end) r.begin = r.end = 0;
     return r;
   }
-  // keys of a part (tiles)
+  // keys of a part (tiles).  A window's keys begin anywhere in a part, and so touch one more than they fill.
   __device__ __forceinline__ int chunk(const PagedArgs& a) const {
-    return a.splits <= 1 ? INT32_MAX : max(a.chunk, ((length + a.splits - 1) / a.splits + 63) & ~63);
+    if (a.splits <= 1) return INT32_MAX;
+    const int seen = a.window > 0 ? min(length, a.window + tokens) : length, full = a.splits - (a.window > 0 ? 1 : 0);
+    return max(a.chunk, ((seen + full - 1) / full + 63) & ~63);
   }
 };
 __device__ __forceinline__ Sequence sequence(const PagedArgs& a, int b) {
@@ -131,14 +133,25 @@ __device__ __forceinline__ u32x4 finite_part(u32x4 x) {
   return x;
 }
 
-// (Both kernels are compiled as if there were no NaNs, which saves a canonicalising instruction for every operand of a maximum: what has to tell them asks for their bits.)
+// Both kernels are compiled as if there were no NaNs, which saves a canonicalising instruction for every operand of a maximum.  So what has to tell them asks for the bits of
+// a number that was loaded as bits, and what adds one does it where the compiler does not look: it takes a test of a float for a test of infinity alone.
 template <typename T>
-__device__ __forceinline__ bool wild_value(T v) {
-  if constexpr (sizeof(T) == 4) return (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) == 0x7f800000u;
-  else {
-    constexpr uint16_t kExp = std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
-    return (__builtin_bit_cast(uint16_t, v) & kExp) == kExp;
+using Bits = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+// sum += *at where that is an infinity or a NaN
+template <typename T>
+__device__ __forceinline__ void add_wild(float& sum, const T* at) {
+  typedef Bits<T> __attribute__((may_alias)) Loaded;
+  constexpr uint32_t kExp = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
+  const uint32_t x = *reinterpret_cast<const Loaded*>(at);
+  if ((x & kExp) != kExp) return;
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (std::is_same<T, f16>::value) {
+    float wide;
+    asm volatile("v_cvt_f32_f16 %1, %2\n\tv_add_f32 %0, %0, %1" : "+v"(sum), "=&v"(wide) : "v"(x));
+  } else {
+    asm volatile("v_add_f32 %0, %0, %1" : "+v"(sum) : "v"(sizeof(T) == 4 ? x : x << 16));
   }
+#endif
 }
 // The reference point of a row's probabilities, in units of scale log2(e) score, a whole number: it moves only where a score lies more than this above it, so the sums are
 // seldom scaled, and then by powers of two.  Probabilities of up to 2^8 lose nothing: they are as exact in their type as those up to 1, and the division by their sum takes the factor back out.  (The

@@ -15,12 +15,12 @@ struct PagedPlan {
   int64_t few_floats, tile_floats;  // of the workspace
 };
 
-void cut(int64_t units, int64_t wanted, int64_t least, int64_t reach, int64_t longest, int* chunk, int* splits) {
+// `reach` keys into parts of at least `least`, so that `units` times their number are `wanted` at most.
+void cut(int64_t units, int64_t wanted, int64_t least, int64_t reach, bool window, int* chunk, int* splits) {
   const int64_t parts = std::min(std::max<int64_t>(1, wanted / std::max<int64_t>(1, units)), std::max<int64_t>(1, ceil_div(reach, least)));
-  int64_t size = ceil_div(ceil_div(reach, parts), 64) * 64;
-  size = std::max(size, ceil_div(ceil_div(longest, 4096), 64) * 64);  // (at most 4096 parts)
-  *splits = parts > 1 ? (int)std::max<int64_t>(1, ceil_div(longest, size)) : 1;
-  *chunk = (int)std::min<int64_t>(size, INT32_MAX - 64);
+  const int64_t size = ceil_div(ceil_div(reach, parts), 64) * 64;
+  *splits = parts > 1 ? (int)(ceil_div(reach, size) + (window ? 1 : 0)) : 1;
+  *chunk = (int)size;
 }
 
 // Few rows: up to so many bytes of keys and values of one sequence and head are one workgroup's.  A CU fetches about 50 GB/s, so these take 6 us, what sharing them out
@@ -44,7 +44,7 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   p.few_waves = p.few_splits == 0 && batch * view.kv_heads < compute_units() ? 8 : 4;
   // Many rows: cut where two workgroups a CU are not reached, into parts of at least as many keys as take longer than their joining (fp32, whose matrix instructions take
   // sixteen times as long: us for one prompt of 200 tokens, 12 heads of 64, parts of 256 / 64 at least 22.0 / 15.7; 16-bit types 9.8 / 11.7).
-  cut(view.kv_heads * (tokens * group / 128 + std::min(batch, tokens)), 512, dtype == TTMI_F32 ? 64 : 256, reach, longest, &p.tile_chunk, &p.tile_splits);
+  cut(view.kv_heads * (tokens * group / 128 + std::min(batch, tokens)), 512, dtype == TTMI_F32 ? 64 : 256, reach, window > 0, &p.tile_chunk, &p.tile_splits);
   const int64_t d = view.head_dim;
   p.few_floats = p.few ? 2ll * p.few_splits * kFewRows * (d + 2) : 0;
   p.tile_floats = p.tiles && p.tile_splits > 1 ? tokens * heads * p.tile_splits * (d + 2) : 0;
@@ -81,7 +81,8 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
   TTMI_REQUIRE(q_pitch >= heads * d && out_pitch >= heads * d, "rows overlap: a pitch is too small");
   TTMI_REQUIRE(dtype == TTMI_F32 || dtype == TTMI_F16 || dtype == TTMI_BF16, "unsupported dtype");
   TTMI_REQUIRE(window >= 0 && max_tokens >= 0 && max_length >= 0, "window, max_tokens and max_length must not be negative");
-  TTMI_REQUIRE(batch->tokens * heads <= 1 << 30 && batch->batch * cache->kv_heads <= 1 << 30, "more rows or sequences than one launch takes");
+  // (a launch has less than 2^32 threads: 512 of them for a sequence and key/value head, or 256 for 128 rows besides)
+  TTMI_REQUIRE(batch->tokens * heads < 1 << 30 && batch->batch * cache->kv_heads < 1 << 23, "more rows or sequences than one launch takes");
   TTMI_REQUIRE(scale > 0.f && scale <= 3e38f, "scale must be positive and finite");
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   TTMI_REQUIRE(q != nullptr && out != nullptr, "q or out is null");

@@ -163,242 +163,243 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
     unit = units * blockIdx.x / workgroups, stop = units * (blockIdx.x + 1) / workgroups;
   }
   while (unit < stop) {
-  Place place;
-  if (a.splits > 0) place = find_unit(a, walk, unit);
-  else place.b = (int)(unit / view.kv_heads), place.kv_head = (int)(unit % view.kv_heads), place.round = 0, place.rounds = INT32_MAX;
-  const int b = place.b, kv_head = place.kv_head;
-  const int64_t ends = a.splits > 0 ? min(stop, unit + place.rounds - place.round) : stop;
-  const int start = a.splits > 0 ? kStart : 0;  // (in a pair's first unit there is nothing to do)
-  const int round0 = max(0, place.round - start), round1 = place.round + (int)(a.splits > 0 ? ends - unit : INT32_MAX) - start;
-  const bool complete = round0 == 0 && round1 == place.rounds - start;
-  unit = ends;
-  if (round1 <= round0) continue;
-  const Sequence seq = sequence(a, b);
-  const int rows_all = seq.tokens * a.group;
-  if (rows_all <= 0 || (rows_all > a.few && !a.every)) return;  // (a workgroup of its own)
-  if (round0 == 0 && kv_head == 0 && tid == 0 && view.lengths[b] > seq.length) page_error(view);
-  PageCursor cursor;
-  cursor.table = view.table + (int64_t)b * view.table_pitch;
-  cursor.first = 0, cursor.ahead = 0, cursor.at = 0;
+    Place place;
+    if (a.splits > 0) place = find_unit(a, walk, unit);
+    else place.b = (int)(unit / view.kv_heads), place.kv_head = (int)(unit % view.kv_heads), place.round = 0, place.rounds = INT32_MAX;
+    const int b = place.b, kv_head = place.kv_head;
+    const int64_t ends = a.splits > 0 ? min(stop, unit + place.rounds - place.round) : stop;
+    const int start = a.splits > 0 ? kStart : 0;  // (in a pair's first unit there is nothing to do)
+    const int round0 = max(0, place.round - start), round1 = place.round + (int)(a.splits > 0 ? ends - unit : INT32_MAX) - start;
+    const bool complete = round0 == 0 && round1 == place.rounds - start;
+    unit = ends;
+    if (round1 <= round0) continue;
+    const Sequence seq = sequence(a, b);
+    const int rows_all = seq.tokens * a.group;
+    if (rows_all <= 0 || (rows_all > a.few && !a.every)) return;  // (a workgroup of its own)
+    if (round0 == 0 && kv_head == 0 && tid == 0 && view.lengths[b] > seq.length) page_error(view);
+    PageCursor cursor;
+    cursor.table = view.table + (int64_t)b * view.table_pitch;
+    cursor.first = 0, cursor.ahead = 0, cursor.at = 0;
 
-  for (int row0 = 0; row0 < rows_all; row0 += kFewRows) {
-    const int rows = min(kFewRows, rows_all - row0);
-    const int token0 = row0 / a.group, token1 = (row0 + rows - 1) / a.group;
-    const int token = row < rows ? (row0 + row) / a.group : token0, head = kv_head * a.group + (row < rows ? row0 + row - token * a.group : 0);
-    const Reach mine = seq.reach(a, token), low = seq.reach(a, token0), high = seq.reach(a, token1);
-    // Keys that some row sees, and those that all rows see: both ends rise with the position.  (A row without keys, before the first one, begins and ends at 0.)
-    const int first = low.begin, end = max(low.end, high.end), sure_first = high.begin, sure_end = low.end;
-    int lo = first & ~(S::kKeys - 1), hi = end;
-    if (!complete) {
-      lo = max(lo, (first / kRound + round0) * kRound);
-      hi = min(hi, (first / kRound + round1) * kRound);
-    }
-    cursor.last = max(0, (end - 1) >> view.page_shift);
-
-    u32x4 qf[S::kSteps];
-#pragma unroll
-    for (int i = 0; i < S::kSteps; ++i) {
-      qf[i] = u32x4{0u, 0u, 0u, 0u};
-      if (row < rows) qf[i] = *reinterpret_cast<const u32x4*>(q + (seq.start + token) * a.q_pitch + (int64_t)head * D + (quarter + 4 * i) * S::kElems);
-    }
-    floatx4 ot[S::kTiles];
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t) ot[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-    float top = -INFINITY, sum = 0.f;  // of scale * log2(e) * score; the sum is this quarter's share
-
-    u32x4 kf[S::kGroups][S::kSteps], vf[S::kGroups][S::kValuePieces];
-    auto load_keys = [&](int key) __attribute__((always_inline)) {
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g) {
-        const T* p;
-        if constexpr (!SMALL) p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(keys) + group_at<S::kRowBytes>(view, cursor, key + 16 * g)) + row * D;
-        else p = keys + row_offset<D>(view, cursor, kv_head, key + 16 * g + row);
-#pragma unroll
-        for (int i = 0; i < S::kSteps; ++i) kf[g][i] = *reinterpret_cast<const u32x4*>(p + (quarter + 4 * i) * S::kElems);
+    for (int row0 = 0; row0 < rows_all; row0 += kFewRows) {
+      const int rows = min(kFewRows, rows_all - row0);
+      const int token0 = row0 / a.group, token1 = (row0 + rows - 1) / a.group;
+      const int token = row < rows ? (row0 + row) / a.group : token0, head = kv_head * a.group + (row < rows ? row0 + row - token * a.group : 0);
+      const Reach mine = seq.reach(a, token), low = seq.reach(a, token0), high = seq.reach(a, token1);
+      // Keys that some row sees, and those that all rows see: both ends rise with the position.  (A row without keys, before the first one, begins and ends at 0.)
+      const int first = low.begin, end = max(low.end, high.end), sure_first = high.begin, sure_end = low.end;
+      int lo = first & ~(S::kKeys - 1), hi = end;
+      if (!complete) {
+        lo = max(lo, (first / kRound + round0) * kRound);
+        hi = min(hi, (first / kRound + round1) * kRound);
       }
-    };
-    auto load_values = [&](int key) __attribute__((always_inline)) {  // before the keys of the tile
-      if constexpr (!SMALL) come_to<S::kRowBytes>(view, cursor, kv_head, key);
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g) {
-        if constexpr (!SMALL) {
-          const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(values) + group_at<S::kRowBytes>(view, cursor, key + 16 * g)) + lane * S::kElems;
-#pragma unroll
-          for (int i = 0; i < S::kValuePieces; ++i) vf[g][i] = *reinterpret_cast<const u32x4*>(p + i * 64 * S::kElems);
-        } else {
-#pragma unroll
-          for (int i = 0; i < S::kValuePieces; ++i) {
-            const int at = i * 1024 + lane * 16, r = at / S::kRowBytes;
-            vf[g][i] = *reinterpret_cast<const u32x4*>(values + row_offset<D>(view, cursor, kv_head, key + 16 * g + r) + at % S::kRowBytes / (int)sizeof(T));
+      cursor.last = max(0, (end - 1) >> view.page_shift);
+
+      u32x4 qf[S::kSteps];
+  #pragma unroll
+      for (int i = 0; i < S::kSteps; ++i) {
+        qf[i] = u32x4{0u, 0u, 0u, 0u};
+        if (row < rows) qf[i] = *reinterpret_cast<const u32x4*>(q + (seq.start + token) * a.q_pitch + (int64_t)head * D + (quarter + 4 * i) * S::kElems);
+      }
+      floatx4 ot[S::kTiles];
+  #pragma unroll
+      for (int t = 0; t < S::kTiles; ++t) ot[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+      float top = -INFINITY, sum = 0.f;  // of scale * log2(e) * score; the sum is this quarter's share
+
+      u32x4 kf[S::kGroups][S::kSteps], vf[S::kGroups][S::kValuePieces];
+      auto load_keys = [&](int key) __attribute__((always_inline)) {
+  #pragma unroll
+        for (int g = 0; g < S::kGroups; ++g) {
+          const T* p;
+          if constexpr (!SMALL) p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(keys) + group_at<S::kRowBytes>(view, cursor, key + 16 * g)) + row * D;
+          else p = keys + row_offset<D>(view, cursor, kv_head, key + 16 * g + row);
+  #pragma unroll
+          for (int i = 0; i < S::kSteps; ++i) kf[g][i] = *reinterpret_cast<const u32x4*>(p + (quarter + 4 * i) * S::kElems);
+        }
+      };
+      auto load_values = [&](int key) __attribute__((always_inline)) {  // before the keys of the tile
+        if constexpr (!SMALL) come_to<S::kRowBytes>(view, cursor, kv_head, key);
+  #pragma unroll
+        for (int g = 0; g < S::kGroups; ++g) {
+          if constexpr (!SMALL) {
+            const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(values) + group_at<S::kRowBytes>(view, cursor, key + 16 * g)) + lane * S::kElems;
+  #pragma unroll
+            for (int i = 0; i < S::kValuePieces; ++i) vf[g][i] = *reinterpret_cast<const u32x4*>(p + i * 64 * S::kElems);
+          } else {
+  #pragma unroll
+            for (int i = 0; i < S::kValuePieces; ++i) {
+              const int at = i * 1024 + lane * 16, r = at / S::kRowBytes;
+              vf[g][i] = *reinterpret_cast<const u32x4*>(values + row_offset<D>(view, cursor, kv_head, key + 16 * g + r) + at % S::kRowBytes / (int)sizeof(T));
+            }
           }
         }
-      }
-    };
+      };
 
-    constexpr int kStep = NW * S::kKeys;
-    // One tile.  Whether another follows is known to the compiler: a load that may or may not have been sent would make it wait for all of them.
-    auto work_on = [&](int key, auto more) __attribute__((always_inline)) {
-      const bool masked = key < sure_first || key + S::kKeys > sure_end || key + S::kKeys > hi;
-      uint32_t wild = 0;
-      if (masked) {  // keys that no row sees may hold anything: their values count as zeros, and one that only some rows see must not reach the others
-#pragma unroll
+      constexpr int kStep = NW * S::kKeys;
+      // One tile.  Whether another follows is known to the compiler: a load that may or may not have been sent would make it wait for all of them.
+      auto work_on = [&](int key, auto more) __attribute__((always_inline)) {
+        const bool masked = key < sure_first || key + S::kKeys > sure_end || key + S::kKeys > hi;
+        uint32_t wild = 0;
+        if (masked) {  // keys that no row sees may hold anything: their values count as zeros, and one that only some rows see must not reach the others
+  #pragma unroll
+          for (int g = 0; g < S::kGroups; ++g)
+  #pragma unroll
+            for (int i = 0; i < S::kValuePieces; ++i) {
+              const int k = key + 16 * g + (i * 1024 + lane * 16) / S::kRowBytes;
+              if (k < first || k >= end) vf[g][i] = u32x4{0u, 0u, 0u, 0u};
+              wild |= not_finite<T>(vf[g][i]);
+            }
+          wild = __any(wild != 0);
+        }
+  #pragma unroll
         for (int g = 0; g < S::kGroups; ++g)
-#pragma unroll
+  #pragma unroll
           for (int i = 0; i < S::kValuePieces; ++i) {
-            const int k = key + 16 * g + (i * 1024 + lane * 16) / S::kRowBytes;
-            if (k < first || k >= end) vf[g][i] = u32x4{0u, 0u, 0u, 0u};
-            wild |= not_finite<T>(vf[g][i]);
+            const int at = i * 1024 + lane * 16, r = 16 * g + at / S::kRowBytes;
+            *reinterpret_cast<u32x4*>(tile + r * S::kRowBytes + value_piece<T, D>(r, at % S::kRowBytes / 16) * 16) = wild ? finite_part<T>(vf[g][i]) : vf[g][i];
           }
-        wild = __any(wild != 0);
-      }
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g)
-#pragma unroll
-        for (int i = 0; i < S::kValuePieces; ++i) {
-          const int at = i * 1024 + lane * 16, r = 16 * g + at / S::kRowBytes;
-          *reinterpret_cast<u32x4*>(tile + r * S::kRowBytes + value_piece<T, D>(r, at % S::kRowBytes / 16) * 16) = wild ? finite_part<T>(vf[g][i]) : vf[g][i];
-        }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the tile is this wavefront's alone: its LDS accesses are in order)
-      if constexpr (decltype(more)::value) load_values(key + kStep);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the tile is this wavefront's alone: its LDS accesses are in order)
+        if constexpr (decltype(more)::value) load_values(key + kStep);
 
-      floatx4 st[S::kGroups];
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g) {
-        st[g] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < S::kSteps; ++i) st[g] = mma16<T>(kf[g][i], qf[i], st[g]);
-      }
-      if constexpr (decltype(more)::value) load_keys(key + kStep);
-      if (masked) {
-#pragma unroll
-        for (int g = 0; g < S::kGroups; ++g)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = key + 16 * g + 4 * quarter + e;
-            if (k < mine.begin || k >= mine.end || k >= hi) st[g][e] = -INFINITY;
-          }
-      }
-      float m = st[0][0];
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, st[g][e]);
-      const float moved = moved_reference(top, quarters_max(m) * a.scale_log2e);
-      const float zero = moved == -INFINITY ? 0.f : moved;  // (a row that has seen no key yet)
-      const float shrink = __builtin_amdgcn_exp2f(top - zero);
-      top = moved;
-      u32x4 pf{};
-      float share = 0.f;
-      float p[S::kGroups][4];
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[g][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[g][e], a.scale_log2e, -zero));
-      if constexpr (sizeof(T) == 2) {
-        // rounded to the type for the second product; the sum is that of the rounded ones, so what rounding does to all of them alike cancels
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          pf[w] = pack2<T>(p[w >> 1][2 * (w & 1)], p[w >> 1][2 * (w & 1) + 1]);
-          share = add_pair<T>(pf[w], share);
+        floatx4 st[S::kGroups];
+  #pragma unroll
+        for (int g = 0; g < S::kGroups; ++g) {
+          st[g] = floatx4{0.f, 0.f, 0.f, 0.f};
+  #pragma unroll
+          for (int i = 0; i < S::kSteps; ++i) st[g] = mma16<T>(kf[g][i], qf[i], st[g]);
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) share += p[0][e];
-      }
-      sum = sum * shrink + share;
-      if (__any(shrink != 1.f)) {
-#pragma unroll
-        for (int t = 0; t < S::kTiles; ++t) ot[t] *= shrink;
-      }
-#pragma unroll
-      for (int t = 0; t < S::kTiles; ++t) {
-        if constexpr (sizeof(T) == 2) {
-          u32x4 v;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const int r = 16 * g + 4 * quarter + (row >> 2);
-            const u32x2 half = read_transposed(tile + r * S::kRowBytes + value_piece<T, D>(r, 2 * t + ((row >> 1) & 1)) * 16 + (row & 1) * 8);
-            v[2 * g] = half[0], v[2 * g + 1] = half[1];
-          }
-          ot[t] = mma16<T>(v, pf, ot[t]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * quarter + e;
-            const float v = *reinterpret_cast<const float*>(tile + r * S::kRowBytes + value_piece<T, D>(r, 4 * t + (row >> 2)) * 16 + (row & 3) * 4);
-            ot[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[0][e], ot[t], 0, 0, 0);
-          }
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if (wild) {  // an infinity or a NaN is what a sum with it is, whatever its weight
-#pragma unroll 1
-        for (int k = key; k < min(key + S::kKeys, hi); ++k) {
-          const T* v = values + row_offset<D>(view, cursor, kv_head, k) + 4 * quarter;
-          const bool seen = k >= mine.begin && k < mine.end;
-#pragma unroll
-          for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
+        if constexpr (decltype(more)::value) load_keys(key + kStep);
+        if (masked) {
+  #pragma unroll
+          for (int g = 0; g < S::kGroups; ++g)
+  #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const T x = v[16 * t + e];
-              if (seen && wild_value(x)) ot[t][e] += to_float(x);
+              const int k = key + 16 * g + 4 * quarter + e;
+              if (k < mine.begin || k >= mine.end || k >= hi) st[g][e] = -INFINITY;
             }
         }
-      }
-    };
-    int key = lo + wave * S::kKeys;
-    if (key < hi) {
-      if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, key);
-      load_values(key);
-      load_keys(key);
-      for (; key + kStep < hi; key += kStep) work_on(key, std::true_type{});
-      work_on(key, std::false_type{});
-    }
-
-    // the wavefronts meet
-    sum = quarters_sum(sum);
-    __syncthreads();
-    float* const stage = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t)
-      *reinterpret_cast<floatx4*>(stage + (wave * kFewRows + row) * S::kPitch + 16 * t + 4 * quarter) = ot[t];
-    if (quarter == 0) met[wave][row][0] = top, met[wave][row][1] = sum;
-    __syncthreads();
-    {
-      constexpr int kThreads = NW * 4, kWide = D / kThreads;  // of a row; columns of a thread
-      const int r = tid / kThreads, d0 = tid % kThreads * kWide;
-      if (r < rows) {
-        float best = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) best = fmaxf(best, met[w][r][0]);
-        const float zero = best == -INFINITY ? 0.f : best;
-        float total = 0.f, o[kWide] = {};
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const float weight = __builtin_amdgcn_exp2f(met[w][r][0] - zero);
-          total += met[w][r][1] * weight;
-#pragma unroll
-          for (int c = 0; c < kWide; ++c) o[c] += stage[(w * kFewRows + r) * S::kPitch + d0 + c] * weight;
-        }
-        if (complete) {
-          const int t = (row0 + r) / a.group, h = kv_head * a.group + row0 + r - t * a.group;
-          const float inv = total != 0.f ? 1.0f / total : 0.f;
-          T* to = static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D + d0;
-          Vec<T, kWide> x;
-#pragma unroll
-          for (int c = 0; c < kWide; ++c) x.v[c] = from_float<T>(o[c] * inv);
-          store_vec<T, kWide>(to, x);
+        float m = st[0][0];
+  #pragma unroll
+        for (int g = 0; g < S::kGroups; ++g)
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) m = fmaxf(m, st[g][e]);
+        const float moved = moved_reference(top, quarters_max(m) * a.scale_log2e);
+        const float zero = moved == -INFINITY ? 0.f : moved;  // (a row that has seen no key yet)
+        const float shrink = __builtin_amdgcn_exp2f(top - zero);
+        top = moved;
+        u32x4 pf{};
+        float share = 0.f;
+        float p[S::kGroups][4];
+  #pragma unroll
+        for (int g = 0; g < S::kGroups; ++g)
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) p[g][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[g][e], a.scale_log2e, -zero));
+        if constexpr (sizeof(T) == 2) {
+          // rounded to the type for the second product; the sum is that of the rounded ones, so what rounding does to all of them alike cancels
+  #pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            pf[w] = pack2<T>(p[w >> 1][2 * (w & 1)], p[w >> 1][2 * (w & 1) + 1]);
+            share = add_pair<T>(pf[w], share);
+          }
         } else {
-          const int64_t at = (2 * (int64_t)blockIdx.x + (round0 == 0 ? 1 : 0)) * kFewRows + r;
-          float* const ml = a.partial + 2 * (int64_t)a.splits * kFewRows * D + at * 2;
-#pragma unroll
-          for (int c = 0; c < kWide; ++c) a.partial[at * D + d0 + c] = o[c];
-          if (d0 == 0) ml[0] = best, ml[1] = total;
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) share += p[0][e];
+        }
+        sum = sum * shrink + share;
+        if (__any(shrink != 1.f)) {
+  #pragma unroll
+          for (int t = 0; t < S::kTiles; ++t) ot[t] *= shrink;
+        }
+  #pragma unroll
+        for (int t = 0; t < S::kTiles; ++t) {
+          if constexpr (sizeof(T) == 2) {
+            u32x4 v;
+  #pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int r = 16 * g + 4 * quarter + (row >> 2);
+              const u32x2 half = read_transposed(tile + r * S::kRowBytes + value_piece<T, D>(r, 2 * t + ((row >> 1) & 1)) * 16 + (row & 1) * 8);
+              v[2 * g] = half[0], v[2 * g + 1] = half[1];
+            }
+            ot[t] = mma16<T>(v, pf, ot[t]);
+          } else {
+  #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = 4 * quarter + e;
+              const float v = *reinterpret_cast<const float*>(tile + r * S::kRowBytes + value_piece<T, D>(r, 4 * t + (row >> 2)) * 16 + (row & 3) * 4);
+              ot[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[0][e], ot[t], 0, 0, 0);
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (wild) {  // an infinity or a NaN is what a sum with it is, whatever its weight
+  #pragma unroll 1
+          for (int k = key; k < min(key + S::kKeys, hi); ++k) {
+            const T* v = values + row_offset<D>(view, cursor, kv_head, k) + 4 * quarter;
+            const bool seen = k >= mine.begin && k < mine.end;
+  #pragma unroll
+            for (int t = 0; t < S::kTiles; ++t)
+  #pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float sum_e = ot[t][e];
+                if (seen) add_wild(sum_e, v + 16 * t + e);
+                ot[t][e] = sum_e;
+              }
+          }
+        }
+      };
+      int key = lo + wave * S::kKeys;
+      if (key < hi) {
+        if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, key);
+        load_values(key);
+        load_keys(key);
+        for (; key + kStep < hi; key += kStep) work_on(key, std::true_type{});
+        work_on(key, std::false_type{});
+      }
+
+      // the wavefronts meet
+      sum = quarters_sum(sum);
+      __syncthreads();
+      float* const stage = reinterpret_cast<float*>(smem);
+  #pragma unroll
+      for (int t = 0; t < S::kTiles; ++t)
+        *reinterpret_cast<floatx4*>(stage + (wave * kFewRows + row) * S::kPitch + 16 * t + 4 * quarter) = ot[t];
+      if (quarter == 0) met[wave][row][0] = top, met[wave][row][1] = sum;
+      __syncthreads();
+      {
+        constexpr int kThreads = NW * 4, kWide = D / kThreads;  // of a row; columns of a thread
+        const int r = tid / kThreads, d0 = tid % kThreads * kWide;
+        if (r < rows) {
+          float best = -INFINITY;
+  #pragma unroll
+          for (int w = 0; w < NW; ++w) best = fmaxf(best, met[w][r][0]);
+          const float zero = best == -INFINITY ? 0.f : best;
+          float total = 0.f, o[kWide] = {};
+  #pragma unroll
+          for (int w = 0; w < NW; ++w) {
+            const float weight = __builtin_amdgcn_exp2f(met[w][r][0] - zero);
+            total += met[w][r][1] * weight;
+  #pragma unroll
+            for (int c = 0; c < kWide; ++c) o[c] += stage[(w * kFewRows + r) * S::kPitch + d0 + c] * weight;
+          }
+          if (complete) {
+            const int t = (row0 + r) / a.group, h = kv_head * a.group + row0 + r - t * a.group;
+            const float inv = total != 0.f ? 1.0f / total : 0.f;
+            T* to = static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D + d0;
+            Vec<T, kWide> x;
+  #pragma unroll
+            for (int c = 0; c < kWide; ++c) x.v[c] = from_float<T>(o[c] * inv);
+            store_vec<T, kWide>(to, x);
+          } else {
+            const int64_t at = (2 * (int64_t)blockIdx.x + (round0 == 0 ? 1 : 0)) * kFewRows + r;
+            float* const ml = a.partial + 2 * (int64_t)a.splits * kFewRows * D + at * 2;
+  #pragma unroll
+            for (int c = 0; c < kWide; ++c) a.partial[at * D + d0 + c] = o[c];
+            if (d0 == 0) ml[0] = best, ml[1] = total;
+          }
         }
       }
+      if (row0 + kFewRows < rows_all || unit < stop) __syncthreads();
     }
-    if (row0 + kFewRows < rows_all || unit < stop) __syncthreads();
-  }
   }
 }
 

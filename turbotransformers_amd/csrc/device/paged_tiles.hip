@@ -59,7 +59,7 @@ __device__ __forceinline__ void store_rows(const PagedArgs& a, const Sequence& s
       }
     return;
   }
-  const int64_t at = (at_token * a.heads + head) * a.splits + part;
+  const int64_t at = (at_token * a.heads + head) * a.splits + part % a.splits;
   float* to = a.partial + at * D + 4 * lhalf;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
@@ -94,11 +94,13 @@ __device__ __forceinline__ bool find_block(const PagedArgs& a, int want, int* b,
         if (lane >= d) upto += below;
       }
       before = upto - blocks, all = __builtin_amdgcn_readlane(upto, kWave - 1);
-    } else for (uint64_t others = __ballot(blocks > 0); others != 0; others &= others - 1) {
-      const int j = __ffsll((unsigned long long)others) - 1;
-      const int their_blocks = __builtin_amdgcn_readlane(blocks, j), their_reach = __builtin_amdgcn_readlane(reach, j);
-      all += their_blocks;
-      if (their_reach > reach || (their_reach == reach && j < lane)) before += their_blocks;
+    } else {
+      for (uint64_t others = __ballot(blocks > 0); others != 0; others &= others - 1) {
+        const int j = __ffsll((unsigned long long)others) - 1;
+        const int their_blocks = __builtin_amdgcn_readlane(blocks, j), their_reach = __builtin_amdgcn_readlane(reach, j);
+        all += their_blocks;
+        if (their_reach > reach || (their_reach == reach && j < lane)) before += their_blocks;
+      }
     }
     if (want < all) {
       const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(want >= before && want < before + blocks)) - 1);
@@ -118,13 +120,13 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   __shared__ __align__(16) char smem[4 * S::kBytes];
   __shared__ int wild;  // whether values that only some rows see hold infinities or NaNs
   const PagedView& view = a.view;
-  const int kv_head = blockIdx.x % view.kv_heads, part = blockIdx.z;
+  const int kv_head = blockIdx.x % view.kv_heads;
   int b, block;
   if (!find_block(a, blockIdx.x / view.kv_heads, &b, &block)) return;
   const Sequence seq = sequence(a, b);
   const int chunk = seq.chunk(a);
   const int row0 = block * kTileRows, rows = min(kTileRows, seq.tokens * a.group - row0);
-  if (part == 0 && kv_head == 0 && block == 0 && threadIdx.x == 0 && view.lengths[b] > seq.length) page_error(view);
+  if (blockIdx.z == 0 && kv_head == 0 && block == 0 && threadIdx.x == 0 && view.lengths[b] > seq.length) page_error(view);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lrow = lane & 31, lhalf = lane >> 5;
   const T* const keys = static_cast<const T*>(a.keys);
@@ -132,8 +134,9 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   // keys that some row of the workgroup sees, and those that all see (both ends rise with the position); the same of this wavefront
   const Reach low = seq.reach(a, row0 / a.group), high = seq.reach(a, (row0 + rows - 1) / a.group);
   const int first = low.begin, end = max(low.end, high.end), sure_first = high.begin, sure_end = low.end;
+  const int part0 = first / chunk, part = part0 + (int)blockIdx.z;
   const int lo = (int)max(part * (int64_t)chunk, (int64_t)(first & ~(S::kKeys - 1))), hi = (int)min((part + 1) * (int64_t)chunk, (int64_t)end);
-  if (lo >= hi && part != 0) return;
+  if (lo >= hi && part != part0) return;
   const int wave_rows = max(0, min(32, rows - wave * 32));
   const int wrow = row0 + wave * 32;
   const Reach wave_low = seq.reach(a, wrow / a.group), wave_high = seq.reach(a, (wrow + max(wave_rows, 1) - 1) / a.group);
@@ -321,7 +324,7 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
-static_assert(sizeof(T) == 2 || S::kSubs == 1, "32 keys");
+        static_assert(sizeof(T) == 2 || S::kSubs == 1, "32 keys");
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           st[0][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][e], a.scale_log2e, -zero));
@@ -352,8 +355,9 @@ static_assert(sizeof(T) == 2 || S::kSubs == 1, "32 keys");
           for (int t = 0; t < S::kOut; ++t) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const T x = v[32 * t + 8 * (e / 4) + e % 4];
-              if (seen && wild_value(x)) ot[t][e] += to_float(x);
+              float sum_e = ot[t][e];
+              if (seen) add_wild(sum_e, v + 32 * t + 8 * (e / 4) + e % 4);
+              ot[t][e] = sum_e;
             }
             __builtin_amdgcn_sched_barrier(0);  // (few registers: this path is cold)
           }
@@ -372,7 +376,8 @@ static_assert(sizeof(T) == 2 || S::kSubs == 1, "32 keys");
     sum = both.a + both.b;
   }
   if (!live) return;
-  store_rows<T, D>(a, seq, token, head, part, mine.begin / chunk, mine.end > 0 ? (mine.end - 1) / chunk : 0, lhalf, ot, top, sum);
+  const bool sees = mine.end > 0;
+  store_rows<T, D>(a, seq, token, head, part, sees ? mine.begin / chunk : part0, sees ? (mine.end - 1) / chunk : part0, lhalf, ot, top, sum);
 }
 
 // Rows whose keys lay in several parts: a wavefront per row and head.
@@ -386,9 +391,9 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(const PagedArgs a) {
   const Reach reach = seq.reach(a, row - seq.start);
   const int chunk = seq.chunk(a), part0 = reach.begin / chunk, part1 = reach.end > 0 ? (reach.end - 1) / chunk : 0;
   if (part0 == part1) return;
-  const int64_t at = ((int64_t)row * a.heads + h) * a.splits + part0;
+  const int64_t at = ((int64_t)row * a.heads + h) * a.splits;
   join_parts_by_wavefront<T, D>(
-      a.partial, a.partial + (int64_t)view.tokens * a.heads * a.splits * D, part1 - part0 + 1, [&](int p) { return at + p; },
+      a.partial, a.partial + (int64_t)view.tokens * a.heads * a.splits * D, part1 - part0 + 1, [&](int p) { return at + (part0 + p) % a.splits; },
       static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D);
 }
 

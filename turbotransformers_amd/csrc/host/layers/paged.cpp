@@ -120,6 +120,16 @@ bool Share(const TensorView& a, const RowArgs& a_rows, const TensorView& b, cons
   return off < a_width || off + b_width > a_pitch;
 }
 
+// Whether rows, or one of two dense tensors, reach into the other's memory.
+bool Meet(const TensorView& a, int64_t a_bytes, const TensorView& b, int64_t b_bytes) {
+  const intptr_t a0 = reinterpret_cast<intptr_t>(a.data), b0 = reinterpret_cast<intptr_t>(b.data);
+  return a_bytes > 0 && b_bytes > 0 && a0 < b0 + b_bytes && b0 < a0 + a_bytes;
+}
+int64_t Bytes(const TensorView& dense) { return dense.numel() * (dense.dtype.bits / 8); }
+int64_t Bytes(const TensorView& t, const RowArgs& rows, int64_t d) {
+  return t.shape[0] > 0 ? ((t.shape[0] - 1) * rows.pitch + rows.heads * d) * (t.dtype.bits / 8) : 0;
+}
+
 }  // namespace
 
 void RotaryAppend(const TensorView& qkv, const TensorView& keys, const TensorView& values, const PagedBatchViews& batch, const TensorView* inv_freq,
@@ -132,6 +142,12 @@ void RotaryAppend(const TensorView& qkv, const TensorView& keys, const TensorVie
   const bool in_place = q_out.data == qkv.data;
   if (in_place && qkv.shape[0] <= 1) out.pitch = in.pitch;  // (a single row has none of its own)
   TT_ENFORCE(in_place || !Share(qkv, in, q_out, out, cache.cache.head_dim), "the queries' place overlaps qkv");
+  const int64_t held = Bytes(keys);
+  TT_ENFORCE(!Meet(keys, held, values, held), "keys and values overlap");
+  for (const TensorView* t : {&keys, &values}) {
+    TT_ENFORCE(!Meet(*t, held, qkv, Bytes(qkv, in, cache.cache.head_dim)) && !Meet(*t, held, q_out, Bytes(q_out, out, cache.cache.head_dim)),
+               "qkv or the queries' place overlaps the cache");
+  }
   const ttmi_paged_batch args = Batch(batch, qkv.shape[0], device);
   int64_t rotary_dim = 0;
   if (inv_freq != nullptr) {
@@ -146,17 +162,19 @@ void RotaryAppend(const TensorView& qkv, const TensorView& keys, const TensorVie
 }
 
 void PagedAttention(const TensorView& q, const TensorView& keys, const TensorView& values, const PagedBatchViews& batch, const TensorView& out,
-                    int64_t max_tokens, int64_t max_length, float scale, bool causal, int64_t window,
+                    int64_t max_tokens, int64_t max_length, const float* scale, bool causal, int64_t window,
                     const std::function<void*(int64_t)>& workspace, int device, void* stream) {
   const CacheArgs cache = Cache(keys, values, device);
   const RowArgs from = Rows(q, cache, device, "q"), to = Rows(out, cache, device, "out");
   TT_ENFORCE(from.heads == to.heads && q.shape[0] == out.shape[0], "q and out differ in shape");
   TT_ENFORCE(!Share(q, from, out, to, cache.cache.head_dim), "out overlaps q");
+  for (const TensorView* t : {&keys, &values})
+    TT_ENFORCE(!Meet(*t, Bytes(*t), out, Bytes(out, to, cache.cache.head_dim)), "out overlaps the cache");
   const ttmi_paged_batch args = Batch(batch, q.shape[0], device);
-  if (scale == 0.f) scale = (float)(1.0 / std::sqrt((double)cache.cache.head_dim));
+  const float factor = scale != nullptr ? *scale : (float)(1.0 / std::sqrt((double)cache.cache.head_dim));
   int64_t bytes = 0;
   TT_DEVICE_CALL(ttmi_paged_attention_workspace(&cache.cache, &args, from.heads, max_tokens, max_length, window, cache.type, &bytes));
-  TT_DEVICE_CALL(ttmi_paged_attention(q.data, from.pitch, out.data, to.pitch, from.heads, &cache.cache, &args, max_tokens, max_length, scale, causal ? 1 : 0,
+  TT_DEVICE_CALL(ttmi_paged_attention(q.data, from.pitch, out.data, to.pitch, from.heads, &cache.cache, &args, max_tokens, max_length, factor, causal ? 1 : 0,
                                       window, bytes > 0 ? workspace(bytes) : nullptr, bytes, cache.type, stream));
 }
 
@@ -170,6 +188,7 @@ void CopyPages(const TensorView& keys, const TensorView& values, const std::vect
   TT_ENFORCE_EQ(keys.n_dim, values.n_dim, "keys and values differ in shape");
   for (int i = 0; i < keys.n_dim; ++i) TT_ENFORCE_EQ(keys.shape[i], values.shape[i], "keys and values differ in shape");
   TT_ENFORCE(core::SameDataType(keys.dtype, values.dtype), "keys and values differ in type");
+  TT_ENFORCE(!Meet(keys, Bytes(keys), values, Bytes(values)), "keys and values overlap");
   TT_ENFORCE_EQ(sources.size(), destinations.size(), "one destination for each source");
   const bool many = keys.n_dim == 5;
   const int64_t layers = many ? keys.shape[0] : 1, pages = keys.shape[many ? 1 : 0];

@@ -39,10 +39,10 @@ namespace kernels {
 // inv_freq float64 [rotary_dim / 2] or null; q_out [tokens, heads * d] or [tokens, heads, d], rows any distance apart.
 void RotaryAppend(const TensorView& qkv, const TensorView& keys, const TensorView& values, const PagedBatchViews& batch, const TensorView* inv_freq,
                   bool interleaved, float amplitude, const TensorView& q_out, int device, void* stream);
-// q, out [tokens, heads * d] or [tokens, heads, d], rows any distance apart.  scale 0: 1 / sqrt(d).  `workspace` gives device memory of as many
+// q, out [tokens, heads * d] or [tokens, heads, d], rows any distance apart.  scale null: 1 / sqrt(d).  `workspace` gives device memory of as many
 // bytes that stays until the call's work on the stream is done.
 void PagedAttention(const TensorView& q, const TensorView& keys, const TensorView& values, const PagedBatchViews& batch, const TensorView& out,
-                    int64_t max_tokens, int64_t max_length, float scale, bool causal, int64_t window,
+                    int64_t max_tokens, int64_t max_length, const float* scale, bool causal, int64_t window,
                     const std::function<void*(int64_t)>& workspace, int device, void* stream);
 // keys, values [pages, ...] or, of several layers, [layers, pages, kv_heads, page_size, d]
 void CopyPages(const TensorView& keys, const TensorView& values, const std::vector<int32_t>& sources, const std::vector<int32_t>& destinations,

@@ -192,13 +192,14 @@ static void RotaryAppend(const py::object& qkv, const py::object& keys, const py
 // `empty_bytes`: a Python function of a number of bytes that gives device memory of the caller's framework, whose allocator knows the stream (and
 // gives a call that is being recorded into a graph memory that stays the graph's).
 static void PagedAttention(const py::object& q, const py::object& keys, const py::object& values, const py::object& table, const py::object& starts,
-                           const py::object& lengths, const py::object& out, int64_t max_tokens, int64_t max_length, float scale, bool causal,
+                           const py::object& lengths, const py::object& out, int64_t max_tokens, int64_t max_length, const py::object& scale, bool causal,
                            int64_t window, const py::object& empty_bytes, int device, uintptr_t stream) {
   const ViewArg in(q, "q"), k(keys, "keys"), v(values, "values"), t(table, "table"), s(starts, "starts"), l(lengths, "lengths"), o(out, "out");
   std::unique_ptr<ViewArg> workspace;
   py::object memory;
+  const float factor = scale.is_none() ? 0.f : scale.cast<float>();
   layers::kernels::PagedAttention(
-      in.view, k.view, v.view, {t.view, s.view, l.view}, o.view, max_tokens, max_length, scale, causal, window,
+      in.view, k.view, v.view, {t.view, s.view, l.view}, o.view, max_tokens, max_length, scale.is_none() ? nullptr : &factor, causal, window,
       [&](int64_t bytes) -> void* {
         memory = empty_bytes(bytes);
         workspace = std::make_unique<ViewArg>(memory, "workspace");

@@ -62,12 +62,12 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     window > 0: only the last `window` up to its own.  A token that sees no key gets zeros.
 
     q: [tokens, heads * head_dim] or [tokens, heads, head_dim], head_dim 64 or 128; rows may lie any distance apart.  heads is a multiple of
-    kv_heads: query head h reads key/value head h // (heads // kv_heads).  scale: 1 / sqrt(head_dim) by default.
+    kv_heads: query head h reads key/value head h // (heads // kv_heads).  scale: positive, 1 / sqrt(head_dim) by default.
     max_tokens, max_length: the most new tokens and keys of a sequence, where known: they choose how the work is cut, not what is computed.
     -> like q: `out` if given."""
     if out is None:
         out = torch.empty_like(q)
-    cxx.paged_attention(q, keys, values, table, starts, lengths, out, max_tokens, max_length, 0.0 if scale is None else scale, causal, window,
+    cxx.paged_attention(q, keys, values, table, starts, lengths, out, max_tokens, max_length, scale, causal, window,
                         _empty_bytes, *_here())
     return out
 
