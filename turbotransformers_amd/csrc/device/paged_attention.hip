@@ -15,9 +15,15 @@ struct PagedPlan {
   int64_t few_floats, tile_floats;  // of the workspace
 };
 
-// `reach` keys into parts of at least `least`, so that `units` times their number are `wanted` at most.
-void cut(int64_t units, int64_t wanted, int64_t least, int64_t reach, bool window, int* chunk, int* splits) {
-  const int64_t parts = std::min(std::max<int64_t>(1, wanted / std::max<int64_t>(1, units)), std::max<int64_t>(1, ceil_div(reach, least)));
+// Many rows, `units` blocks of them with up to `reach` keys: into parts of at least `least` keys, where it is two of them.  A workgroup alone on its CU is done a third earlier than one of two, so the
+// parts are as many as the CUs hold one each, but where those would be long (five times the least and more), and a CU that has none idles long: then as many as make two.
+// us, whole chip / twice that: bf16, 8 key heads of 64, a prompt of 1000 tokens 21.7 / 26.2, 400 tokens behind 1500 keys 27.0 / 27.4, behind 6000 58.0 / 51.8, 700 behind 6000
+// 100.6 / 78.8; head_dim 128 30.4 / 41.1, 39.2 / 39.4, 81.8 / 75.0, 146 / 118.5.
+void cut(int64_t units, int64_t least, int64_t reach, bool window, int* chunk, int* splits) {
+  const int64_t most = reach < 2 * least ? 1 : ceil_div(reach, least), cus = compute_units();
+  auto made = [&](int64_t workgroups) { return std::min(std::max<int64_t>(1, workgroups / std::max<int64_t>(1, units)), most); };
+  int64_t parts = made(cus);
+  if (reach >= 5 * least * parts) parts = made(2 * cus);
   const int64_t size = ceil_div(ceil_div(reach, parts), 64) * 64;
   *splits = parts > 1 ? (int)(ceil_div(reach, size) + (window ? 1 : 0)) : 1;
   *chunk = (int)size;
@@ -42,9 +48,9 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   p.few_rows = p.tiles ? kFewRows : (int)(most * group);
   p.few_splits = reach * 2 * view.head_dim * (int64_t)dtype_size(dtype) <= kWholeBytes ? 0 : 2 * compute_units();
   p.few_waves = p.few_splits == 0 && batch * view.kv_heads < compute_units() ? 8 : 4;
-  // Many rows: cut where two workgroups a CU are not reached, into parts of at least as many keys as take longer than their joining (fp32, whose matrix instructions take
-  // sixteen times as long: us for one prompt of 200 tokens, 12 heads of 64, parts of 256 / 64 at least 22.0 / 15.7; 16-bit types 9.8 / 11.7).
-  cut(view.kv_heads * (tokens * group / 128 + std::min(batch, tokens)), 512, dtype == TTMI_F32 ? 64 : 256, reach, window > 0, &p.tile_chunk, &p.tile_splits);
+  // (The least that takes longer than joining: fp32, whose matrix instructions take sixteen times as long, us for one prompt of 200 tokens, 4 key heads of 64, parts of 256 / 64
+  // at least 20.9 / 15.1; 16-bit types, 400 tokens, 8 key heads, parts of 512 / 256 / 128 11.9 / 14.3 / 15.7, 100 tokens behind 8000 keys, one key head, 17.1 / 15.0 / 16.6.)
+  cut(view.kv_heads * (tokens * group / 128 + std::min(batch, tokens)), dtype == TTMI_F32 ? 64 : 256, reach, window > 0, &p.tile_chunk, &p.tile_splits);
   const int64_t d = view.head_dim;
   p.few_floats = p.few ? 2ll * p.few_splits * kFewRows * (d + 2) : 0;
   p.tile_floats = p.tiles && p.tile_splits > 1 ? tokens * heads * p.tile_splits * (d + 2) : 0;

@@ -23,6 +23,9 @@ struct Tiles {
   static constexpr int kPieces = kBytes / 4096;         // 16-byte pieces of a tile per thread
   static constexpr int kSteps = kRowBytes / 32;         // pieces of a row per lane, for the first product
   static constexpr int kOut = D / 32;
+  // Tiles on their way in registers.  us, 6 chunks of 400 to 600 tokens behind 1500 to 9000 keys, 32 query and 8 key heads of 64, one / two: fp32 936 / 838, bf16 151 / 154
+  // (head_dim 128 has no registers for two).
+  static constexpr int kDepth = sizeof(T) == 4 && D == 64 ? 2 : 1;
 };
 
 // Places of a row's 16-byte pieces in LDS.  Keys: sixteen rows read the same piece at a time.  Values: 64 bytes of four rows at a time (fp32: 128 bytes of two rows that lie
@@ -162,39 +165,39 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   cursor.table = view.table + (int64_t)b * view.table_pitch;
   cursor.last = max(0, (end - 1) >> view.page_shift);
   cursor.first = 0, cursor.ahead = 0, cursor.at = 0;
-  u32x4 kr[S::kPieces], vr[S::kPieces];
+  u32x4 kr[S::kDepth][S::kPieces], vr[S::kDepth][S::kPieces];
   // 16-byte pieces of a tile: thread by thread, 4 KB after 4 KB.  A wavefront's 1 KB lies in one group of 16 rows.
-  auto load_piece = [&](int i, int key) __attribute__((always_inline)) {
+  auto load_piece = [&](int i, int key, int set) __attribute__((always_inline)) {
     if constexpr (!SMALL) {
       const int group = (i * 4096 + wave * 1024) / (16 * S::kRowBytes) * 16;
       const int64_t from = group_at<S::kRowBytes>(view, cursor, key + group);
       const uint32_t in_group = (uint32_t)(i * 4096 + tid * 16) % (16 * S::kRowBytes);
-      kr[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(keys) + from + in_group);
-      vr[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(values) + from + in_group);
+      kr[set][i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(keys) + from + in_group);
+      vr[set][i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(values) + from + in_group);
     } else {
       const int at = i * 4096 + tid * 16;
       const int64_t from = row_offset<D>(view, cursor, kv_head, key + at / S::kRowBytes) + at % S::kRowBytes / (int)sizeof(T);
-      kr[i] = *reinterpret_cast<const u32x4*>(keys + from);
-      vr[i] = *reinterpret_cast<const u32x4*>(values + from);
+      kr[set][i] = *reinterpret_cast<const u32x4*>(keys + from);
+      vr[set][i] = *reinterpret_cast<const u32x4*>(values + from);
     }
   };
   auto key_stage = [&](int s) __attribute__((always_inline)) { return smem + s * 2 * S::kBytes; };
   auto value_stage = [&](int s) __attribute__((always_inline)) { return smem + s * 2 * S::kBytes + S::kBytes; };
-  auto store_piece = [&](int i, int s) __attribute__((always_inline)) {
+  auto store_piece = [&](int i, int s, int set) __attribute__((always_inline)) {
     const int at = i * 4096 + tid * 16, r = at / S::kRowBytes, c = at % S::kRowBytes / 16;
-    *reinterpret_cast<u32x4*>(key_stage(s) + r * S::kRowBytes + key_piece<T, D>(r, c) * 16) = kr[i];
-    *reinterpret_cast<u32x4*>(value_stage(s) + r * S::kRowBytes + value_piece<T, D>(r, c) * 16) = vr[i];
+    *reinterpret_cast<u32x4*>(key_stage(s) + r * S::kRowBytes + key_piece<T, D>(r, c) * 16) = kr[set][i];
+    *reinterpret_cast<u32x4*>(value_stage(s) + r * S::kRowBytes + value_piece<T, D>(r, c) * 16) = vr[set][i];
   };
   // Keys that no row sees may hold anything: their values count as zeros.  Where only some rows see a key, infinities and NaNs of its values must not
   // reach the others: they are left out here, noted, and added where they are seen.
   auto partly_seen = [&](int key) __attribute__((always_inline)) { return key < sure_first || key + S::kKeys > sure_end; };
-  auto clean_values = [&](int key) __attribute__((always_inline)) {
+  auto clean_values = [&](int key, int set) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < S::kPieces; ++i) {
       const int k = key + (i * 4096 + tid * 16) / S::kRowBytes;
-      if (k < first || k >= end) vr[i] = u32x4{0u, 0u, 0u, 0u};
-      if (not_finite<T>(vr[i])) wild = 1;
-      vr[i] = finite_part<T>(vr[i]);
+      if (k < first || k >= end) vr[set][i] = u32x4{0u, 0u, 0u, 0u};
+      if (not_finite<T>(vr[set][i])) wild = 1;
+      vr[set][i] = finite_part<T>(vr[set][i]);
     }
   };
   if (lo < hi) {
@@ -202,27 +205,30 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
     const int last = lo + (hi - 1 - lo) / S::kKeys * S::kKeys;
     if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, lo);
 #pragma unroll
-    for (int i = 0; i < S::kPieces; ++i) load_piece(i, lo);
+    for (int i = 0; i < S::kPieces; ++i) load_piece(i, lo, 0);
     if (tid == 0) wild = 0;
     __syncthreads();
-    if (partly_seen(lo)) clean_values(lo);
+    if (partly_seen(lo)) clean_values(lo, 0);
 #pragma unroll
-    for (int i = 0; i < S::kPieces; ++i) store_piece(i, 0);
+    for (int i = 0; i < S::kPieces; ++i) store_piece(i, 0, 0);
 #pragma unroll
-    for (int i = 0; i < S::kPieces; ++i) load_piece(i, min(lo + S::kKeys, last));  // (in the same 64 pages)
+    for (int n = 1; n <= S::kDepth; ++n)
+#pragma unroll
+      for (int i = 0; i < S::kPieces; ++i) load_piece(i, min(lo + n * S::kKeys, last), n % S::kDepth);  // (in the same 64 pages)
     __syncthreads();
     // One tile; its stage is known to the compiler, so that places in LDS are fixed numbers behind one of the lane's.
     auto work_on = [&](int key, auto stage) __attribute__((always_inline)) {
       constexpr int s = decltype(stage)::value;
       // The other stage is free: what was fetched for it while the last tile was worked on goes there, and the tile behind it is sent for.
-      const int after = min(key + 2 * S::kKeys, last);
+      constexpr int set = (s + 1) % S::kDepth;
+      const int after = min(key + (1 + S::kDepth) * S::kKeys, last);
       if constexpr (!SMALL) come_to<S::kRowBytes>(view, cursor, kv_head, after);
-      if (__builtin_expect(partly_seen(key + S::kKeys), 0)) clean_values(key + S::kKeys);
+      if (__builtin_expect(partly_seen(key + S::kKeys), 0)) clean_values(key + S::kKeys, set);
       if (key >= wave_end || key + S::kKeys <= wave_first) {  // nothing to do for this wavefront's rows
 #pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) store_piece(i, s ^ 1);
+        for (int i = 0; i < S::kPieces; ++i) store_piece(i, s ^ 1, set);
 #pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) load_piece(i, after);
+        for (int i = 0; i < S::kPieces; ++i) load_piece(i, after, set);
         __syncthreads();
         return;
       }
@@ -246,11 +252,11 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
       for (int n = 0; n < kScores; ++n) {
         st[n % S::kSubs] = mma32<T>(f[n % kAhead], qf[n / S::kSubs], st[n % S::kSubs]);
         if (n + kAhead < kScores) f[n % kAhead] = read_keys(n + kAhead);
-        if (n < S::kPieces) store_piece(n, s ^ 1);
+        if (n < S::kPieces) store_piece(n, s ^ 1, set);
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int i = 0; i < S::kPieces; ++i) load_piece(i, after);
+      for (int i = 0; i < S::kPieces; ++i) load_piece(i, after, set);
       if (__builtin_expect(key < wave_high.begin || key + S::kKeys > wave_low.end, 0)) {
         const int from = mine.begin - key - 4 * lhalf;
         const uint32_t span = (uint32_t)(mine.end - mine.begin);
@@ -380,21 +386,59 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   store_rows<T, D>(a, seq, token, head, part, sees ? mine.begin / chunk : part0, sees ? (mine.end - 1) / chunk : part0, lhalf, ot, top, sum);
 }
 
-// Rows whose keys lay in several parts: a wavefront per row and head.
-template <typename T, int D>
+// Rows whose keys lay in several parts.  What their bytes take is little; what counts is how many trips to memory follow one another: the sequence, its length, the parts.  So
+// a thread has four columns of a row and head and asks for up to MOST parts at once.  (us for two parts, 32 heads of 64: a wavefront per row and head 10.4 for 600 tokens and 14.8
+// for 1000, this 4.9 for 700.)  MOST 0, many parts: a workgroup per row and head, whose threads share them.
+constexpr int kFewParts = 16;
+template <typename T, int D, int MOST>
 __global__ __launch_bounds__(256) void join_tiles_kernel(const PagedArgs a) {
   const PagedView& view = a.view;
-  const int row = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = sequence_of(view, row);
-  if (b >= view.batch || h >= a.heads) return;
+  const int row = blockIdx.x, b = sequence_of(view, row);
+  if (b >= view.batch) return;
   const Sequence seq = sequence(a, b);
   if (row < seq.start || (seq.tokens * a.group <= kFewRows && !a.every)) return;
   const Reach reach = seq.reach(a, row - seq.start);
-  const int chunk = seq.chunk(a), part0 = reach.begin / chunk, part1 = reach.end > 0 ? (reach.end - 1) / chunk : 0;
-  if (part0 == part1) return;
-  const int64_t at = ((int64_t)row * a.heads + h) * a.splits;
-  join_parts_by_wavefront<T, D>(
-      a.partial, a.partial + (int64_t)view.tokens * a.heads * a.splits * D, part1 - part0 + 1, [&](int p) { return at + (part0 + p) % a.splits; },
-      static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D);
+  const int chunk = seq.chunk(a), part0 = reach.begin / chunk, parts = (reach.end > 0 ? (reach.end - 1) / chunk : 0) - part0 + 1;
+  if (parts <= 1) return;
+  const float* const met = a.partial + (int64_t)view.tokens * a.heads * a.splits * D;
+  if constexpr (MOST == 0) {
+    const int h = blockIdx.y;
+    const int64_t at = ((int64_t)row * a.heads + h) * a.splits;
+    join_parts<T, D>(
+        a.partial, met, parts, [&](int p) { return at + (part0 + p) % a.splits; }, static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D);
+  } else {
+    constexpr int kThreads = D / 4;
+    const int h = blockIdx.y * (256 / kThreads) + threadIdx.x / kThreads, d0 = threadIdx.x % kThreads * 4;
+    if (h >= a.heads) return;
+    const int64_t at = ((int64_t)row * a.heads + h) * a.splits;
+    floatx4 x[MOST];
+    floatx2 ml[MOST];
+#pragma unroll
+    for (int p = 0; p < MOST; ++p)
+      if (p < parts) {
+        const int64_t from = at + (part0 + p) % a.splits;
+        x[p] = *reinterpret_cast<const floatx4*>(a.partial + from * D + d0);
+        ml[p] = *reinterpret_cast<const floatx2*>(met + from * 2);
+      }
+    float best = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int p = 0; p < MOST; ++p)
+      if (p < parts) best = fmaxf(best, ml[p][0]);
+    const float zero = best == -INFINITY ? 0.f : best;
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < MOST; ++p)
+      if (p < parts) {
+        const float weight = __builtin_amdgcn_exp2f(ml[p][0] - zero);
+        total += ml[p][1] * weight;
+        sum += x[p] * weight;
+      }
+    const float inv = total != 0.f ? 1.0f / total : 0.f;
+    Vec<T, 4> y;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) y.v[c] = from_float<T>(sum[c] * inv);
+    store_vec<T, 4>(static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D + d0, y);
+  }
 }
 
 }  // namespace
@@ -406,14 +450,20 @@ int launch_tiles(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t st
   PagedArgs args = a;
   args.ordered = blocks * a.view.kv_heads * a.splits > 2 * compute_units();
   TTMI_DISPATCH_FLOAT(dtype, T, {
-    auto launch = [&](auto kernel, auto join) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * a.view.kv_heads), 1, (unsigned)a.splits), dim3(256), 0, stream, args);
-      if (a.splits > 1) hipLaunchKernelGGL(join, dim3((unsigned)a.view.tokens, (unsigned)ceil_div(a.heads, 4)), dim3(256), 0, stream, a);
+    auto launch = [&](auto d, auto small_pages) {
+      constexpr int D = decltype(d)::value;
+      hipLaunchKernelGGL((tiles_kernel<T, D, decltype(small_pages)::value>), dim3((unsigned)(blocks * a.view.kv_heads), 1, (unsigned)a.splits), dim3(256), 0, stream, args);
+      const unsigned tokens = (unsigned)a.view.tokens, few = (unsigned)ceil_div(a.heads, 256 / (D / 4));
+      if (a.splits > kFewParts) hipLaunchKernelGGL((join_tiles_kernel<T, D, 0>), dim3(tokens, a.heads), dim3(256), 0, stream, a);
+      else if (a.splits > 2) hipLaunchKernelGGL((join_tiles_kernel<T, D, kFewParts>), dim3(tokens, few), dim3(256), 0, stream, a);
+      else if (a.splits > 1) hipLaunchKernelGGL((join_tiles_kernel<T, D, 2>), dim3(tokens, few), dim3(256), 0, stream, a);
     };
-    if (head_dim == 64 && small) launch(tiles_kernel<T, 64, true>, join_tiles_kernel<T, 64>);
-    else if (head_dim == 64) launch(tiles_kernel<T, 64, false>, join_tiles_kernel<T, 64>);
-    else if (small) launch(tiles_kernel<T, 128, true>, join_tiles_kernel<T, 128>);
-    else launch(tiles_kernel<T, 128, false>, join_tiles_kernel<T, 128>);
+    const std::integral_constant<int, 64> d64;
+    const std::integral_constant<int, 128> d128;
+    if (head_dim == 64 && small) launch(d64, std::true_type{});
+    else if (head_dim == 64) launch(d64, std::false_type{});
+    else if (small) launch(d128, std::true_type{});
+    else launch(d128, std::false_type{});
   });
   return launch_status("paged_attention");
 }
