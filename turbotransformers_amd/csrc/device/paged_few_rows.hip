@@ -7,7 +7,12 @@
 // second operand of
 //     Ot[d, row] += Vt[d, keys] . Pt[keys, row]
 // wants them: its order of keys is ours to choose.  Vt is what the transposing reads give of a tile that lies in LDS row by row as it came (fp32: plain reads of a
-// column).  Tiles are fetched into registers one ahead: 8 KB of keys and as many of values per wavefront are on their way while one is worked on.
+// column).  Tiles are fetched into registers one ahead: 8 KB of keys and as many of values per wavefront are on their way while one is worked on; what a CU has on its way is
+// what it gets (about 50 GB/s whatever runs on the others), so the loads are never behind a condition, which would make the compiler wait for all of them.
+//
+// Measured, 32 query and 8 key heads of 128: 64 sequences of 100 to 6000 keys, bf16, 85 us and 6 to join the parts (5.1 TB/s while it reads; a large copy here 4.8);
+// 4 sequences of 60000 to 131071 keys, fp16, 264 and 7 (6.0 TB/s, part of it out of the last-level cache).  One sequence of 387 keys, 12 heads of 64, fp16: 6.7, of which
+// most is the trips to memory that follow one another: length, pages, keys.
 #include "paged_attention.h"
 
 namespace ttmi {
@@ -403,7 +408,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
   }
 }
 
-// Pairs that were several workgroups': their rows' partial results are joined.  A workgroup per pair and row, or per pair where there are many of them: then a wavefront
+// Pairs that were several workgroups': their rows' partial results are joined, in 5 to 7 us, nearly all of them the launch and three trips to memory.  A workgroup per pair and row, or per pair where there are many of them: then a wavefront
 // takes a row, unless the pair had many parts.
 constexpr int kManyPairs = 64, kManyParts = 16;
 template <typename T, int D>
