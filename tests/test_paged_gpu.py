@@ -650,3 +650,69 @@ def test_many_sequences(dt, batch):
     case.check_attention(case.run_attention(max_length=5000))  # (long enough for sharing out)
     new = [40 if i % 11 == 0 else m for i, m in enumerate(new)]
     check(dt, new, lengths, 4, 2, 64, 16)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_more_heads_of_a_group_than_rows_of_a_tile(dt):
+    check(dt, [1, 3, 2], [20, 5, 300], 200, 1, 64, 16)
+    check(dt, [2], [700], 150, 1, 128, 32, window=33)
+
+
+def test_calls_on_two_streams_at_a_time():
+    """Two batches over one cache, cut and joined, in turn on two streams without waiting for one another: their workspaces are their own."""
+    cases = [Case("bf16", [1] * 3, [3000, 2000, 900], 8, 2, 128, 16, seed=1), Case("bf16", [40, 1], [2500, 1200], 8, 2, 128, 16, seed=2)]
+    tensors = [[x.cuda() for x in (case.q, case.keys, case.values)] + case.device_args() for case in cases]
+    hints = [dict(max_tokens=max(case.new), max_length=max(case.lengths)) for case in cases]
+    want = [tt.paged_attention(*t, **h) for t, h in zip(tensors, hints)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(tt.paged_attention(*tensors[i], **hints[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        cases[i].check_attention(want[i])
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_recorded_copies():
+    """The list of a recorded copy is the recording's own: the lists it was given may change, the pages' contents may."""
+    keys, values = (torch.randn(2, 30, 2, 16, 64, device="cuda", dtype=torch.float16) for _ in range(2))
+    src, dst = [1, 5, 7], [10, 20, 3]
+    tt.copy_pages(keys, values, [0], [29])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tt.copy_pages(keys, values, src, dst)
+    src[0], dst[0] = 2, 4
+    for _ in range(3):
+        keys.normal_(), values.normal_()
+        want = [x.clone() for x in (keys, values)]
+        for w in want:
+            w[:, [10, 20, 3]] = w[:, [1, 5, 7]]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(keys, want[0]) and torch.equal(values, want[1])
+
+
+def test_sequences_without_keys_and_calls_without_tokens():
+    """No tokens at all, no sequences, a table without columns for sequences that are empty: nothing is written, nothing goes wrong."""
+    case = Case("f16", [1, 1], [20, 3], 4, 2, 64, 16)
+    k, v = case.keys.cuda(), case.values.cuda()
+    table, starts, lengths = case.device_args()
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    assert tt.paged_attention(case.q.cuda()[:0], k, v, table, starts * 0, lengths).shape == (0, 4, 64)
+    out = torch.full((2, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    tt.paged_attention(case.q.cuda(), k, v, table[:0], ints(0), ints(), out=out)
+    tt.paged_attention(case.q.cuda(), k, v, table, ints(0, 0, 0), lengths, out=out)
+    assert (out == 7).all()
+    tt.paged_attention(case.q.cuda(), k, v, table[:, :0].contiguous(), ints(0, 1, 2), ints(0, 0), causal=False, out=out)
+    assert (out == 0).all()
+    qkv = torch.ones(2, 8, 64, dtype=torch.float16, device="cuda")
+    before = k.clone()
+    assert tt.rotary_append(qkv[:0], k, v, table, starts * 0, lengths).shape == (0, 4, 64)
+    tt.rotary_append(qkv, k, v, table, ints(0, 0, 0), lengths)
+    assert torch.equal(k.nan_to_num(), before.nan_to_num())
+    tt.cxx.synchronize()

@@ -10,7 +10,7 @@
 // Measured, 32 query and 8 key heads of 128, bf16: a prompt of 8192 tokens 580 to 620 us (0.89 to 0.94 PFLOP/s; a large product here 1.26), a multiplication by zeros 530 to 565:
 // the chip is at its power limit.  Heads of 64: 343 us (0.80), where an exponential takes a lane as long as its share of the products.  A workgroup by itself takes about 7 us to
 // its first tile and 0.95 a tile of 64 keys, heads of 64, where four instructions' worth of products would be 0.2: a chain of reads, products, maximum, exponentials, products.
-// What was built and taken out: 256 rows a workgroup with the products of 32 keys beside the exponentials of the 32 before, 3 % for heads of 128, a loss for those of 64.
+// What was built and taken out: 256 rows a workgroup with the products of 32 keys beside the exponentials of the 32 before, level to 3 % faster for heads of 128, 2 % slower for those of 64.
 #include "paged_attention.h"
 
 namespace ttmi {
