@@ -584,7 +584,7 @@ typedef struct ttmi_paged_cache {
 } ttmi_paged_cache;
 
 /* A batch of sequences and their new tokens.  All three arrays lie on the device and may change between replays of a recorded call.
- *   table    [batch, table_pitch] the pages of each sequence, in order; entries past its last page are not read
+ *   table    [batch, table_pitch] the pages of each sequence, in order; entries past its last page are not read; table_pitch * page_size is 2^30 at most
  *   starts   [batch + 1], never falling: the new tokens of sequence b are rows starts[b] to starts[b + 1] of the packed tensors (none, one or many);
  *            rows from starts[batch] on are neither read nor written
  *   lengths  [batch] keys of the sequence, those of its new tokens included: the i-th of n new tokens has position lengths[b] - n + i
@@ -605,7 +605,7 @@ typedef struct ttmi_paged_batch {
  *   The first rotary_dim (even, 0: none) elements of each head are turned: the pair number i by the angle position * inv_freq[i] (radians; inv_freq
  *   DEVICE double[rotary_dim / 2]; angles are formed in 64 bits, any position keeps its place on the circle), times `amplitude`.  Pairs are elements
  *   (2i, 2i + 1) where `interleaved`, else (i, i + rotary_dim / 2).  The rest of a head is copied.
- * Two new tokens must not share a slot.  No counterpart in the reference. */
+ * Two new tokens must not share a slot, and neither keys and values nor cache and rows may overlap.  No counterpart in the reference. */
 TTMI_API int ttmi_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t q_pitch, int64_t heads,
                                 const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, const double* inv_freq,
                                 int64_t rotary_dim, int interleaved, float amplitude, int dtype, void* stream);
@@ -615,6 +615,7 @@ TTMI_API int ttmi_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out,
  * `causal`: keys up to the token's own position, else all keys of its sequence; window > 0: of these only positions from its own - window + 1 on.
  * A token that sees no key gets zeros.  q and out [tokens, heads, 64 or 128], rows q_pitch and out_pitch elements apart (a multiple of 16
  * bytes); out must not overlap anything else; heads is a multiple of kv_heads, query head h reads key/value head h / (heads / kv_heads).
+ * scale is positive.  tokens * heads is less than 2^30, batch * kv_heads less than 2^23.
  * max_tokens, max_length: the most new tokens and keys that a sequence has, or 0 if unknown.  They only choose how the work is cut; a
  * call whose sequences have more is computed all the same.
  * workspace: DEVICE memory of ttmi_paged_attention_workspace bytes (0: none is needed), 16-byte aligned, for this call alone while it runs.
@@ -628,7 +629,7 @@ TTMI_API int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int
 
 /* Page destinations[i] becomes a copy of page sources[i], i < count, in `layers` caches that lie behind each other ([layers, pages, page_bytes]
  * each of keys and values).  sources, destinations: HOST arrays.  A page must not be a destination twice, nor both a
- * source and a destination; a source may be copied many times.  page_bytes a multiple of 16. */
+ * source and a destination; a source may be copied many times.  page_bytes a multiple of 16, 2^36 at most. */
 TTMI_API int ttmi_copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t page_bytes, const int32_t* sources,
                              const int32_t* destinations, int64_t count, void* stream);
 
