@@ -128,6 +128,96 @@ def test_pool_refuses():
     assert pool.table([], 3).shape == (0, 3)
 
 
+def test_pool_says_beforehand_what_it_will_copy_and_move():
+    """`copies_of` and `moves_of` change nothing, name what `extend` and `compact` then return, and refuse what `extend` refuses."""
+    rng = random.Random(1)
+    pool = tt.cxx.PagePool(30, 4)
+    held = [pool.add()]
+    book = lambda: [(s, pool.pages_of(s), pool.length(s)) for s in held] + [pool.free_pages] + [pool.references(p) for p in range(30)]
+    seen = 0
+    for _ in range(300):
+        names = rng.sample(held, rng.randint(1, len(held)))
+        tokens = [rng.choice([0, 1, 2, 7]) for _ in names]
+        before = book()
+        try:
+            copies = pool.copies_of(names, tokens)
+        except tt.cxx.EnforceNotMet:
+            assert book() == before
+            with pytest.raises(tt.cxx.EnforceNotMet):
+                pool.extend(names, tokens)
+            assert book() == before
+            for s in held[1:]:
+                pool.free(s)
+            held = held[:1]
+            pool.truncate(held[0], rng.randint(0, 9))
+            continue
+        assert book() == before
+        free = {p for p in range(30) if pool.references(p) == 0}
+        assert {to for _, to in copies} <= free
+        assert pool.extend(names, tokens) == copies
+        seen += len(copies)
+        if len(held) < 6:
+            held.append(pool.fork(rng.choice(held)))
+        if rng.random() < 0.2:
+            before, moves = book(), pool.moves_of()
+            assert book() == before
+            assert {to for _, to in moves} <= {p for p in range(30) if pool.references(p) == 0}
+            assert pool.compact() == moves
+            seen += len(moves)
+    assert seen > 50
+
+
+class FailsOnce(Exception):
+    pass
+
+
+@pytest.mark.parametrize("fails", ["copy", "batch"])
+def test_a_step_that_cannot_be_made_leaves_the_sequences_as_they_were(fails, monkeypatch):
+    """The copy of a shared page is refused (here: memory of the host), or the batch cannot be built: every sequence has its tokens as before, and the same
+    call made again copies the page."""
+    from turbotransformers_amd.layers import paged
+    cache = tt.PagedCache(1, 1, 16, 8, 4, torch.float32, device="cpu")
+    a = cache.add()
+    cache.extend([a], [6])
+    b = cache.fork(a)
+    shared = cache.pool.pages_of(a)[1]
+    held = lambda: [(cache.pool.length(s), cache.pool.pages_of(s)[0]) for s in (a, b)]
+    before, copied = held(), []
+    if fails == "copy":
+        with pytest.raises(tt.cxx.EnforceNotMet, match="not on the GPU"):
+            cache.extend([a, b], [1, 7])
+        assert cache.pool.pages_of(a) == cache.pool.pages_of(b) and cache.pool.free_pages == 6
+    monkeypatch.setattr(paged, "copy_pages", lambda keys, values, src, dst: copied.extend(zip(src, dst)))
+    if fails == "batch":
+        def no_batch(*args):
+            raise FailsOnce
+        with monkeypatch.context() as m:
+            m.setattr(paged, "PagedBatch", no_batch)
+            with pytest.raises(FailsOnce):
+                cache.extend([a, b], [1, 7])
+    assert held() == before
+    batch = cache.extend([a, b], [1, 7])
+    assert [cache.length(s) for s in (a, b)] == [7, 13] and batch.lengths.tolist() == [7, 13] and batch.starts.tolist() == [0, 1, 8]
+    last = [cache.pool.pages_of(s)[1] for s in (a, b)]
+    assert last[0] != last[1] and len(copied) == 1 and copied[0][0] == shared and copied[0][1] in last
+
+
+def test_a_compaction_that_cannot_be_made_changes_nothing(monkeypatch):
+    from turbotransformers_amd.layers import paged
+    cache = tt.PagedCache(1, 1, 16, 8, 4, torch.float32, device="cpu")
+    a, b = cache.add(), cache.add()
+    cache.extend([a, b], [9, 5])
+    cache.free(a)
+    book = lambda: (cache.pool.pages_of(b), cache.pool.free_pages, [cache.pool.references(p) for p in range(8)])
+    before = book()
+    with pytest.raises(tt.cxx.EnforceNotMet, match="not on the GPU"):
+        cache.compact()
+    assert book() == before
+    moved = []
+    monkeypatch.setattr(paged, "copy_pages", lambda keys, values, src, dst: moved.extend(zip(src, dst)))
+    assert cache.compact() == 2 and [src for src, _ in moved] == before[0] and cache.pool.pages_of(b) == [0, 1]
+
+
 # ----------------------------------------------------------------------------------------------------- refusals ------
 P = ctypes.c_void_p
 ADDRESS = 1 << 20  # (nothing is read: every call below is refused before a launch)

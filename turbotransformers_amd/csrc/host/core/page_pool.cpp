@@ -1,8 +1,8 @@
 #include "core/page_pool.h"
 
 #include <algorithm>
-#include <functional>
 #include <limits>
+#include <numeric>
 
 #include "core/enforce.h"
 
@@ -37,7 +37,7 @@ int64_t PagePool::Add() {
   return next_++;
 }
 
-PagePool::Copies PagePool::Extend(const std::vector<int64_t>& sequences, const std::vector<int64_t>& tokens) {
+PagePool::Growth PagePool::GrowthOf(const std::vector<int64_t>& sequences, const std::vector<int64_t>& tokens) const {
   TT_ENFORCE_EQ(sequences.size(), tokens.size(), "one number of tokens for each sequence");
   std::vector<int64_t> named(sequences);
   std::sort(named.begin(), named.end());
@@ -46,23 +46,34 @@ PagePool::Copies PagePool::Extend(const std::vector<int64_t>& sequences, const s
   // depends on the order in which they come, so the pages are counted as they will be taken.
   std::unordered_map<int32_t, int32_t> left;
   int64_t needed = 0;
-  std::vector<bool> splits(sequences.size(), false);
+  Growth growth;
+  growth.splits.assign(sequences.size(), false);
+  std::vector<std::pair<int32_t, int64_t>> replaced;  // a shared page, and how many pages are taken before that which takes its place
   for (size_t i = 0; i < sequences.size(); ++i) {
     const Sequence& s = Of(sequences[i]);
     TT_ENFORCE(tokens[i] >= 0 && tokens[i] <= std::numeric_limits<int32_t>::max() - s.length, "bad number of tokens");
-    needed += PagesFor(s.length + tokens[i]) - (int64_t)s.pages.size();
     if (tokens[i] > 0 && s.length % page_size_ != 0) {
       const int32_t last = s.pages.back();
       const auto it = left.emplace(last, references_[(size_t)last]).first;
       if (it->second > 1) {
-        splits[i] = true;
+        growth.splits[i] = true;
         --it->second;
-        ++needed;
+        replaced.emplace_back(last, needed++);
       }
     }
+    needed += PagesFor(s.length + tokens[i]) - (int64_t)s.pages.size();
   }
   TT_ENFORCE(needed <= free_pages(), "%ld pages are needed, %ld are free", (long)needed, (long)free_pages());
-  Copies copies;
+  for (const auto& page : replaced) growth.copies.emplace_back(page.first, free_[free_.size() - 1 - (size_t)page.second]);
+  return growth;
+}
+
+PagePool::Copies PagePool::CopiesOf(const std::vector<int64_t>& sequences, const std::vector<int64_t>& tokens) const {
+  return GrowthOf(sequences, tokens).copies;
+}
+
+PagePool::Copies PagePool::Extend(const std::vector<int64_t>& sequences, const std::vector<int64_t>& tokens) {
+  Growth growth = GrowthOf(sequences, tokens);
   for (size_t i = 0; i < sequences.size(); ++i) {
     Sequence& s = sequences_[sequences[i]];
     auto take = [&] {
@@ -71,16 +82,14 @@ PagePool::Copies PagePool::Extend(const std::vector<int64_t>& sequences, const s
       references_[(size_t)page] = 1;
       return page;
     };
-    if (splits[i]) {
-      const int32_t shared = s.pages.back();
+    if (growth.splits[i]) {
+      --references_[(size_t)s.pages.back()];  // (others still hold it)
       s.pages.back() = take();
-      --references_[(size_t)shared];  // (others still hold it)
-      copies.emplace_back(shared, s.pages.back());
     }
     s.length += tokens[i];
     while ((int64_t)s.pages.size() < PagesFor(s.length)) s.pages.push_back(take());
   }
-  return copies;
+  return std::move(growth.copies);
 }
 
 int64_t PagePool::Fork(int64_t sequence) {
@@ -106,24 +115,31 @@ void PagePool::Free(int64_t sequence) {
   sequences_.erase(sequence);
 }
 
-PagePool::Copies PagePool::Compact() {
-  std::vector<int32_t> to((size_t)pages());
+PagePool::Copies PagePool::MovesOf() const {
   int32_t hole = 0, live = 0;
   for (int32_t n : references_) live += n > 0;
   Copies moves;
   // live pages from number `live` on go to the free ones below it, in order: no page is read that another move writes
-  for (int32_t page = 0; page < (int32_t)pages(); ++page) {
-    to[(size_t)page] = page;
-    if (page < live || references_[(size_t)page] == 0) continue;
+  for (int32_t page = live; page < (int32_t)pages(); ++page) {
+    if (references_[(size_t)page] == 0) continue;
     while (references_[(size_t)hole] != 0) ++hole;
-    to[(size_t)page] = hole;
     moves.emplace_back(page, hole++);
   }
-  for (const auto& move : moves) std::swap(references_[(size_t)move.first], references_[(size_t)move.second]);
+  return moves;
+}
+
+PagePool::Copies PagePool::Compact() {
+  const Copies moves = MovesOf();
+  std::vector<int32_t> to((size_t)pages());
+  std::iota(to.begin(), to.end(), 0);
+  for (const auto& move : moves) {
+    to[(size_t)move.first] = move.second;
+    std::swap(references_[(size_t)move.first], references_[(size_t)move.second]);
+  }
   for (auto& entry : sequences_)
     for (int32_t& page : entry.second.pages) page = to[(size_t)page];
   free_.clear();
-  for (int32_t page = (int32_t)pages() - 1; page >= live; --page) free_.push_back(page);
+  for (int32_t page = (int32_t)pages() - 1; page >= 0 && references_[(size_t)page] == 0; --page) free_.push_back(page);
   return moves;
 }
 

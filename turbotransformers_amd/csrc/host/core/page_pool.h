@@ -21,10 +21,14 @@ class PagePool {
   // Sequence sequences[i] grows by tokens[i] (a sequence may be named once).  A last page that is shared and not full is replaced by a page of its own,
   // whose copy is returned and has to be made before the new tokens are stored.  Without enough free pages nothing changes and the call throws.
   Copies Extend(const std::vector<int64_t>& sequences, const std::vector<int64_t>& tokens);
+  // The copies that Extend would return (it throws where that would), with nothing changed: they go to free pages, so whoever makes them first and then calls
+  // Extend has lost nothing where a copy fails.
+  Copies CopiesOf(const std::vector<int64_t>& sequences, const std::vector<int64_t>& tokens) const;
   int64_t Fork(int64_t sequence);                         // a sequence with the same tokens in the same pages -> its number
   void Truncate(int64_t sequence, int64_t length);        // back to its first `length` tokens
   void Free(int64_t sequence);
   Copies Compact();  // live pages move to the lowest numbers; the moves have to be made before anything else reads or writes the cache
+  Copies MovesOf() const;  // what Compact would return, with nothing changed: moves to free pages as well
 
   int64_t Length(int64_t sequence) const { return Of(sequence).length; }
   const std::vector<int32_t>& Pages(int64_t sequence) const { return Of(sequence).pages; }
@@ -40,6 +44,11 @@ class PagePool {
     int64_t length = 0;
   };
   const Sequence& Of(int64_t sequence) const;
+  struct Growth {
+    std::vector<bool> splits;  // whether a sequence's last page is replaced
+    Copies copies;
+  };
+  Growth GrowthOf(const std::vector<int64_t>& sequences, const std::vector<int64_t>& tokens) const;
   int64_t PagesFor(int64_t tokens) const { return (tokens + page_size_ - 1) / page_size_; }
   void Release(int32_t page);
 

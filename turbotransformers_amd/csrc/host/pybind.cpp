@@ -499,10 +499,12 @@ PYBIND11_MODULE(turbo_transformers_cxx, m) {
       .def(py::init<int64_t, int64_t>(), py::arg("pages"), py::arg("page_size"))
       .def("add", &core::PagePool::Add)
       .def("extend", &core::PagePool::Extend, py::arg("sequences"), py::arg("tokens"))
+      .def("copies_of", &core::PagePool::CopiesOf, py::arg("sequences"), py::arg("tokens"))
       .def("fork", &core::PagePool::Fork, py::arg("sequence"))
       .def("truncate", &core::PagePool::Truncate, py::arg("sequence"), py::arg("length"))
       .def("free", &core::PagePool::Free, py::arg("sequence"))
       .def("compact", &core::PagePool::Compact)
+      .def("moves_of", &core::PagePool::MovesOf)
       .def("length", &core::PagePool::Length, py::arg("sequence"))
       .def("pages_of", &core::PagePool::Pages, py::arg("sequence"))
       .def("references", &core::PagePool::References, py::arg("page"))

@@ -152,9 +152,18 @@ class PagedCache:
 
     def extend(self, sequences: Sequence[int], tokens: Sequence[int]) -> PagedBatch:
         """Room for tokens[i] new tokens of sequences[i], and the batch of that step.  Shared pages that would be written are copied first.
-        Raises, with nothing changed, where there are not enough free pages."""
-        self._move(self.pool.extend(sequences, tokens))
-        lengths = [self.pool.length(s) for s in sequences]
+        A call that raises, for want of free pages or because a copy or the batch cannot be made, leaves every sequence with the tokens it had."""
+        self._move(self.pool.copies_of(sequences, tokens))  # (to free pages: the book follows when they have been enqueued)
+        before = [self.pool.length(s) for s in sequences]
+        self.pool.extend(sequences, tokens)
+        try:
+            return self._batch(sequences, tokens, [n + more for n, more in zip(before, tokens)])
+        except BaseException:
+            for s, n in zip(sequences, before):
+                self.pool.truncate(s, n)
+            raise
+
+    def _batch(self, sequences, tokens, lengths):
         longest = max(lengths, default=0)
         starts = [0]
         for n in tokens:
@@ -169,9 +178,10 @@ class PagedCache:
                           max(tokens, default=0), longest)
 
     def compact(self) -> int:
-        """Moves live pages to the lowest numbers -> how many moved.  Batches made before are void."""
-        moves = self.pool.compact()
-        self._move(moves)
+        """Moves live pages to the lowest numbers -> how many moved.  Batches made before are void.  A call that raises has changed nothing."""
+        moves = self.pool.moves_of()
+        self._move(moves)  # (to free pages, as above)
+        self.pool.compact()
         return len(moves)
 
     def append(self, layer: int, qkv: torch.Tensor, batch: PagedBatch, inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
