@@ -290,6 +290,14 @@ def test_attention_refuses(lib):
     assert lib.ttmi_paged_attention_workspace(ctypes.byref(cache()), ctypes.byref(batch()), 4, 0, 0, 0, capi.F16, None) == -1
 
 
+def test_scales_whose_product_with_log2_e_is_not_finite_are_refused(lib):
+    """The kernels multiply scores by scale * log2(e), 1.4427 of it: 2.3585e38 * 1.4427 is below the largest fp32 number 3.4028e38, 2.3587e38 * 1.4427 is above."""
+    for scale in (2.3587e38, 2.5e38, 3e38, 3.4e38):
+        assert attend(lib, cache(), batch(), scale=scale) == -1, scale
+        assert b"scale" in lib.ttmi_last_error()
+    assert attend(lib, cache(), batch(tokens=0), scale=2.3585e38) == 0
+
+
 def test_launches_that_are_too_large_are_refused(lib):
     """Before anything is started: more rows, or more sequences, than a launch has threads for."""
     assert attend(lib, cache(kv_heads=1), batch(tokens=1 << 20), heads=1 << 10, q_pitch=1 << 16, out_pitch=1 << 16) == -1

@@ -6,6 +6,8 @@
 // paged_tiles.hip.  This file cuts the work: keys of a sequence into parts, where there are few rows and heads, whose results a small kernel joins.
 #include "paged_attention.h"
 
+#include <limits>
+
 namespace ttmi {
 namespace {
 
@@ -89,7 +91,8 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
   TTMI_REQUIRE(window >= 0 && max_tokens >= 0 && max_length >= 0, "window, max_tokens and max_length must not be negative");
   // (a launch has less than 2^32 threads: 512 of them for a sequence and key/value head, or 256 for 128 rows besides)
   TTMI_REQUIRE(batch->tokens * heads < 1 << 30 && batch->batch * cache->kv_heads < 1 << 23, "more rows or sequences than one launch takes");
-  TTMI_REQUIRE(scale > 0.f && scale <= 3e38f, "scale must be positive and finite");
+  const float scale_log2e = scale * 1.4426950408889634f;
+  TTMI_REQUIRE(scale > 0.f && scale_log2e <= std::numeric_limits<float>::max(), "scale must be positive, and finite times log2(e)");
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   TTMI_REQUIRE(q != nullptr && out != nullptr, "q or out is null");
   TTMI_REQUIRE(rows_aligned(q, q_pitch, dtype) && rows_aligned(out, out_pitch, dtype), "rows of q and out must be 16-byte aligned");
@@ -100,7 +103,7 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
   a.q = q, a.out = out, a.keys = cache->keys, a.values = cache->values, a.q_pitch = q_pitch, a.out_pitch = out_pitch;
   a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads), a.causal = causal != 0;
   a.window = (int)std::min<int64_t>(window, 1 << 30);  // (beyond every position)
-  a.scale_log2e = scale * 1.4426950408889634f;
+  a.scale_log2e = scale_log2e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.tiles) {
     a.every = !p.few, a.chunk = p.tile_chunk, a.splits = p.tile_splits;
