@@ -317,6 +317,19 @@ def test_workspace_does_not_grow_with_keys_that_a_window_hides(lib, dtype):
     assert sizes[0] == sizes[1] and 0 < sizes[0] <= 300 * 4 * 66 * 4 * 20
 
 
+@pytest.mark.parametrize("dtype", [capi.F32, capi.F16])
+@pytest.mark.parametrize("tokens", [1, 300])
+def test_workspace_of_a_window_that_hides_nothing(lib, dtype, tokens):
+    """However far a window reaches beyond the longest context, to the largest number there is: the same cut (one that needs room)."""
+    sizes = []
+    for window in (1 << 22, 1 << 30, (1 << 31) + 5, (1 << 63) - 1 - tokens, (1 << 63) - 1):
+        n = ctypes.c_int64(-7)
+        assert lib.ttmi_paged_attention_workspace(ctypes.byref(cache(pages=1 << 20)), ctypes.byref(batch(batch=1, tokens=tokens, table_pitch=1 << 12)), 4, tokens, 0,
+                                                  window, dtype, ctypes.byref(n)) == 0
+        sizes.append(n.value)
+    assert len(set(sizes)) == 1 and sizes[0] > 0, sizes
+
+
 def copy(ttmi, sources, destinations, keys=ADDRESS, values=ADDRESS, layers=1, pages=8, page_bytes=64):
     a, b = (np.asarray(x, np.int32) for x in (sources, destinations))
     return ttmi.ttmi_copy_pages(P(keys), P(values), layers, pages, page_bytes, P(a.ctypes.data), P(b.ctypes.data), len(a), None)

@@ -11,6 +11,8 @@
 namespace ttmi {
 namespace {
 
+constexpr int64_t kWidest = 1 << 30;  // windows: no position lies beyond it
+
 struct PagedPlan {
   bool few, tiles;  // which kernels run; one alone takes all sequences
   int few_rows, few_splits, few_waves, tile_chunk, tile_splits;
@@ -38,6 +40,7 @@ constexpr int64_t kWholeBytes = 320 << 10;
 
 PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, int64_t window, int dtype) {
   PagedPlan p;
+  window = std::min(window, kWidest);
   const int64_t group = heads / view.kv_heads, tokens = view.tokens, batch = std::max(1, view.batch);
   const int64_t held = view.table_pitch << view.page_shift;
   const int64_t longest = std::max<int64_t>(1, max_length > 0 ? std::min(max_length, held) : held);
@@ -102,7 +105,7 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
                "the workspace is too small or not 16-byte aligned");
   a.q = q, a.out = out, a.keys = cache->keys, a.values = cache->values, a.q_pitch = q_pitch, a.out_pitch = out_pitch;
   a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads), a.causal = causal != 0;
-  a.window = (int)std::min<int64_t>(window, 1 << 30);  // (beyond every position)
+  a.window = (int)std::min(window, kWidest);
   a.scale_log2e = scale_log2e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.tiles) {
