@@ -269,6 +269,13 @@ def test_bad_caches_and_batches_are_refused(lib, call):
         assert call(lib, cache(), batch(), **changes) == -1, changes
 
 
+@pytest.mark.parametrize("call", [append, attend])
+def test_tables_whose_slots_pass_64_bits_are_refused(lib, call):
+    """table_pitch * page_size of 2^64, 2^63 and 2^52 + 1 times 4096, of which 64 bits hold 0, a negative number and 4096."""
+    for pitch, size in ((1 << 52, 4096), (1 << 51, 4096), ((1 << 52) + 1, 4096), ((1 << 60) + 4, 16), ((1 << 63) - 1, 2)):
+        assert call(lib, cache(page_size=size), batch(table_pitch=pitch)) == -1, (pitch, size)
+
+
 def test_append_refuses(lib):
     for changes in (dict(qkv=None), dict(q=None), dict(inv_freq=None), dict(rotary=63), dict(rotary=66), dict(rotary=-2), dict(qkv_pitch=511), dict(q_pitch=255),
                     dict(q=ADDRESS), dict(qkv=ADDRESS + 1), dict(qkv=ADDRESS + 2, interleaved=1)):

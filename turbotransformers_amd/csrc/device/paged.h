@@ -26,7 +26,7 @@ inline int paged_view(const ttmi_paged_cache* cache, const ttmi_paged_batch* bat
   TTMI_REQUIRE(cache->head_dim >= 16 && cache->head_dim <= 256 && cache->head_dim % 16 == 0, "head_dim must be a multiple of 16 up to 256");
   TTMI_REQUIRE(cache->kv_heads >= 1 && cache->kv_heads <= 65535 && heads >= 1 && heads <= 65535 && heads % cache->kv_heads == 0,
                "heads must be a multiple of kv_heads, at most 65535");
-  TTMI_REQUIRE(cache->pages >= 0 && cache->pages <= kMost && batch->table_pitch >= 0 && batch->table_pitch * cache->page_size <= 1 << 30,
+  TTMI_REQUIRE(cache->pages >= 0 && cache->pages <= kMost && batch->table_pitch >= 0 && batch->table_pitch <= (1 << 30) / cache->page_size,
                "too many pages: positions must not pass 2^30");
   TTMI_REQUIRE(batch->batch >= 0 && batch->batch <= kMost / 2 && batch->tokens >= 0 && batch->tokens <= kMost / 256, "batch is too large");
   if (batch->batch > 0 && batch->tokens > 0) {
