@@ -1,0 +1,70 @@
+"""Attention over pages where scores, values and queries are infinite, not numbers or very large, in every way that the work is cut; and long prompts side by side."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import turbotransformers_amd as tt
+from test_paged_gpu import DTYPES, Case
+
+pytestmark = pytest.mark.gpu
+
+# (new tokens, keys before them in 16-bit types and in fp32, heads, kv_heads, head_dim): which kernel works on the sequences, and which one joins their parts
+WAYS = {
+    "few rows, whole": ([1, 3], [200, 90], [200, 90], 4, 2, 64),
+    "few rows, joined by row": ([1, 3], [5000, 3000], [5000, 3000], 4, 2, 64),
+    "few rows, joined by pair": ([1] * 40, [2500 + 7 * i for i in range(40)], [1500 + 7 * i for i in range(40)], 4, 2, 64),
+    "tiles, whole": ([30, 60], [20, 10], [20, 10], 4, 2, 128),
+    "tiles, two parts": ([20], [492], [108], 48, 12, 64),
+    "tiles, some parts": ([20], [3000], [800], 4, 2, 64),
+    "tiles, many parts": ([20], [9000], [2500], 4, 1, 128),
+}
+
+
+def made(way, dt, **kw):
+    new, past16, past32, heads, kv_heads, d = WAYS[way]
+    return Case(dt, new, past32 if dt == "f32" else past16, heads, kv_heads, d, 16, **kw)
+
+
+def slot(case, b, key):
+    return int(case.table[b, key // case.page]), slice(None), key % case.page
+
+
+def rows_of(case, b):
+    return range(int(case.starts[b]), int(case.starts[b + 1]))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("way", WAYS)
+def test_rows_whose_scores_are_all_minus_infinity(dt, way):
+    """Zero divided by zero is NaN; zeros are for tokens that see no key.  The first element of every key is 1, that of one query minus infinity: its other heads and the
+    other tokens have what they have without it."""
+    case = made(way, dt)
+    case.keys[..., 0] = torch.where(torch.isnan(case.keys[..., 0]), case.keys[..., 0], torch.ones_like(case.keys[..., 0]))
+    clean = case.run_attention()
+    case.check_attention(clean)
+    hit = [(rows_of(case, b)[0], 1) for b in range(len(case.new))] + [(rows_of(case, len(case.new) - 1)[-1], 2)]
+    for row, head in hit:
+        case.q[row, head, 0] = -math.inf
+    got = case.run_attention()
+    for row, head in hit:
+        assert torch.isnan(got[row, head]).all(), (row, head)
+        got[row, head] = clean[row, head]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("way", WAYS)
+def test_keys_of_weight_zero(dt, way):
+    """Scores of minus infinity among others, the first keys' of a sequence among them: the bits of scores so low that their weights are zero."""
+    case = made(way, dt)
+    case.q[..., 0] = 8.0  # times -60000 and a scale of at least 128^-1/2: 2^-60000 and less is 0
+    hit = [(b, key) for b, n in enumerate(case.lengths) for key in [*range(10), n // 2]]
+    for b, key in hit:
+        case.keys[slot(case, b, key)][..., 0] = -60000.0
+    low = case.run_attention()
+    case.check_attention(low)
+    for b, key in hit:
+        case.keys[slot(case, b, key)][..., 0] = -math.inf
+    assert torch.equal(case.run_attention(), low)

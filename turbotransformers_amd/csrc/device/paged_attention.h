@@ -169,10 +169,14 @@ __device__ __forceinline__ u32x2 read_transposed(const void* p) {
 #endif
 }
 
+// What a row's sum is multiplied by in the end.  A row that sees no key has zeros.  Where one does, the sum of its probabilities is at least 1, or 0 if all its scores are
+// minus infinity: then 0 times 1 / 0 makes the NaN that the division of zero by zero is.
+__device__ __forceinline__ float inverse_sum(float sum, bool sees) { return sees ? 1.0f / sum : 0.f; }
+
 // o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over `parts` partial results of a row, the p-th of which is row at(p) of `partial` [.., D] and `ml` [.., 2];
-// 256 threads.
+// sees: whether the row sees a key.  256 threads.
 template <typename T, int D, typename At>
-__device__ __forceinline__ void join_parts(const float* partial, const float* ml, int parts, At at, T* out) {
+__device__ __forceinline__ void join_parts(const float* partial, const float* ml, int parts, bool sees, At at, T* out) {
   constexpr int kWide = 4, kThreads = D / kWide, kShares = 256 / kThreads;  // columns of a thread; threads of a part; parts at a time
   const int d0 = threadIdx.x % kThreads * kWide, share = threadIdx.x / kThreads;
   __shared__ float met[kShares][D + 2];
@@ -205,12 +209,12 @@ __device__ __forceinline__ void join_parts(const float* partial, const float* ml
     l += met[i][D + 1] * weight;
     x += met[i][threadIdx.x] * weight;
   }
-  out[threadIdx.x] = from_float<T>(l != 0.f ? x / l : 0.f);
+  out[threadIdx.x] = from_float<T>(sees ? x / l : 0.f);
 }
 
 // The same for one wavefront and few parts: four columns a lane, the parts shared by the lanes that are left.
 template <typename T, int D, typename At>
-__device__ __forceinline__ void join_parts_by_wavefront(const float* partial, const float* ml, int parts, At at, T* out) {
+__device__ __forceinline__ void join_parts_by_wavefront(const float* partial, const float* ml, int parts, bool sees, At at, T* out) {
   constexpr int kThreads = D / 4, kShares = kWave / kThreads;
   const int lane = (int)(threadIdx.x % kWave), d0 = lane % kThreads * 4, share = lane / kThreads;
   float best = -INFINITY;
@@ -233,7 +237,7 @@ __device__ __forceinline__ void join_parts_by_wavefront(const float* partial, co
     for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], d, kWave);
   }
   if (share != 0) return;
-  const float inv = total != 0.f ? 1.0f / total : 0.f;
+  const float inv = inverse_sum(total, sees);
   Vec<T, 4> x;
 #pragma unroll
   for (int c = 0; c < 4; ++c) x.v[c] = from_float<T>(sum[c] * inv);

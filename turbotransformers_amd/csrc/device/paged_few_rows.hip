@@ -388,7 +388,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
           }
           if (complete) {
             const int t = (row0 + r) / a.group, h = kv_head * a.group + row0 + r - t * a.group;
-            const float inv = total != 0.f ? 1.0f / total : 0.f;
+            const float inv = inverse_sum(total, seq.reach(a, t).end > 0);
             T* to = static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D + d0;
             Vec<T, kWide> x;
   #pragma unroll
@@ -428,6 +428,7 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a) {
   if (first == last) return;
   const int parts = (int)(last - first) + 1;
   const float* const ml = a.partial + 2 * (int64_t)a.splits * kFewRows * D;
+  auto sees = [&](int r) { return seq.reach(a, r / a.group).end > 0; };
   auto place = [&](int r) {
     const int t = r / a.group, h = kv_head * a.group + r - t * a.group;
     return static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D;
@@ -435,12 +436,12 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a) {
   if (gridDim.y == 1 && parts <= kManyParts) {
     for (int r = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < rows; r += 4)
       join_parts_by_wavefront<T, D>(
-          a.partial, ml, parts, [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
+          a.partial, ml, parts, sees(r), [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
     return;
   }
   for (int r = blockIdx.y; r < rows; r += gridDim.y) {
     join_parts<T, D>(
-        a.partial, ml, parts, [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
+        a.partial, ml, parts, sees(r), [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
     __syncthreads();
   }
 }

@@ -49,12 +49,12 @@ __device__ __forceinline__ int value_piece(int row, int piece) {
 
 // A row's sums over one part of its keys: divided and stored, or, where its keys lie in several parts, kept for the kernel that joins those.
 template <typename T, int D>
-__device__ __forceinline__ void store_rows(const PagedArgs& a, const Sequence& seq, int token, int head, int part, int part0, int part1, int lhalf,
+__device__ __forceinline__ void store_rows(const PagedArgs& a, const Sequence& seq, int token, int head, int part, int part0, int part1, bool sees, int lhalf,
                                            const floatx16 (&ot)[D / 32], float top, float sum) {
   const int64_t at_token = seq.start + token;
   if (part0 == part1) {
     if (part != part0) return;
-    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+    const float inv = inverse_sum(sum, sees);
     T* to = static_cast<T*>(a.out) + at_token * a.out_pitch + (int64_t)head * D + 4 * lhalf;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   }
   if (!live) return;
   const bool sees = mine.end > 0;
-  store_rows<T, D>(a, seq, token, head, part, sees ? mine.begin / chunk : part0, sees ? (mine.end - 1) / chunk : part0, lhalf, ot, top, sum);
+  store_rows<T, D>(a, seq, token, head, part, sees ? mine.begin / chunk : part0, sees ? (mine.end - 1) / chunk : part0, sees, lhalf, ot, top, sum);
 }
 
 // Rows whose keys lay in several parts.  What their bytes take is little; what counts is how many trips to memory follow one another: the sequence, its length, the parts.  So
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(const PagedArgs a) {
     const int h = blockIdx.y;
     const int64_t at = ((int64_t)row * a.heads + h) * a.splits;
     join_parts<T, D>(
-        a.partial, met, parts, [&](int p) { return at + (part0 + p) % a.splits; }, static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D);
+        a.partial, met, parts, true, [&](int p) { return at + (part0 + p) % a.splits; }, static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)h * D);
   } else {
     constexpr int kThreads = D / 4;
     const int h = blockIdx.y * (256 / kThreads) + threadIdx.x / kThreads, d0 = threadIdx.x % kThreads * 4;
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(const PagedArgs a) {
         total += ml[p][1] * weight;
         sum += x[p] * weight;
       }
-    const float inv = total != 0.f ? 1.0f / total : 0.f;
+    const float inv = inverse_sum(total, true);  // (a row of several parts sees keys)
     Vec<T, 4> y;
 #pragma unroll
     for (int c = 0; c < 4; ++c) y.v[c] = from_float<T>(sum[c] * inv);

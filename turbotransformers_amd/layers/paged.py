@@ -59,7 +59,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
                     lengths: torch.Tensor, max_tokens: int = 0, max_length: int = 0, scale: Optional[float] = None, causal: bool = True,
                     window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(scale * q k^T) v of the new tokens over their sequences' keys: up to a token's own position if causal, all of them otherwise;
-    window > 0: only the last `window` up to its own.  A token that sees no key gets zeros.
+    window > 0: only the last `window` up to its own.  A token that sees no key gets zeros; where it sees some, all with a score of minus
+    infinity, NaN, as zero divided by zero is.
 
     q: [tokens, heads * head_dim] or [tokens, heads, head_dim], head_dim 64 or 128; rows may lie any distance apart.  heads is a multiple of
     kv_heads: query head h reads key/value head h // (heads // kv_heads).  scale: positive, 1 / sqrt(head_dim) by default.
