@@ -613,8 +613,11 @@ TTMI_API int ttmi_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out,
 /* Attention of the new tokens over their sequences' pages:
  *   out[t, h, :] = sum_j p_j v_j, p = softmax over the keys j that token t sees of scale * q[t, h, :] . k_j
  * `causal`: keys up to the token's own position, else all keys of its sequence; window > 0: of these only positions from its own - window + 1 on.
- * A token that sees no key gets zeros, one all of whose scores are minus infinity NaN.  q and out [tokens, heads, 64 or 128], rows q_pitch and out_pitch elements apart (a multiple of 16
- * bytes); out must not overlap anything else; heads is a multiple of kv_heads, query head h reads key/value head h / (heads / kv_heads).
+ * A token that sees no key gets zeros, one all of whose scores are minus infinity NaN, one that sees an infinite value or a NaN an infinity or a NaN.
+ * Scores, sums and statistics are held in fp32; in 16-bit types the probabilities are rounded to the type for their product with the values, and what
+ * they are divided by is the sum of the rounded ones.  The sum of |v| over the keys that a token sees must stay below 2^120 (as it does in fp16).
+ * q and out [tokens, heads, 64 or 128], rows q_pitch and out_pitch elements apart (a multiple of 16 bytes); out must not overlap anything else;
+ * heads is a multiple of kv_heads, query head h reads key/value head h / (heads / kv_heads).
  * scale is positive, scale * log2(e) finite.  tokens * heads is less than 2^30, batch * kv_heads less than 2^23.
  * max_tokens, max_length: the most new tokens and keys that a sequence has, or 0 if unknown.  They only choose how the work is cut; a
  * call whose sequences have more is computed all the same.

@@ -1,7 +1,6 @@
 """Attention over pages where scores, values and queries are infinite, not numbers or very large, in every way that the work is cut; and long prompts side by side."""
 import math
 
-import numpy as np
 import pytest
 import torch
 
@@ -68,3 +67,22 @@ def test_keys_of_weight_zero(dt, way):
     for b, key in hit:
         case.keys[slot(case, b, key)][..., 0] = -math.inf
     assert torch.equal(case.run_attention(), low)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("way", WAYS)
+def test_the_largest_values(dt, way):
+    """Values of one sign whose sum over a token's keys is just below 2^120, where every weight but the first tile's is 2^7.9 before the division: no sum leaves fp32, and
+    the mean of equal values is that value."""
+    case = made(way, dt)
+    case.q.zero_()
+    case.q[..., 0] = 8.0
+    kept = torch.isnan(case.keys)
+    case.keys.zero_()
+    for b, n in enumerate(case.lengths):
+        for key in range(16, n):
+            case.keys[slot(case, b, key)][..., 0] = 7.9 * math.log(2) * math.sqrt(case.d) / 8
+    case.keys[kept] = math.nan
+    value = 2.0 ** (119 - math.ceil(math.log2(max(case.lengths)))) * 1.875
+    case.values = torch.where(torch.isnan(case.values), case.values, torch.full_like(case.values, value))
+    case.check_attention(case.run_attention())

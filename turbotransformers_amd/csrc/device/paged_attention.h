@@ -137,7 +137,8 @@ __device__ __forceinline__ u32x4 finite_part(u32x4 x) {
 // a number that was loaded as bits, and what adds one does it where the compiler does not look: it takes a test of a float for a test of infinity alone.
 template <typename T>
 using Bits = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
-// sum += *at where that is an infinity or a NaN
+// sum += *at where that is an infinity or a NaN.  (Where its weight rounds to zero the matrix instruction, in tiles that all rows see, makes a NaN of an infinity: it multiplies.  Which of the
+// two a token gets that sees one is not promised.)
 template <typename T>
 __device__ __forceinline__ void add_wild(float& sum, const T* at) {
   typedef Bits<T> __attribute__((may_alias)) Loaded;
@@ -154,8 +155,9 @@ __device__ __forceinline__ void add_wild(float& sum, const T* at) {
 #endif
 }
 // The reference point of a row's probabilities, in units of scale log2(e) score, a whole number: it moves only where a score lies more than this above it, so the sums are
-// seldom scaled, and then by powers of two.  Probabilities of up to 2^8 lose nothing: they are as exact in their type as those up to 1, and the division by their sum takes the factor back out.  (The
-// decision is the row's own: what is in the tile with it moves no bit of it.)
+// seldom scaled, and then by powers of two.  Probabilities of up to 2^8 lose no places: they are as exact in their type as those up to 1, and the division by their sum takes the factor back out.  What
+// they cost is range: the sums before the division are at most 2^8 times the sum of |v| over the row's keys, which has to stay below 2^120 (fp16 values are far from that).  (The decision is the
+// row's own: what is in the tile with it moves no bit of it.)
 constexpr float kSlack = 8.f;
 __device__ __forceinline__ float moved_reference(float top, float highest) { return highest > top + kSlack || top == -INFINITY ? fmaxf(__builtin_floorf(highest), top) : top; }
 

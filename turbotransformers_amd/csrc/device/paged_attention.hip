@@ -1,6 +1,7 @@
 // Attention of new tokens over keys and values in pages: o = sum_j p_j v_j with p = softmax_j(scale q . k_j) over the keys that a token sees.
 // One pass over the keys: with the maximum m and the sum l of exp(s_j - m) so far, a tile of new scores moves m to m', scales what was summed by
-// exp(m - m') and adds its own exp(s_j - m') and exp(s_j - m') v_j.  All of it in fp32; exp(x) as 2^(x log2 e).
+// exp(m - m') and adds its own exp(s_j - m') and exp(s_j - m') v_j.  Scores, m, l and the sums in fp32; exp(x) as 2^(x log2 e).  In 16-bit types the probabilities are rounded to the type for the second product,
+// which the matrix instructions take no wider, and l sums the rounded ones.
 //
 // Two kernels share a batch by the rows (new tokens times query heads of a key/value head) of its sequences: up to 16 of them paged_few_rows.hip, more
 // paged_tiles.hip.  This file cuts the work: keys of a sequence into parts, where there are few rows and heads, whose results a small kernel joins.

@@ -336,7 +336,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
           }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (wild) {  // an infinity or a NaN is what a sum with it is, whatever its weight
+        if (wild) {  // a sum with an infinity or a NaN is one or the other
   #pragma unroll 1
           for (int k = key; k < min(key + S::kKeys, hi); ++k) {
             const T* v = values + row_offset<D>(view, cursor, kv_head, k) + 4 * quarter;

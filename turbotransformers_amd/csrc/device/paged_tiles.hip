@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (__builtin_expect(partly_seen(key), 0) && wild) {  // an infinity or a NaN is what a sum with it is, whatever its weight
+      if (__builtin_expect(partly_seen(key), 0) && wild) {  // a sum with an infinity or a NaN is one or the other
 #pragma unroll 1
         for (int k = key; k < min(key + S::kKeys, hi); ++k) {
           const T* v = values + row_offset<D>(view, cursor, kv_head, k) + 4 * lhalf;

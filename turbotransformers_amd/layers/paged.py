@@ -60,7 +60,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
                     window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(scale * q k^T) v of the new tokens over their sequences' keys: up to a token's own position if causal, all of them otherwise;
     window > 0: only the last `window` up to its own.  A token that sees no key gets zeros; where it sees some, all with a score of minus
-    infinity, NaN, as zero divided by zero is.
+    infinity, NaN, as zero divided by zero is.  Sums and statistics are held in 32 bits; in 16-bit types the probabilities are rounded to the type for
+    their product with v (and divided by the sum of the rounded ones).  The sum of |v| over a token's keys has to stay below 2^120.
 
     q: [tokens, heads * head_dim] or [tokens, heads, head_dim], head_dim 64 or 128; rows may lie any distance apart.  heads is a multiple of
     kv_heads: query head h reads key/value head h // (heads // kv_heads).  scale: positive, 1 / sqrt(head_dim) by default.
