@@ -86,3 +86,77 @@ def test_the_largest_values(dt, way):
     value = 2.0 ** (119 - math.ceil(math.log2(max(case.lengths)))) * 1.875
     case.values = torch.where(torch.isnan(case.values), case.values, torch.full_like(case.values, value))
     case.check_attention(case.run_attention())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("way", WAYS)
+def test_what_is_not_finite_stays_with_the_rows_that_see_it(dt, bad, way):
+    """A value of the last key/value head, at the first key, in the middle, at the first new token and at the last: NaN (or an infinity) in its column for the tokens that
+    see it, the same bits as without it everywhere else.  A query's element: NaN in its own row and head."""
+    case = made(way, dt)
+    clean = case.run_attention()
+    case.check_attention(clean)
+    kept, group = case.values.clone(), case.heads // case.kv_heads
+    for where in (lambda n, m: 0, lambda n, m: (n - m) // 2, lambda n, m: n - m, lambda n, m: n - 1):
+        case.values.copy_(kept)
+        spoiled = torch.zeros(case.q.shape, dtype=torch.bool)
+        for b, (n, m) in enumerate(zip(case.lengths, case.new)):
+            key = where(n, m)
+            case.values[slot(case, b, key)][-1, 7] = bad
+            for row in rows_of(case, b):
+                spoiled[row, case.heads - group:, 7] = n - m + row - rows_of(case, b)[0] >= key
+        got = case.run_attention().cpu()
+        assert torch.equal(torch.isnan(got) if math.isnan(bad) else ~torch.isfinite(got), spoiled)
+        assert torch.equal(got[~spoiled], clean.cpu()[~spoiled])
+    case.values.copy_(kept)
+    spoiled = torch.zeros(case.q.shape, dtype=torch.bool)
+    for b in range(len(case.new)):
+        case.q[rows_of(case, b)[-1], 1, 5] = bad
+        spoiled[rows_of(case, b)[-1], 1] = True
+    got = case.run_attention().cpu()
+    assert torch.equal(torch.isnan(got), spoiled)
+    assert torch.equal(got[~spoiled], clean.cpu()[~spoiled])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+@pytest.mark.parametrize("way", WAYS)
+def test_an_infinite_value_behind_a_weight_of_zero(dt, bad, way):
+    """Its key has a score so low that its weight is zero: an infinity or NaN for those who see it (which one is not said), in its column alone."""
+    case = made(way, dt)
+    case.q[..., 0] = 8.0
+    for b, n in enumerate(case.lengths):
+        case.keys[slot(case, b, 3)][..., 0] = -60000.0
+    clean = case.run_attention().cpu()
+    for b in range(len(case.new)):
+        case.values[slot(case, b, 3)][0, 9] = bad
+    spoiled = torch.zeros(case.q.shape, dtype=torch.bool)
+    spoiled[:, :case.heads // case.kv_heads, 9] = True
+    got = case.run_attention().cpu()
+    assert torch.equal(~torch.isfinite(got), spoiled)
+    assert torch.equal(got[~spoiled], clean[~spoiled])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("window", [0, 400])
+def test_prompts_of_many_blocks_side_by_side(dt, window):
+    """More workgroups than the chip takes at a time: they begin with the sequences of most keys, in these with the last rows; single tokens among them."""
+    case = Case(dt, [300, 1, 1500, 700, 1, 1100, 513], [0, 90, 7, 200, 0, 0, 33], 24, 12, 64, 16, spare_rows=1)
+    case.check_attention(case.run_attention(window=window), window=window)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_a_sequence_alone_and_among_others(dt):
+    """How the work is cut depends on the whole batch, so bits may differ; both are within the tolerance of the formula."""
+    case = Case(dt, [1, 40, 1, 300, 7], [3000, 100, 17, 0, 900], 8, 2, 128, 16)
+    together = case.run_attention()
+    want, tol = case.attention()
+    keys, values, (table, _, lengths) = case.keys.cuda(), case.values.cuda(), case.device_args()
+    for b, n in enumerate(case.new):
+        rows = slice(int(case.starts[b]), int(case.starts[b + 1]))
+        alone = tt.paged_attention(case.q[rows].cuda(), keys, values, table[b:b + 1], torch.tensor([0, n], dtype=torch.int32, device="cuda"), lengths[b:b + 1],
+                                   max_tokens=n, max_length=case.lengths[b])
+        for got in (alone, together[rows]):
+            assert ((got.cpu().double() - want[rows]).abs() <= tol[rows]).all(), b
+    tt.cxx.synchronize()
