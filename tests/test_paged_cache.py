@@ -337,6 +337,23 @@ def test_workspace_of_a_window_that_hides_nothing(lib, dtype, tokens):
     assert len(set(sizes)) == 1 and sizes[0] > 0, sizes
 
 
+@pytest.mark.parametrize("dtype", [capi.F32, capi.F16, capi.BF16])
+def test_long_contexts_beside_a_prompt_are_shared_out(lib, dtype):
+    """Single tokens over 100000 keys and a prompt that fills the chip by itself: room for the parts that their keys are cut into.  The prompt alone, prompts of one
+    length and short contexts beside a prompt need none."""
+    def room(sequences, tokens, most, longest):
+        n = ctypes.c_int64(-7)
+        assert lib.ttmi_paged_attention_workspace(ctypes.byref(cache(pages=1 << 20, kv_heads=8, head_dim=128)),
+                                                  ctypes.byref(batch(batch=sequences, tokens=tokens, table_pitch=1 << 14)), 32, most, longest, 0, dtype,
+                                                  ctypes.byref(n)) == 0
+        return n.value
+    assert room(9, 4104, 4096, 100000) > 0
+    assert room(2, 4097, 4096, 100000) > 0
+    assert room(1, 4096, 4096, 100000) == 0
+    assert room(3, 12288, 4096, 100000) == 0
+    assert room(9, 4104, 4096, 1000) == 0
+
+
 def copy(ttmi, sources, destinations, keys=ADDRESS, values=ADDRESS, layers=1, pages=8, page_bytes=64):
     a, b = (np.asarray(x, np.int32) for x in (sources, destinations))
     return ttmi.ttmi_copy_pages(P(keys), P(values), layers, pages, page_bytes, P(a.ctypes.data), P(b.ctypes.data), len(a), None)

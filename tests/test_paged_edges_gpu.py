@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import turbotransformers_amd as tt
-from test_paged_gpu import DTYPES, Case
+from test_paged_gpu import DTYPES, Case, check
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +160,10 @@ def test_a_sequence_alone_and_among_others(dt):
         for got in (alone, together[rows]):
             assert ((got.cpu().double() - want[rows]).abs() <= tol[rows]).all(), b
     tt.cxx.synchronize()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("window", [0, 6000])
+def test_long_contexts_beside_prompts(dt, window):
+    """Few tokens over thousands of keys, cut and joined, in one call with a prompt and a chunk behind many keys; sequences without new tokens among them."""
+    check(dt, [1, 700, 3, 0, 90], [9000, 0, 5000, 70, 3000], 8, 2, 64, 16, window=window, spare_rows=1)

@@ -48,9 +48,19 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   const int64_t most = max_tokens > 0 ? std::min(max_tokens, tokens) : tokens;
   const int64_t reach = window > 0 ? std::min(longest, window + most) : longest;
   p.tiles = most * group > kFewRows;
-  // One launch instead of two where sequences have many rows on average: the kernel for many rows takes those with few as well.  us, 40 sequences decoding and 3 chunks of
-  // 200 to 900 tokens (143 rows on average): two kernels 41.3, one 29.3.
-  p.few = !p.tiles || tokens * group / batch < 64;
+  // One launch instead of two where sequences have many rows on average and none of them many keys: the kernel for many rows takes those with few as well.  Where one may have more than
+  // 64 of its tiles, a workgroup would walk over them with a row or four of 128 alive, and sequences with few rows keep a kernel that cuts their keys, if there can be
+  // any (the tokens would make so many sequences of the most only).
+  // us, one launch / two, one key length for all decoding sequences (1000, 4000, 8000, 16000, 100000), chunks without keys before them:
+  //   bf16, 32 and 8 heads of 128: 1 decoding, a chunk of 512     26.5 / 31.6,    43.2 / 36.0,   66.4 / 38.6,  115 / 46,   640 / 110
+  //                                8, one of 2048                 63.1 / 77.8,    93.2 / 88.1,    166 / 108,   315 / 165, 1893 / 619
+  //                                40, 3 of 500                   51.7 / 63.8,     139 / 160,     256 / 266,   495 / 492
+  //   fp16, 16 and 4 heads of 64:  8, one of 2048                 36.3 / 45.9,    57.2 / 48.7,    105 / 53,    203 / 63,  1252 / 187
+  //   fp32, 12 heads of 64:        8, one of 2048                  155 / 173,      309 / 193,     595 / 234,  1166 / 301, 7117 / 973  (2000: 168 / 180)
+  // Sequences that all have many rows pay the launches of the other kernel: 6 chunks of 400 to 600 tokens behind up to 9000 keys 220 / 224.
+  const int64_t long_walk = 64 * (dtype == TTMI_F32 ? 32 : 64);
+  const bool some_few = most * batch > tokens;
+  p.few = !p.tiles || tokens * group / batch < 64 || (reach > long_walk && some_few);
   p.few_rows = p.tiles ? kFewRows : (int)(most * group);
   p.few_splits = reach * 2 * view.head_dim * (int64_t)dtype_size(dtype) <= kWholeBytes ? 0 : 2 * compute_units();
   p.few_waves = p.few_splits == 0 && batch * view.kv_heads < compute_units() ? 8 : 4;
