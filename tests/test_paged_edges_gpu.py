@@ -13,7 +13,8 @@ pytestmark = pytest.mark.gpu
 WAYS = {
     "few rows, whole": ([1, 3], [200, 90], [200, 90], 4, 2, 64),
     "few rows, joined by row": ([1, 3], [5000, 3000], [5000, 3000], 4, 2, 64),
-    "few rows, joined by pair": ([1] * 40, [2500 + 7 * i for i in range(40)], [1500 + 7 * i for i in range(40)], 4, 2, 64),
+    "few rows of many, joined by row": ([1] * 40, [2500 + 7 * i for i in range(40)], [1500 + 7 * i for i in range(40)], 4, 2, 64),
+    "few rows, joined by pair": ([1] * 64, [1500, 1700] + [100 + i for i in range(62)], [1500, 1700] + [100 + i for i in range(62)], 16, 8, 64),
     "tiles, whole": ([30, 60], [20, 10], [20, 10], 4, 2, 128),
     "tiles, two parts": ([20], [492], [108], 48, 12, 64),
     "tiles, some parts": ([20], [3000], [800], 4, 2, 64),

@@ -34,8 +34,9 @@ void cut(int64_t units, int64_t least, int64_t reach, bool window, int* chunk, i
   *chunk = (int)size;
 }
 
-// Few rows: up to so many bytes of keys and values of one sequence and head are one workgroup's.  A CU fetches about 50 GB/s, so these take 6 us, what sharing them out
-// and joining the parts costs besides their share.  us a call, one workgroup / shared: bf16, head_dim 128, 8 sequences of 255 keys (130 KB) 7.2 / 12.4, 500 10.6 / 13.5,
+// Few rows: up to so many bytes of keys and values of one sequence and head are one workgroup's.  A CU fetches about 50 GB/s while few others read, so these take 6 us, what sharing them out
+// and joining the parts costs besides their share.  Where the pairs fill the chip it is the launch to join that counts: 256 sequences of 620 keys, 8 key heads of 128, 115 / 126, 64 of 1 to 600 keys
+// 18.0 / 24.7.  us a call, one workgroup / shared: bf16, head_dim 128, 8 sequences of 255 keys (130 KB) 7.2 / 12.4, 500 10.6 / 13.5,
 // 1000 (512 KB) 15.6 / 15.9, 2000 25.2 / 22.6, 1 sequence of 1000 14.8 / 12.6; fp16, head_dim 64, 12 heads, 1 sequence of 1000 (256 KB) 9.7 / 12.1, 2000 14.4 / 12.1.
 constexpr int64_t kWholeBytes = 320 << 10;
 
@@ -48,7 +49,8 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   const int64_t most = max_tokens > 0 ? std::min(max_tokens, tokens) : tokens;
   const int64_t reach = window > 0 ? std::min(longest, window + most) : longest;
   p.tiles = most * group > kFewRows;
-  // One launch instead of two where sequences have many rows on average and none of them many keys: the kernel for many rows takes those with few as well.  Where one may have more than
+  // One launch instead of two where sequences have many rows on average and none of them many keys: the kernel for many rows takes those with few as well (40 sequences decoding and 3
+  // chunks of 200 to 900 tokens, 1000 keys seen: two launches 38.0 us, one 25.6).  Where one may have more than
   // 64 of its tiles, a workgroup would walk over them with a row or four of 128 alive, and sequences with few rows keep a kernel that cuts their keys, if there can be
   // any (the tokens would make so many sequences of the most only).
   // us, one launch / two, one key length for all decoding sequences (1000, 4000, 8000, 16000, 100000), chunks without keys before them:

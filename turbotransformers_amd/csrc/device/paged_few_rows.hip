@@ -1,14 +1,16 @@
 // Attention over pages where a sequence has few rows (new tokens times query heads of a key/value head): decoding.
 //
-// What it has to read, every key and value once, bounds it.  A workgroup has up to 16 rows of one sequence and head and a part of the keys; its four wavefronts
-// take every fourth tile of it, each with a running maximum, sum and output of its own, without a barrier until they meet at the end.  Scores are computed transposed,
+// What it has to read, every key and value once, bounds it.  A workgroup has up to 16 rows of one sequence and head and a part of the keys; its NW wavefronts (four,
+// or eight where a launch leaves CUs without a workgroup) take its tiles in turn, each with a running maximum, sum and output of its own, without a barrier until they meet at the end.  Scores are
+// computed transposed,
 //     St[key, row] = K[key, :] . Q[row, :]        v_mfma_f32_16x16x32 (fp32: 16x16x4), K as it comes from memory, a 16-byte piece of a row a lane,
 // so a lane has one row and four keys of each 16: the statistics need one exchange over the four quarters of the wavefront, and the probabilities lie as the
 // second operand of
 //     Ot[d, row] += Vt[d, keys] . Pt[keys, row]
 // wants them: its order of keys is ours to choose.  Vt is what the transposing reads give of a tile that lies in LDS row by row as it came (fp32: plain reads of a
 // column).  Tiles are fetched into registers one ahead: 8 KB of keys and as many of values per wavefront are on their way while one is worked on; what a CU has on its way is
-// what it gets (about 50 GB/s whatever runs on the others), so the loads are never behind a condition, which would make the compiler wait for all of them.
+// what it gets (about 50 GB/s while the others leave the memory room for that; 20 where all 256 read, which is its 5 TB/s), so the loads are never behind a condition, which would make
+// the compiler wait for all of them.
 //
 // Measured, 32 query and 8 key heads of 128: 64 sequences of 100 to 6000 keys, bf16, 85 us and 6 to join the parts (5.1 TB/s while it reads; a large copy here 4.8);
 // 4 sequences of 60000 to 131071 keys, fp16, 264 and 7 (6.0 TB/s, part of it out of the last-level cache).  One sequence of 387 keys, 12 heads of 64, fp16: 6.7, of which
@@ -142,7 +144,8 @@ __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t 
   p.kv_head = rest / p.rounds, p.round = rest - p.kv_head * p.rounds;
   return p;
 }
-// Workgroups that share the work.  At least kFewest rounds each, so that a wavefront has more than its first tile's wait.
+// Workgroups that share the work.  At least kFewest rounds each, so that a wavefront has more than its first tile's wait.  us, 1 / 2 / 4 of them, 8 key heads of 128: 1 sequence
+// of 1500 keys 11.6 / 12.5 / 15.6, of 8000 16.4 / 14.1 / 15.6, 8 of 1000 19.0 / 16.7 / 17.7, 8 of 2000 21.2 / 21.4 / 25.8.
 constexpr int kFewest = 2;
 __device__ __forceinline__ int64_t sharers(const PagedArgs& a, int64_t units) { return max((int64_t)1, min((int64_t)a.splits, (units + kFewest - 1) / kFewest)); }
 
@@ -409,10 +412,12 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
 }
 
 // Pairs that were several workgroups': their rows' partial results are joined, in 5 to 7 us, nearly all of them the launch and three trips to memory.  A workgroup per pair and row, or per pair where there are many of them: then a wavefront
-// takes a row, unless the pair had many parts.
-constexpr int kManyPairs = 64, kManyParts = 16;
+// takes a row.
+// us, a workgroup per row / per pair, 32 query and 8 key heads of 128: 1 sequence of 3000 keys 12.8 / 14.2, 8 (64 pairs) 24.9 / 25.4, 64 of 1500 (512) 75.4 / 73.8, 200 (1600)
+// 241 / 228; 16 query heads of one key head, one sequence of 100000 keys beside 63 of 500, whose pair has most of the parts, 45.7 / 145.
+constexpr int kManyPairs = 512;
 template <typename T, int D>
-__global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a, bool by_pair) {
   const PagedView& view = a.view;
   const int kv_head = blockIdx.x % view.kv_heads, b = blockIdx.x / view.kv_heads;
   const Sequence seq = sequence(a, b);
@@ -433,27 +438,26 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a) {
     const int t = r / a.group, h = kv_head * a.group + r - t * a.group;
     return static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D;
   };
-  if (gridDim.y == 1 && parts <= kManyParts) {
+  if (by_pair) {
     for (int r = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < rows; r += 4)
       join_parts_by_wavefront<T, D>(
           a.partial, ml, parts, sees(r), [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
     return;
   }
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    join_parts<T, D>(
-        a.partial, ml, parts, sees(r), [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
-    __syncthreads();
-  }
+  const int r = blockIdx.y;
+  join_parts<T, D>(
+      a.partial, ml, parts, sees(r), [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
 }
 
 }  // namespace
 
 int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream) {
   const unsigned pairs = (unsigned)((int64_t)a.view.batch * a.view.kv_heads);
+  const bool by_pair = pairs >= kManyPairs;
   TTMI_DISPATCH_FLOAT(dtype, T, {
     auto launch = [&](auto kernel, auto join) {
       hipLaunchKernelGGL(kernel, dim3(a.splits > 0 ? (unsigned)a.splits : pairs), dim3(a.waves * 64), 0, stream, a);
-      if (a.splits > 0) hipLaunchKernelGGL(join, dim3(pairs, pairs >= kManyPairs ? 1u : (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0, stream, a);
+      if (a.splits > 0) hipLaunchKernelGGL(join, dim3(pairs, by_pair ? 1u : (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0, stream, a, by_pair);
     };
     const bool small = a.view.page_shift < 4;
     auto sized = [&](auto d) {
