@@ -124,7 +124,7 @@ static void launch_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out
 // ---- pages copied to pages ----------------------------------------------------------------------------------------------
 // The list goes along with the launch: nothing is copied to the device, and a recorded call keeps its own.  A page goes through the registers of ceil(bytes / 16 KB) workgroups,
 // four pieces of 16 bytes a lane on their way: 901 pages of 64 KB in keys and values of 24 layers 1124 us, 5.05 TB/s (a large copy here 4.8); 4 pages of 24 KB in 12 layers 3.3.
-constexpr int kCopyPairs = 448, kCopyFew = 16;  // what fits the arguments of a launch (4 KB); a short list, whose launch is shorter: a call for 4 pairs 4.85 / 4.4 us
+constexpr int kCopyPairs = 448, kCopyFew = 16;  // what fits the arguments of a launch (4 KB); a short list, whose launch is shorter: a call for 1, 4, 16 pairs 5.3 / 4.1, 5.3 / 4.7, 5.5 / 5.1 us
 constexpr int kCopyBytes = 16384;  // of a workgroup
 template <int N>
 struct PagePairs {

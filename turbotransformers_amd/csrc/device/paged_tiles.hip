@@ -7,9 +7,12 @@
 // row by row as in the cache (fp32: plain reads of a column).  Packing a group's heads into one tile of rows reads the keys of a head once for all of them and keeps
 // tiles full whatever the group.
 //
-// Measured, 32 query and 8 key heads of 128, bf16: a prompt of 8192 tokens 580 to 620 us (0.89 to 0.94 PFLOP/s; a large product here 1.26), a multiplication by zeros 530 to 565:
-// the chip is at its power limit.  Heads of 64: 343 us (0.80), where an exponential takes a lane as long as its share of the products.  A workgroup by itself takes about 7 us to
+// Measured, 32 query and 8 key heads of 128, bf16: a prompt of 8192 tokens 580 to 620 us (0.89 to 0.94 PFLOP/s; a large product here 1.26).  Of a SIMD's 1.19e6 cycles
+// the matrix pipe is busy for 0.53e6 and vector instructions, the exponentials first, are at work for as many: the two hardly overlap.  Power comes second: on zeros the same launch takes 530 to 565 us.
+// Heads of 64: 343 us (0.80), where an exponential takes a lane as long as its share of the products.  A workgroup by itself takes about 7 us to
 // its first tile and 0.95 a tile of 64 keys, heads of 64, where four instructions' worth of products would be 0.2: a chain of reads, products, maximum, exponentials, products.
+// The last blocks of a launch run on few CUs: 6 chunks of 400 to 600 tokens behind up to 9000 keys 220 us (0.85 PFLOP/s), 93 tiles for each of 512 places, 125 in the longest block.
+// fp32 with heads of 128 has no registers left (256 and 96 bytes of scratch a lane): a prompt of 1000 tokens 153 us.
 // What was built and taken out: 256 rows a workgroup with the products of 32 keys beside the exponentials of the 32 before, level to 3 % faster for heads of 128, 2 % slower for those of 64.
 #include "paged_attention.h"
 

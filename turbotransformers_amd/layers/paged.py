@@ -63,8 +63,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     infinity, NaN, as zero divided by zero is.  Sums and statistics are held in 32 bits; in 16-bit types the probabilities are rounded to the type for
     their product with v (and divided by the sum of the rounded ones).  The sum of |v| over a token's keys has to stay below 2^120.
 
-    q: [tokens, heads * head_dim] or [tokens, heads, head_dim], head_dim 64 or 128; rows may lie any distance apart.  heads is a multiple of
-    kv_heads: query head h reads key/value head h // (heads // kv_heads).  scale: positive, 1 / sqrt(head_dim) by default.
+    q: [tokens, heads * head_dim] or [tokens, heads, head_dim], head_dim 64 or 128; rows may lie any multiple of 16 bytes apart.  heads is a
+    multiple of kv_heads: query head h reads key/value head h // (heads // kv_heads).  scale: positive, 1 / sqrt(head_dim) by default.
     max_tokens, max_length: the most new tokens and keys of a sequence, where known: they choose how the work is cut, not what is computed.
     -> like q: `out` if given."""
     if out is None:
@@ -122,7 +122,7 @@ class PagedCache:
         b = cache.fork(a)                                 # shares a's pages; a page that both would write is copied by extend()
         cache.free(a)
 
-    `pool` is the book itself (cxx.PagePool).  Pages that are freed may be handed out by the next `extend`; work of earlier steps that still reads
+    `attend` reads heads of 64 or 128; the rest takes any multiple of 16 up to 256.  `pool` is the book itself (cxx.PagePool).  Pages that are freed may be handed out by the next `extend`; work of earlier steps that still reads
     them has to be on the same stream."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page_size: int = 16, dtype: torch.dtype = torch.float16, device=None):
