@@ -1,0 +1,677 @@
+"""Norms of heads in the append, attention with windows and first tokens that stay visible, and families of sequences that share their first pages, against the
+formulas in 64 bits."""
+import ctypes
+import math
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import turbotransformers_amd as tt
+from helpers import TORCH_DTYPES
+from test_paged_gpu import DTYPES, E32, EPS, Case, turned
+from turbotransformers_amd import capi
+
+pytestmark = pytest.mark.gpu
+
+
+class Sight(Case):
+    """A batch with families.  families: (sequences, keys they have in common) in order; the common keys' full pages are the first one's, and what would have been the
+    others' pages holds NaN."""
+
+    def __init__(self, dt, new, past, heads, kv_heads, d, page, families=(), **kw):
+        super().__init__(dt, new, past, heads, kv_heads, d, page, **kw)
+        self.rows = np.array([[b, b + 1, 0] for b in range(len(new))], np.int32).reshape(-1, 3)
+        first = 0
+        for members, keys in families:
+            self.share(first, first + members, keys)
+            first += members
+        self.families = any(row[2] for row in self.rows)
+
+    def share(self, first, end, keys):
+        n = keys // self.page
+        for b in range(first + 1, end):
+            own = self.table[b, :n].tolist()
+            self.keys[own], self.values[own] = math.nan, math.nan
+            self.table[b, :n] = self.table[first, :n]
+        self.rows[first:end] = (first, end, n * self.page)
+
+    def attention(self, causal=True, window=0, sinks=0, scale=None):
+        """-> (out, tolerance), as Case.attention, whose docstring derives the tolerance (joining partial results of a family's keys and of a sequence's own is one
+        join, as that of parts is)."""
+        scale = scale if scale is not None else 1 / math.sqrt(self.d)
+        eps = EPS[self.dt]
+        out = torch.full((self.tokens, self.heads, self.d), math.nan, dtype=torch.float64)
+        tol = torch.zeros_like(out)
+        group = self.heads // self.kv_heads
+        for b, n in enumerate(self.lengths):
+            rows = slice(int(self.starts[b]), int(self.starts[b + 1]))
+            m = rows.stop - rows.start
+            if m == 0:
+                continue
+            k, v = self.history(b, self.keys), self.history(b, self.values)
+            position, key = torch.arange(n - m, n)[:, None], torch.arange(n)[None]
+            hidden = key > position if causal else torch.zeros(m, n, dtype=torch.bool)
+            if window:
+                hidden = hidden | ((key <= position - window) & (key >= sinks))
+            for h in range(self.heads):
+                q = self.q[rows, h].double()
+                kh, vh = k[:, h // group], v[:, h // group]
+                s = (q @ kh.T * scale).masked_fill(hidden, -math.inf)
+                size = (q.abs() @ kh.abs().T * scale).masked_fill(hidden, 0)
+                top = s.amax(1, keepdim=True) if n else torch.zeros(m, 1)
+                p = torch.exp(s - torch.where(top.isinf(), torch.zeros_like(top), top)).masked_fill(hidden, 0)
+                total = p.sum(1, keepdim=True)
+                p = torch.where(total > 0, p / total, torch.zeros_like(p))
+                o, a = p @ vh, p @ vh.abs()
+                ds = (self.d + 6) * E32 * (size.amax(1, keepdim=True) if n else 0)
+                t = a * (4 * ds + 2 * (n + 8) * E32 + 8 * E32) + eps / 2 * o.abs()
+                if self.dt != "f32":
+                    t = t + eps * a
+                if self.dt == "f16" and n:
+                    t = t + 2 * n * 2.0 ** -25 * vh.abs().max()
+                out[rows, h], tol[rows, h] = o, t
+        return out, tol
+
+    def run_attention(self, families=None, hints=None, **kw):
+        rows = self.rows if families is None else np.asarray(families, np.int32)
+        if self.families or families is not None:
+            count, most = (len({row[0] for row in rows.tolist() if row[2]}), int(rows[:, 2].max())) if hints is None else hints
+            kw.update(families=torch.from_numpy(rows.copy()).cuda(), family_count=count, max_shared=most)
+        return super().run_attention(**kw)
+
+
+def check(*args, causal=True, window=0, sinks=0, scale=None, **kw):
+    case = Sight(*args, **kw)
+    got = case.run_attention(causal=causal, window=window, sinks=sinks, scale=scale)
+    case.check_attention(got, causal=causal, window=window, sinks=sinks, scale=scale)
+    assert (got[int(case.starts[-1]):] == 7.0).all()  # rows behind the last sequence are left as they were
+
+
+# ------------------------------------------------------------------------------------------- windows and first tokens ------
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(1, 1), (16, 4), (50, 31), (64, 64), (100, 33), (33, 200), (10000, 4), (5, 10000)])
+def test_windows_with_sinks(dt, d, window, sinks):
+    """Single tokens, chunks, prompts that begin before the window does, sequences without new tokens; first keys that end anywhere in a tile or reach into the window."""
+    check(dt, [1, 90, 1, 0, 7, 40], [300, 40, 0, 50, 129, 0], 4, 2, d, 16, window=window, sinks=sinks, spare_rows=2, spare_width=1)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,page", [(2, 2, 1), (6, 2, 2), (8, 1, 8), (32, 2, 32), (20, 1, 128), (4, 4, 4096)])
+def test_windows_with_sinks_heads_and_pages(dt, heads, kv_heads, page):
+    check(dt, [1, 20, 1, 3], [700, 400, 5, 260], heads, kv_heads, 64, page, window=70, sinks=9)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("window,sinks", [(1, 3), (40, 17), (128, 128)])
+def test_windows_with_sinks_without_causality(dt, window, sinks):
+    check(dt, [1, 70, 3, 20], [5, 30, 400, 900], 4, 2, 64, 16, causal=False, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_long_windows_with_sinks_are_cut_and_joined(dt, causal):
+    for window, sinks, new, past in ((1000, 4, [40], [5000]), (700, 300, [130, 9, 20], [2999, 100, 4000]), (2000, 70, [20], [1500]), (3000, 5, [1, 2], [9000, 3500]),
+                                     (20, 3000, [30, 1], [5000, 6000])):
+        check(dt, new, past, 4, 2, 64, 16, causal=causal, window=window, sinks=sinks, spare_rows=1)
+    case = Sight(dt, [90, 30, 1], [3000, 17, 4000], 4, 2, 64, 16)
+    for most in ((30, 400), (0, 0), (1 << 30, 1 << 40)):
+        got = case.run_attention(max_tokens=most[0], max_length=most[1], window=900, sinks=77, causal=causal)
+        case.check_attention(got, window=900, sinks=77, causal=causal)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_sinks_without_a_window_say_nothing(dt):
+    case = Sight(dt, [1, 40], [600, 100], 4, 2, 64, 16)
+    assert torch.equal(case.run_attention(sinks=5), case.run_attention())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("new,past", [([1, 5, 150], [300, 290, 200]), ([1], [9000]), ([60], [5000]), ([1] * 70, [400 + i for i in range(70)])])
+def test_what_is_not_finite_reaches_only_the_tokens_that_see_it(dt, bad, new, past):
+    """A value among the first keys that are seen, one behind them, one at the window's edge: other rows and columns keep their bits."""
+    window, sinks = 100, 5
+    case = Sight(dt, new, past, 4, 2, 64, 16)
+    clean = case.run_attention(window=window, sinks=sinks).cpu()
+    case.check_attention(clean, window=window, sinks=sinks)
+    kept = case.values.clone()
+    for key in (lambda n, p: 4, lambda n, p: 5, lambda n, p: 31, lambda n, p: p - window, lambda n, p: p - window + 1, lambda n, p: p + n - 1):
+        case.values.copy_(kept)
+        spoiled = torch.zeros(case.q.shape, dtype=torch.bool)
+        for b, (n, p) in enumerate(zip(new, past)):
+            at = key(n, p)
+            case.values[case.table[b, at // 16], 1, at % 16, 7] = bad
+            for i in range(n):
+                spoiled[int(case.starts[b]) + i, 2:, 7] = at <= p + i and (at > p + i - window or at < sinks)
+        got = case.run_attention(window=window, sinks=sinks).cpu()
+        assert torch.equal(~torch.isfinite(got), spoiled)
+        assert torch.equal(got[~spoiled], clean[~spoiled])
+
+
+# ------------------------------------------------------------------------------------------------------- families ------
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (6, 2), (16, 1)])
+def test_families_of_single_tokens(dt, d, heads, kv_heads):
+    """Two and more samples of texts that end around the steps of sharing, some alone, some with nothing of their own but the new token."""
+    families = [(3, 128), (1, 0), (2, 127), (5, 144), (4, 256), (1, 0), (2, 640), (3, 16), (2, 0)]
+    rng = random.Random(heads)
+    past = [keys + rng.choice([0, 1, 15, 16, 60, 200]) for members, keys in families for _ in range(members)]
+    check(dt, [1] * len(past), past, heads, kv_heads, d, 16, families=families, spare_rows=3, spare_width=1)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("members,keys,heads,kv_heads", [(2, 3000, 4, 4), (40, 1500, 8, 2), (9, 5000, 16, 1), (70, 700, 4, 2), (3, 9000, 6, 2)])
+def test_long_families_are_cut_and_joined(dt, members, keys, heads, kv_heads):
+    rng = random.Random(members)
+    past = [keys + rng.choice([1, 30, 200, 900 if i % 9 == 0 else 40]) for i in range(members)]
+    check(dt, [1] * members, past, heads, kv_heads, 64, 16, families=[(members, keys)])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (8, 2, 128), (200, 1, 64)])
+def test_families_with_chunks(dt, heads, kv_heads, d):
+    """Questions of many tokens about a text, speculated tokens, sequences without new tokens, the first of a family among them."""
+    check(dt, [20, 1, 0, 130, 3, 0, 5, 1, 1, 16], [700, 650, 900, 640, 645, 512, 520, 513, 90, 40], heads, kv_heads, d, 16,
+          families=[(5, 640), (3, 512), (2, 0)], spare_rows=1)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("page", [1, 2, 8, 16, 128, 256])
+def test_families_and_page_sizes(dt, page):
+    check(dt, [1, 2, 1, 1, 40], [600, 530, 700, 300, 512], 4, 2, 64, page, families=[(3, 512), (2, 256)])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_new_tokens_among_the_common_keys(dt, causal):
+    """A family's keys are the first of its sequences, whatever is new: tokens that see a part of them, one of them, none."""
+    case = Sight(dt, [300, 1, 200, 40, 1], [0, 299, 100, 260, 600], 4, 2, 64, 16, families=[(4, 256), (1, 0)])
+    case.check_attention(case.run_attention(causal=causal), causal=causal)
+    case = Sight(dt, [1, 1, 20], [400, 500, 380], 4, 2, 64, 16, families=[(3, 384)])
+    case.lengths[2] = 7  # its 20 tokens have positions -13 to 6
+    got = case.run_attention(max_length=501)
+    assert (got[2:15] == 0).all()
+    case.check_attention(got)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (100, 0), (700, 0), (100, 4), (300, 130), (50, 512), (200, 900), (10000, 7)])
+def test_families_with_windows_and_sinks(dt, window, sinks):
+    """Windows that end before the common keys, in them, and not at all; first keys that stay visible: some, the common ones, more."""
+    check(dt, [1, 1, 30, 1, 1, 1, 0, 2], [900, 520, 600, 3000, 1, 700, 400, 2900], 4, 2, 64, 16, families=[(3, 512), (1, 0), (1, 0), (3, 384)], window=window,
+          sinks=sinks, spare_rows=1)
+    check(dt, [1] * 6, [2600, 2500, 2999, 2450, 5000, 2447], 8, 2, 128, 16, families=[(6, 2432)], window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("hints", [(0, 0), (1, 1), (1 << 40, 1 << 40), (7, 200)])
+def test_hints_of_families_choose_nothing_but_the_cut(dt, hints):
+    case = Sight(dt, [1, 40, 1, 1, 1, 3], [1600, 1400, 1500, 300, 260, 90], 8, 2, 64, 16, families=[(3, 1392), (2, 256), (1, 0)])
+    case.check_attention(case.run_attention(hints=hints))
+    case.check_attention(case.run_attention(hints=hints, max_tokens=1, max_length=10))
+
+
+def test_rows_of_families_that_disagree_are_sequences_on_their_own():
+    """Numbers outside the batch, firsts that name another first or an end before the sequence, families that claim each other's sequences: no key is lost or read twice."""
+    case = Sight("f16", [1, 2, 1, 1, 30, 1], [700, 600, 650, 620, 610, 640], 8, 2, 64, 16, families=[(6, 512)])
+    big = 1 << 31
+    for rows in ([[0, 6, 0]] * 6, [[0, 6, -5]] * 6, [[-1, 6, 512]] * 6, [[9, 6, 512]] * 6, [[big - 1, big - 1, big - 1]] * 6, [[-big, -big, -big]] * 6, [[0, 3, 512]] * 6,
+                 [[0, 6, 512]] * 3 + [[3, 6, 256]] * 3, [[1, 6, 512], [0, 6, 512]] + [[0, 6, 512]] * 4, [[0, 6, 512], [0, 2, 256], [2, 6, 512], [2, 6, 512], [0, 6, 512], [4, 9, 400]],
+                 [[0, 100, big - 1]] * 6, [[5, 6, 512]] * 5 + [[5, 6, 512]], [[0, 6, 512]] + [[b, b + 1, 512] for b in range(1, 6)], [[0, 0, 512]] * 6):
+        case.check_attention(case.run_attention(families=rows, hints=(1, 512)))
+    tt.cxx.synchronize()
+
+
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+def test_common_keys_end_where_the_first_sequence_does(dt):
+    """A row that promises more keys than the first sequence of the family has: what it has not is each sequence's own."""
+    case = Sight(dt, [1, 1, 1], [300, 700, 650], 4, 2, 64, 16, families=[(3, 288)])
+    case.check_attention(case.run_attention(families=[[0, 3, 640]] * 3))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("batch", [63, 64, 65, 200])
+def test_many_families(dt, batch):
+    """More sequences than a wavefront has lanes, families across that border, some sequences without new tokens and some long ones."""
+    rng = random.Random(batch)
+    families, left = [], batch
+    while left:
+        members = min(left, rng.choice([1, 1, 2, 5, 17]))
+        families.append((members, rng.choice([128, 200, 384]) if members > 1 else 0))
+        left -= members
+    past = [keys + rng.choice([0, 3, 70, 1500 if rng.random() < 0.1 else 130]) for members, keys in families for _ in range(members)]
+    new = [0 if i % 7 == 3 else 1 for i in range(batch)]
+    check(dt, new, past, 4, 2, 64, 16, families=families, spare_rows=1)
+    new = [40 if i % 31 == 0 else m for i, m in enumerate(new)]
+    check(dt, new, past, 4, 2, 64, 16, families=families)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_what_is_not_finite_in_common_keys(dt, bad):
+    """A value of a common key reaches every token that sees it, in its column alone; one behind every token's position, or in front of some tokens' windows, only those who see it."""
+    new, past, window = [1, 30, 1, 1], [700, 300, 400, 500], 330
+    case = Sight(dt, new, past, 4, 2, 64, 16, families=[(4, 320)])  # (tokens 300 to 319 of the second sequence are common keys)
+    for w in (0, window):
+        clean = case.run_attention(window=w).cpu()
+        case.check_attention(clean, window=w)
+        kept = case.values.clone()
+        for key in (0, 63, 100, 255, 310, 319):
+            case.values[case.table[0, key // 16], 1, key % 16, 7] = bad
+            spoiled = torch.zeros(case.q.shape, dtype=torch.bool)
+            for b, (n, p) in enumerate(zip(new, past)):
+                for i in range(n):
+                    spoiled[int(case.starts[b]) + i, 2:, 7] = key <= p + i and (w == 0 or key > p + i - w)
+            got = case.run_attention(window=w).cpu()
+            assert torch.equal(~torch.isfinite(got), spoiled), (w, key)
+            assert torch.equal(got[~spoiled], clean[~spoiled]), (w, key)
+            case.values.copy_(kept)
+    case.q[:, 0, 0] = -math.inf  # scores of minus infinity alone: NaN; among others: weights of zero
+    case.keys[..., 0] = torch.where(torch.isnan(case.keys[..., 0]), case.keys[..., 0], torch.ones_like(case.keys[..., 0]))
+    got = case.run_attention().cpu()
+    assert torch.isnan(got[:, 0]).all() and torch.isfinite(got[:, 1:]).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_scores_far_apart_in_common_and_own_keys(dt):
+    case = Sight(dt, [1, 30, 1], [900, 800, 790], 4, 2, 64, 16, families=[(3, 768)], scale_q=30.0)
+    case.check_attention(case.run_attention())
+    for scale in (1e-4, 3.0):
+        case.check_attention(case.run_attention(scale=scale), scale=scale)
+
+
+def test_the_same_call_twice_gives_the_same_bits():
+    for dt in DTYPES:
+        case = Sight(dt, [1, 40, 1, 1, 1], [3000, 2000, 2700, 300, 20], 8, 2, 128, 16, families=[(3, 1984), (2, 0)])
+        assert torch.equal(case.run_attention(), case.run_attention())
+        assert torch.equal(case.run_attention(window=700, sinks=40), case.run_attention(window=700, sinks=40))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_offsets_beyond_32_bits(dt):
+    """A cache of more than 2^32 bytes whose last pages hold the common and the own keys."""
+    d, page, kv_heads = 128, 64, 8
+    pages = (1 << 31) // (kv_heads * page * d) + 60
+    keys = torch.zeros((pages, kv_heads, page, d), dtype=TORCH_DTYPES[dt], device="cuda")
+    values = torch.zeros_like(keys)
+    case = Sight(dt, [1, 20, 1], [500, 437, 440], 16, kv_heads, d, page, families=[(3, 384)])
+    used = sorted({int(p) for row, n in zip(case.table, case.lengths) for p in row[:-(-n // page)]})
+    high = {p: pages - 1 - i for i, p in enumerate(used)}
+    for p, h in high.items():
+        keys[h], values[h] = case.keys[p].cuda(), case.values[p].cuda()
+    table = torch.tensor([[high.get(int(p), 0) for p in row] for row in case.table], dtype=torch.int32, device="cuda")
+    _, starts, lengths = case.device_args()
+    rows = torch.from_numpy(case.rows).cuda()
+    for window, sinks in ((0, 0), (60, 30)):
+        got = tt.paged_attention(case.q.cuda(), keys, values, table, starts, lengths, max_length=600, families=rows, window=window, sinks=sinks)
+        case.check_attention(got, window=window, sinks=sinks)
+    norm = torch.ones(d, device="cuda")
+    qkv = torch.randn(case.tokens, 32, d, device="cuda").to(keys.dtype)
+    tt.rotary_append(qkv, keys, values, table, starts, lengths, q_norm=norm, k_norm=norm)
+    last = int(table[1, (case.lengths[1] - 1) // page])
+    assert torch.equal(values[last, :, (case.lengths[1] - 1) % page], qkv[20, 24:])
+    tt.cxx.synchronize()
+
+
+def test_pages_outside_the_cache_are_reported():
+    case = Sight("f16", [1, 30, 1, 1], [400, 307, 290, 100], 4, 2, 64, 16, families=[(3, 256), (1, 0)])
+    case.keys, case.values = case.keys.nan_to_num(), case.values.nan_to_num()
+    for kw in (dict(families=torch.from_numpy(case.rows).cuda()), dict(window=200, sinks=20), dict(families=torch.from_numpy(case.rows).cuda(), window=200, sinks=20)):
+        for bad in (-1, 1 << 20):
+            for column in (1, 17):
+                table, starts, lengths = case.device_args()
+                table[0, column] = bad
+                out = tt.paged_attention(case.q.cuda(), case.keys.cuda(), case.values.cuda(), table, starts, lengths, **kw)
+                torch.cuda.synchronize()
+                with pytest.raises(tt.cxx.EnforceNotMet, match="out of range"):
+                    tt.cxx.synchronize()
+                tt.cxx.synchronize()  # reported once
+                want, tol = case.attention(window=kw.get("window", 0), sinks=kw.get("sinks", 0))
+                assert ((out.cpu().double() - want).abs() <= tol)[-1].all()  # the sequence that is on its own
+    # more keys than the table has pages for: those there are
+    table, starts, lengths = case.device_args()
+    lengths[0] = 5000
+    tt.paged_attention(case.q.cuda(), case.keys.cuda(), case.values.cuda(), table.clamp(0, 3)[:, :20].contiguous(), starts, lengths, window=100, sinks=3)
+    torch.cuda.synchronize()
+    with pytest.raises(tt.cxx.EnforceNotMet, match="out of range"):
+        tt.cxx.synchronize()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_rows_that_lie_apart(dt):
+    case = Sight(dt, [1, 20, 1], [300, 267, 290], 4, 2, 64, 16, families=[(3, 256)])
+    wide = torch.zeros(case.tokens, 8 * 64, dtype=case.q.dtype, device="cuda")
+    wide[:, 64:64 + 256] = case.q.cuda().view(-1, 256)
+    result = torch.full((case.tokens, 512), 7.0, dtype=case.q.dtype, device="cuda")
+    for kw in (dict(), dict(window=40, sinks=3)):
+        got = tt.paged_attention(wide[:, 64:320], case.keys.cuda(), case.values.cuda(), *case.device_args(), out=result[:, 128:384],
+                                 families=torch.from_numpy(case.rows).cuda(), **kw)
+        case.check_attention(got, **kw)
+        assert (result[:, :128] == 7).all() and (result[:, 384:] == 7).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_recorded_steps(dt):
+    """A step recorded into two graphs and replayed with growing lengths, other tables and other families, eager work and synchronisations between the replays."""
+    case = Sight(dt, [1, 1, 1, 1], [690, 600, 555, 30], 8, 2, 128, 16, families=[(3, 512), (1, 0)], spare_width=3)
+    table, starts, lengths = case.device_args()
+    table.clamp_(0, case.keys.shape[0] - 1)
+    keys, values = case.keys.nan_to_num().cuda(), case.values.nan_to_num().cuda()
+    qkv = torch.randn(4, 12, 128, generator=torch.Generator().manual_seed(2)).to(keys.dtype).cuda()
+    inv_freq, norm, rows = tt.rotary_frequencies(128), torch.rand(128, device="cuda"), torch.from_numpy(case.rows).cuda()
+
+    def call():
+        q = tt.rotary_append(qkv, keys, values, table, starts, lengths, inv_freq, q_norm=norm, k_norm=norm)
+        return (tt.paged_attention(q, keys, values, table, starts, lengths, max_tokens=1, max_length=720, families=rows, family_count=1, max_shared=512),
+                tt.paged_attention(q, keys, values, table, starts, lengths, max_tokens=1, max_length=720, window=300, sinks=70))
+
+    call()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call())
+        graphs.append(graph)
+    for turn in range(4):
+        qkv.copy_(torch.randn(4, 12, 128, generator=torch.Generator().manual_seed(10 + turn)).to(keys.dtype))
+        lengths.add_(1)
+        rows[:3, 2] = [512, 384, 0, 200][turn]
+        want = call()
+        torch.cuda.synchronize()
+        for graph, out in zip(graphs, outs):
+            for x in out:
+                x.fill_(math.nan)
+            graph.replay()
+            torch.randn(1 << 16, device="cuda").sum()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, w) for x, w in zip(out, want)), turn
+    tt.cxx.synchronize()
+
+
+def test_calls_on_two_streams_at_a_time():
+    """Two batches with families in turn on two streams without waiting for one another: their workspaces are their own."""
+    cases = [Sight("bf16", [1] * 3, [3000, 2000, 2900], 8, 2, 128, 16, seed=1, families=[(3, 1984)]),
+             Sight("bf16", [40, 1], [2500, 1200], 8, 2, 128, 16, seed=2, families=[(2, 1200)])]
+    tensors = [[x.cuda() for x in (case.q, case.keys, case.values)] + case.device_args() for case in cases]
+    hints = [dict(max_tokens=max(case.new), max_length=max(case.lengths), families=torch.from_numpy(case.rows).cuda()) for case in cases]
+    want = [tt.paged_attention(*t, **h) for t, h in zip(tensors, hints)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(tt.paged_attention(*tensors[i], **hints[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        cases[i].check_attention(want[i])
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_c_interface():
+    """The calls through the C ABI: the workspace they ask for, and their refusal of a smaller one."""
+    lib = capi.load()
+    case = Sight("f16", [1, 1, 1], [5000, 4800, 20], 4, 1, 64, 16, families=[(2, 4800), (1, 0)])
+    q, k, v = case.q.cuda(), case.keys.cuda(), case.values.cuda()
+    table, starts, lengths = case.device_args()
+    rows = torch.from_numpy(case.rows).cuda()
+    cache = capi.PagedCache(k.data_ptr(), v.data_ptr(), k.shape[0], 1, 16, 64)
+    batch = capi.PagedBatch(table.data_ptr(), table.shape[1], starts.data_ptr(), lengths.data_ptr(), 3, 3)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for window, sinks, families in ((0, 0, rows), (3000, 9, None), (3000, 9, rows), (0, 0, None), (0, 5, None)):
+        sight = capi.PagedSight(window, sinks, families.data_ptr() if families is not None else None, 0, 0)
+        n = ctypes.c_int64(-1)
+        capi.check(lib.ttmi_paged_attention_sight_workspace(ctypes.byref(cache), ctypes.byref(batch), 4, 1, 5001, ctypes.byref(sight), capi.F16, ctypes.byref(n)))
+        assert n.value >= 0
+        work = torch.empty(max(16, n.value), dtype=torch.uint8, device="cuda")
+        out = torch.empty_like(q)
+        call = lambda bytes: lib.ttmi_paged_attention_sight(q.data_ptr(), 256, out.data_ptr(), 256, 4, ctypes.byref(cache), ctypes.byref(batch), 1, 5001, 0.125, 1,
+                                                            ctypes.byref(sight), work.data_ptr(), bytes, capi.F16, stream)
+        capi.check(call(n.value))
+        torch.cuda.synchronize()
+        case.check_attention(out, window=window, sinks=sinks)
+        if n.value:
+            assert call(n.value - 1) == -1
+    tt.cxx.synchronize()
+
+
+def test_calls_without_tokens_or_sequences():
+    case = Sight("f16", [1, 1], [300, 290], 4, 2, 64, 16, families=[(2, 256)])
+    k, v = case.keys.cuda(), case.values.cuda()
+    table, starts, lengths = case.device_args()
+    rows = torch.from_numpy(case.rows).cuda()
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    assert tt.paged_attention(case.q.cuda()[:0], k, v, table, starts * 0, lengths, families=rows).shape == (0, 4, 64)
+    out = torch.full((2, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    tt.paged_attention(case.q.cuda(), k, v, table[:0], ints(0), ints(), out=out, families=rows[:0])
+    tt.paged_attention(case.q.cuda(), k, v, table, ints(0, 0, 0), lengths, out=out, families=rows)
+    tt.paged_attention(case.q.cuda(), k, v, table, ints(0, 0, 0), lengths, out=out, window=5, sinks=2)
+    assert (out == 7).all()
+    for kw in (dict(families=rows), dict(window=3, sinks=2)):
+        tt.paged_attention(case.q.cuda(), k, v, table[:, :0].contiguous(), ints(0, 1, 2), ints(0, 0), causal=False, out=out, **kw)
+        assert (out == 0).all()
+        out.fill_(7)
+    tt.cxx.synchronize()
+
+
+def test_python_refusals_with_device_tensors():
+    case = Sight("f16", [1, 3], [300, 290], 4, 2, 64, 16, families=[(2, 256)])
+    k, v, q = case.keys.cuda(), case.values.cuda(), case.q.cuda()
+    ints = case.device_args()
+    rows = torch.from_numpy(case.rows).cuda()
+    for bad in (dict(families=rows.long()), dict(families=rows[:1]), dict(families=rows[:, :2]), dict(families=rows.t()), dict(families=rows.cpu()), dict(families=rows[0]),
+                dict(families=rows, family_count=-1), dict(families=rows, max_shared=-1), dict(sinks=-1), dict(window=-1, sinks=1), dict(families=rows, scale=0.0)):
+        with pytest.raises(tt.cxx.EnforceNotMet):
+            tt.paged_attention(q, k, v, *ints, **bad)
+    qkv = torch.zeros(case.tokens, 8, 64, dtype=torch.float16, device="cuda")
+    norm = torch.ones(64, dtype=torch.float16, device="cuda")
+    for bad in (dict(q_norm=norm[:32]), dict(q_norm=norm.cpu()), dict(k_norm=norm.int()), dict(q_norm=norm.view(1, 64)), dict(k_norm=norm.expand(4, 64)),
+                dict(q_norm=norm, k_norm=norm.float()), dict(q_norm=norm.bfloat16()), dict(q_norm=norm, eps=-1.0), dict(q_norm=norm, eps=math.nan),
+                dict(q_norm=norm, eps=math.inf), dict(q_norm=k.view(-1)[:64]), dict(q_norm=torch.ones(128, dtype=torch.float16, device="cuda")[::2])):
+        with pytest.raises(tt.cxx.EnforceNotMet):
+            tt.rotary_append(qkv, k, v, *ints, **bad)
+    with pytest.raises(tt.cxx.EnforceNotMet):
+        tt.rotary_append(qkv, k, v, *ints, inv_freq=tt.rotary_frequencies(64), interleaved=True, q_norm=torch.ones(65, dtype=torch.float16, device="cuda")[1:])
+
+
+# ------------------------------------------------------------------------------------------------ norms of heads ------
+def normed(x, weight, eps):
+    """x [.., d] in 64 bits -> (normed, tolerance).
+
+    The tolerance, relative to the result: the sum of squares of d numbers in fp32 (d + 8) 2^-24, 1 / d and its product with it and the sum with eps 3 2^-24, of which the
+    root takes half; root, division and two products 5 2^-24."""
+    d = x.shape[-1]
+    y = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight
+    return y, ((d + 11) / 2 + 5) * E32 * y.abs()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rotary", [(64, 64), (128, 128), (64, 32), (128, 20), (80, 80), (96, 0), (48, 2), (256, 254), (16, 16), (256, 0)])
+@pytest.mark.parametrize("which", ["both", "q", "k", "per head"])
+def test_rotary_append_with_norms(dt, interleaved, d, rotary, which):
+    """Heads of very different sizes, slots besides the new tokens' untouched, values as they were."""
+    heads, kv_heads, page = 6, 2, 16
+    case = Case(dt, [1, 5, 0, 40], [7, 0, 9, 30], heads, kv_heads, d, page, spare_rows=2)
+    gen = torch.Generator().manual_seed(1)
+    sizes = torch.tensor([1.0, 1e-3, 30.0, 0.1, 1.0, 5.0, 1e-2, 20.0, 1.0, 1.0])[:, None]
+    qkv = (torch.randn(case.tokens, heads + 2 * kv_heads, d, generator=gen) * sizes).to(TORCH_DTYPES[dt])
+    eps = 1e-5
+    kinds = [torch.float32] if dt == "f32" else [torch.float32, TORCH_DTYPES[dt]]
+    inv_freq = tt.rotary_frequencies(rotary, device="cpu", stretch=2.0)
+    for kind in kinds:
+        shape = lambda n: (n, d) if which == "per head" else (d,)
+        weights = [(1 + 0.3 * torch.randn(shape(n), generator=gen)).to(kind) for n in (heads, kv_heads)]
+        args = {"q_norm": weights[0].cuda() if which != "k" else None, "k_norm": weights[1].cuda() if which != "q" else None}
+        keys, values = case.keys.cuda(), case.values.cuda()
+        out = torch.full((case.tokens, heads, d), 7.0, dtype=qkv.dtype, device="cuda")
+        q = tt.rotary_append(qkv.cuda(), keys, values, *case.device_args(), inv_freq.cuda(), interleaved, 1.25, out, eps=eps, **args)
+        tt.cxx.synchronize()
+        n = int(case.starts[-1])
+        position = torch.cat([torch.arange(length - m, length) for length, m in zip(case.lengths, case.new)])
+        x = qkv[:n, :heads + kv_heads].double()
+        y, off = x.clone(), torch.zeros_like(x)
+        if which != "k":
+            y[:, :heads], off[:, :heads] = normed(x[:, :heads], weights[0].double(), eps)
+        if which != "q":
+            y[:, heads:], off[:, heads:] = normed(x[:, heads:], weights[1].double(), eps)
+        want, tol = turned(y, position, inv_freq, interleaved, 1.25)
+        # what the norm is off by goes through the turn: at most the sum of both of a pair, times the amplitude
+        through = off.clone()
+        i = torch.arange(rotary // 2)
+        first, second = (2 * i, 2 * i + 1) if interleaved else (i, i + rotary // 2)
+        both = 1.25 * (off[..., first] + off[..., second])
+        through[..., first], through[..., second] = both, both
+        tol = tol + through * (1 + 2 ** -10) + EPS[dt] / 2 * want.abs() * (1 + 2 ** -10) + (2.0 ** -25 if dt == "f16" else 0)
+        assert ((q[:n].cpu().double() - want[:, :heads]).abs() <= tol[:, :heads]).all()
+        assert (q[n:] == 7).all()
+        keys, values = keys.cpu(), values.cpu()
+        want_keys, want_values = case.keys.double(), case.values.clone()
+        tol_keys = torch.zeros_like(want_keys)
+        row = 0
+        for b, m in enumerate(case.new):
+            for i in range(case.lengths[b] - m, case.lengths[b]):
+                at = case.table[b, i // page], slice(None), i % page
+                want_keys[at], tol_keys[at], want_values[at] = want[row, heads:], tol[row, heads:], qkv[row, heads + kv_heads:]
+                row += 1
+        assert torch.equal(values.nan_to_num(nan=99.0), want_values.nan_to_num(nan=99.0))
+        assert torch.equal(torch.isnan(keys), torch.isnan(want_keys))
+        assert ((keys.double() - want_keys).abs().nan_to_num() <= tol_keys).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("tokens,heads,kv_heads", [(1, 4, 2), (9, 4, 2), (3, 200, 1), (70, 3, 3)])
+def test_norms_in_place_and_from_rows_that_lie_apart(dt, tokens, heads, kv_heads):
+    """Queries turned where they lie, rows and weights of any alignment: the bits of a call with tensors of their own where the sum's order is the same, else within the
+    tolerance."""
+    case = Case(dt, [tokens], [30], heads, kv_heads, 64, 16)
+    inv_freq = tt.rotary_frequencies(64)
+    width = (heads + 2 * kv_heads) * 64
+    wide = torch.randn(tokens, width + 128, generator=torch.Generator().manual_seed(3)).to(TORCH_DTYPES[dt]).cuda()
+    weight = torch.rand(200 * 64 + 1, generator=torch.Generator().manual_seed(4)).to(TORCH_DTYPES[dt]).cuda()
+    for first, off in ((0, 0), (1, 0), (64, 1)):
+        qkv = wide[:, first:first + width]
+        q_norm, k_norm = weight[off:off + heads * 64].view(heads, 64), weight[off:off + 64]
+        keys, values = [case.keys.cuda() for _ in range(2)], [case.values.cuda() for _ in range(2)]
+        q = tt.rotary_append(qkv, keys[0], values[0], *case.device_args(), inv_freq, q_norm=q_norm, k_norm=k_norm)
+        x, tol = normed(qkv.cpu().double().view(tokens, -1, 64)[:, :heads], q_norm.cpu().double(), 1e-6)
+        want, more = turned(x, torch.arange(30, 30 + tokens), inv_freq.cpu(), False, 1.0)
+        both = tol[..., :32] + tol[..., 32:]
+        tol = torch.cat((both, both), -1) * (1 + 2 ** -10) + more + EPS[dt] / 2 * want.abs() * (1 + 2 ** -10) + (2.0 ** -25 if dt == "f16" else 0)
+        assert ((q.cpu().double() - want).abs() <= tol).all()
+        kept = wide.clone()
+        inside = kept[:, first:first + width]
+        tt.rotary_append(inside, keys[1], values[1], *case.device_args(), inv_freq, out=inside[:, :heads * 64], q_norm=q_norm, k_norm=k_norm)
+        assert torch.equal(inside[:, :heads * 64], q.view(tokens, heads * 64))
+        assert torch.equal(inside[:, heads * 64:], qkv[:, heads * 64:])
+        assert torch.equal(keys[0].nan_to_num(), keys[1].nan_to_num()) and torch.equal(values[0].nan_to_num(), values[1].nan_to_num())
+    tt.cxx.synchronize()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_norms_of_zeros_and_of_what_is_not_finite(dt):
+    """A head of zeros stays zeros, without eps it is NaN; a NaN or an infinity stays in its head; eps alone of a head far smaller."""
+    case = Case(dt, [1, 2], [7, 30], 4, 2, 64, 16)
+    keys, values = case.keys.cuda(), case.values.cuda()
+    norm = torch.ones(64, device="cuda")
+    qkv = torch.randn(3, 8, 64, generator=torch.Generator().manual_seed(3)).to(TORCH_DTYPES[dt]).cuda()
+    clean = tt.rotary_append(qkv, keys, values, *case.device_args(), q_norm=norm, k_norm=norm)
+    qkv[0, 1] = 0
+    qkv[1, 0, 5], qkv[2, 3, 0] = math.nan, math.inf
+    got = tt.rotary_append(qkv, keys, values, *case.device_args(), q_norm=norm, k_norm=norm)
+    assert (got[0, 1] == 0).all() and torch.isnan(got[1, 0]).all() and torch.isnan(got[2, 3, 0]) and (got[2, 3, 1:] == 0).all()
+    for row, head in ((0, 1), (1, 0), (2, 3)):
+        got[row, head] = clean[row, head]
+    assert torch.equal(got, clean)
+    got = tt.rotary_append(qkv, keys, values, *case.device_args(), q_norm=norm, k_norm=norm, eps=0.0)
+    assert torch.isnan(got[0, 1]).all() and torch.isfinite(got[0, [0, 2, 3]]).all()
+    qkv[0, 2] = 2.0 ** -20
+    got = tt.rotary_append(qkv, keys, values, *case.device_args(), q_norm=norm, k_norm=norm, eps=1.0)
+    assert ((got[0, 2].double() / 2.0 ** -20 - 1).abs() <= EPS[dt] + 30 * E32).all()
+
+
+# -------------------------------------------------------------------------------------------------------- together ------
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (60, 150)])
+def test_a_decoder_whose_samples_share_their_prompt(dt, window, sinks):
+    """A prompt, samples of it that grow apart, one of them refused tokens, a fork of a fork, a second prompt among them, a compaction: the context of every step, made with
+    `share`, is that of the sequence's own tokens; heads are normed on their way into the cache."""
+    layers, heads, kv_heads, d, page = 2, 4, 2, 64, 16
+    dtype = TORCH_DTYPES[dt]
+    cache = tt.PagedCache(layers, kv_heads, d, 80, page, dtype)
+    inv_freq = tt.rotary_frequencies(d)
+    gen = torch.Generator().manual_seed(5)
+    norms = [[1 + 0.2 * torch.randn(n, d, generator=gen) for n in (heads, kv_heads)] for _ in range(layers)]
+    told, families = {}, []
+
+    def step(names, tokens):
+        batch = cache.extend(names, tokens, share=True)
+        families.append(batch.family_count)
+        for layer in range(layers):
+            qkv = torch.randn(sum(tokens), heads + 2 * kv_heads, d, generator=gen).to(dtype)
+            at = 0
+            for name, n in zip(names, tokens):
+                told[name][layer].extend(qkv[at:at + n])
+                at += n
+            q = cache.append(layer, qkv.cuda(), batch, inv_freq, q_norm=norms[layer][0].cuda(), k_norm=norms[layer][1].cuda())
+            got = cache.attend(layer, q, batch, window=window, sinks=sinks).cpu().double()
+            at = 0
+            for name, n in zip(names, tokens):
+                if n:
+                    rows = torch.stack(told[name][layer]).double()
+                    length = rows.shape[0]
+                    y, _ = normed(rows[:, :heads + kv_heads], torch.cat(norms[layer]).double(), 1e-6)
+                    y, _ = turned(y, torch.arange(length), inv_freq.cpu(), False, 1.0)
+                    y = y.to(dtype).double()
+                    key, position = torch.arange(length)[None], torch.arange(length - n, length)[:, None]
+                    hidden = key > position
+                    if window:
+                        hidden |= (key <= position - window) & (key >= sinks)
+                    for h in range(heads):
+                        s = (y[length - n:, h] @ y[:, heads + h // 2].T / math.sqrt(d)).masked_fill(hidden, -math.inf)
+                        v = rows[:, heads + kv_heads + h // 2]
+                        want = torch.softmax(s, 1) @ v
+                        # half a step of q, k and the result each, of the probabilities twice; scores of size 8 at most take the error of q and k
+                        bound = (EPS[dt] * 12 + 400 * E32) * max(1.0, float(v.abs().max()))
+                        assert (got[at:at + n, h] - want).abs().max() <= bound, (name, layer, h)
+                at += n
+
+    def new():
+        name = cache.add()
+        told[name] = [[] for _ in range(layers)]
+        return name
+
+    def fork(name):
+        other = cache.fork(name)
+        told[other] = [list(rows) for rows in told[name]]
+        return other
+
+    a, z = new(), new()
+    step([a, z], [200, 150])
+    b, c = fork(a), fork(a)
+    step([a, b, c, z], [1, 1, 1, 1])
+    y = fork(z)
+    step([a, b, c, z, y], [1, 40, 3, 1, 1])
+    e = fork(b)
+    step([c, a, b, e, y, z], [1, 1, 1, 1, 0, 1])
+    cache.truncate(b, 205)
+    told[b] = [rows[:205] for rows in told[b]]
+    cache.free(a)
+    cache.compact()
+    step([c, b, e, z, y], [1, 2, 1, 30, 1])
+    assert families == [0, 1, 2, 2, 2]
+    tt.cxx.synchronize()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_families_and_none_agree(dt):
+    """The same batch with and without its families: both within the tolerance of the formula, and what has no family has the same bits as in a call where nobody has."""
+    case = Sight(dt, [1] * 9, [700 + 40 * i for i in range(8)] + [400], 8, 2, 128, 16, families=[(8, 640), (1, 0)])
+    plain = Case.run_attention(case)
+    case.check_attention(plain)
+    case.check_attention(case.run_attention())

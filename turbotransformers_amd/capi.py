@@ -46,6 +46,12 @@ class PagedBatch(ctypes.Structure):
                 ("batch", ctypes.c_int64), ("tokens", ctypes.c_int64)]
 
 
+class PagedSight(ctypes.Structure):
+    """Mirror of ``ttmi_paged_sight``."""
+    _fields_ = [("window", ctypes.c_int64), ("sinks", ctypes.c_int64), ("families", ctypes.c_void_p), ("family_count", ctypes.c_int64),
+                ("max_shared", ctypes.c_int64)]
+
+
 _SCALARS = {
     "int": ctypes.c_int, "int64_t": ctypes.c_int64, "int32_t": ctypes.c_int32, "float": ctypes.c_float,
     "size_t": ctypes.c_size_t,

@@ -1,6 +1,7 @@
 // A decoder's keys and values in pages: new tokens turned by their positions and stored, pages copied.
 #include "paged.h"
 
+#include <limits>
 #include <new>
 #include <utility>
 #include <vector>
@@ -121,6 +122,140 @@ static void launch_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out
                      static_cast<T*>(q_out), q_pitch, heads, static_cast<T*>(cache->keys), static_cast<T*>(cache->values), view, inv_freq, half, amplitude);
 }
 
+// ---- the same with norms of heads -----------------------------------------------------------------------------------------
+// x -> x / sqrt(sum x^2 / d + eps) * w of each head of queries and keys, then the turn.  A head's row is what LANES neighbouring lanes hold, N items each (as above: W elements,
+// or the two halves' W elements of W pairs), so the sum of its squares is a few exchanges within a wavefront, and each row is read once.
+struct NormView {
+  const void *q, *k;  // weights; null: not normed
+  int64_t q_pitch, k_pitch;
+  float eps, inv_d;
+};
+
+template <typename T, typename WT, int W, int N, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_append_normed_kernel(const T* qkv, int64_t qkv_pitch, T* q_out, int64_t q_pitch, int heads, T* __restrict__ keys,
+                                                                   T* __restrict__ values, const PagedView view, const double* __restrict__ inv_freq, int half,
+                                                                   float amplitude, const NormView norm, int lanes) {
+  const int token = blockIdx.x;
+  const int b = sequence_of(view, token);
+  if (b >= view.batch) return;
+  const int start = view.starts[b];
+  if (token < start) return;
+  const int position = view.lengths[b] - view.starts[b + 1] + token;
+  __shared__ float2 turn[128];
+  for (int i = threadIdx.x; i < half; i += blockDim.x) {
+    const float2 u = unit_turn((double)position * inv_freq[i]);
+    turn[i] = make_float2(u.x * amplitude, u.y * amplitude);
+  }
+  __syncthreads();
+
+  const int d = view.head_dim, hk = view.kv_heads;
+  bool stored = position >= 0 && (position >> view.page_shift) < view.table_pitch;
+  int page = 0;
+  if (stored) {
+    page = view.table[(int64_t)b * view.table_pitch + (position >> view.page_shift)];
+    stored = (unsigned)page < (unsigned)view.pages;
+  }
+  if (!stored && threadIdx.x == 0) page_error(view);
+  const int slot = position & ((1 << view.page_shift) - 1);
+  const int64_t row0 = (((int64_t)page * hk) << view.page_shift) + slot;
+
+  const int pairs = INTERLEAVED ? 0 : half / W;
+  const int items = d / W - pairs, plain = d / W;
+  const T* const in = qkv + (int64_t)token * qkv_pitch;
+  const int lane = (int)threadIdx.x % lanes, all = heads + 2 * hk;
+  // (a wavefront's lanes go round together: those whose head does not exist take part in the exchanges)
+  const int per = (int)blockDim.x / lanes;
+  for (int base = blockIdx.y * per; base < all; base += gridDim.y * per) {
+    const int head = base + (int)threadIdx.x / lanes;
+    const bool query = head < heads, value = head >= heads + hk, there = head < all && (query || stored);
+    const T* const x = in + (int64_t)(head < all ? head : 0) * d;
+    T* const y = query ? q_out + (int64_t)token * q_pitch + (int64_t)head * d
+                       : (value ? values : keys) + (row0 + ((int64_t)(value ? head - heads - hk : head - heads) << view.page_shift)) * d;
+    if (there && value) {
+      for (int i = lane; i < plain; i += lanes) store_vec<T, W>(y + i * W, load_vec<T, W>(x + i * W));
+    }
+    const bool turned = there && !value;
+    const WT* const w = static_cast<const WT*>(query ? norm.q : norm.k);
+    const bool normed = turned && w != nullptr;
+    const WT* const weights = normed ? w + (query ? (int64_t)head * norm.q_pitch : (int64_t)(head - heads) * norm.k_pitch) : nullptr;
+    Vec<T, W> lo[N], hi[N];
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int item = lane + n * lanes;
+      if (!turned || item >= items) continue;
+      const bool pair = !INTERLEAVED && item < pairs;
+      lo[n] = load_vec<T, W>(x + (INTERLEAVED || pair ? item : item + pairs) * W);
+      if (pair) hi[n] = load_vec<T, W>(x + half + item * W);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float a = to_float(lo[n].v[e]);
+        sum = __builtin_fmaf(a, a, sum);
+        if (pair) {
+          const float c = to_float(hi[n].v[e]);
+          sum = __builtin_fmaf(c, c, sum);
+        }
+      }
+    }
+    for (int step = lanes / 2; step > 0; step /= 2) sum += __shfl_xor(sum, step, kWave);
+    const float factor = normed ? 1.0f / sqrtf(__builtin_fmaf(sum, norm.inv_d, norm.eps)) : 1.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int item = lane + n * lanes;
+      if (!turned || item >= items) continue;
+      const bool pair = !INTERLEAVED && item < pairs;
+      const int at = (INTERLEAVED || pair ? item : item + pairs) * W;
+      float a[W], c[W];
+#pragma unroll
+      for (int e = 0; e < W; ++e) a[e] = to_float(lo[n].v[e]) * factor;
+      if (normed) {
+        const Vec<WT, W> u = load_vec<WT, W>(weights + at);
+#pragma unroll
+        for (int e = 0; e < W; ++e) a[e] *= to_float(u.v[e]);
+      }
+      if (pair) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) c[e] = to_float(hi[n].v[e]) * factor;
+        if (normed) {
+          const Vec<WT, W> u = load_vec<WT, W>(weights + half + at);
+#pragma unroll
+          for (int e = 0; e < W; ++e) c[e] *= to_float(u.v[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float2 t = turn[at + e];
+          lo[n].v[e] = from_float<T>(__builtin_fmaf(a[e], t.x, -c[e] * t.y));
+          hi[n].v[e] = from_float<T>(__builtin_fmaf(a[e], t.y, c[e] * t.x));
+        }
+        store_vec<T, W>(y + half + at, hi[n]);
+      } else if (INTERLEAVED && at < 2 * half) {
+#pragma unroll
+        for (int e = 0; e + 1 < W; e += 2) {
+          const float2 t = turn[(at + e) / 2];
+          lo[n].v[e] = from_float<T>(__builtin_fmaf(a[e], t.x, -a[e + 1] * t.y));
+          lo[n].v[e + 1] = from_float<T>(__builtin_fmaf(a[e], t.y, a[e + 1] * t.x));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) lo[n].v[e] = from_float<T>(a[e]);
+      }
+      store_vec<T, W>(y + at, lo[n]);
+    }
+  }
+}
+
+template <typename T, typename WT, int W, int N, bool INTERLEAVED>
+static void launch_rotary_append_normed(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t q_pitch, int heads, const ttmi_paged_cache* cache,
+                                        const PagedView& view, const double* inv_freq, int half, float amplitude, const NormView& norm, hipStream_t stream) {
+  const int items = view.head_dim / W - (INTERLEAVED ? 0 : half / W);
+  int lanes = 1;
+  while (lanes < items && lanes < kWave) lanes *= 2;
+  const int parts = (int)std::min<int64_t>(ceil_div((int64_t)(heads + 2 * view.kv_heads) * lanes, 256), 64);
+  hipLaunchKernelGGL((rotary_append_normed_kernel<T, WT, W, N, INTERLEAVED>), dim3(view.tokens, parts), dim3(256), 0, stream, static_cast<const T*>(qkv), qkv_pitch,
+                     static_cast<T*>(q_out), q_pitch, heads, static_cast<T*>(cache->keys), static_cast<T*>(cache->values), view, inv_freq, half, amplitude, norm,
+                     lanes);
+}
+
 // ---- pages copied to pages ----------------------------------------------------------------------------------------------
 // The list goes along with the launch: nothing is copied to the device, and a recorded call keeps its own.  A page goes through the registers of ceil(bytes / 16 KB) workgroups,
 // four pieces of 16 bytes a lane on their way: 901 pages of 64 KB in keys and values of 24 layers 1124 us, 5.05 TB/s (a large copy here 4.8); 4 pages of 24 KB in 12 layers 3.3.
@@ -161,6 +296,35 @@ static void launch_copy_pages(void* keys, void* values, int64_t layers, int64_t 
   hipLaunchKernelGGL(copy_pages_kernel<N>, grid, dim3(256), 0, stream, static_cast<char*>(keys), static_cast<char*>(values), pages, page_bytes, pairs);
 }
 
+// What both appends check and choose.
+struct AppendPlan {
+  PagedView view;
+  int half;
+  bool vectors, nothing;
+};
+static int plan_append(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t q_pitch, int64_t heads, const ttmi_paged_cache* cache,
+                       const ttmi_paged_batch* batch, const double* inv_freq, int64_t rotary_dim, int interleaved, int dtype, AppendPlan* p) {
+  if (int rc = paged_view(cache, batch, heads, &p->view)) return rc;
+  const int64_t d = cache->head_dim;
+  TTMI_REQUIRE(rotary_dim >= 0 && rotary_dim <= d && rotary_dim % 2 == 0, "rotary_dim must be even and at most head_dim");
+  TTMI_REQUIRE(rotary_dim == 0 || inv_freq != nullptr, "inv_freq is null");
+  TTMI_REQUIRE(qkv_pitch >= (heads + 2 * cache->kv_heads) * d && q_pitch >= heads * d, "rows overlap: a pitch is too small");
+  TTMI_REQUIRE(dtype == TTMI_F32 || dtype == TTMI_F16 || dtype == TTMI_BF16, "unsupported dtype");
+  p->nothing = batch->tokens == 0 || batch->batch == 0;
+  if (p->nothing) return 0;
+  TTMI_REQUIRE(qkv != nullptr && q_out != nullptr, "qkv or q_out is null");
+  TTMI_REQUIRE(q_out != qkv || q_pitch == qkv_pitch, "queries turned in place keep their pitch");
+  const int wide = 16 / (int)dtype_size(dtype);
+  p->half = (int)(rotary_dim / 2);
+  p->vectors = rows_aligned(qkv, qkv_pitch, dtype) && rows_aligned(q_out, q_pitch, dtype) && (interleaved ? rotary_dim : p->half) % wide == 0;
+  // (rows that are not aligned to 16 bytes, and parts of a head that are no whole pieces, go by the element or the pair)
+  TTMI_REQUIRE(((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & (dtype_size(dtype) - 1)) == 0, "qkv or q_out is not aligned to its elements");
+  const bool pairs_aligned = ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & (2 * dtype_size(dtype) - 1)) == 0 && qkv_pitch % 2 == 0 &&
+                             q_pitch % 2 == 0;
+  TTMI_REQUIRE(!interleaved || p->vectors || pairs_aligned, "interleaved pairs must be aligned to two elements");
+  return 0;
+}
+
 }  // namespace ttmi
 
 using namespace ttmi;
@@ -170,35 +334,59 @@ extern "C" {
 int ttmi_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t q_pitch, int64_t heads, const ttmi_paged_cache* cache,
                        const ttmi_paged_batch* batch, const double* inv_freq, int64_t rotary_dim, int interleaved, float amplitude,
                        int dtype, void* stream) {
-  PagedView view;
-  if (int rc = paged_view(cache, batch, heads, &view)) return rc;
-  const int64_t d = cache->head_dim;
-  TTMI_REQUIRE(rotary_dim >= 0 && rotary_dim <= d && rotary_dim % 2 == 0, "rotary_dim must be even and at most head_dim");
-  TTMI_REQUIRE(rotary_dim == 0 || inv_freq != nullptr, "inv_freq is null");
-  TTMI_REQUIRE(qkv_pitch >= (heads + 2 * cache->kv_heads) * d && q_pitch >= heads * d, "rows overlap: a pitch is too small");
-  TTMI_REQUIRE(dtype == TTMI_F32 || dtype == TTMI_F16 || dtype == TTMI_BF16, "unsupported dtype");
-  if (batch->tokens == 0 || batch->batch == 0) return 0;
-  TTMI_REQUIRE(qkv != nullptr && q_out != nullptr, "qkv or q_out is null");
-  TTMI_REQUIRE(q_out != qkv || q_pitch == qkv_pitch, "queries turned in place keep their pitch");
-  const int half = (int)(rotary_dim / 2), wide = 16 / (int)dtype_size(dtype);
-  const bool vectors = rows_aligned(qkv, qkv_pitch, dtype) && rows_aligned(q_out, q_pitch, dtype) &&
-                       (interleaved ? rotary_dim : half) % wide == 0;
-  // (rows that are not aligned to 16 bytes, and parts of a head that are no whole pieces, go by the element or the pair)
-  TTMI_REQUIRE(((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & (dtype_size(dtype) - 1)) == 0, "qkv or q_out is not aligned to its elements");
-  const bool pairs_aligned = ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & (2 * dtype_size(dtype) - 1)) == 0 &&
-                             qkv_pitch % 2 == 0 && q_pitch % 2 == 0;
-  TTMI_REQUIRE(!interleaved || vectors || pairs_aligned, "interleaved pairs must be aligned to two elements");
+  AppendPlan p;
+  if (int rc = plan_append(qkv, qkv_pitch, q_out, q_pitch, heads, cache, batch, inv_freq, rotary_dim, interleaved, dtype, &p)) return rc;
+  if (p.nothing) return 0;
+  const PagedView& view = p.view;
+  const int half = p.half;
   const hipStream_t s = static_cast<hipStream_t>(stream);
 #define TTMI_APPEND(W, I) launch_rotary_append<T, W, I>(qkv, qkv_pitch, q_out, q_pitch, (int)heads, cache, view, inv_freq, half, amplitude, s)
   TTMI_DISPATCH_FLOAT(dtype, T, {
     constexpr int kWide = 16 / (int)sizeof(T);
-    if (vectors && interleaved) TTMI_APPEND(kWide, true);
-    else if (vectors) TTMI_APPEND(kWide, false);
+    if (p.vectors && interleaved) TTMI_APPEND(kWide, true);
+    else if (p.vectors) TTMI_APPEND(kWide, false);
     else if (interleaved) TTMI_APPEND(2, true);
     else TTMI_APPEND(1, false);
   });
 #undef TTMI_APPEND
   return launch_status("rotary_append");
+}
+
+int ttmi_rotary_append_normed(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t q_pitch, int64_t heads, const ttmi_paged_cache* cache,
+                              const ttmi_paged_batch* batch, const double* inv_freq, int64_t rotary_dim, int interleaved, float amplitude, const void* q_norm,
+                              int64_t q_norm_pitch, const void* k_norm, int64_t k_norm_pitch, int norm_dtype, float eps, int dtype, void* stream) {
+  AppendPlan p;
+  if (int rc = plan_append(qkv, qkv_pitch, q_out, q_pitch, heads, cache, batch, inv_freq, rotary_dim, interleaved, dtype, &p)) return rc;
+  const int64_t d = cache->head_dim;
+  TTMI_REQUIRE(norm_dtype == TTMI_F32 || norm_dtype == dtype, "weights of a norm must be float32 or of the tensors' type");
+  TTMI_REQUIRE((q_norm_pitch == 0 || q_norm_pitch >= d) && (k_norm_pitch == 0 || k_norm_pitch >= d), "rows of a norm's weights overlap: a pitch is too small");
+  TTMI_REQUIRE(eps >= 0.f && eps <= std::numeric_limits<float>::max(), "eps must be finite and not negative");
+  const uintptr_t weights = reinterpret_cast<uintptr_t>(q_norm) | reinterpret_cast<uintptr_t>(k_norm);
+  TTMI_REQUIRE((weights & (dtype_size(norm_dtype) - 1)) == 0, "weights of a norm are not aligned to their elements");
+  if (p.nothing) return 0;
+  const int64_t weight_bytes = (int64_t)dtype_size(norm_dtype);
+  const bool aligned = (weights & 15) == 0 && q_norm_pitch * weight_bytes % 16 == 0 && k_norm_pitch * weight_bytes % 16 == 0;
+  // (weights that are not aligned to 16 bytes take the kernels that go by the element; interleaved pairs are two elements)
+  const bool pairs = (weights & (2 * dtype_size(norm_dtype) - 1)) == 0 && q_norm_pitch % 2 == 0 && k_norm_pitch % 2 == 0;
+  TTMI_REQUIRE(!interleaved || pairs, "weights of interleaved pairs must be aligned to two elements");
+  const NormView norm = {q_norm, k_norm, q_norm_pitch, k_norm_pitch, eps, 1.0f / (float)d};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+#define TTMI_APPEND(WT, W, N, I) \
+  launch_rotary_append_normed<T, WT, W, N, I>(qkv, qkv_pitch, q_out, q_pitch, (int)heads, cache, p.view, inv_freq, p.half, amplitude, norm, s)
+  TTMI_DISPATCH_FLOAT(dtype, T, {
+    constexpr int kWide = 16 / (int)sizeof(T);
+    auto launch = [&](auto zero) {
+      using WT = decltype(zero);
+      if (p.vectors && aligned && interleaved) TTMI_APPEND(WT, kWide, 1, true);
+      else if (p.vectors && aligned) TTMI_APPEND(WT, kWide, 1, false);
+      else if (interleaved) TTMI_APPEND(WT, 2, 2, true);
+      else TTMI_APPEND(WT, 1, 4, false);
+    };
+    if (norm_dtype == TTMI_F32) launch(0.f);
+    else launch(T{});
+  });
+#undef TTMI_APPEND
+  return launch_status("rotary_append_normed");
 }
 
 int ttmi_copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t page_bytes, const int32_t* sources,

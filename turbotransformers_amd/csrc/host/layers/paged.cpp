@@ -125,6 +125,14 @@ bool Meet(const TensorView& a, int64_t a_bytes, const TensorView& b, int64_t b_b
   const intptr_t a0 = reinterpret_cast<intptr_t>(a.data), b0 = reinterpret_cast<intptr_t>(b.data);
   return a_bytes > 0 && b_bytes > 0 && a0 < b0 + b_bytes && b0 < a0 + a_bytes;
 }
+// Weights of a norm: how far rows of heads are apart (0: one for all).
+int64_t NormPitch(const TensorView& t, int64_t heads, int64_t d, int device, const char* what) {
+  RequireOn(t, device, what);
+  FloatType(t, what);
+  TT_ENFORCE((t.n_dim == 1 && t.shape[0] == d) || (t.n_dim == 2 && t.shape[0] == heads && t.shape[1] == d), "%s: expected [head_dim] or [heads, head_dim]", what);
+  TT_ENFORCE(t.IsDense(t.n_dim - 1) && (t.n_dim == 1 || t.stride[0] >= 0), "%s: rows must be dense", what);
+  return t.n_dim == 2 && heads > 1 ? t.stride[0] : 0;
+}
 int64_t Bytes(const TensorView& dense) { return dense.numel() * (dense.dtype.bits / 8); }
 int64_t Bytes(const TensorView& t, const RowArgs& rows, int64_t d) {
   return t.shape[0] > 0 ? ((t.shape[0] - 1) * rows.pitch + rows.heads * d) * (t.dtype.bits / 8) : 0;
@@ -133,7 +141,7 @@ int64_t Bytes(const TensorView& t, const RowArgs& rows, int64_t d) {
 }  // namespace
 
 void RotaryAppend(const TensorView& qkv, const TensorView& keys, const TensorView& values, const PagedBatchViews& batch, const TensorView* inv_freq,
-                  bool interleaved, float amplitude, const TensorView& q_out, int device, void* stream) {
+                  bool interleaved, float amplitude, const HeadNorms& norms, const TensorView& q_out, int device, void* stream) {
   const CacheArgs cache = Cache(keys, values, device);
   const RowArgs in = Rows(qkv, cache, device, "qkv");
   RowArgs out = Rows(q_out, cache, device, "queries");
@@ -156,13 +164,29 @@ void RotaryAppend(const TensorView& qkv, const TensorView& keys, const TensorVie
                "inv_freq: expected a dense float64 tensor of one dimension");
     rotary_dim = 2 * inv_freq->shape[0];
   }
-  TT_DEVICE_CALL(ttmi_rotary_append(qkv.data, in.pitch, q_out.data, out.pitch, out.heads, &cache.cache, &args,
-                                    inv_freq != nullptr ? static_cast<const double*>(inv_freq->data) : nullptr, rotary_dim, interleaved ? 1 : 0, amplitude,
-                                    cache.type, stream));
+  const double* const frequencies = inv_freq != nullptr ? static_cast<const double*>(inv_freq->data) : nullptr;
+  if (norms.q == nullptr && norms.k == nullptr) {
+    TT_DEVICE_CALL(ttmi_rotary_append(qkv.data, in.pitch, q_out.data, out.pitch, out.heads, &cache.cache, &args, frequencies, rotary_dim, interleaved ? 1 : 0,
+                                      amplitude, cache.type, stream));
+    return;
+  }
+  const int64_t d = cache.cache.head_dim;
+  const int64_t q_norm_pitch = norms.q != nullptr ? NormPitch(*norms.q, out.heads, d, device, "q_norm") : 0;
+  const int64_t k_norm_pitch = norms.k != nullptr ? NormPitch(*norms.k, cache.cache.kv_heads, d, device, "k_norm") : 0;
+  TT_ENFORCE(norms.q == nullptr || norms.k == nullptr || core::SameDataType(norms.q->dtype, norms.k->dtype), "q_norm and k_norm differ in type");
+  for (const TensorView* t : {norms.q, norms.k}) {
+    if (t == nullptr) continue;
+    const int64_t bytes = ((t->n_dim == 2 ? (t->shape[0] - 1) * t->stride[0] : 0) + d) * (t->dtype.bits / 8);
+    for (const TensorView* cached : {&keys, &values}) TT_ENFORCE(!Meet(*t, bytes, *cached, held), "weights of a norm overlap the cache");
+    TT_ENFORCE(!Meet(*t, bytes, q_out, Bytes(q_out, out, d)), "weights of a norm overlap the queries' place");
+  }
+  TT_DEVICE_CALL(ttmi_rotary_append_normed(qkv.data, in.pitch, q_out.data, out.pitch, out.heads, &cache.cache, &args, frequencies, rotary_dim, interleaved ? 1 : 0,
+                                           amplitude, norms.q != nullptr ? norms.q->data : nullptr, q_norm_pitch, norms.k != nullptr ? norms.k->data : nullptr,
+                                           k_norm_pitch, FloatType(norms.q != nullptr ? *norms.q : *norms.k, "weights of a norm"), norms.eps, cache.type, stream));
 }
 
 void PagedAttention(const TensorView& q, const TensorView& keys, const TensorView& values, const PagedBatchViews& batch, const TensorView& out,
-                    int64_t max_tokens, int64_t max_length, const float* scale, bool causal, int64_t window,
+                    int64_t max_tokens, int64_t max_length, const float* scale, bool causal, const PagedSight& sight,
                     const std::function<void*(int64_t)>& workspace, int device, void* stream) {
   const CacheArgs cache = Cache(keys, values, device);
   const RowArgs from = Rows(q, cache, device, "q"), to = Rows(out, cache, device, "out");
@@ -173,9 +197,21 @@ void PagedAttention(const TensorView& q, const TensorView& keys, const TensorVie
   const ttmi_paged_batch args = Batch(batch, q.shape[0], device);
   const float factor = scale != nullptr ? *scale : (float)(1.0 / std::sqrt((double)cache.cache.head_dim));
   int64_t bytes = 0;
-  TT_DEVICE_CALL(ttmi_paged_attention_workspace(&cache.cache, &args, from.heads, max_tokens, max_length, window, cache.type, &bytes));
-  TT_DEVICE_CALL(ttmi_paged_attention(q.data, from.pitch, out.data, to.pitch, from.heads, &cache.cache, &args, max_tokens, max_length, factor, causal ? 1 : 0,
-                                      window, bytes > 0 ? workspace(bytes) : nullptr, bytes, cache.type, stream));
+  if (sight.families == nullptr && sight.sinks == 0) {
+    TT_DEVICE_CALL(ttmi_paged_attention_workspace(&cache.cache, &args, from.heads, max_tokens, max_length, sight.window, cache.type, &bytes));
+    TT_DEVICE_CALL(ttmi_paged_attention(q.data, from.pitch, out.data, to.pitch, from.heads, &cache.cache, &args, max_tokens, max_length, factor, causal ? 1 : 0,
+                                        sight.window, bytes > 0 ? workspace(bytes) : nullptr, bytes, cache.type, stream));
+    return;
+  }
+  ttmi_paged_sight seen = {sight.window, sight.sinks, nullptr, sight.family_count, sight.max_shared};
+  if (sight.families != nullptr) {
+    RequireInts(*sight.families, 2, device, "families");
+    TT_ENFORCE(sight.families->shape[0] == args.batch && sight.families->shape[1] == 3, "families: expected [batch, 3]");
+    seen.families = static_cast<const int32_t*>(sight.families->data);
+  }
+  TT_DEVICE_CALL(ttmi_paged_attention_sight_workspace(&cache.cache, &args, from.heads, max_tokens, max_length, &seen, cache.type, &bytes));
+  TT_DEVICE_CALL(ttmi_paged_attention_sight(q.data, from.pitch, out.data, to.pitch, from.heads, &cache.cache, &args, max_tokens, max_length, factor, causal ? 1 : 0,
+                                            &seen, bytes > 0 ? workspace(bytes) : nullptr, bytes, cache.type, stream));
 }
 
 void CopyPages(const TensorView& keys, const TensorView& values, const std::vector<int32_t>& sources, const std::vector<int32_t>& destinations, int device,

@@ -181,25 +181,30 @@ struct ViewArg {
 
 static void RotaryAppend(const py::object& qkv, const py::object& keys, const py::object& values, const py::object& table, const py::object& starts,
                          const py::object& lengths, const py::object& inv_freq, bool interleaved, float amplitude, const py::object& q_out, int device,
-                         uintptr_t stream) {
+                         uintptr_t stream, const py::object& q_norm, const py::object& k_norm, float eps) {
   const ViewArg in(qkv, "qkv"), k(keys, "keys"), v(values, "values"), t(table, "table"), s(starts, "starts"), l(lengths, "lengths"), out(q_out, "out");
-  std::unique_ptr<ViewArg> f;
+  std::unique_ptr<ViewArg> f, qn, kn;
   if (!inv_freq.is_none()) f = std::make_unique<ViewArg>(inv_freq, "inv_freq");
-  layers::kernels::RotaryAppend(in.view, k.view, v.view, {t.view, s.view, l.view}, f ? &f->view : nullptr, interleaved, amplitude, out.view, device,
-                                reinterpret_cast<void*>(stream));
+  if (!q_norm.is_none()) qn = std::make_unique<ViewArg>(q_norm, "q_norm");
+  if (!k_norm.is_none()) kn = std::make_unique<ViewArg>(k_norm, "k_norm");
+  layers::kernels::RotaryAppend(in.view, k.view, v.view, {t.view, s.view, l.view}, f ? &f->view : nullptr, interleaved, amplitude,
+                                {qn ? &qn->view : nullptr, kn ? &kn->view : nullptr, eps}, out.view, device, reinterpret_cast<void*>(stream));
 }
 
 // `empty_bytes`: a Python function of a number of bytes that gives device memory of the caller's framework, whose allocator knows the stream (and
 // gives a call that is being recorded into a graph memory that stays the graph's).
 static void PagedAttention(const py::object& q, const py::object& keys, const py::object& values, const py::object& table, const py::object& starts,
                            const py::object& lengths, const py::object& out, int64_t max_tokens, int64_t max_length, const py::object& scale, bool causal,
-                           int64_t window, const py::object& empty_bytes, int device, uintptr_t stream) {
+                           int64_t window, const py::object& empty_bytes, int device, uintptr_t stream, int64_t sinks, const py::object& families,
+                           int64_t family_count, int64_t max_shared) {
   const ViewArg in(q, "q"), k(keys, "keys"), v(values, "values"), t(table, "table"), s(starts, "starts"), l(lengths, "lengths"), o(out, "out");
-  std::unique_ptr<ViewArg> workspace;
+  std::unique_ptr<ViewArg> workspace, f;
   py::object memory;
+  if (!families.is_none()) f = std::make_unique<ViewArg>(families, "families");
   const float factor = scale.is_none() ? 0.f : scale.cast<float>();
   layers::kernels::PagedAttention(
-      in.view, k.view, v.view, {t.view, s.view, l.view}, o.view, max_tokens, max_length, scale.is_none() ? nullptr : &factor, causal, window,
+      in.view, k.view, v.view, {t.view, s.view, l.view}, o.view, max_tokens, max_length, scale.is_none() ? nullptr : &factor, causal,
+      {window, sinks, f ? &f->view : nullptr, family_count, max_shared},
       [&](int64_t bytes) -> void* {
         memory = empty_bytes(bytes);
         workspace = std::make_unique<ViewArg>(memory, "workspace");
@@ -527,8 +532,12 @@ PYBIND11_MODULE(turbo_transformers_cxx, m) {
       .def_property_readonly("pages", &core::PagePool::pages)
       .def_property_readonly("page_size", &core::PagePool::page_size)
       .def_property_readonly("sequences", &core::PagePool::sequences);
-  m.def("rotary_append", &RotaryAppend);
-  m.def("paged_attention", &PagedAttention);
+  m.def("rotary_append", &RotaryAppend, py::arg("qkv"), py::arg("keys"), py::arg("values"), py::arg("table"), py::arg("starts"), py::arg("lengths"),
+        py::arg("inv_freq"), py::arg("interleaved"), py::arg("amplitude"), py::arg("out"), py::arg("device"), py::arg("stream"), py::arg("q_norm") = py::none(),
+        py::arg("k_norm") = py::none(), py::arg("eps") = 1e-6f);
+  m.def("paged_attention", &PagedAttention, py::arg("q"), py::arg("keys"), py::arg("values"), py::arg("table"), py::arg("starts"), py::arg("lengths"),
+        py::arg("out"), py::arg("max_tokens"), py::arg("max_length"), py::arg("scale"), py::arg("causal"), py::arg("window"), py::arg("empty_bytes"),
+        py::arg("device"), py::arg("stream"), py::arg("sinks") = 0, py::arg("families") = py::none(), py::arg("family_count") = 0, py::arg("max_shared") = 0);
   m.def("copy_pages", &CopyPages);
 
   m.def("bind_torch", [](const py::object& tensor_type, const py::object& to_capsule, const py::object& from_capsule) {

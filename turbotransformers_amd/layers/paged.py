@@ -13,11 +13,14 @@ replayed with other contents of all tensors.  A page outside the cache, or a tok
 import math
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from .. import cxx
 
 __all__ = ['PagedCache', 'PagedBatch', 'rotary_append', 'paged_attention', 'copy_pages', 'rotary_frequencies']
+
+_LEAST_SHARED = 128  # keys that the kernels take as shared: the step of their work
 
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)  # absent from builds without a device
 _current_device, _is_initialized = torch.cuda.current_device, torch.cuda.is_initialized
@@ -37,12 +40,15 @@ def _empty_bytes(n):
 
 def rotary_append(qkv: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                   lengths: torch.Tensor, inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
-                  amplitude: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  amplitude: float = 1.0, out: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
+                  k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
     """Turns the new tokens' queries and keys by their positions and stores keys and values into their pages.
 
     qkv: [tokens, (heads + 2 kv_heads) * head_dim] or [tokens, heads + 2 kv_heads, head_dim], queries first; rows may lie any distance apart.
     inv_freq: float64 on the GPU; pair i of the first 2 * len(inv_freq) elements of a head turns by position * inv_freq[i] (`rotary_frequencies`
     makes them), None: nothing turns.  interleaved: pairs are neighbours (2i, 2i + 1), else (i, i + len(inv_freq)).
+    q_norm, k_norm: where given, queries / keys are normed head by head before they turn, x / sqrt(mean(x^2) + eps) * weight: float32 or qkv's type, [head_dim] for
+    all heads or [heads, head_dim] / [kv_heads, head_dim].  Everything is computed in 32 bits (a head's sum of squares has to stay below 2^128) and rounded once.
     -> the queries [tokens, heads, head_dim]: `out` if given, which may be the queries' part of qkv itself."""
     if out is None:
         shape = qkv.shape
@@ -51,26 +57,37 @@ def rotary_append(qkv: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
         if heads < 1:
             raise ValueError("qkv has no room for queries beside the cache's heads")
         out = qkv.new_empty((shape[0], heads, d))
-    cxx.rotary_append(qkv, keys, values, table, starts, lengths, inv_freq, interleaved, amplitude, out, *_here())
+    if q_norm is None and k_norm is None:
+        cxx.rotary_append(qkv, keys, values, table, starts, lengths, inv_freq, interleaved, amplitude, out, *_here())
+    else:
+        cxx.rotary_append(qkv, keys, values, table, starts, lengths, inv_freq, interleaved, amplitude, out, *_here(), q_norm, k_norm, eps)
     return out
 
 
 def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                     lengths: torch.Tensor, max_tokens: int = 0, max_length: int = 0, scale: Optional[float] = None, causal: bool = True,
-                    window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    window: int = 0, out: Optional[torch.Tensor] = None, sinks: int = 0, families: Optional[torch.Tensor] = None,
+                    family_count: int = 0, max_shared: int = 0) -> torch.Tensor:
     """softmax(scale * q k^T) v of the new tokens over their sequences' keys: up to a token's own position if causal, all of them otherwise;
-    window > 0: only the last `window` up to its own.  A token that sees no key gets zeros; where it sees some, all with a score of minus
+    window > 0: only the last `window` up to its own, and with sinks > 0 the first `sinks` of its sequence besides.  A token that sees no key gets zeros; where it sees some, all with a score of minus
     infinity, NaN, as zero divided by zero is.  Sums and statistics are held in 32 bits; in 16-bit types the probabilities are rounded to the type for
     their product with v (and divided by the sum of the rounded ones).  The sum of |v| over a token's keys has to stay below 2^120.
 
     q: [tokens, heads * head_dim] or [tokens, heads, head_dim], head_dim 64 or 128; rows may lie any multiple of 16 bytes apart.  heads is a
     multiple of kv_heads: query head h reads key/value head h // (heads // kv_heads).  scale: positive, 1 / sqrt(head_dim) by default.
     max_tokens, max_length: the most new tokens and keys of a sequence, where known: they choose how the work is cut, not what is computed.
+    families: int32 [batch, 3] on the GPU: neighbouring sequences whose first keys lie in the same pages may be a family, whose common keys are read once for all of them.
+    The row of each of its sequences is (number of the first of them, number behind the last, keys they have in common); of one that is on its own (its own number, the next,
+    0).  The common keys are read where the first one's row of the table says, in steps of 128 (fewer are not shared).  The result is that without families but for roundings.
+    family_count, max_shared: how many families there are and the most keys of one, where known: hints as well.  `PagedCache.extend(..., share=True)` fills in all three.
     -> like q: `out` if given."""
     if out is None:
         out = torch.empty_like(q)
-    cxx.paged_attention(q, keys, values, table, starts, lengths, out, max_tokens, max_length, scale, causal, window,
-                        _empty_bytes, *_here())
+    if sinks == 0 and families is None:
+        cxx.paged_attention(q, keys, values, table, starts, lengths, out, max_tokens, max_length, scale, causal, window, _empty_bytes, *_here())
+    else:
+        cxx.paged_attention(q, keys, values, table, starts, lengths, out, max_tokens, max_length, scale, causal, window, _empty_bytes, *_here(), sinks, families,
+                            family_count, max_shared)
     return out
 
 
@@ -103,11 +120,42 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, stretch: float = 
     return inv_freq.to(device if device is not None else 'cuda')
 
 
+def _families(table: np.ndarray, before: Sequence[int], page_size: int):
+    """Families of neighbours whose first pages are the same ones, full before this step -> rows [batch, 3], how many families, the most keys of one."""
+    n = len(before)
+    rows = np.stack([np.arange(n), np.arange(1, n + 1), np.zeros(n, np.int64)], axis=1).astype(np.int32)
+    if n < 2:
+        return rows, 0, 0
+    full = np.asarray(before, np.int64) // page_size
+    differs = table[1:] != table[:-1]
+    common = np.where(differs.any(axis=1), differs.argmax(axis=1), table.shape[1]) if table.shape[1] else np.zeros(n - 1, np.int64)
+    links = np.minimum(common, np.minimum(full[1:], full[:-1])) * page_size
+    links[links < _LEAST_SHARED] = 0
+    count = most = first = 0
+    keys = int(links[0])  # what sequences first .. b - 1 have in common with b - 1's next
+    for b in range(1, n + 1):
+        link = int(links[b - 1]) if b < n else 0
+        members = b - first
+        if members == 1:
+            keys = link
+        # one more member, if that saves more keys than the shorter prefix loses for the others
+        if link and (members == 1 or members * min(keys, link) >= (members - 1) * keys):
+            keys = min(keys, link)
+            continue
+        if members > 1:
+            rows[first:b] = (first, b, keys)
+            count, most = count + 1, max(most, keys)
+        first = b
+    return rows, count, most
+
+
 class PagedBatch:
     """The sequences of one step as the operators take them; all layers of the step share it."""
 
-    def __init__(self, table: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, max_tokens: int = 0, max_length: int = 0):
+    def __init__(self, table: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, max_tokens: int = 0, max_length: int = 0,
+                 families: Optional[torch.Tensor] = None, family_count: int = 0, max_shared: int = 0):
         self.table, self.starts, self.lengths, self.max_tokens, self.max_length = table, starts, lengths, max_tokens, max_length
+        self.families, self.family_count, self.max_shared = families, family_count, max_shared
 
 
 class PagedCache:
@@ -152,32 +200,39 @@ class PagedCache:
         if pairs:
             copy_pages(self.keys, self.values, [p[0] for p in pairs], [p[1] for p in pairs])
 
-    def extend(self, sequences: Sequence[int], tokens: Sequence[int]) -> PagedBatch:
+    def extend(self, sequences: Sequence[int], tokens: Sequence[int], share: bool = False) -> PagedBatch:
         """Room for tokens[i] new tokens of sequences[i], and the batch of that step.  Shared pages that would be written are copied first.
+        share: neighbours in `sequences` that begin with the same 128 or more tokens in the same pages (forks of one another) are a family in this step, and `attend`
+        reads those keys once for all of them.
         A call that raises, for want of free pages or because a copy or the batch cannot be made, leaves every sequence with the tokens it had."""
         self._move(self.pool.copies_of(sequences, tokens))  # (to free pages: the book follows when they have been enqueued)
         before = [self.pool.length(s) for s in sequences]
         self.pool.extend(sequences, tokens)
         try:
-            return self._batch(sequences, tokens, [n + more for n, more in zip(before, tokens)])
+            return self._batch(sequences, tokens, [n + more for n, more in zip(before, tokens)], before if share else None)
         except BaseException:
             for s, n in zip(sequences, before):
                 self.pool.truncate(s, n)
             raise
 
-    def _batch(self, sequences, tokens, lengths):
+    def _batch(self, sequences, tokens, lengths, before):
         longest = max(lengths, default=0)
         starts = [0]
         for n in tokens:
             starts.append(starts[-1] + n)
         table = self.pool.table(sequences, max(1, -(-longest // self.pool.page_size)))
-        # one copy to the device: [table | starts | lengths]
-        packed = torch.cat((torch.from_numpy(table).flatten(), torch.tensor(starts + lengths, dtype=torch.int32)))
+        rows, family_count, max_shared = _families(table, before, self.pool.page_size) if before is not None else (None, 0, 0)
+        # one copy to the device: [table | starts | lengths | families]
+        parts = [torch.from_numpy(table).flatten(), torch.tensor(starts + lengths, dtype=torch.int32)]
+        if family_count:
+            parts.append(torch.from_numpy(rows).flatten())
+        packed = torch.cat(parts)
         if self.keys.is_cuda:
             packed = packed.pin_memory().to(self.keys.device, non_blocking=True)
         n, width = table.shape
-        return PagedBatch(packed[:n * width].view(n, width), packed[n * width:n * width + n + 1], packed[n * width + n + 1:],
-                          max(tokens, default=0), longest)
+        at = n * width + n + 1
+        return PagedBatch(packed[:n * width].view(n, width), packed[n * width:at], packed[at:at + n], max(tokens, default=0), longest,
+                          packed[at + n:].view(n, 3) if family_count else None, family_count, max_shared)
 
     def compact(self) -> int:
         """Moves live pages to the lowest numbers -> how many moved.  Batches made before are void.  A call that raises has changed nothing."""
@@ -187,12 +242,14 @@ class PagedCache:
         return len(moves)
 
     def append(self, layer: int, qkv: torch.Tensor, batch: PagedBatch, inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
-               amplitude: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               amplitude: float = 1.0, out: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
+               k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
         """`rotary_append` into this cache."""
-        return rotary_append(qkv, self.keys[layer], self.values[layer], batch.table, batch.starts, batch.lengths, inv_freq, interleaved, amplitude, out)
+        return rotary_append(qkv, self.keys[layer], self.values[layer], batch.table, batch.starts, batch.lengths, inv_freq, interleaved, amplitude, out,
+                             q_norm, k_norm, eps)
 
     def attend(self, layer: int, q: torch.Tensor, batch: PagedBatch, scale: Optional[float] = None, causal: bool = True, window: int = 0,
-               out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """`paged_attention` over this cache."""
+               out: Optional[torch.Tensor] = None, sinks: int = 0) -> torch.Tensor:
+        """`paged_attention` over this cache, with the families of a batch made with `share`."""
         return paged_attention(q, self.keys[layer], self.values[layer], batch.table, batch.starts, batch.lengths, batch.max_tokens, batch.max_length,
-                               scale, causal, window, out)
+                               scale, causal, window, out, sinks, batch.families, batch.family_count, batch.max_shared)
