@@ -185,7 +185,7 @@ def test_workspace_does_not_grow_with_keys_that_a_window_hides(lib, dtype):
     """300 tokens that see their last 500 keys and the first 20: as much room with a table for 2^24 positions as with one for 2^12, and with the largest numbers as with
     those that hide nothing."""
     sizes = [room(lib, 1, 300, 4, 2, 64, 300, 0, 500, 20, None, dtype=dtype, pitch=pitch) for pitch in (1 << 8, 1 << 20)]
-    assert sizes[0] == sizes[1] and 0 <= sizes[0] <= 300 * 4 * 66 * 4 * 20
+    assert sizes[0] == sizes[1] and 0 < sizes[0] <= 300 * 4 * 66 * 4 * 20
     for tokens in (1, 300):
         sizes = [room(lib, 1, tokens, 4, 2, 64, tokens, 0, window, sinks, None, dtype=dtype, pitch=1 << 12)
                  for window in (1 << 22, 1 << 30, (1 << 31) + 5, (1 << 63) - 1 - tokens, (1 << 63) - 1) for sinks in (7, 1 << 20, (1 << 63) - 1)]

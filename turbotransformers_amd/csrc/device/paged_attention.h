@@ -10,6 +10,7 @@
 namespace ttmi {
 
 constexpr int kFewRows = 16;  // rows of a sequence and key/value head that are the few-rows kernel's
+constexpr int kShareStep = 128;  // keys of a family are taken in steps of this, a multiple of every tile: what is left of them is each sequence's own
 
 struct PagedArgs {
   const void *q, *keys, *values;
@@ -26,26 +27,56 @@ struct PagedArgs {
   // ordered: its workgroups begin with those that have the most keys.
   int splits, waves, few, chunk, ordered;
   float* partial;  // sums of rows whose keys are several workgroups' [..][d], behind them the maxima and sums of their probabilities [..][2]
+  // Of the kernels that know of first keys that stay visible and of families (SIGHT).
+  int sinks;
+  const int32_t* families;  // null: none
+  // Keys of families are cut like those of sequences with many rows; family_blocks blocks of 128 rows at a time are worked on.
+  int family_chunk, family_splits, family_blocks;
+  // With families `partial` holds the rows of all results that are joined: those of the few-rows kernel (2 splits kFewRows), and from these on, for each row of q and head:
+  int64_t own_at, family_at, whole_at, rows;  // of a sequence's own keys in parts, of its family's in parts, of its own where one workgroup had them all; the end
 };
 
 struct Reach {
   int begin, end;  // keys
+  int low;         // SIGHT: keys below, from the sequence's own first on, are seen besides
 };
 struct Sequence {
   int start, tokens, length, first;  // its first row, new tokens, keys, position of the first new token
+  int base = 0;                      // SIGHT: keys below are its family's
   __device__ __forceinline__ Reach reach(const PagedArgs& a, int token) const {
     const int position = first + token;
     Reach r;
     r.begin = a.window > 0 ? max(0, position - a.window + 1) : 0;
     r.end = a.causal ? max(0, min(length, position + 1)) : length;
     if (r.begin >= r.end) r.begin = r.end = 0;
+    r.low = 0;
     return r;
+  }
+  // The same with the first keys that stay visible, of the sequence's own keys alone (where it sees none of them, begin, end and low are `base`); all ends rise with the token.
+  __device__ __forceinline__ Reach own_reach(const PagedArgs& a, int token) const {
+    Reach r = reach(a, token);
+    r.low = max(base, a.window > 0 ? min(a.sinks, r.end) : 0);
+    r.end = max(base, r.end);
+    r.begin = min(max(base, r.begin), r.end);
+    return r;
+  }
+  template <bool SIGHT>
+  __device__ __forceinline__ Reach reach_of(const PagedArgs& a, int token) const {
+    if constexpr (SIGHT) return own_reach(a, token);
+    else return reach(a, token);
   }
   // keys of a part (tiles).  A window's keys begin anywhere in a part, and so touch one more than they fill.
   __device__ __forceinline__ int chunk(const PagedArgs& a) const {
     if (a.splits <= 1) return INT32_MAX;
     const int seen = a.window > 0 ? min(length, a.window + tokens) : length, full = a.splits - (a.window > 0 ? 1 : 0);
     return max(a.chunk, ((seen + full - 1) / full + 63) & ~63);
+  }
+  // SIGHT: the same of the keys that a block of its rows sees, laid behind each other (Span): whole tiles of first keys, a window that begins anywhere in a tile.
+  __device__ __forceinline__ int span_chunk(const PagedArgs& a) const {
+    if (a.splits <= 1) return INT32_MAX;
+    const int own = max(0, length - base);
+    const int seen = a.window > 0 ? (int)min((int64_t)own, (int64_t)max(0, a.sinks - base) + a.window + tokens + 128) : own;
+    return max(a.chunk, ((seen + a.splits - 1) / a.splits + 63) & ~63);
   }
 };
 __device__ __forceinline__ Sequence sequence(const PagedArgs& a, int b) {
@@ -56,6 +87,109 @@ __device__ __forceinline__ Sequence sequence(const PagedArgs& a, int b) {
   s.first = length - s.tokens;
   s.length = max(0, (int)min((int64_t)length, a.view.table_pitch << a.view.page_shift));
   return s;
+}
+
+
+// Keys that a block of rows sees: those from first to end, of which all rows see those from sure_first to sure_end; SIGHT: and those below low, of which all see those below
+// sure_low.
+struct Sight {
+  int first, end, sure_first, sure_end, low, sure_low;
+};
+// Of rows whose ends rise from the first to the last.  (A row without keys, before the first one that has some, begins and ends where the sequence's own keys do.)
+__device__ __forceinline__ Sight sight_of(const Reach& first_row, const Reach& last_row) {
+  Sight s;
+  s.first = first_row.begin, s.end = max(first_row.end, last_row.end), s.sure_first = last_row.begin, s.sure_end = first_row.end;
+  s.low = max(first_row.low, last_row.low), s.sure_low = min(first_row.low, last_row.low);
+  return s;
+}
+template <bool SIGHT>
+__device__ __forceinline__ bool all_see(const Sight& s, int key, int keys) {
+  return (key >= s.sure_first && key + keys <= s.sure_end) || (SIGHT && key + keys <= s.sure_low);
+}
+template <bool SIGHT>
+__device__ __forceinline__ bool some_see(const Sight& s, int key) {
+  return (key >= s.first && key < s.end) || (SIGHT && key < s.low);
+}
+template <bool SIGHT>
+__device__ __forceinline__ bool sees(const Reach& r, int key) {
+  return (key >= r.begin && key < r.end) || (SIGHT && key < r.low);
+}
+// SIGHT: whole tiles of the first keys that some row sees and, right behind them, whole tiles of the others: places lo to hi, the tile at a place holds the keys from key_at on.
+struct Span {
+  int lo, hi, seam, skip;
+  __device__ __forceinline__ int key_at(int place) const { return place + (place >= seam ? skip : 0); }
+  __device__ __forceinline__ int place_of(int key) const { return key - (key >= seam + skip ? skip : 0); }
+};
+template <int TILE>
+__device__ __forceinline__ Span span_of(const Sight& s, int base) {
+  Span span;
+  const int start = s.first & ~(TILE - 1);
+  if (s.low <= base) return {start, s.end, 0, 0};
+  span.seam = (s.low + TILE - 1) & ~(TILE - 1);
+  span.skip = max(0, start - span.seam);
+  span.lo = base, span.hi = s.end - span.skip;
+  return span;
+}
+
+// A family: sequences that follow one another and begin with the same keys.  What the rows of `families` say counts where the first sequence of a family and
+// another one agree on it, so that no key is left out or read twice whatever they hold.
+struct Family {
+  int first, end, keys;  // sequences; keys in common, a multiple of kShareStep, 0: no family
+};
+__device__ __forceinline__ Family family_led_by(const PagedArgs& a, int b) {
+  const PagedView& view = a.view;
+  const int32_t* const row = a.families + 3 * (int64_t)b;
+  Family f;
+  f.first = b, f.end = min(row[1], view.batch);
+  const int held = (int)min((int64_t)view.lengths[b], view.table_pitch << view.page_shift);
+  f.keys = row[0] == b && f.end > b + 1 ? max(0, min(row[2], held)) & ~(kShareStep - 1) : 0;
+  return f;
+}
+// The number of the first sequence of b's family, where that is one, and its keys (0: b is on its own).
+__device__ __forceinline__ int shared_keys(const PagedArgs& a, int b, int* first) {
+  *first = a.families[3 * (int64_t)b];
+  if ((unsigned)*first > (unsigned)b) return 0;
+  const Family f = family_led_by(a, *first);
+  return b < f.end ? f.keys : 0;
+}
+template <bool SIGHT>
+__device__ __forceinline__ Sequence sequence_of_batch(const PagedArgs& a, int b) {
+  Sequence s = sequence(a, b);
+  if constexpr (SIGHT) {
+    int first;
+    if (a.families != nullptr) s.base = shared_keys(a, b, &first);
+  }
+  return s;
+}
+// A family as a sequence: the rows of all of its sequences over the keys they have in common.
+__device__ __forceinline__ Sequence family_sequence(const PagedArgs& a, const Family& f) {
+  Sequence s;
+  s.start = max(0, a.view.starts[f.first]);
+  s.tokens = f.keys > 0 ? max(0, min(a.view.starts[f.end], a.view.tokens) - s.start) : 0;
+  s.length = f.keys, s.first = 0;
+  return s;
+}
+// The sequence of a family that a row of q belongs to, each lane's own.  Where each has one new token that is one trip to memory.
+__device__ __forceinline__ int member_of(const PagedArgs& a, const Family& f, int start, int row) {
+  const int32_t* const starts = a.view.starts;
+  int lo = min(f.first + row - start, f.end - 1), hi = f.end;
+  if (starts[lo] <= row && starts[lo + 1] > row) return lo;
+  lo = f.first;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= row) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+// What a row of member b sees of its family's keys.
+__device__ __forceinline__ Reach family_reach(const PagedArgs& a, const Family& f, int b, int row) {
+  const Sequence s = sequence(a, b);
+  Reach r = s.reach(a, row - s.start);
+  r.low = min(f.keys, a.window > 0 ? min(a.sinks, r.end) : 0);
+  r.end = min(f.keys, r.end);
+  r.begin = min(r.begin, r.end);
+  return r;
 }
 
 // The pages that a wavefront is about to read, 64 of them, a lane each: where their rows of one key/value head begin; and the numbers of the 64 behind those, which are on
@@ -248,5 +382,15 @@ __device__ __forceinline__ void join_parts_by_wavefront(const float* partial, co
 
 int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream);
 int launch_tiles(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream);
+
+// How the work of a call is laid out: `tiles` takes families and sequences with many rows, `few` the others.
+struct SightLaunch {
+  PagedArgs tiles, few;
+  bool run_tiles, run_few;
+  int own_blocks;  // blocks of 128 rows of sequences' own keys
+};
+void launch_sight_f16(const SightLaunch& l, int64_t head_dim, hipStream_t stream);
+void launch_sight_bf16(const SightLaunch& l, int64_t head_dim, hipStream_t stream);
+void launch_sight_f32(const SightLaunch& l, int64_t head_dim, hipStream_t stream);
 
 }  // namespace ttmi

@@ -75,6 +75,66 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   return p;
 }
 
+// With first keys that stay visible and with families.  The sequences' own keys are cut as ever (their number is guessed from max_length: a sequence on its own may be that long); families
+// have blocks of 128 rows each, of which the few tokens of a decoding batch fill one or two, and their keys are cut to match.
+struct SightPlan {
+  PagedPlan own;
+  int family_chunk, family_splits, family_blocks, own_blocks;
+  int64_t few_rows, own_rows, family_rows, whole_rows, floats;  // of the workspace
+};
+SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, const ttmi_paged_sight& sight, int dtype) {
+  SightPlan p;
+  const int64_t sinks = std::min(sight.sinks, kWidest), window = sight.window > 0 ? std::min(std::min(sight.window, kWidest) + sinks + 128, kWidest) : 0;
+  p.own = plan(view, heads, max_tokens, max_length, window, dtype);
+  const int64_t group = heads / view.kv_heads, tokens = view.tokens, d = view.head_dim;
+  p.own_blocks = p.own.tiles ? (int)(tokens * group / 128 + std::min<int64_t>(view.batch, tokens)) : 0;
+  p.family_chunk = p.family_splits = 1, p.family_blocks = 0, p.family_rows = p.whole_rows = 0;
+  const bool families = sight.families != nullptr;
+  if (families) {
+    const int64_t held = view.table_pitch << view.page_shift, shared = std::max<int64_t>(1, sight.max_shared > 0 ? std::min(sight.max_shared, held) : held);
+    const int64_t blocks = tokens * group / 128 + std::max<int64_t>(1, std::min<int64_t>(sight.family_count, view.batch / 2));
+    cut(view.kv_heads * blocks, dtype == TTMI_F32 ? 64 : 256, shared, false, &p.family_chunk, &p.family_splits);
+    p.family_blocks = (int)blocks;
+    p.family_rows = tokens * heads * p.family_splits;
+    p.whole_rows = p.own.few ? tokens * heads : 0;
+  }
+  p.few_rows = p.own.few ? 2ll * p.own.few_splits * kFewRows : 0;
+  p.own_rows = p.own.tiles && (families || p.own.tile_splits > 1) ? tokens * heads * p.own.tile_splits : 0;
+  p.floats = (p.few_rows + p.own_rows + p.family_rows + p.whole_rows) * (d + 2);
+  return p;
+}
+
+int check_sight(const ttmi_paged_sight* sight) {
+  TTMI_REQUIRE(sight != nullptr, "sight is null");
+  TTMI_REQUIRE(sight->window >= 0 && sight->sinks >= 0 && sight->family_count >= 0 && sight->max_shared >= 0,
+               "window, sinks, family_count and max_shared must not be negative");
+  TTMI_REQUIRE((reinterpret_cast<uintptr_t>(sight->families) & 3) == 0, "families is not aligned to its elements");
+  return 0;
+}
+
+// What both forms of the call check; the arguments that they have in common.
+int attention_args(const void* q, int64_t q_pitch, void* out, int64_t out_pitch, int64_t heads, const ttmi_paged_cache* cache, const ttmi_paged_batch* batch,
+                   int64_t max_tokens, int64_t max_length, float scale, int causal, int64_t window, int dtype, PagedArgs* a) {
+  if (int rc = paged_view(cache, batch, heads, &a->view)) return rc;
+  const int64_t d = cache->head_dim;
+  TTMI_REQUIRE(d == 64 || d == 128, "paged attention needs head_dim 64 or 128");
+  TTMI_REQUIRE(q_pitch >= heads * d && out_pitch >= heads * d, "rows overlap: a pitch is too small");
+  TTMI_REQUIRE(dtype == TTMI_F32 || dtype == TTMI_F16 || dtype == TTMI_BF16, "unsupported dtype");
+  TTMI_REQUIRE(window >= 0 && max_tokens >= 0 && max_length >= 0, "window, max_tokens and max_length must not be negative");
+  // (a launch has less than 2^32 threads: 512 of them for a sequence and key/value head, or 256 for 128 rows besides)
+  TTMI_REQUIRE(batch->tokens * heads < 1 << 30 && batch->batch * cache->kv_heads < 1 << 23, "more rows or sequences than one launch takes");
+  a->scale_log2e = scale * 1.4426950408889634f;
+  TTMI_REQUIRE(scale > 0.f && a->scale_log2e <= std::numeric_limits<float>::max(), "scale must be positive, and finite times log2(e)");
+  if (batch->tokens == 0 || batch->batch == 0) return 0;
+  TTMI_REQUIRE(q != nullptr && out != nullptr, "q or out is null");
+  TTMI_REQUIRE(rows_aligned(q, q_pitch, dtype) && rows_aligned(out, out_pitch, dtype), "rows of q and out must be 16-byte aligned");
+  a->q = q, a->out = out, a->keys = cache->keys, a->values = cache->values, a->q_pitch = q_pitch, a->out_pitch = out_pitch;
+  a->heads = (int)heads, a->group = (int)(heads / cache->kv_heads), a->causal = causal != 0;
+  a->window = (int)std::min(window, kWidest);
+  a->sinks = 0, a->families = nullptr;
+  return 0;
+}
+
 }  // namespace
 }  // namespace ttmi
 
@@ -99,27 +159,13 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
                          const ttmi_paged_batch* batch, int64_t max_tokens, int64_t max_length, float scale, int causal, int64_t window,
                          void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
   PagedArgs a;
-  if (int rc = paged_view(cache, batch, heads, &a.view)) return rc;
-  const int64_t d = cache->head_dim;
-  TTMI_REQUIRE(d == 64 || d == 128, "paged attention needs head_dim 64 or 128");
-  TTMI_REQUIRE(q_pitch >= heads * d && out_pitch >= heads * d, "rows overlap: a pitch is too small");
-  TTMI_REQUIRE(dtype == TTMI_F32 || dtype == TTMI_F16 || dtype == TTMI_BF16, "unsupported dtype");
-  TTMI_REQUIRE(window >= 0 && max_tokens >= 0 && max_length >= 0, "window, max_tokens and max_length must not be negative");
-  // (a launch has less than 2^32 threads: 512 of them for a sequence and key/value head, or 256 for 128 rows besides)
-  TTMI_REQUIRE(batch->tokens * heads < 1 << 30 && batch->batch * cache->kv_heads < 1 << 23, "more rows or sequences than one launch takes");
-  const float scale_log2e = scale * 1.4426950408889634f;
-  TTMI_REQUIRE(scale > 0.f && scale_log2e <= std::numeric_limits<float>::max(), "scale must be positive, and finite times log2(e)");
+  if (int rc = attention_args(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, window, dtype, &a)) return rc;
   if (batch->tokens == 0 || batch->batch == 0) return 0;
-  TTMI_REQUIRE(q != nullptr && out != nullptr, "q or out is null");
-  TTMI_REQUIRE(rows_aligned(q, q_pitch, dtype) && rows_aligned(out, out_pitch, dtype), "rows of q and out must be 16-byte aligned");
+  const int64_t d = cache->head_dim;
   const PagedPlan p = plan(a.view, heads, max_tokens, max_length, window, dtype);
   const int64_t bytes = (p.few_floats + p.tile_floats) * 4;
   TTMI_REQUIRE(bytes == 0 || (workspace != nullptr && workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                "the workspace is too small or not 16-byte aligned");
-  a.q = q, a.out = out, a.keys = cache->keys, a.values = cache->values, a.q_pitch = q_pitch, a.out_pitch = out_pitch;
-  a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads), a.causal = causal != 0;
-  a.window = (int)std::min(window, kWidest);
-  a.scale_log2e = scale_log2e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.tiles) {
     a.every = !p.few, a.chunk = p.tile_chunk, a.splits = p.tile_splits;
@@ -132,6 +178,46 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
     if (int rc = launch_few_rows(a, dtype, d, s)) return rc;
   }
   return 0;
+}
+
+int ttmi_paged_attention_sight_workspace(const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, int64_t heads, int64_t max_tokens, int64_t max_length,
+                                         const ttmi_paged_sight* sight, int dtype, int64_t* bytes) {
+  if (int rc = check_sight(sight)) return rc;
+  if (sight->families == nullptr && (sight->sinks == 0 || sight->window == 0))
+    return ttmi_paged_attention_workspace(cache, batch, heads, max_tokens, max_length, sight->window, dtype, bytes);
+  PagedView view;
+  TTMI_REQUIRE(bytes != nullptr, "bytes is null");
+  if (int rc = paged_view(cache, batch, heads, &view)) return rc;
+  TTMI_REQUIRE(max_tokens >= 0 && max_length >= 0, "max_tokens and max_length must not be negative");
+  *bytes = batch->tokens == 0 || batch->batch == 0 ? 0 : plan_sight(view, heads, max_tokens, max_length, *sight, dtype).floats * 4;
+  return 0;
+}
+
+int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_t out_pitch, int64_t heads, const ttmi_paged_cache* cache,
+                               const ttmi_paged_batch* batch, int64_t max_tokens, int64_t max_length, float scale, int causal, const ttmi_paged_sight* sight,
+                               void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  if (int rc = check_sight(sight)) return rc;
+  if (sight->families == nullptr && (sight->sinks == 0 || sight->window == 0))
+    return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, sight->window, workspace, workspace_bytes,
+                                dtype, stream);
+  SightLaunch l;
+  PagedArgs& a = l.tiles;
+  if (int rc = attention_args(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, sight->window, dtype, &a)) return rc;
+  if (batch->tokens == 0 || batch->batch == 0) return 0;
+  const SightPlan p = plan_sight(a.view, heads, max_tokens, max_length, *sight, dtype);
+  TTMI_REQUIRE(p.floats == 0 || (workspace != nullptr && workspace_bytes >= p.floats * 4 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+               "the workspace is too small or not 16-byte aligned");
+  a.sinks = (int)std::min(sight->sinks, kWidest), a.families = sight->families;
+  a.partial = static_cast<float*>(workspace);
+  a.every = !p.own.few, a.chunk = p.own.tile_chunk, a.splits = p.own.tile_splits, a.ordered = 1;
+  a.family_chunk = p.family_chunk, a.family_splits = p.family_splits, a.family_blocks = p.family_blocks;
+  a.own_at = p.few_rows, a.family_at = a.own_at + p.own_rows, a.whole_at = a.family_at + p.family_rows, a.rows = a.whole_at + p.whole_rows;
+  l.few = a;
+  l.few.every = !p.own.tiles, l.few.few = p.own.few_rows, l.few.splits = p.own.few_splits, l.few.waves = p.own.few_waves;
+  l.run_tiles = p.own.tiles || p.family_blocks > 0, l.run_few = p.own.few, l.own_blocks = p.own_blocks;
+  const auto launch = dtype == TTMI_F32 ? launch_sight_f32 : dtype == TTMI_F16 ? launch_sight_f16 : launch_sight_bf16;
+  launch(l, cache->head_dim, static_cast<hipStream_t>(stream));
+  return launch_status("paged_attention_sight");
 }
 
 }  // extern "C"

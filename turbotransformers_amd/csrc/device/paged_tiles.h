@@ -1,0 +1,522 @@
+// Attention over pages where sequences have many rows (new tokens times query heads of a key/value head): prompts and chunks of them.
+//
+// The matrix instructions bound it, and with them the exponentials and what LDS can feed.  A workgroup has 128 rows of one sequence and head, 32 a wavefront, and
+// walks over tiles of 64 keys (fp32: 32) that all four share in LDS, fetched into registers one ahead and stored while the other stage is worked on.
+// Scores are computed transposed, St[key, row] = K . Q^T (v_mfma_f32_32x32x16, fp32: 32x32x2), so a lane has one row, its statistics need one exchange of the two
+// half-wavefronts, and the probabilities lie in the accumulators as Ot[d, row] += Vt . Pt wants them; Vt is what the transposing reads give of values that lie in LDS
+// row by row as in the cache (fp32: plain reads of a column).  Packing a group's heads into one tile of rows reads the keys of a head once for all of them and keeps
+// tiles full whatever the group.
+//
+// Measured, 32 query and 8 key heads of 128, bf16: a prompt of 8192 tokens 580 to 620 us (0.89 to 0.94 PFLOP/s; a large product here 1.26).  Of a SIMD's 1.19e6 cycles
+// the matrix pipe is busy for 0.53e6 and vector instructions, the exponentials first, are at work for as many: the two hardly overlap.  Power comes second: on zeros the same launch takes 530 to 565 us.
+// Heads of 64: 343 us (0.80), where an exponential takes a lane as long as its share of the products.  A workgroup by itself takes about 7 us to
+// its first tile and 0.95 a tile of 64 keys, heads of 64, where four instructions' worth of products would be 0.2: a chain of reads, products, maximum, exponentials, products.
+// The last blocks of a launch run on few CUs: 6 chunks of 400 to 600 tokens behind up to 9000 keys 220 us (0.85 PFLOP/s), 93 tiles for each of 512 places, 125 in the longest block.
+// fp32 with heads of 128 has no registers left (256 and 96 bytes of scratch a lane): a prompt of 1000 tokens 153 us.
+// What was built and taken out: 256 rows a workgroup with the products of 32 keys beside the exponentials of the 32 before, level to 3 % faster for heads of 128, 2 % slower for those of 64.
+//
+// SIGHT: rows that see the first keys of their sequence besides a window (the keys that a block sees lie behind each other in whole tiles, Span), sequences whose first keys are their family's,
+// and families: the rows of all sequences of one over the keys that they have in common, each of which sees what its own position lets it see.
+#pragma once
+
+#include "paged_attention.h"
+
+namespace ttmi {
+namespace {
+
+constexpr int kTileRows = 128;  // of a workgroup
+constexpr int kSpanTiles = 64;  // a tile or two
+// Keys of a part of a family's, which has at most a.family_splits of them.
+__device__ __forceinline__ int family_chunk(const PagedArgs& a, const Sequence& family) {
+  return max(a.family_chunk, ((family.length + a.family_splits - 1) / a.family_splits + 63) & ~63);
+}
+// Parts that a row's own keys lie in (1 where it sees none of them).
+__device__ __forceinline__ int own_parts(const Reach& r, const Span& span, int base, int chunk) {
+  return r.end > base ? (span.place_of(r.end - 1) - span.lo) / chunk + 1 : 1;
+}
+
+template <typename T, int D>
+struct Tiles {
+  static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // (a part of kSpanTiles)
+  static constexpr int kSubs = kKeys / 32;
+  static constexpr int kElems = 16 / (int)sizeof(T);
+  static constexpr int kRowBytes = D * (int)sizeof(T);
+  static constexpr int kBytes = kKeys * kRowBytes;      // of a tile of keys, or of values
+  static constexpr int kPieces = kBytes / 4096;         // 16-byte pieces of a tile per thread
+  static constexpr int kSteps = kRowBytes / 32;         // pieces of a row per lane, for the first product
+  static constexpr int kOut = D / 32;
+  // Tiles on their way in registers.  us, 6 chunks of 400 to 600 tokens behind 1500 to 9000 keys, 32 query and 8 key heads of 64, one / two: fp32 936 / 838, bf16 151 / 154
+  // (head_dim 128 has no registers for two).
+  static constexpr int kDepth = sizeof(T) == 4 && D == 64 ? 2 : 1;
+};
+
+// Places of a row's 16-byte pieces in LDS.  Keys: sixteen rows read the same piece at a time.  Values: 64 bytes of four rows at a time (fp32: 128 bytes of two rows that lie
+// four apart).  The exclusive or takes them to different banks.
+template <typename T, int D>
+__device__ __forceinline__ int key_piece(int row, int piece) {
+  if constexpr (sizeof(T) == 2 && D == 64) return piece ^ ((row >> 1) & 7);
+  else return piece ^ (row & 15);
+}
+template <typename T, int D>
+__device__ __forceinline__ int tile_value_piece(int row, int piece) {
+  if constexpr (sizeof(T) == 4) return piece ^ (((row >> 2) & 1) << 3);
+  else if constexpr (D == 128) return piece ^ ((row & 3) << 2);
+  else return piece ^ (((row >> 1) & 1) << 2);
+}
+
+// A row's sums, divided and stored.
+template <typename T, int D>
+__device__ __forceinline__ void store_out(const PagedArgs& a, int64_t token, int head, bool sees, int lhalf, const floatx16 (&ot)[D / 32], float sum) {
+  const float inv = inverse_sum(sum, sees);
+  T* to = static_cast<T*>(a.out) + token * a.out_pitch + (int64_t)head * D + 4 * lhalf;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      Vec<T, 4> x;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x.v[c] = from_float<T>(ot[t][4 * g + c] * inv);
+      store_vec<T, 4>(to + 32 * t + 8 * g, x);
+    }
+}
+// The same where the row's keys lie in several parts: kept for the kernel that joins those, in row `at` of `rows` partial results.
+template <int D>
+__device__ __forceinline__ void store_part(const PagedArgs& a, int64_t at, int64_t rows, int lhalf, const floatx16 (&ot)[D / 32], float top, float sum) {
+  float* to = a.partial + at * D + 4 * lhalf;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<floatx4*>(to + 32 * t + 8 * g) = floatx4{ot[t][4 * g], ot[t][4 * g + 1], ot[t][4 * g + 2], ot[t][4 * g + 3]};
+  if (lhalf == 0) {
+    float* ml = a.partial + rows * D + at * 2;
+    ml[0] = top, ml[1] = sum;
+  }
+}
+
+// The `want`-th block of rows of all sequences -> its sequence and number in it (false: there are fewer).  Every lane looks at a sequence of 64.
+// Where there are more workgroups than the chip takes at a time, those with the most keys come first: sequences by their keys (64 of them at a time), and in a sequence the
+// last rows, which have the most keys before them.
+// SIGHT: those of families, or of the sequences' own keys; *upto: a number from which on there are none.
+template <bool SIGHT>
+__device__ __forceinline__ bool find_block(const PagedArgs& a, int want, bool families, int* b, int* block, int* upto) {
+  const int lane = (int)(threadIdx.x % kWave);
+  int passed = 0;
+  for (int base = 0; base < a.view.batch; base += kWave) {
+    int blocks = 0, reach = 0;
+    if (SIGHT && families) {
+      if (base + lane < a.view.batch) {
+        const Sequence seq = family_sequence(a, family_led_by(a, base + lane));
+        blocks = (seq.tokens * a.group + kTileRows - 1) / kTileRows, reach = seq.length;
+      }
+    } else if (base + lane < a.view.batch) {
+      const Sequence seq = sequence(a, base + lane);
+      const int rows = seq.tokens * a.group;
+      if (rows > kFewRows || a.every) blocks = (rows + kTileRows - 1) / kTileRows;
+      reach = a.window > 0 ? min(seq.length, a.window + seq.tokens) : seq.length;
+    }
+    int before = 0, all = 0;
+    if (!a.ordered) {
+      int upto = blocks;
+#pragma unroll
+      for (int d = 1; d < kWave; d *= 2) {
+        const int below = __shfl_up(upto, d, kWave);
+        if (lane >= d) upto += below;
+      }
+      before = upto - blocks, all = __builtin_amdgcn_readlane(upto, kWave - 1);
+    } else {
+      for (uint64_t others = __ballot(blocks > 0); others != 0; others &= others - 1) {
+        const int j = __ffsll((unsigned long long)others) - 1;
+        const int their_blocks = __builtin_amdgcn_readlane(blocks, j), their_reach = __builtin_amdgcn_readlane(reach, j);
+        all += their_blocks;
+        if (their_reach > reach || (their_reach == reach && j < lane)) before += their_blocks;
+      }
+    }
+    if (want < all) {
+      const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(want >= before && want < before + blocks)) - 1);
+      *b = base + found;
+      *block = __builtin_amdgcn_readlane(before + blocks, found) - 1 - want;
+      if constexpr (SIGHT) *upto = base + kWave < a.view.batch ? INT32_MAX : passed + all;
+      return true;
+    }
+    want -= all, passed += all;
+  }
+  return false;
+}
+
+template <typename T, int D>
+struct TilesShared {
+  __align__(16) char tiles[4 * Tiles<T, D>::kBytes];
+  int wild;  // whether values that only some rows see hold infinities or NaNs
+  int sights[4][6];  // of a family's rows, wavefront by wavefront
+};
+
+// What the rows of a family that a wavefront's lanes have see (`live`: this lane has one), and what all rows of the workgroup do.  Mostly everything.
+template <typename Shared>
+__device__ __forceinline__ void family_sights(const Family& f, const Reach& mine, bool live, int wave, Shared& shared, Sight* of_wave, Sight* of_all) {
+  Sight s = {0, f.keys, 0, f.keys, 0, 0};
+  if (!__all(!live || (mine.begin == 0 && mine.end == f.keys && mine.low == 0))) {
+    s.first = live ? mine.begin : INT32_MAX, s.end = live ? mine.end : 0, s.sure_first = live ? mine.begin : 0, s.sure_end = live ? mine.end : INT32_MAX;
+    s.low = live ? mine.low : 0, s.sure_low = live ? mine.low : INT32_MAX;
+#pragma unroll 1
+    for (int d = 1; d < kWave; d *= 2) {
+      s.first = min(s.first, __shfl_xor(s.first, d, kWave)), s.end = max(s.end, __shfl_xor(s.end, d, kWave));
+      s.sure_first = max(s.sure_first, __shfl_xor(s.sure_first, d, kWave)), s.sure_end = min(s.sure_end, __shfl_xor(s.sure_end, d, kWave));
+      s.low = max(s.low, __shfl_xor(s.low, d, kWave)), s.sure_low = min(s.sure_low, __shfl_xor(s.sure_low, d, kWave));
+    }
+    s = {__builtin_amdgcn_readfirstlane(s.first), __builtin_amdgcn_readfirstlane(s.end), __builtin_amdgcn_readfirstlane(s.sure_first),
+         __builtin_amdgcn_readfirstlane(s.sure_end), __builtin_amdgcn_readfirstlane(s.low), __builtin_amdgcn_readfirstlane(s.sure_low)};
+  } else if (!__any(live)) s = {INT32_MAX, 0, 0, INT32_MAX, 0, INT32_MAX};
+  *of_wave = s;
+  const int lane = (int)(threadIdx.x % kWave);
+  if (lane == 0) {
+    int* const to = shared.sights[wave];
+    to[0] = s.first, to[1] = s.end, to[2] = s.sure_first, to[3] = s.sure_end, to[4] = s.low, to[5] = s.sure_low;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int* const from = shared.sights[w];
+    s.first = min(s.first, from[0]), s.end = max(s.end, from[1]), s.sure_first = max(s.sure_first, from[2]), s.sure_end = min(s.sure_end, from[3]);
+    s.low = max(s.low, from[4]), s.sure_low = min(s.sure_low, from[5]);
+  }
+  *of_all = {__builtin_amdgcn_readfirstlane(s.first), __builtin_amdgcn_readfirstlane(s.end), __builtin_amdgcn_readfirstlane(s.sure_first),
+             __builtin_amdgcn_readfirstlane(s.sure_end), __builtin_amdgcn_readfirstlane(s.low), __builtin_amdgcn_readfirstlane(s.sure_low)};
+}
+
+// Part `z` of block `want` of rows -> a number from which on there are none; SIGHT: of families, or of the sequences' own keys.  SMALL: pages of fewer than 16 slots
+template <typename T, int D, bool SMALL, bool SIGHT>
+__device__ __forceinline__ int tiles(const PagedArgs& a, int want, int kv_head, int z, bool families, TilesShared<T, D>& shared) {
+  using S = Tiles<T, D>;
+  char* const smem = shared.tiles;
+  int& wild = shared.wild;
+  const PagedView& view = a.view;
+  int b, block, upto = 0;
+  if (!find_block<SIGHT>(a, want, families, &b, &block, &upto)) return 0;
+  Family family{};
+  Sequence seq;
+  if (SIGHT && families) {
+    family = family_led_by(a, b);
+    seq = family_sequence(a, family);
+  } else seq = sequence_of_batch<SIGHT>(a, b);
+  const int row0 = block * kTileRows, rows = min(kTileRows, seq.tokens * a.group - row0);
+  if (z == 0 && kv_head == 0 && block == 0 && threadIdx.x == 0 && !families && view.lengths[b] > seq.length) page_error(view);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lrow = lane & 31, lhalf = lane >> 5;
+  const T* const keys = static_cast<const T*>(a.keys);
+  const T* const values = static_cast<const T*>(a.values);
+  const int wave_rows = max(0, min(32, rows - wave * 32));
+  const int wrow = row0 + wave * 32;
+  bool live = lrow < wave_rows;
+  const int token = (wrow + (live ? lrow : 0)) / a.group, head = kv_head * a.group + (live ? wrow + lrow - token * a.group : 0);
+  // what the rows of the workgroup see, and those of this wavefront
+  Reach mine;
+  Sight sight, wave_sight;
+  if (SIGHT && families) {
+    const int row = seq.start + (wave_rows > 0 ? token : 0), member = member_of(a, family, seq.start, row);
+    mine = family_reach(a, family, member, row);
+    live = live && a.families[3 * (int64_t)member] == family.first;  // (others' rows are not this family's, whatever it says)
+    family_sights(family, mine, live, wave, shared, &wave_sight, &sight);
+  } else {
+    mine = seq.reach_of<SIGHT>(a, token);
+    sight = sight_of(seq.reach_of<SIGHT>(a, row0 / a.group), seq.reach_of<SIGHT>(a, (row0 + rows - 1) / a.group));
+    wave_sight = sight_of(seq.reach_of<SIGHT>(a, wrow / a.group), seq.reach_of<SIGHT>(a, (wrow + max(wave_rows, 1) - 1) / a.group));
+    if (wave_rows <= 0) wave_sight.end = wave_sight.low = 0;
+  }
+  // its part of them; SIGHT: places
+  int chunk, part0, part, lo, hi;
+  Span span;
+  if constexpr (!SIGHT) {
+    chunk = seq.chunk(a);
+    part0 = sight.first / chunk, part = part0 + z;
+    lo = (int)max(part * (int64_t)chunk, (int64_t)(sight.first & ~(S::kKeys - 1))), hi = (int)min((part + 1) * (int64_t)chunk, (int64_t)sight.end);
+    if (lo >= hi && part != part0) return upto;
+  } else {
+    part0 = 0, part = z;
+    if (families) {  // all rows of a family have the same parts, and write them
+      chunk = family_chunk(a, seq);
+      span = {0, 0, 0, 0};
+      if (z * (int64_t)chunk >= seq.length) return upto;
+      lo = z * chunk, hi = (int)min((z + 1) * (int64_t)chunk, (int64_t)seq.length);
+      if (a.window > 0) {  // of this part: the first keys that stay visible, the windows' or, from the one to the other, both
+        if (lo >= sight.low) lo = max(lo, min(hi, sight.first & ~(S::kKeys - 1)));
+        hi = min(hi, sight.end);
+        if (hi <= sight.first) hi = min(hi, sight.low);
+        hi = max(lo, hi);
+      }
+    } else {
+      chunk = seq.span_chunk(a);
+      span = span_of<kSpanTiles>(sight, seq.base);
+      lo = (int)min(span.lo + part * (int64_t)chunk, (int64_t)span.hi), hi = (int)min(span.lo + (part + 1) * (int64_t)chunk, (int64_t)span.hi);
+      if (lo >= hi && part != 0) return upto;
+    }
+  }
+  auto key_at = [&](int place) __attribute__((always_inline)) {
+    if constexpr (SIGHT) return span.key_at(place);
+    else return place;
+  };
+
+  u32x4 qf[S::kSteps];
+#pragma unroll
+  for (int i = 0; i < S::kSteps; ++i) {
+    qf[i] = u32x4{0u, 0u, 0u, 0u};
+    if (live) qf[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + (seq.start + token) * a.q_pitch + (int64_t)head * D + (2 * i + lhalf) * S::kElems);
+  }
+  floatx16 ot[S::kOut];
+#pragma unroll
+  for (int t = 0; t < S::kOut; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ot[t][e] = 0.f;
+  float top = -INFINITY, sum = 0.f;
+
+  PageCursor cursor;
+  cursor.table = view.table + (int64_t)b * view.table_pitch;
+  cursor.last = max(0, (sight.end - 1) >> view.page_shift);
+  cursor.first = 0, cursor.ahead = 0, cursor.at = 0;
+  u32x4 kr[S::kDepth][S::kPieces], vr[S::kDepth][S::kPieces];
+  // 16-byte pieces of a tile: thread by thread, 4 KB after 4 KB.  A wavefront's 1 KB lies in one group of 16 rows.
+  auto load_piece = [&](int i, int key, int set) __attribute__((always_inline)) {
+    if constexpr (!SMALL) {
+      const int group = (i * 4096 + wave * 1024) / (16 * S::kRowBytes) * 16;
+      const int64_t from = group_at<S::kRowBytes>(view, cursor, key + group);
+      const uint32_t in_group = (uint32_t)(i * 4096 + tid * 16) % (16 * S::kRowBytes);
+      kr[set][i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(keys) + from + in_group);
+      vr[set][i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(values) + from + in_group);
+    } else {
+      const int at = i * 4096 + tid * 16;
+      const int64_t from = row_offset<D>(view, cursor, kv_head, key + at / S::kRowBytes) + at % S::kRowBytes / (int)sizeof(T);
+      kr[set][i] = *reinterpret_cast<const u32x4*>(keys + from);
+      vr[set][i] = *reinterpret_cast<const u32x4*>(values + from);
+    }
+  };
+  auto key_stage = [&](int s) __attribute__((always_inline)) { return smem + s * 2 * S::kBytes; };
+  auto value_stage = [&](int s) __attribute__((always_inline)) { return smem + s * 2 * S::kBytes + S::kBytes; };
+  auto store_piece = [&](int i, int s, int set) __attribute__((always_inline)) {
+    const int at = i * 4096 + tid * 16, r = at / S::kRowBytes, c = at % S::kRowBytes / 16;
+    *reinterpret_cast<u32x4*>(key_stage(s) + r * S::kRowBytes + key_piece<T, D>(r, c) * 16) = kr[set][i];
+    *reinterpret_cast<u32x4*>(value_stage(s) + r * S::kRowBytes + tile_value_piece<T, D>(r, c) * 16) = vr[set][i];
+  };
+  // Keys that no row sees may hold anything: their values count as zeros.  Where only some rows see a key, infinities and NaNs of its values must not
+  // reach the others: they are left out here, noted, and added where they are seen.
+  auto partly_seen = [&](int key) __attribute__((always_inline)) { return !all_see<SIGHT>(sight, key, S::kKeys); };
+  auto clean_values = [&](int key, int set) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < S::kPieces; ++i) {
+      const int k = key + (i * 4096 + tid * 16) / S::kRowBytes;
+      if (!some_see<SIGHT>(sight, k)) vr[set][i] = u32x4{0u, 0u, 0u, 0u};
+      if (not_finite<T>(vr[set][i])) wild = 1;
+      vr[set][i] = finite_part<T>(vr[set][i]);
+    }
+  };
+  if (lo < hi) {
+    // (Loads past the last tile fetch that once more, out of L2: a load that may or may not have been sent would make the compiler wait for all of them.)
+    const int last = lo + (hi - 1 - lo) / S::kKeys * S::kKeys;
+    if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, key_at(lo));
+#pragma unroll
+    for (int i = 0; i < S::kPieces; ++i) load_piece(i, key_at(lo), 0);
+    if (tid == 0) wild = 0;
+    __syncthreads();
+    if (partly_seen(key_at(lo))) clean_values(key_at(lo), 0);
+#pragma unroll
+    for (int i = 0; i < S::kPieces; ++i) store_piece(i, 0, 0);
+#pragma unroll
+    for (int n = 1; n <= S::kDepth; ++n) {
+      const int next = key_at(min(lo + n * S::kKeys, last));
+      if constexpr (SIGHT && !SMALL) come_to<S::kRowBytes>(view, cursor, kv_head, next);
+#pragma unroll
+      for (int i = 0; i < S::kPieces; ++i) load_piece(i, next, n % S::kDepth);  // (in the same 64 pages, or SIGHT behind a gap)
+    }
+    __syncthreads();
+    // One tile; its stage is known to the compiler, so that places in LDS are fixed numbers behind one of the lane's.
+    auto work_on = [&](int place, auto stage) __attribute__((always_inline)) {
+      constexpr int s = decltype(stage)::value;
+      const int key = key_at(place);
+      // The other stage is free: what was fetched for it while the last tile was worked on goes there, and the tile behind it is sent for.
+      constexpr int set = (s + 1) % S::kDepth;
+      const int after = key_at(min(place + (1 + S::kDepth) * S::kKeys, last));
+      if constexpr (!SMALL) come_to<S::kRowBytes>(view, cursor, kv_head, after);
+      if (__builtin_expect(partly_seen(key_at(place + S::kKeys)), 0)) clean_values(key_at(place + S::kKeys), set);
+      if ((key >= wave_sight.end || key + S::kKeys <= wave_sight.first) && (!SIGHT || key >= wave_sight.low)) {  // nothing to do for this wavefront's rows
+#pragma unroll
+        for (int i = 0; i < S::kPieces; ++i) store_piece(i, s ^ 1, set);
+#pragma unroll
+        for (int i = 0; i < S::kPieces; ++i) load_piece(i, after, set);
+        __syncthreads();
+        return;
+      }
+      const char* const kt = key_stage(s);
+      const char* const vt = value_stage(s);
+      floatx16 st[S::kSubs];
+#pragma unroll
+      for (int u = 0; u < S::kSubs; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[u][e] = 0.f;
+      auto read_keys = [&](int n) __attribute__((always_inline)) {  // the operand of the n-th matrix instruction of St
+        const int r = 32 * (n % S::kSubs) + lrow;
+        return *reinterpret_cast<const u32x4*>(kt + r * S::kRowBytes + key_piece<T, D>(r, 2 * (n / S::kSubs) + lhalf) * 16);
+      };
+      // Reads run kAhead instructions before their use.  The fences keep that order: left to itself the compiler waits for each read in front of its use.
+      constexpr int kAhead = 4, kScores = S::kSubs * S::kSteps;
+      u32x4 f[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) f[n] = read_keys(n);
+#pragma unroll
+      for (int n = 0; n < kScores; ++n) {
+        st[n % S::kSubs] = mma32<T>(f[n % kAhead], qf[n / S::kSubs], st[n % S::kSubs]);
+        if (n + kAhead < kScores) f[n % kAhead] = read_keys(n + kAhead);
+        if (n < S::kPieces) store_piece(n, s ^ 1, set);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < S::kPieces; ++i) load_piece(i, after, set);
+      if (__builtin_expect(!all_see<SIGHT>(wave_sight, key, S::kKeys), 0)) {
+        const int from = mine.begin - key - 4 * lhalf, low = mine.low - key - 4 * lhalf;
+        const uint32_t span = (uint32_t)(mine.end - mine.begin);
+#pragma unroll
+        for (int u = 0; u < S::kSubs; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if ((uint32_t)(32 * u + 8 * (e / 4) + e % 4 - from) >= span && (!SIGHT || 32 * u + 8 * (e / 4) + e % 4 >= low)) st[u][e] = -INFINITY;
+      }
+      float m;
+      {
+        float part[4];  // (chains of a quarter of the length)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          part[j] = st[0][j];
+#pragma unroll
+          for (int u = 0; u < S::kSubs; ++u)
+#pragma unroll
+            for (int e = j; e < 16; e += 4) part[j] = fmaxf(part[j], st[u][e]);
+        }
+        const LanePair sw = swap_halves(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+        m = fmaxf(sw.a, sw.b);
+      }
+      const float moved = moved_reference(top, m * a.scale_log2e);
+      const float zero = moved == -INFINITY ? 0.f : moved;  // (a row that has seen no key yet)
+      const float shrink = __builtin_amdgcn_exp2f(top - zero);
+      top = moved;
+      if (__builtin_expect(__any(shrink != 1.f), 0)) {
+        sum *= shrink;
+#pragma unroll
+        for (int t = 0; t < S::kOut; ++t) ot[t] *= shrink;
+      }
+      if constexpr (sizeof(T) == 2) {
+        auto read_values = [&](int n) __attribute__((always_inline)) {  // the operand of the n-th matrix instruction of Ot: kOut of them for each 16 keys
+          const int r0 = 16 * (n / S::kOut) + 4 * lhalf + ((lane >> 2) & 3), t = n % S::kOut;
+          u32x4 v;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int r = r0 + 8 * g;
+            const u32x2 half = read_transposed(vt + r * S::kRowBytes + tile_value_piece<T, D>(r, 4 * t + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8);
+            v[2 * g] = half[0], v[2 * g + 1] = half[1];
+          }
+          return v;
+        };
+        // Probabilities, rounded to the type for the second product; their sum is that of the rounded ones, so what rounding does to all of them alike cancels.  Eight
+        // of a row's at a time are what a lane gives the instructions of 16 keys.
+        u32x4 pf[2 * S::kSubs];
+        auto probabilities = [&](int pair) __attribute__((always_inline)) {
+          float p[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[pair / 8][2 * (pair % 8) + j], a.scale_log2e, -zero));
+          pf[pair / 4][pair % 4] = pack2<T>(p[0], p[1]);
+          sum = add_pair<T>(pf[pair / 4][pair % 4], sum);
+        };
+        constexpr int kProducts = 2 * S::kSubs * S::kOut, kPairs = 8 * S::kSubs, kFirst = 4;
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) f[n] = read_values(n);
+#pragma unroll
+        for (int n = 0; n < kFirst; ++n) probabilities(n);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < kProducts; ++n) {
+          ot[n % S::kOut] = mma32<T>(f[n % kAhead], pf[n / S::kOut], ot[n % S::kOut]);
+          if (n + kAhead < kProducts) f[n % kAhead] = read_values(n + kAhead);
+          // the next 16 keys' probabilities beside this 16 keys' instructions
+          if (n / S::kOut + 1 < 2 * S::kSubs) {
+            constexpr int kEach = 4 / S::kOut;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) probabilities(kFirst + n * kEach + j);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        static_assert(sizeof(T) == 2 || S::kSubs == 1, "32 keys");
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          st[0][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][e], a.scale_log2e, -zero));
+          sum += st[0][e];
+        }
+        auto read_value = [&](int n) __attribute__((always_inline)) {  // the operand of the n-th matrix instruction of Ot: kOut of them for each pair of keys
+          const int e = n / S::kOut, r = 8 * (e / 4) + 4 * lhalf + e % 4;
+          return *reinterpret_cast<const float*>(vt + r * S::kRowBytes + tile_value_piece<T, D>(r, 8 * (n % S::kOut) + (lrow >> 2)) * 16 + (lrow & 3) * 4);
+        };
+        constexpr int kProducts = 16 * S::kOut;
+        float v[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) v[n] = read_value(n);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < kProducts; ++n) {
+          ot[n % S::kOut] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[n % kAhead], st[0][n / S::kOut], ot[n % S::kOut], 0, 0, 0);
+          if (n + kAhead < kProducts) v[n % kAhead] = read_value(n + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (__builtin_expect(partly_seen(key), 0) && wild) {  // a sum with an infinity or a NaN is one or the other
+#pragma unroll 1
+        for (int k = key; k < (SIGHT ? key + S::kKeys : min(key + S::kKeys, hi)); ++k) {
+          const T* v = values + row_offset<D>(view, cursor, kv_head, k) + 4 * lhalf;
+          const bool seen = sees<SIGHT>(mine, k);
+#pragma unroll
+          for (int t = 0; t < S::kOut; ++t) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float sum_e = ot[t][e];
+              if (seen) add_wild(sum_e, v + 32 * t + 8 * (e / 4) + e % 4);
+              ot[t][e] = sum_e;
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (few registers: this path is cold)
+          }
+        }
+      }
+      __syncthreads();
+    };
+    for (int place = lo; place < hi; place += 2 * S::kKeys) {
+      work_on(place, std::integral_constant<int, 0>{});
+      if (place + S::kKeys < hi) work_on(place + S::kKeys, std::integral_constant<int, 1>{});
+    }
+  }
+
+  {
+    const LanePair both = swap_halves(sum);
+    sum = both.a + both.b;
+  }
+  if (!live) return upto;
+  const int64_t at_token = seq.start + token;
+  if constexpr (!SIGHT) {
+    const bool sees_some = mine.end > 0;
+    const int first_part = sees_some ? mine.begin / chunk : part0, last_part = sees_some ? (mine.end - 1) / chunk : part0;
+    if (first_part == last_part) {
+      if (part == first_part) store_out<T, D>(a, at_token, head, sees_some, lhalf, ot, sum);
+    } else store_part<D>(a, (at_token * a.heads + head) * a.splits + part % a.splits, (int64_t)view.tokens * a.heads * a.splits, lhalf, ot, top, sum);
+  } else if (families) store_part<D>(a, a.family_at + (at_token * a.heads + head) * a.family_splits + part, a.rows, lhalf, ot, top, sum);
+  else {
+    const int last_part = own_parts(mine, span, seq.base, chunk) - 1;
+    if (last_part == 0 && seq.base == 0) {
+      if (part == 0) store_out<T, D>(a, at_token, head, mine.end > 0, lhalf, ot, sum);
+    } else if (part <= last_part) store_part<D>(a, a.own_at + (at_token * a.heads + head) * a.splits + part, a.rows, lhalf, ot, top, sum);
+  }
+  return upto;
+}
+
+template <typename T, int D, bool SMALL>
+__global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
+  __shared__ TilesShared<T, D> shared;
+  const int kv_head = blockIdx.x % a.view.kv_heads;
+  tiles<T, D, SMALL, false>(a, blockIdx.x / a.view.kv_heads, kv_head, blockIdx.z, false, shared);
+}
+
+}  // namespace
+}  // namespace ttmi
