@@ -30,8 +30,9 @@ struct PagedArgs {
   // Of the kernels that know of first keys that stay visible and of families (SIGHT).
   int sinks;
   const int32_t* families;  // null: none
-  // Keys of families are cut like those of sequences with many rows; family_blocks blocks of 128 rows at a time are worked on.
-  int family_chunk, family_splits, family_blocks;
+  // shares: workgroups that the families' keys, in at most family_splits parts of at least family_least steps of 64, and the sequences with few rows take among them;
+  // few_splits, few_every: splits and every of the few-rows kernel, where it runs (run_few); own_blocks: blocks of 128 rows of sequences' own keys, tile_groups workgroups.
+  int shares, family_splits, family_least, run_few, few_splits, few_every, own_blocks, tile_groups;
   // With families `partial` holds the rows of all results that are joined: those of the few-rows kernel (2 splits kFewRows), and from these on, for each row of q and head:
   int64_t own_at, family_at, whole_at, rows;  // of a sequence's own keys in parts, of its family's in parts, of its own where one workgroup had them all; the end
 };
@@ -131,6 +132,18 @@ __device__ __forceinline__ Span span_of(const Sight& s, int base) {
   return span;
 }
 
+// Sums over the lanes up to this one, it included, and over all.
+__device__ __forceinline__ int sum_up_to_here(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+__device__ __forceinline__ int sum_of_lanes(int v) { return __builtin_amdgcn_readlane(sum_up_to_here(v), kWave - 1); }
+
 // A family: sequences that follow one another and begin with the same keys.  What the rows of `families` say counts where the first sequence of a family and
 // another one agree on it, so that no key is left out or read twice whatever they hold.
 struct Family {
@@ -145,47 +158,84 @@ __device__ __forceinline__ Family family_led_by(const PagedArgs& a, int b) {
   f.keys = row[0] == b && f.end > b + 1 ? max(0, min(row[2], held)) & ~(kShareStep - 1) : 0;
   return f;
 }
-// The number of the first sequence of b's family, where that is one, and its keys (0: b is on its own).
-__device__ __forceinline__ int shared_keys(const PagedArgs& a, int b, int* first) {
-  *first = a.families[3 * (int64_t)b];
-  if ((unsigned)*first > (unsigned)b) return 0;
-  const Family f = family_led_by(a, *first);
-  return b < f.end ? f.keys : 0;
-}
-template <bool SIGHT>
-__device__ __forceinline__ Sequence sequence_of_batch(const PagedArgs& a, int b) {
-  Sequence s = sequence(a, b);
-  if constexpr (SIGHT) {
-    int first;
-    if (a.families != nullptr) s.base = shared_keys(a, b, &first);
+
+// 64 sequences, a lane each, with one trip to memory: what they are, the families that they lead and whose keys are not their own.
+struct LaneSequences {
+  int base;                            // number of the first
+  int starts, ends;                    // of the packed rows, as they are given
+  int start, tokens, length, first, own;  // as in Sequence (own: its base)
+  int leader;                          // the first of its family, as its row says
+  int family_end, family_keys, family_tokens;  // of the family that it leads; keys 0: none
+
+  __device__ __forceinline__ Sequence sequence(int lane) const {
+    Sequence s;
+    s.start = __builtin_amdgcn_readlane(start, lane), s.tokens = __builtin_amdgcn_readlane(tokens, lane), s.length = __builtin_amdgcn_readlane(length, lane);
+    s.first = __builtin_amdgcn_readlane(first, lane), s.base = __builtin_amdgcn_readlane(own, lane);
+    return s;
   }
+  __device__ __forceinline__ Family family(int lane) const {
+    return {base + lane, __builtin_amdgcn_readlane(family_end, lane), __builtin_amdgcn_readlane(family_keys, lane)};
+  }
+  // A family as a sequence: the rows of all of its sequences over the keys they have in common.
+  __device__ __forceinline__ Sequence family_sequence(int lane) const {
+    Sequence s;
+    s.start = __builtin_amdgcn_readlane(start, lane), s.tokens = __builtin_amdgcn_readlane(family_tokens, lane);
+    s.length = __builtin_amdgcn_readlane(family_keys, lane), s.first = 0;
+    return s;
+  }
+};
+__device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int base) {
+  const PagedView& view = a.view;
+  const int lane = (int)(threadIdx.x % kWave), b = base + lane, at = min(b, view.batch - 1);
+  LaneSequences s;
+  s.base = base;
+  s.starts = view.starts[at], s.ends = view.starts[at + 1];
+  const int length = view.lengths[at];
+  int row[3] = {-1, 0, 0};
+  if (a.families != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) row[i] = a.families[3 * (int64_t)at + i];
+  }
+  const int held = (int)min((int64_t)length, view.table_pitch << view.page_shift);
+  s.start = max(0, s.starts), s.tokens = b < view.batch ? max(0, min(s.ends, view.tokens) - s.start) : 0;
+  s.length = max(0, held), s.first = length - s.tokens;
+  s.own = 0, s.leader = row[0], s.family_end = min(row[1], view.batch), s.family_keys = s.family_tokens = 0;
+  if (a.families == nullptr) return s;
+  if (b < view.batch && row[0] == b && s.family_end > b + 1) s.family_keys = max(0, min(row[2], held)) & ~(kShareStep - 1);
+  const int last = s.family_end - 1 - base;
+  int rows_end = __shfl(s.ends, max(0, min(last, kWave - 1)), kWave);
+  if (s.family_keys > 0 && last >= kWave) rows_end = view.starts[s.family_end];
+  if (s.family_keys > 0) s.family_tokens = max(0, min(rows_end, view.tokens) - s.start);
+  const int from = row[0] - base, there = max(0, min(from, kWave - 1));
+  int keys = __shfl(s.family_keys, there, kWave), end = __shfl(s.family_end, there, kWave);
+  if ((unsigned)row[0] > (unsigned)b) keys = 0;
+  else if (from < 0) {
+    const Family f = family_led_by(a, row[0]);
+    keys = f.keys, end = f.end;
+  }
+  if (b < end) s.own = keys;
   return s;
 }
-// A family as a sequence: the rows of all of its sequences over the keys they have in common.
-__device__ __forceinline__ Sequence family_sequence(const PagedArgs& a, const Family& f) {
-  Sequence s;
-  s.start = max(0, a.view.starts[f.first]);
-  s.tokens = f.keys > 0 ? max(0, min(a.view.starts[f.end], a.view.tokens) - s.start) : 0;
-  s.length = f.keys, s.first = 0;
-  return s;
-}
-// The sequence of a family that a row of q belongs to, each lane's own.  Where each has one new token that is one trip to memory.
-__device__ __forceinline__ int member_of(const PagedArgs& a, const Family& f, int start, int row) {
-  const int32_t* const starts = a.view.starts;
-  int lo = min(f.first + row - start, f.end - 1), hi = f.end;
-  if (starts[lo] <= row && starts[lo + 1] > row) return lo;
-  lo = f.first;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= row) lo = mid;
-    else hi = mid;
+// The sequence of a family that a row of q belongs to, each lane's own, and what of the family's keys the row sees; *member: whether that sequence says that it is of the family.  Where each
+// sequence has one new token and they lie among the 64, no trip to memory.
+__device__ __forceinline__ Reach family_reach(const PagedArgs& a, const LaneSequences& s, const Family& f, int start, int row, bool* member) {
+  const PagedView& view = a.view;
+  const int guess = min(f.first + row - start, f.end - 1), at = min(guess - s.base, kWave - 1);
+  int leader = __shfl(s.leader, at, kWave);
+  Sequence q;
+  q.start = __shfl(s.start, at, kWave), q.tokens = __shfl(s.tokens, at, kWave), q.length = __shfl(s.length, at, kWave), q.first = __shfl(s.first, at, kWave);
+  if (!(guess - s.base < kWave && q.start <= row && row < q.start + q.tokens)) {
+    int lo = f.first, hi = f.end;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (view.starts[mid] <= row) lo = mid;
+      else hi = mid;
+    }
+    q = sequence(a, lo);
+    leader = a.families[3 * (int64_t)lo];
   }
-  return lo;
-}
-// What a row of member b sees of its family's keys.
-__device__ __forceinline__ Reach family_reach(const PagedArgs& a, const Family& f, int b, int row) {
-  const Sequence s = sequence(a, b);
-  Reach r = s.reach(a, row - s.start);
+  *member = leader == f.first;
+  Reach r = q.reach(a, row - q.start);
   r.low = min(f.keys, a.window > 0 ? min(a.sinks, r.end) : 0);
   r.end = min(f.keys, r.end);
   r.begin = min(r.begin, r.end);
@@ -383,11 +433,10 @@ __device__ __forceinline__ void join_parts_by_wavefront(const float* partial, co
 int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream);
 int launch_tiles(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream);
 
-// How the work of a call is laid out: `tiles` takes families and sequences with many rows, `few` the others.
+// How the work of a call is laid out: `all` for the launch of everything, `few` for that of the sequences with few rows where they have one of their own.
 struct SightLaunch {
-  PagedArgs tiles, few;
-  bool run_tiles, run_few;
-  int own_blocks;  // blocks of 128 rows of sequences' own keys
+  PagedArgs all, few;
+  bool run_tiles;
 };
 void launch_sight_f16(const SightLaunch& l, int64_t head_dim, hipStream_t stream);
 void launch_sight_bf16(const SightLaunch& l, int64_t head_dim, hipStream_t stream);

@@ -75,11 +75,12 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   return p;
 }
 
-// With first keys that stay visible and with families.  The sequences' own keys are cut as ever (their number is guessed from max_length: a sequence on its own may be that long); families
-// have blocks of 128 rows each, of which the few tokens of a decoding batch fill one or two, and their keys are cut to match.
+// With first keys that stay visible and with families.  The sequences' own keys are cut as ever (their number is guessed from max_length: a sequence on its own may be that long).  A family's are
+// cut on the device, which knows how many there are; here it is said how many workgroups there will be, two a CU or, where each would have more than 32 steps of 64 keys, four times as many
+// (16 questions about 20000 tokens, 32 and 8 heads of 128: 1 / 2 / 3 / 5 / 8 parts 650 / 570 / 498 / 475 / 487 us).
 struct SightPlan {
   PagedPlan own;
-  int family_chunk, family_splits, family_blocks, own_blocks;
+  int shares, family_splits, family_least, own_blocks;
   int64_t few_rows, own_rows, family_rows, whole_rows, floats;  // of the workspace
 };
 SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, const ttmi_paged_sight& sight, int dtype) {
@@ -88,19 +89,22 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
   p.own = plan(view, heads, max_tokens, max_length, window, dtype);
   const int64_t group = heads / view.kv_heads, tokens = view.tokens, d = view.head_dim;
   p.own_blocks = p.own.tiles ? (int)(tokens * group / 128 + std::min<int64_t>(view.batch, tokens)) : 0;
-  p.family_chunk = p.family_splits = 1, p.family_blocks = 0, p.family_rows = p.whole_rows = 0;
+  p.shares = p.family_splits = p.family_least = 0, p.family_rows = p.whole_rows = 0;
   const bool families = sight.families != nullptr;
   if (families) {
     const int64_t held = view.table_pitch << view.page_shift, shared = std::max<int64_t>(1, sight.max_shared > 0 ? std::min(sight.max_shared, held) : held);
-    const int64_t blocks = tokens * group / 128 + std::max<int64_t>(1, std::min<int64_t>(sight.family_count, view.batch / 2));
-    cut(view.kv_heads * blocks, dtype == TTMI_F32 ? 64 : 256, shared, false, &p.family_chunk, &p.family_splits);
-    p.family_blocks = (int)blocks;
+    const int64_t count = std::max<int64_t>(1, std::min<int64_t>(sight.family_count, view.batch / 2)), cus = compute_units();
+    const int64_t steps = ceil_div(shared, 64), all = std::max(count, ceil_div(tokens * group, 128)) * steps * view.kv_heads;
+    p.shares = (int)std::max(all > 64 * cus ? 8 * cus : 2 * cus, 2 * (int64_t)view.kv_heads);  // (each head has one, and leaves as many)
+    p.family_least = dtype == TTMI_F32 ? 1 : 2;
+    // (where the sequences' own keys have a share too, parts are longer and so fewer)
+    p.family_splits = (int)ceil_div(steps, std::max<int64_t>(p.family_least, all / p.shares)) + 1;
     p.family_rows = tokens * heads * p.family_splits;
     p.whole_rows = p.own.few ? tokens * heads : 0;
   }
   p.few_rows = p.own.few ? 2ll * p.own.few_splits * kFewRows : 0;
   p.own_rows = p.own.tiles && (families || p.own.tile_splits > 1) ? tokens * heads * p.own.tile_splits : 0;
-  p.floats = (p.few_rows + p.own_rows + p.family_rows + p.whole_rows) * (d + 2);
+  p.floats = (p.few_rows + p.own_rows + p.family_rows + p.whole_rows) * (d + 2) + (families ? 4 : 0);
   return p;
 }
 
@@ -201,7 +205,7 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
     return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, sight->window, workspace, workspace_bytes,
                                 dtype, stream);
   SightLaunch l;
-  PagedArgs& a = l.tiles;
+  PagedArgs& a = l.all;
   if (int rc = attention_args(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, sight->window, dtype, &a)) return rc;
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   const SightPlan p = plan_sight(a.view, heads, max_tokens, max_length, *sight, dtype);
@@ -210,11 +214,14 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
   a.sinks = (int)std::min(sight->sinks, kWidest), a.families = sight->families;
   a.partial = static_cast<float*>(workspace);
   a.every = !p.own.few, a.chunk = p.own.tile_chunk, a.splits = p.own.tile_splits, a.ordered = 1;
-  a.family_chunk = p.family_chunk, a.family_splits = p.family_splits, a.family_blocks = p.family_blocks;
+  a.shares = p.shares, a.family_splits = p.family_splits, a.family_least = p.family_least;
   a.own_at = p.few_rows, a.family_at = a.own_at + p.own_rows, a.whole_at = a.family_at + p.family_rows, a.rows = a.whole_at + p.whole_rows;
+  l.run_tiles = p.own.tiles || p.shares > 0;
+  a.run_few = p.own.few, a.few = p.own.few_rows, a.few_splits = p.own.few_splits, a.few_every = !p.own.tiles;
+  a.own_blocks = p.own_blocks, a.tile_groups = (int)(p.own_blocks * a.view.kv_heads * p.own.tile_splits);
   l.few = a;
-  l.few.every = !p.own.tiles, l.few.few = p.own.few_rows, l.few.splits = p.own.few_splits, l.few.waves = p.own.few_waves;
-  l.run_tiles = p.own.tiles || p.family_blocks > 0, l.run_few = p.own.few, l.own_blocks = p.own_blocks;
+  l.few.splits = p.own.few_splits;
+  l.few.waves = l.run_tiles && a.view.page_shift >= 4 ? 4 : p.own.few_waves;  // (4 in one launch with the others)
   const auto launch = dtype == TTMI_F32 ? launch_sight_f32 : dtype == TTMI_F16 ? launch_sight_f16 : launch_sight_bf16;
   launch(l, cache->head_dim, static_cast<hipStream_t>(stream));
   return launch_status("paged_attention_sight");

@@ -82,18 +82,24 @@ constexpr int kRound = 128;
 // A pair has a unit more than rounds: what a workgroup waits for when it comes to one (its length, its pages, its first tile) is time that others have for theirs.
 // us, 64 sequences of 100 to 6000 keys (three draws, and all of 1450), without / with it / with two: 105 / 89 / 91, 87 / 75 / 77, 107 / 94 / 97, 104 / 95 / 98, 75 / 75 / 75.
 constexpr int kStart = 1;
+// Of this lane (without tokens behind the last sequence).
+__device__ __forceinline__ Sequence own_sequence(const LaneSequences& lanes) {
+  Sequence s;
+  s.start = lanes.start, s.tokens = lanes.tokens, s.length = lanes.length, s.first = lanes.first, s.base = lanes.own;
+  return s;
+}
 struct Walk {  // 64 sequences, a lane each
+  LaneSequences lanes;    // SIGHT
   int base, rounds;       // number of the first; rounds of this lane's, for one head
   int64_t before, upto;   // units of all sequences before these; of these up to this lane's, it included
   int64_t groups;         // of batches of more than 64 sequences: units of this lane's 64th of them and of those before it
 };
 constexpr int kSpanTile = 32;  // a tile or two
 template <bool SIGHT>
-__device__ __forceinline__ int rounds_of(const PagedArgs& a, int b) {
-  const Sequence seq = sequence_of_batch<SIGHT>(a, b);
+__device__ __forceinline__ int rounds_of(const PagedArgs& a, const Sequence& seq) {
   const int rows = seq.tokens * a.group;
   if (rows <= 0) return 0;
-  if (rows > a.few) return a.every ? kStart + 1 : 0;  // (more rows than was said: not cut)
+  if (rows > a.few) return (SIGHT ? a.few_every : a.every) ? kStart + 1 : 0;  // (more rows than was said: not cut)
   if constexpr (SIGHT) {
     const Span span = span_of<kSpanTile>(sight_of(seq.own_reach(a, 0), seq.own_reach(a, seq.tokens - 1)), seq.base);
     return kStart + max(1, (span.hi - span.lo + kRound - 1) / kRound);
@@ -116,10 +122,16 @@ __device__ __forceinline__ int64_t sum_up_to_lane(int64_t v) {
 }
 template <bool SIGHT>
 __device__ __forceinline__ void walk_to(const PagedArgs& a, Walk& w, int base, int64_t before) {
-  const int lane = (int)(threadIdx.x % kWave);
   w.base = base, w.before = before;
-  w.rounds = base + lane < a.view.batch ? rounds_of<SIGHT>(a, base + lane) : 0;
-  w.upto = sum_up_to_lane((int64_t)w.rounds * a.view.kv_heads);
+  if constexpr (SIGHT) {
+    w.lanes = lane_sequences(a, base);
+    w.rounds = rounds_of<true>(a, own_sequence(w.lanes));
+    w.upto = (int64_t)sum_up_to_here(w.rounds) * a.view.kv_heads;
+  } else {
+    const int lane = (int)(threadIdx.x % kWave);
+    w.rounds = base + lane < a.view.batch ? rounds_of<false>(a, sequence(a, base + lane)) : 0;
+    w.upto = sum_up_to_lane((int64_t)w.rounds * a.view.kv_heads);
+  }
 }
 template <bool SIGHT>
 __device__ __forceinline__ void walk_on(const PagedArgs& a, Walk& w) { walk_to<SIGHT>(a, w, w.base + kWave, w.before + lane_of(w.upto, kWave - 1)); }
@@ -138,8 +150,18 @@ __device__ __forceinline__ int64_t count_units(const PagedArgs& a, Walk& w) {
   }
   const int size = group_size(a), first = (int)(threadIdx.x % kWave) * size;
   int64_t mine = 0;
+  if constexpr (SIGHT) {
+    // 64 sequences at a time; what each group of `size` has is kept by its lane
+    for (int base = 0; base < a.view.batch; base += kWave) {
+      const int upto = sum_up_to_here(rounds_of<true>(a, own_sequence(lane_sequences(a, base))));
+      const int from = min(max(first - base, 0), kWave), to = min(max(first + size - base, 0), kWave);
+      const int low = __shfl(upto, max(from - 1, 0), kWave), high = __shfl(upto, max(to - 1, 0), kWave);
+      mine += (to > 0 ? high : 0) - (from > 0 ? low : 0);
+    }
+  } else {
 #pragma unroll 4
-  for (int i = 0; i < size; ++i) mine += first + i < a.view.batch ? rounds_of<SIGHT>(a, first + i) : 0;
+    for (int i = 0; i < size; ++i) mine += first + i < a.view.batch ? rounds_of<false>(a, sequence(a, first + i)) : 0;
+  }
   w.groups = sum_up_to_lane(mine * a.view.kv_heads);
   w.base = 0, w.rounds = 0, w.before = w.upto = 0;
   return lane_of(w.groups, kWave - 1);
@@ -163,7 +185,7 @@ __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t 
 // Workgroups that share the work.  At least kFewest rounds each, so that a wavefront has more than its first tile's wait.  us, 1 / 2 / 4 of them, 8 key heads of 128: 1 sequence
 // of 1500 keys 11.6 / 12.5 / 15.6, of 8000 16.4 / 14.1 / 15.6, 8 of 1000 19.0 / 16.7 / 17.7, 8 of 2000 21.2 / 21.4 / 25.8.
 constexpr int kFewest = 2;
-__device__ __forceinline__ int64_t sharers(const PagedArgs& a, int64_t units) { return max((int64_t)1, min((int64_t)a.splits, (units + kFewest - 1) / kFewest)); }
+__device__ __forceinline__ int64_t sharers(int splits, int64_t units) { return max((int64_t)1, min((int64_t)splits, (units + kFewest - 1) / kFewest)); }
 
 template <typename T, int D, int NW>
 struct FewRowsShared {
@@ -171,9 +193,9 @@ struct FewRowsShared {
   float met[NW][kFewRows][2];
 };
 
-// The share of one of a.splits workgroups (0: of a pair).  SMALL: pages of fewer than 16 slots
+// The share of one of `splits` workgroups (0: of a pair); SIGHT: units and walk as count_units gives them, if units >= 0.  SMALL: pages of fewer than 16 slots
 template <typename T, int D, int NW, bool SMALL, bool SIGHT>
-__device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, FewRowsShared<T, D, NW>& shared) {
+__device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int splits, Walk& walk, int64_t all_units, FewRowsShared<T, D, NW>& shared) {
   using S = FewRows<T, D, NW>;
   char* const smem = shared.tiles;
   auto& met = shared.met;
@@ -185,27 +207,30 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, FewR
   char* const tile = smem + wave * S::kValueBytes;
 
   // splits 0: a workgroup for each pair
-  Walk walk;
   int64_t unit = workgroup, stop = unit + 1;
-  if (a.splits > 0) {
-    const int64_t units = count_units<SIGHT>(a, walk), workgroups = sharers(a, units);
+  if (splits > 0) {
+    const int64_t units = SIGHT && all_units >= 0 ? all_units : count_units<SIGHT>(a, walk), workgroups = sharers(splits, units);
     if (workgroup >= workgroups) return;
     unit = units * workgroup / workgroups, stop = units * (workgroup + 1) / workgroups;
   }
   while (unit < stop) {
     Place place;
-    if (a.splits > 0) place = find_unit<SIGHT>(a, walk, unit);
+    if (splits > 0) place = find_unit<SIGHT>(a, walk, unit);
     else place.b = (int)(unit / view.kv_heads), place.kv_head = (int)(unit % view.kv_heads), place.round = 0, place.rounds = INT32_MAX;
     const int b = place.b, kv_head = place.kv_head;
-    const int64_t ends = a.splits > 0 ? min(stop, unit + place.rounds - place.round) : stop;
-    const int start = a.splits > 0 ? kStart : 0;  // (in a pair's first unit there is nothing to do)
-    const int round0 = max(0, place.round - start), round1 = place.round + (int)(a.splits > 0 ? ends - unit : INT32_MAX) - start;
+    const int64_t ends = splits > 0 ? min(stop, unit + place.rounds - place.round) : stop;
+    const int start = splits > 0 ? kStart : 0;  // (in a pair's first unit there is nothing to do)
+    const int round0 = max(0, place.round - start), round1 = place.round + (int)(splits > 0 ? ends - unit : INT32_MAX) - start;
     const bool complete = round0 == 0 && round1 == place.rounds - start;
     unit = ends;
     if (round1 <= round0) continue;
-    const Sequence seq = sequence_of_batch<SIGHT>(a, b);
+    Sequence seq;
+    if constexpr (SIGHT) {
+      if (splits == 0) walk.lanes = lane_sequences(a, b & ~(kWave - 1));
+      seq = walk.lanes.sequence(b - walk.lanes.base);
+    } else seq = sequence(a, b);
     const int rows_all = seq.tokens * a.group;
-    if (rows_all <= 0 || (rows_all > a.few && !a.every)) return;  // (a workgroup of its own)
+    if (rows_all <= 0 || (rows_all > a.few && !(SIGHT ? a.few_every : a.every))) return;  // (a workgroup of its own)
     if (round0 == 0 && kv_head == 0 && tid == 0 && view.lengths[b] > seq.length) page_error(view);
     PageCursor cursor;
     cursor.table = view.table + (int64_t)b * view.table_pitch;
@@ -437,7 +462,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, FewR
           } else {
             const bool whole = SIGHT && complete;  // (of a family's: what it has of its own)
             const int64_t at = whole ? a.whole_at + (seq.start + t) * (int64_t)a.heads + h : (2 * (int64_t)workgroup + (round0 == 0 ? 1 : 0)) * kFewRows + r;
-            float* const ml = a.partial + (SIGHT ? a.rows : 2 * (int64_t)a.splits * kFewRows) * D + at * 2;
+            float* const ml = a.partial + (SIGHT ? a.rows : 2 * (int64_t)splits * kFewRows) * D + at * 2;
   #pragma unroll
             for (int c = 0; c < kWide; ++c) a.partial[at * D + d0 + c] = o[c];
             if (d0 == 0) ml[0] = best, ml[1] = total;
@@ -452,7 +477,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, FewR
 template <typename T, int D, int NW, bool SMALL, bool SIGHT>
 __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedArgs a) {
   __shared__ FewRowsShared<T, D, NW> shared;
-  few_rows<T, D, NW, SMALL, SIGHT>(a, blockIdx.x, shared);
+  Walk walk{};
+  few_rows<T, D, NW, SMALL, SIGHT>(a, blockIdx.x, a.splits, walk, -1, shared);
 }
 
 // Which workgroups had a part of a pair: from first to last.
@@ -460,9 +486,7 @@ struct Sharers {
   int64_t first, last;
 };
 template <bool SIGHT>
-__device__ __forceinline__ Sharers sharers_of(const PagedArgs& a, int b, int kv_head) {
-  Walk walk;
-  const int64_t units = count_units<SIGHT>(a, walk), workgroups = sharers(a, units);
+__device__ __forceinline__ Sharers sharers_of(const PagedArgs& a, Walk& walk, int64_t units, int64_t workgroups, int b, int kv_head) {
   if (a.view.batch > kWave) walk_to_group<SIGHT>(a, walk, b / group_size(a));
   while (walk.base + kWave <= b) walk_on<SIGHT>(a, walk);
   const int lane = b - walk.base, rounds = __builtin_amdgcn_readlane(walk.rounds, lane);
@@ -479,10 +503,12 @@ template <typename T, int D, bool SIGHT>
 __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a, bool by_pair) {
   const PagedView& view = a.view;
   const int kv_head = blockIdx.x % view.kv_heads, b = blockIdx.x / view.kv_heads;
-  const Sequence seq = sequence(a, b);
+  const Sequence seq = sequence(a, b);  // (without families, whose parts are joined elsewhere)
   const int rows = seq.tokens * a.group;
   if (rows > a.few || (int)blockIdx.y >= rows) return;
-  const Sharers shared = sharers_of<SIGHT>(a, b, kv_head);
+  Walk walk{};
+  const int64_t units = count_units<SIGHT>(a, walk), workgroups = sharers(a.splits, units);
+  const Sharers shared = sharers_of<SIGHT>(a, walk, units, workgroups, b, kv_head);
   const int64_t first = shared.first, last = shared.last;
   if (first == last) return;
   const int parts = (int)(last - first) + 1;
@@ -503,22 +529,26 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a, b
       a.partial, ml, parts, sees(r), [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
 }
 
+template <typename T, int D, bool SIGHT>
+void start_join_few_rows(const PagedArgs& a, hipStream_t stream) {
+  if (a.splits == 0 || a.families != nullptr) return;
+  const unsigned pairs = (unsigned)((int64_t)a.view.batch * a.view.kv_heads);
+  const bool by_pair = pairs >= kManyPairs;
+  hipLaunchKernelGGL((join_few_rows_kernel<T, D, SIGHT>), dim3(pairs, by_pair ? 1u : (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0,
+                     stream, a, by_pair);
+}
 template <typename T, bool SIGHT>
 void start_few_rows(const PagedArgs& a, int64_t head_dim, hipStream_t stream) {
   const unsigned pairs = (unsigned)((int64_t)a.view.batch * a.view.kv_heads);
-  const bool by_pair = pairs >= kManyPairs;
-  auto launch = [&](auto kernel, auto join) {
-    hipLaunchKernelGGL(kernel, dim3(a.splits > 0 ? (unsigned)a.splits : pairs), dim3(a.waves * 64), 0, stream, a);
-    if (a.splits > 0 && a.families == nullptr)
-      hipLaunchKernelGGL(join, dim3(pairs, by_pair ? 1u : (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0, stream, a, by_pair);
-  };
   const bool small = a.view.page_shift < 4;
   auto sized = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (small && a.waves == 4) launch(few_rows_kernel<T, D, 4, true, SIGHT>, join_few_rows_kernel<T, D, SIGHT>);
-    else if (small) launch(few_rows_kernel<T, D, 8, true, SIGHT>, join_few_rows_kernel<T, D, SIGHT>);
-    else if (a.waves == 4) launch(few_rows_kernel<T, D, 4, false, SIGHT>, join_few_rows_kernel<T, D, SIGHT>);
-    else launch(few_rows_kernel<T, D, 8, false, SIGHT>, join_few_rows_kernel<T, D, SIGHT>);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.splits > 0 ? (unsigned)a.splits : pairs), dim3(a.waves * 64), 0, stream, a); };
+    if (small && a.waves == 4) launch(few_rows_kernel<T, D, 4, true, SIGHT>);
+    else if (small) launch(few_rows_kernel<T, D, 8, true, SIGHT>);
+    else if (a.waves == 4) launch(few_rows_kernel<T, D, 4, false, SIGHT>);
+    else launch(few_rows_kernel<T, D, 8, false, SIGHT>);
+    start_join_few_rows<T, D, SIGHT>(a, stream);
   };
   if (head_dim == 64) sized(std::integral_constant<int, 64>{});
   else sized(std::integral_constant<int, 128>{});

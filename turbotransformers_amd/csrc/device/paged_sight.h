@@ -14,42 +14,178 @@ namespace ttmi {
 
 namespace {
 
+// How a.shares workgroups are divided.  Work on a family is counted in steps of 64 keys of a block of 128 rows, that on the others in rounds of the few-rows kernel.  What a step costs a workgroup, in
+// sixteenths of a microsecond with two workgroups on a CU, and what a round does where all of them read: its bytes at 9.8 GB/s.
+template <typename T, int D>
+constexpr int kStepCost = sizeof(T) == 4 ? (D == 128 ? 96 : 56) : (D == 128 ? 28 : 24);
+template <typename T, int D>
+constexpr int kRoundCost = 16 * kRound * 2 * D * (int)sizeof(T) / 9800;
+struct Shares {
+  int steps;          // of a part of a family's keys, at most
+  int items;          // parts of blocks of rows of all families, for one key/value head
+  int family_groups;  // workgroups that take them, for one head
+  int few_groups;     // and those that are left for sequences with few rows
+};
+struct FamilyWork {  // of a lane's family
+  int blocks, steps;
+};
+__device__ __forceinline__ FamilyWork family_work(const PagedArgs& a, const LaneSequences& lanes) {
+  return {(int)(((int64_t)lanes.family_tokens * a.group + kTileRows - 1) / kTileRows), lanes.family_keys / 64};
+}
+__device__ __forceinline__ int family_parts(int steps, int most) { return (steps + most - 1) / most; }
+// For kernels that follow, behind the partial results.
+struct ShareNote {
+  int steps, few_groups;
+  int64_t units;
+};
+template <int D>
+__device__ __forceinline__ ShareNote* share_note(const PagedArgs& a) {
+  return reinterpret_cast<ShareNote*>(a.partial + a.rows * (D + 2));
+}
+// walk, *units: those of the few-rows kernel (and the first 64 sequences, where there are no more).
+template <typename T, int D>
+__device__ __forceinline__ Shares shares_of(const PagedArgs& a, Walk& walk, int64_t* units) {
+  const int kv_heads = a.view.kv_heads;
+  const bool few = a.run_few && a.few_splits > 0, single = a.view.batch <= kWave;
+  *units = 0;
+  if (few) *units = count_units<true>(a, walk);
+  else if (single) walk.lanes = lane_sequences(a, 0);
+  // (sums of 64 numbers that are capped for the balance alone)
+  constexpr int kCap = 1 << 24;
+  int64_t steps = 0;
+  int longest = 0;
+  for (int base = 0; base < a.view.batch; base += kWave) {
+    const FamilyWork w = family_work(a, single ? walk.lanes : lane_sequences(a, base));
+    steps += sum_of_lanes((int)min((int64_t)w.blocks * w.steps, (int64_t)kCap));
+    for (uint64_t more = __ballot(w.steps > longest); more != 0; more = __ballot(w.steps > longest))
+      longest = __builtin_amdgcn_readlane(w.steps, __ffsll((unsigned long long)more) - 1);
+  }
+  Shares s;
+  const int64_t family_cost = steps * kStepCost<T, D>, cost = family_cost + *units / kv_heads * kRoundCost<T, D>;
+  const int groups = max(kv_heads, (int)(cost > 0 ? (uint64_t)(a.shares * family_cost) / (uint64_t)cost : 0));
+  s.steps = max(max(a.family_least, (longest + a.family_splits - 1) / a.family_splits), (int)min((steps * kv_heads + groups - 1) / groups, (int64_t)INT32_MAX));
+  s.items = 0;
+  for (int base = 0; base < a.view.batch; base += kWave) {
+    const FamilyWork w = family_work(a, single ? walk.lanes : lane_sequences(a, base));
+    s.items += sum_of_lanes(w.blocks * family_parts(w.steps, s.steps));
+  }
+  // (at least an eighth is left for the others)
+  s.family_groups = min(s.items, max(1, (few ? a.shares - a.shares / 8 : a.shares) / kv_heads));
+  s.few_groups = max(1, min(a.few_splits, a.shares - s.family_groups * kv_heads));
+  return s;
+}
+
+// The item-th part of a block of a family's rows -> whether there is one.
+struct Job {
+  int b, block, part, chunk;
+  Sequence seq;
+  Family family;
+};
+__device__ __forceinline__ bool find_family_job(const PagedArgs& a, const Shares& s, int item, bool there, LaneSequences& lanes, Job* job) {
+  int passed = 0;
+  for (int base = 0; base < a.view.batch; base += kWave) {
+    if (!there) lanes = lane_sequences(a, base);
+    const FamilyWork w = family_work(a, lanes);
+    const int mine = w.blocks * family_parts(w.steps, s.steps), upto = passed + sum_up_to_here(mine), all = __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (item >= all) {
+      passed = all;
+      continue;
+    }
+    const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(item < upto)) - 1);
+    const int at = item - __builtin_amdgcn_readlane(upto - mine, found), blocks = __builtin_amdgcn_readlane(w.blocks, found);
+    const int steps = __builtin_amdgcn_readlane(w.steps, found), parts = family_parts(steps, s.steps);
+    // (workgroups beside each other have the same keys of a head, on one XCD where there are eight heads)
+    job->b = base + found, job->part = at / blocks, job->block = at - job->part * blocks, job->chunk = (steps + parts - 1) / parts * 64;
+    job->seq = lanes.family_sequence(found), job->family = lanes.family(found);
+    return true;
+  }
+  return false;
+}
+// The share of a workgroup in the families' keys (`lanes`: the first 64 sequences, where there are no more), or in blocks of sequences with many rows, over their own keys.  More
+// blocks than was said are taken in turns.
 template <typename T, int D, bool SMALL>
-__global__ __launch_bounds__(256, 2) void sight_tiles_kernel(const PagedArgs a, int own_blocks) {
-  __shared__ TilesShared<T, D> shared;
-  const int kv_heads = a.view.kv_heads, family_groups = a.families != nullptr ? kv_heads * a.family_blocks * a.family_splits : 0;
-  const bool families = (int)blockIdx.x < family_groups;
-  const int group = families ? blockIdx.x : blockIdx.x - family_groups, splits = families ? a.family_splits : a.splits;
-  const int kv_head = group % kv_heads, part = group / kv_heads % splits;
-  // (more blocks than was said are taken in turns)
-  const int step = families ? a.family_blocks : own_blocks;
-  for (int block = group / kv_heads / splits, upto = INT32_MAX; block < upto; block += step) {
-    upto = tiles<T, D, SMALL, true>(a, block, kv_head, part, families, shared);
+__device__ __forceinline__ void sight_tiles(const PagedArgs& a, bool families, const Shares& s, int group, LaneSequences lanes, TilesShared<T, D>& shared) {
+  const int kv_heads = a.view.kv_heads, kv_head = group % kv_heads, own_part = group / kv_heads % a.splits;
+  const int step = families ? s.family_groups : a.own_blocks;
+  bool there = a.view.batch <= kWave;
+  for (int item = group / kv_heads / (families ? 1 : a.splits), stop = families ? s.items : INT32_MAX; item < stop; item += step) {
+    Job job;
+    if (families) {
+      if (!find_family_job(a, s, item, there, lanes, &job)) return;
+    } else {
+      if (!find_block<true>(a, item, &lanes, &job.b, &job.block, &stop)) return;
+      job.part = own_part, job.chunk = 0, job.seq = lanes.sequence(job.b - lanes.base), job.family = Family{};
+    }
+    there = false;  // (they are not kept where the registers are needed)
+    tiles<T, D, SMALL, true>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, kv_head, job.part, shared);
     __syncthreads();
   }
 }
 
+// One launch: a.shares workgroups (none without families) for families and for sequences with few rows, a.tile_groups for those with many, the rest, if any, for few rows.  So a
+// CU has workgroups that multiply beside others that read.  SMALL: sequences with few rows have a launch of their own.
+template <typename T, int D, bool SMALL>
+__global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
+  __shared__ union {
+    TilesShared<T, D> tiles;
+    FewRowsShared<T, D, 4> few;
+  } shared;
+  int group = blockIdx.x, few_groups = a.few_splits;
+  Walk walk{};
+  Shares s{};
+  int64_t units = -1;
+  const int shares = a.families != nullptr ? a.shares : 0;
+  bool families = false, own = false;
+  if (group < shares) {
+    s = shares_of<T, D>(a, walk, &units);
+    if (group == 0 && threadIdx.x == 0) *share_note<D>(a) = {s.steps, s.few_groups, units};
+    families = group < s.family_groups * a.view.kv_heads;
+    if (!families) group -= s.family_groups * a.view.kv_heads, few_groups = s.few_groups;
+    if (!families && (SMALL || units == 0 || group >= few_groups)) return;
+  } else {
+    group -= shares;
+    own = group < a.tile_groups;
+    if (!own) group -= a.tile_groups;
+  }
+  if (families || own) {
+    sight_tiles<T, D, SMALL>(a, families, s, group, walk.lanes, shared.tiles);
+    return;
+  }
+  if constexpr (!SMALL) few_rows<T, D, 4, false, true>(a, group, few_groups, walk, units, shared.few);
+}
+
 // A wavefront a row and head.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a, const PagedArgs few, bool run_few) {
+__global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
   const PagedView& view = a.view;
-  const int row = blockIdx.x, b = sequence_of(view, row), head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (b >= view.batch || head >= a.heads) return;
-  const Sequence seq = sequence_of_batch<true>(a, b);
-  if (row < seq.start) return;
+  const int row = blockIdx.x, head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (head >= a.heads) return;
+  ShareNote note{};
+  if (a.families != nullptr) note = *share_note<D>(a);
+  // the row's sequence: the first that ends behind it
+  Walk walk{};
+  int b = -1;
+  for (int base = 0; base < view.batch; base += kWave) {
+    walk.lanes = lane_sequences(a, base);
+    const int before = __popcll(__ballot(base + (int)(threadIdx.x % kWave) < view.batch && walk.lanes.ends <= row));
+    if (before == kWave) continue;
+    b = base + before;
+    break;
+  }
+  if (b < 0 || b >= view.batch) return;
+  const Sequence seq = walk.lanes.sequence(b - walk.lanes.base);
+  if (row < seq.start || row >= seq.start + seq.tokens) return;
   const int kv_head = head / a.group, r = (row - seq.start) * a.group + head % a.group, rows = seq.tokens * a.group;
   const int64_t at = (int64_t)row * a.heads + head;
-  int family_parts = 0;
-  if (seq.base > 0) {
-    Sequence family;
-    family.length = seq.base;
-    const int chunk = family_chunk(a, family);
-    family_parts = (seq.base + chunk - 1) / chunk;
+  int of_family = 0;
+  if (seq.base > 0) {  // (as many parts as there are chunks, which are equal but for the last)
+    const int steps = seq.base / 64, parts = family_parts(steps, note.steps), chunk = (steps + parts - 1) / parts;
+    of_family = (steps + chunk - 1) / chunk;
   }
-  int parts = 1;                     // of the sequence's own keys
-  int64_t place = few.whole_at + at;  // of them, and how far they lie apart
+  int parts = 1;                    // of the sequence's own keys
+  int64_t place = a.whole_at + at;  // of them, and how far they lie apart
   int64_t second = 0, step = 0;
-  if (!run_few || (rows > kFewRows && !few.every)) {
+  if (!a.run_few || (rows > kFewRows && !a.few_every)) {
     const Reach mine = seq.own_reach(a, row - seq.start);
     const int row0 = r / kTileRows * kTileRows, last = min(rows, row0 + kTileRows) - 1;
     const Span span = span_of<kSpanTiles>(sight_of(seq.own_reach(a, row0 / a.group), seq.own_reach(a, last / a.group)), seq.base);
@@ -57,19 +193,23 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a, cons
     place = a.own_at + at * a.splits, second = place + 1, step = 1;
   } else if (a.families == nullptr) {
     return;
-  } else if (few.splits > 0) {
-    const Sharers shared = sharers_of<true>(few, b, kv_head);
+  } else if (a.few_splits > 0) {
+    int64_t units = note.units;
+    if (view.batch <= kWave) walk.base = 0, walk.before = 0, walk.rounds = rounds_of<true>(a, own_sequence(walk.lanes)),
+                             walk.upto = (int64_t)sum_up_to_here(walk.rounds) * view.kv_heads;
+    else units = count_units<true>(a, walk);
+    const Sharers shared = sharers_of<true>(a, walk, units, sharers(view.page_shift >= 4 ? note.few_groups : a.few_splits, units), b, kv_head);
     if (shared.last > shared.first) {
       parts = (int)(shared.last - shared.first) + 1;
       place = (2 * shared.first + 1) * kFewRows + r, second = 2 * (shared.first + 1) * kFewRows + r, step = 2 * kFewRows;
     }
   }
-  if (family_parts == 0 && parts == 1) return;  // (there already)
+  if (of_family == 0 && parts == 1) return;  // (there already)
   const int64_t family_place = a.family_at + at * a.family_splits;
   join_parts_by_wavefront<T, D>(
-      a.partial, a.partial + a.rows * D, family_parts + parts, seq.reach(a, row - seq.start).end > 0,
+      a.partial, a.partial + a.rows * D, of_family + parts, seq.reach(a, row - seq.start).end > 0,
       [&](int p) {
-        const int own = p - family_parts;
+        const int own = p - of_family;
         return own < 0 ? family_place + p : own == 0 ? place : second + (own - 1) * step;
       },
       static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)head * D);
@@ -77,22 +217,25 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a, cons
 
 template <typename T>
 void start_sight(const SightLaunch& l, int64_t head_dim, hipStream_t stream) {
-  const PagedArgs& a = l.tiles;
+  const PagedArgs& a = l.all;
   auto sized = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (l.run_tiles) {
-      const int64_t groups = (int64_t)a.view.kv_heads * ((a.families != nullptr ? (int64_t)a.family_blocks * a.family_splits : 0) + (int64_t)l.own_blocks * a.splits);
-      if (a.view.page_shift < 4) hipLaunchKernelGGL((sight_tiles_kernel<T, D, true>), dim3((unsigned)groups), dim3(256), 0, stream, a, l.own_blocks);
-      else hipLaunchKernelGGL((sight_tiles_kernel<T, D, false>), dim3((unsigned)groups), dim3(256), 0, stream, a, l.own_blocks);
+    const int shares = a.families != nullptr ? a.shares : 0;
+    if (!l.run_tiles) start_few_rows<T, true>(l.few, head_dim, stream);
+    else if (a.view.page_shift < 4) {
+      hipLaunchKernelGGL((sight_kernel<T, D, true>), dim3(shares + a.tile_groups), dim3(256), 0, stream, a);
+      if (a.run_few) start_few_rows<T, true>(l.few, head_dim, stream);
+    } else {
+      const int few_groups = !a.run_few ? 0 : a.few_splits == 0 ? a.view.batch * a.view.kv_heads : shares > 0 ? 0 : a.few_splits;
+      hipLaunchKernelGGL((sight_kernel<T, D, false>), dim3(shares + a.tile_groups + few_groups), dim3(256), 0, stream, a);
+      if (a.run_few) start_join_few_rows<T, D, true>(l.few, stream);
     }
-    if (l.run_few) start_few_rows<T, true>(l.few, head_dim, stream);
     if (a.families != nullptr || (l.run_tiles && a.splits > 1))
-      hipLaunchKernelGGL((join_sight_kernel<T, D>), dim3(a.view.tokens, (unsigned)ceil_div(a.heads, 4)), dim3(256), 0, stream, a, l.few, l.run_few);
+      hipLaunchKernelGGL((join_sight_kernel<T, D>), dim3(a.view.tokens, (unsigned)ceil_div(a.heads, 4)), dim3(256), 0, stream, a);
   };
   if (head_dim == 64) sized(std::integral_constant<int, 64>{});
   else sized(std::integral_constant<int, 128>{});
 }
 
 }  // namespace
-
 }  // namespace ttmi

@@ -26,10 +26,6 @@ namespace {
 
 constexpr int kTileRows = 128;  // of a workgroup
 constexpr int kSpanTiles = 64;  // a tile or two
-// Keys of a part of a family's, which has at most a.family_splits of them.
-__device__ __forceinline__ int family_chunk(const PagedArgs& a, const Sequence& family) {
-  return max(a.family_chunk, ((family.length + a.family_splits - 1) / a.family_splits + 63) & ~63);
-}
 // Parts that a row's own keys lie in (1 where it sees none of them).
 __device__ __forceinline__ int own_parts(const Reach& r, const Span& span, int base, int chunk) {
   return r.end > base ? (span.place_of(r.end - 1) - span.lo) / chunk + 1 : 1;
@@ -97,18 +93,18 @@ __device__ __forceinline__ void store_part(const PagedArgs& a, int64_t at, int64
 // The `want`-th block of rows of all sequences -> its sequence and number in it (false: there are fewer).  Every lane looks at a sequence of 64.
 // Where there are more workgroups than the chip takes at a time, those with the most keys come first: sequences by their keys (64 of them at a time), and in a sequence the
 // last rows, which have the most keys before them.
-// SIGHT: those of families, or of the sequences' own keys; *upto: a number from which on there are none.
+// SIGHT: *upto: a number from which on there are none.
 template <bool SIGHT>
-__device__ __forceinline__ bool find_block(const PagedArgs& a, int want, bool families, int* b, int* block, int* upto) {
+__device__ __forceinline__ bool find_block(const PagedArgs& a, int want, LaneSequences* lanes, int* b, int* block, int* upto) {
   const int lane = (int)(threadIdx.x % kWave);
   int passed = 0;
   for (int base = 0; base < a.view.batch; base += kWave) {
     int blocks = 0, reach = 0;
-    if (SIGHT && families) {
-      if (base + lane < a.view.batch) {
-        const Sequence seq = family_sequence(a, family_led_by(a, base + lane));
-        blocks = (seq.tokens * a.group + kTileRows - 1) / kTileRows, reach = seq.length;
-      }
+    if constexpr (SIGHT) {
+      *lanes = lane_sequences(a, base);
+      const int rows = lanes->tokens * a.group;
+      if (rows > kFewRows || a.every) blocks = (rows + kTileRows - 1) / kTileRows;
+      reach = a.window > 0 ? min(lanes->length, a.window + lanes->tokens) : lanes->length;
     } else if (base + lane < a.view.batch) {
       const Sequence seq = sequence(a, base + lane);
       const int rows = seq.tokens * a.group;
@@ -184,23 +180,18 @@ __device__ __forceinline__ void family_sights(const Family& f, const Reach& mine
              __builtin_amdgcn_readfirstlane(s.sure_end), __builtin_amdgcn_readfirstlane(s.low), __builtin_amdgcn_readfirstlane(s.sure_low)};
 }
 
-// Part `z` of block `want` of rows -> a number from which on there are none; SIGHT: of families, or of the sequences' own keys.  SMALL: pages of fewer than 16 slots
+// Part `z` of a block of rows of sequence b; SIGHT: of the sequence's own keys, or (family.keys > 0) of the family's that it leads, in parts of family_chunk keys.
+// SMALL: pages of fewer than 16 slots
 template <typename T, int D, bool SMALL, bool SIGHT>
-__device__ __forceinline__ int tiles(const PagedArgs& a, int want, int kv_head, int z, bool families, TilesShared<T, D>& shared) {
+__device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, const Sequence& seq, const LaneSequences& lanes, const Family& family, int family_chunk,
+                                      int kv_head, int z, TilesShared<T, D>& shared) {
   using S = Tiles<T, D>;
   char* const smem = shared.tiles;
   int& wild = shared.wild;
   const PagedView& view = a.view;
-  int b, block, upto = 0;
-  if (!find_block<SIGHT>(a, want, families, &b, &block, &upto)) return 0;
-  Family family{};
-  Sequence seq;
-  if (SIGHT && families) {
-    family = family_led_by(a, b);
-    seq = family_sequence(a, family);
-  } else seq = sequence_of_batch<SIGHT>(a, b);
+  const bool families = SIGHT && family.keys > 0;
   const int row0 = block * kTileRows, rows = min(kTileRows, seq.tokens * a.group - row0);
-  if (z == 0 && kv_head == 0 && block == 0 && threadIdx.x == 0 && !families && view.lengths[b] > seq.length) page_error(view);
+  if (z == 0 && kv_head == 0 && block == 0 && threadIdx.x == 0 && !families && seq.first + seq.tokens > seq.length) page_error(view);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lrow = lane & 31, lhalf = lane >> 5;
   const T* const keys = static_cast<const T*>(a.keys);
@@ -213,9 +204,9 @@ __device__ __forceinline__ int tiles(const PagedArgs& a, int want, int kv_head, 
   Reach mine;
   Sight sight, wave_sight;
   if (SIGHT && families) {
-    const int row = seq.start + (wave_rows > 0 ? token : 0), member = member_of(a, family, seq.start, row);
-    mine = family_reach(a, family, member, row);
-    live = live && a.families[3 * (int64_t)member] == family.first;  // (others' rows are not this family's, whatever it says)
+    bool member;
+    mine = family_reach(a, lanes, family, seq.start, seq.start + (wave_rows > 0 ? token : 0), &member);
+    live = live && member;  // (others' rows are not this family's, whatever it says)
     family_sights(family, mine, live, wave, shared, &wave_sight, &sight);
   } else {
     mine = seq.reach_of<SIGHT>(a, token);
@@ -230,13 +221,13 @@ __device__ __forceinline__ int tiles(const PagedArgs& a, int want, int kv_head, 
     chunk = seq.chunk(a);
     part0 = sight.first / chunk, part = part0 + z;
     lo = (int)max(part * (int64_t)chunk, (int64_t)(sight.first & ~(S::kKeys - 1))), hi = (int)min((part + 1) * (int64_t)chunk, (int64_t)sight.end);
-    if (lo >= hi && part != part0) return upto;
+    if (lo >= hi && part != part0) return;
   } else {
     part0 = 0, part = z;
     if (families) {  // all rows of a family have the same parts, and write them
-      chunk = family_chunk(a, seq);
+      chunk = family_chunk;
       span = {0, 0, 0, 0};
-      if (z * (int64_t)chunk >= seq.length) return upto;
+      if (z * (int64_t)chunk >= seq.length) return;
       lo = z * chunk, hi = (int)min((z + 1) * (int64_t)chunk, (int64_t)seq.length);
       if (a.window > 0) {  // of this part: the first keys that stay visible, the windows' or, from the one to the other, both
         if (lo >= sight.low) lo = max(lo, min(hi, sight.first & ~(S::kKeys - 1)));
@@ -248,7 +239,7 @@ __device__ __forceinline__ int tiles(const PagedArgs& a, int want, int kv_head, 
       chunk = seq.span_chunk(a);
       span = span_of<kSpanTiles>(sight, seq.base);
       lo = (int)min(span.lo + part * (int64_t)chunk, (int64_t)span.hi), hi = (int)min(span.lo + (part + 1) * (int64_t)chunk, (int64_t)span.hi);
-      if (lo >= hi && part != 0) return upto;
+      if (lo >= hi && part != 0) return;
     }
   }
   auto key_at = [&](int place) __attribute__((always_inline)) {
@@ -493,7 +484,7 @@ __device__ __forceinline__ int tiles(const PagedArgs& a, int want, int kv_head, 
     const LanePair both = swap_halves(sum);
     sum = both.a + both.b;
   }
-  if (!live) return upto;
+  if (!live) return;
   const int64_t at_token = seq.start + token;
   if constexpr (!SIGHT) {
     const bool sees_some = mine.end > 0;
@@ -508,14 +499,15 @@ __device__ __forceinline__ int tiles(const PagedArgs& a, int want, int kv_head, 
       if (part == 0) store_out<T, D>(a, at_token, head, mine.end > 0, lhalf, ot, sum);
     } else if (part <= last_part) store_part<D>(a, a.own_at + (at_token * a.heads + head) * a.splits + part, a.rows, lhalf, ot, top, sum);
   }
-  return upto;
 }
 
 template <typename T, int D, bool SMALL>
 __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   __shared__ TilesShared<T, D> shared;
   const int kv_head = blockIdx.x % a.view.kv_heads;
-  tiles<T, D, SMALL, false>(a, blockIdx.x / a.view.kv_heads, kv_head, blockIdx.z, false, shared);
+  int b, block, upto;
+  if (!find_block<false>(a, blockIdx.x / a.view.kv_heads, nullptr, &b, &block, &upto)) return;
+  tiles<T, D, SMALL, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, blockIdx.z, shared);
 }
 
 }  // namespace
