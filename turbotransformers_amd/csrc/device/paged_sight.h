@@ -17,7 +17,7 @@ namespace {
 // How a.shares workgroups are divided.  Work on a family is counted in steps of 64 keys of a block of 128 rows, that on the others in rounds of the few-rows kernel.  What a step costs a workgroup, in
 // sixteenths of a microsecond with two workgroups on a CU, and what a round does where all of them read: its bytes at 9.8 GB/s.
 template <typename T, int D>
-constexpr int kStepCost = sizeof(T) == 4 ? (D == 128 ? 96 : 56) : (D == 128 ? 28 : 24);
+constexpr int kStepCost = sizeof(T) == 4 ? (D == 128 ? 200 : 120) : (D == 128 ? 88 : 64);
 template <typename T, int D>
 constexpr int kRoundCost = 16 * kRound * 2 * D * (int)sizeof(T) / 9800;
 struct Shares {
@@ -103,9 +103,10 @@ __device__ __forceinline__ bool find_family_job(const PagedArgs& a, const Shares
 }
 // The share of a workgroup in the families' keys (`lanes`: the first 64 sequences, where there are no more), or in blocks of sequences with many rows, over their own keys.  More
 // blocks than was said are taken in turns.
-template <typename T, int D, bool SMALL>
+template <typename T, int D, bool SMALL, bool FAMILIES>
 __device__ __forceinline__ void sight_tiles(const PagedArgs& a, bool families, const Shares& s, int group, LaneSequences lanes, TilesShared<T, D>& shared) {
   const int kv_heads = a.view.kv_heads, kv_head = group % kv_heads, own_part = group / kv_heads % a.splits;
+  families = FAMILIES && families;
   const int step = families ? s.family_groups : a.own_blocks;
   bool there = a.view.batch <= kWave;
   for (int item = group / kv_heads / (families ? 1 : a.splits), stop = families ? s.items : INT32_MAX; item < stop; item += step) {
@@ -117,15 +118,17 @@ __device__ __forceinline__ void sight_tiles(const PagedArgs& a, bool families, c
       job.part = own_part, job.chunk = 0, job.seq = lanes.sequence(job.b - lanes.base), job.family = Family{};
     }
     there = false;  // (they are not kept where the registers are needed)
-    tiles<T, D, SMALL, true>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, kv_head, job.part, shared);
+    tiles<T, D, SMALL, true, FAMILIES>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, kv_head, job.part, shared);
     __syncthreads();
   }
 }
 
-// One launch: a.shares workgroups (none without families) for families and for sequences with few rows, a.tile_groups for those with many, the rest, if any, for few rows.  So a
-// CU has workgroups that multiply beside others that read.  SMALL: sequences with few rows have a launch of their own.
-template <typename T, int D, bool SMALL>
+// One launch: a.shares workgroups (FAMILIES) for families and for sequences with few rows, a.tile_groups for those with many, the rest, if any, for few rows (FEW).  So a
+// CU has workgroups that multiply beside others that read.  (Families take registers and FEW does not cost any, but instructions: a prompt of 8192 tokens in a window of 1024, 32 and 8
+// heads of 128, 206 us with both, 195 without.)
+template <typename T, int D, bool SMALL, bool FAMILIES, bool FEW>
 __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
+  static_assert(!FEW || !SMALL, "with small pages sequences with few rows have a launch of their own");
   __shared__ union {
     TilesShared<T, D> tiles;
     FewRowsShared<T, D, 4> few;
@@ -134,24 +137,21 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
   Walk walk{};
   Shares s{};
   int64_t units = -1;
-  const int shares = a.families != nullptr ? a.shares : 0;
-  bool families = false, own = false;
-  if (group < shares) {
+  const int shares = FAMILIES ? a.shares : 0;
+  bool families = false, own = !FEW;
+  if (FAMILIES && group < shares) {
     s = shares_of<T, D>(a, walk, &units);
     if (group == 0 && threadIdx.x == 0) *share_note<D>(a) = {s.steps, s.few_groups, units};
     families = group < s.family_groups * a.view.kv_heads;
     if (!families) group -= s.family_groups * a.view.kv_heads, few_groups = s.few_groups;
-    if (!families && (SMALL || units == 0 || group >= few_groups)) return;
+    if (!families && (!FEW || units == 0 || group >= few_groups)) return;
   } else {
     group -= shares;
-    own = group < a.tile_groups;
+    own = !FEW || group < a.tile_groups;
     if (!own) group -= a.tile_groups;
   }
-  if (families || own) {
-    sight_tiles<T, D, SMALL>(a, families, s, group, walk.lanes, shared.tiles);
-    return;
-  }
-  if constexpr (!SMALL) few_rows<T, D, 4, false, true>(a, group, few_groups, walk, units, shared.few);
+  if (families || own) sight_tiles<T, D, SMALL, FAMILIES>(a, families, s, group, walk.lanes, shared.tiles);
+  else if constexpr (FEW) few_rows<T, D, 4, false, true>(a, group, few_groups, walk, units, shared.few);
 }
 
 // A wavefront a row and head.
@@ -206,13 +206,54 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
   }
   if (of_family == 0 && parts == 1) return;  // (there already)
   const int64_t family_place = a.family_at + at * a.family_splits;
-  join_parts_by_wavefront<T, D>(
-      a.partial, a.partial + a.rows * D, of_family + parts, seq.reach(a, row - seq.start).end > 0,
-      [&](int p) {
-        const int own = p - of_family;
-        return own < 0 ? family_place + p : own == 0 ? place : second + (own - 1) * step;
-      },
-      static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)head * D);
+  const int all = of_family + parts;
+  const bool sees = seq.reach(a, row - seq.start).end > 0;
+  T* const out = static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)head * D;
+  const float* const ml = a.partial + a.rows * D;
+  auto place_of = [&](int p) {
+    const int own = p - of_family;
+    return own < 0 ? family_place + p : own == 0 ? place : second + (own - 1) * step;
+  };
+  if (all > kWave) {
+    join_parts_by_wavefront<T, D>(a.partial, ml, all, sees, place_of, out);
+    return;
+  }
+  // up to 64 parts: each lane has what one weighs, and the sums, four columns a lane and a few parts at a time, are asked for without waiting for that
+  constexpr int kThreads = D / 4, kBeside = kWave / kThreads, kAsked = 8;
+  const int lane = (int)(threadIdx.x % kWave), d0 = lane % kThreads * 4, share = lane / kThreads;
+  const int64_t mine = place_of(min(lane, all - 1));
+  const floatx2 met = *reinterpret_cast<const floatx2*>(ml + 2 * mine);
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+  float weight = 0.f, total = 0.f;
+  for (int first = 0; first < all; first += kAsked * kBeside) {
+    floatx4 x[kAsked];
+#pragma unroll
+    for (int i = 0; i < kAsked; ++i) {
+      const int p = min(first + i * kBeside + share, all - 1);
+      x[i] = *reinterpret_cast<const floatx4*>(a.partial + place_of(p) * D + d0);
+    }
+    if (first == 0) {
+      const float best = group_max<kWave>(lane < all ? met[0] : -INFINITY);
+      weight = lane < all ? __builtin_amdgcn_exp2f(met[0] - (best == -INFINITY ? 0.f : best)) : 0.f;
+      total = group_sum<kWave>(lane < all ? met[1] * weight : 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < kAsked; ++i) {
+      const int p = first + i * kBeside + share;
+      const float w = __shfl(weight, min(p, kWave - 1), kWave);
+      if (p < all) sum += x[i] * w;
+    }
+  }
+#pragma unroll
+  for (int d = kThreads; d < kWave; d *= 2)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], d, kWave);
+  if (share != 0) return;
+  const float inv = inverse_sum(total, sees);
+  Vec<T, 4> y;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) y.v[c] = from_float<T>(sum[c] * inv);
+  store_vec<T, 4>(out + d0, y);
 }
 
 template <typename T>
@@ -221,14 +262,21 @@ void start_sight(const SightLaunch& l, int64_t head_dim, hipStream_t stream) {
   auto sized = [&](auto d) {
     constexpr int D = decltype(d)::value;
     const int shares = a.families != nullptr ? a.shares : 0;
+    const bool small = a.view.page_shift < 4;
+    // (where sequences with few rows are shared out among all workgroups, those are a.shares)
+    const int few_groups = a.few_splits == 0 ? a.view.batch * a.view.kv_heads : shares > 0 ? 0 : a.few_splits;
+    auto launch = [&](auto kernel, int groups) { hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), 0, stream, a); };
     if (!l.run_tiles) start_few_rows<T, true>(l.few, head_dim, stream);
-    else if (a.view.page_shift < 4) {
-      hipLaunchKernelGGL((sight_kernel<T, D, true>), dim3(shares + a.tile_groups), dim3(256), 0, stream, a);
-      if (a.run_few) start_few_rows<T, true>(l.few, head_dim, stream);
+    else if (!small && a.run_few) {
+      if (shares > 0) launch(sight_kernel<T, D, false, true, true>, shares + a.tile_groups + few_groups);
+      else launch(sight_kernel<T, D, false, false, true>, a.tile_groups + few_groups);
+      start_join_few_rows<T, D, true>(l.few, stream);
     } else {
-      const int few_groups = !a.run_few ? 0 : a.few_splits == 0 ? a.view.batch * a.view.kv_heads : shares > 0 ? 0 : a.few_splits;
-      hipLaunchKernelGGL((sight_kernel<T, D, false>), dim3(shares + a.tile_groups + few_groups), dim3(256), 0, stream, a);
-      if (a.run_few) start_join_few_rows<T, D, true>(l.few, stream);
+      if (small && shares > 0) launch(sight_kernel<T, D, true, true, false>, shares + a.tile_groups);
+      else if (small) launch(sight_kernel<T, D, true, false, false>, a.tile_groups);
+      else if (shares > 0) launch(sight_kernel<T, D, false, true, false>, shares + a.tile_groups);
+      else launch(sight_kernel<T, D, false, false, false>, a.tile_groups);
+      if (a.run_few) start_few_rows<T, true>(l.few, head_dim, stream);
     }
     if (a.families != nullptr || (l.run_tiles && a.splits > 1))
       hipLaunchKernelGGL((join_sight_kernel<T, D>), dim3(a.view.tokens, (unsigned)ceil_div(a.heads, 4)), dim3(256), 0, stream, a);

@@ -182,14 +182,14 @@ __device__ __forceinline__ void family_sights(const Family& f, const Reach& mine
 
 // Part `z` of a block of rows of sequence b; SIGHT: of the sequence's own keys, or (family.keys > 0) of the family's that it leads, in parts of family_chunk keys.
 // SMALL: pages of fewer than 16 slots
-template <typename T, int D, bool SMALL, bool SIGHT>
+template <typename T, int D, bool SMALL, bool SIGHT, bool FAMILIES>
 __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, const Sequence& seq, const LaneSequences& lanes, const Family& family, int family_chunk,
                                       int kv_head, int z, TilesShared<T, D>& shared) {
   using S = Tiles<T, D>;
   char* const smem = shared.tiles;
   int& wild = shared.wild;
   const PagedView& view = a.view;
-  const bool families = SIGHT && family.keys > 0;
+  const bool families = FAMILIES && family.keys > 0;
   const int row0 = block * kTileRows, rows = min(kTileRows, seq.tokens * a.group - row0);
   if (z == 0 && kv_head == 0 && block == 0 && threadIdx.x == 0 && !families && seq.first + seq.tokens > seq.length) page_error(view);
 
@@ -203,7 +203,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
   // what the rows of the workgroup see, and those of this wavefront
   Reach mine;
   Sight sight, wave_sight;
-  if (SIGHT && families) {
+  if (families) {
     bool member;
     mine = family_reach(a, lanes, family, seq.start, seq.start + (wave_rows > 0 ? token : 0), &member);
     live = live && member;  // (others' rows are not this family's, whatever it says)
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   const int kv_head = blockIdx.x % a.view.kv_heads;
   int b, block, upto;
   if (!find_block<false>(a, blockIdx.x / a.view.kv_heads, nullptr, &b, &block, &upto)) return;
-  tiles<T, D, SMALL, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, blockIdx.z, shared);
+  tiles<T, D, SMALL, false, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, blockIdx.z, shared);
 }
 
 }  // namespace
