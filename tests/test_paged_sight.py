@@ -210,3 +210,12 @@ def test_python_calls_that_are_refused():
     for call in (lambda: tt.paged_attention(q, kv, kv.clone(), *ints, families=3), lambda: tt.rotary_append(qkv, kv, kv.clone(), *ints, k_norm=[1.0])):
         with pytest.raises(tt.cxx.EnforceNotMet, match="expected a tensor"):
             call()
+
+
+def test_families_are_taken_where_they_save_reads(lib):
+    """One token each of 8 or 64 sequences, 32 and 8 heads of 128 in fp16 (4 KB a key): common keys are read once, which needs room for partial results, where that is much or not known."""
+    alone = [room(lib, n, n, most=1, longest=longest, families=None) for n, longest in ((8, 600), (64, 600))]
+    assert alone == [0, 0]  # (short contexts are not cut)
+    call = lambda n, shared, count=1: room(lib, n, n, most=1, longest=600, count=count, shared=shared)
+    assert call(8, 512) == call(64, 64) == call(64, 512, 60) == 0
+    assert call(64, 512) > 0 and call(8, 8192) > 0 and call(8, 0) > 0 and call(8, 512, 0) > 0

@@ -74,7 +74,8 @@ class Sight(Case):
                 out[rows, h], tol[rows, h] = o, t
         return out, tol
 
-    def run_attention(self, families=None, hints=None, **kw):
+    def run_attention(self, families=None, hints=(0, 0), **kw):
+        """hints: family_count and max_shared.  Where neither is known families are made use of however little there is to gain; None: both as they are."""
         rows = self.rows if families is None else np.asarray(families, np.int32)
         if self.families or families is not None:
             count, most = (len({row[0] for row in rows.tolist() if row[2]}), int(rows[:, 2].max())) if hints is None else hints
@@ -85,7 +86,12 @@ class Sight(Case):
 def check(*args, causal=True, window=0, sinks=0, scale=None, **kw):
     case = Sight(*args, **kw)
     got = case.run_attention(causal=causal, window=window, sinks=sinks, scale=scale)
-    case.check_attention(got, causal=causal, window=window, sinks=sinks, scale=scale)
+    want = case.check_attention(got, causal=causal, window=window, sinks=sinks, scale=scale)
+    if case.families:
+        _, tol = case.attention(causal=causal, window=window, sinks=sinks, scale=scale)
+        n = int(case.starts[-1])
+        hinted = case.run_attention(causal=causal, window=window, sinks=sinks, scale=scale, hints=None).cpu().double()
+        assert ((hinted[:n] - want[:n]).abs() <= tol[:n]).all()
     assert (got[int(case.starts[-1]):] == 7.0).all()  # rows behind the last sequence are left as they were
 
 
@@ -208,7 +214,7 @@ def test_families_with_windows_and_sinks(dt, window, sinks):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("hints", [(0, 0), (1, 1), (1 << 40, 1 << 40), (7, 200)])
+@pytest.mark.parametrize("hints", [(0, 0), (1, 1), (1 << 40, 1 << 40), (7, 200), (1, 0), (0, 64), (1, 1 << 40)])
 def test_hints_of_families_choose_nothing_but_the_cut(dt, hints):
     case = Sight(dt, [1, 40, 1, 1, 1, 3], [1600, 1400, 1500, 300, 260, 90], 8, 2, 64, 16, families=[(3, 1392), (2, 256), (1, 0)])
     case.check_attention(case.run_attention(hints=hints))
@@ -222,9 +228,9 @@ def test_rows_of_families_that_disagree_are_sequences_on_their_own():
     for rows in ([[0, 6, 0]] * 6, [[0, 6, -5]] * 6, [[-1, 6, 512]] * 6, [[9, 6, 512]] * 6, [[big - 1, big - 1, big - 1]] * 6, [[-big, -big, -big]] * 6, [[0, 3, 512]] * 6,
                  [[0, 6, 512]] * 3 + [[3, 6, 256]] * 3, [[1, 6, 512], [0, 6, 512]] + [[0, 6, 512]] * 4, [[0, 6, 512], [0, 2, 256], [2, 6, 512], [2, 6, 512], [0, 6, 512], [4, 9, 400]],
                  [[5, 6, 512]] * 5 + [[5, 6, 512]], [[0, 6, 512]] + [[b, b + 1, 512] for b in range(1, 6)], [[0, 0, 512]] * 6):
-        case.check_attention(case.run_attention(families=rows, hints=(1, 512)))
+        case.check_attention(case.run_attention(families=rows))
     # more keys promised than lie in the same pages: they are read from the first sequence's, whose own result that is
-    got = case.run_attention(families=[[0, 100, big - 1]] * 6, hints=(1, 512))
+    got = case.run_attention(families=[[0, 100, big - 1]] * 6)
     want, tol = case.attention()
     assert ((got[0].cpu().double() - want[0]).abs() <= tol[0]).all()
     tt.cxx.synchronize()
@@ -370,7 +376,7 @@ def test_recorded_steps(dt):
 
     def call():
         q = tt.rotary_append(qkv, keys, values, table, starts, lengths, inv_freq, q_norm=norm, k_norm=norm)
-        return (tt.paged_attention(q, keys, values, table, starts, lengths, max_tokens=1, max_length=720, families=rows, family_count=1, max_shared=512),
+        return (tt.paged_attention(q, keys, values, table, starts, lengths, max_tokens=1, max_length=720, families=rows),
                 tt.paged_attention(q, keys, values, table, starts, lengths, max_tokens=1, max_length=720, window=300, sinks=70))
 
     call()
@@ -616,6 +622,7 @@ def test_a_decoder_whose_samples_share_their_prompt(dt, window, sinks):
     def step(names, tokens):
         batch = cache.extend(names, tokens, share=True)
         families.append(batch.family_count)
+        batch.family_count = batch.max_shared = 0  # (so few keys are read once only where it is not known how few they are)
         for layer in range(layers):
             qkv = torch.randn(sum(tokens), heads + 2 * kv_heads, d, generator=gen).to(dtype)
             at = 0
@@ -679,3 +686,16 @@ def test_families_and_none_agree(dt):
     plain = Case.run_attention(case)
     case.check_attention(plain)
     case.check_attention(case.run_attention())
+    assert torch.equal(case.run_attention(hints=None), plain)  # (too few keys to gain anything)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("new,window,sinks", [(1, 0, 0), (1, 900, 40), (6, 0, 0)])
+def test_families_that_are_worth_it(dt, new, window, sinks):
+    """As many common keys as are read once where all is known: those of 70 sequences, cut and joined, and the same bits without hints."""
+    rng = random.Random(new)
+    past = [2048 + rng.choice([1, 20, 300]) for _ in range(70)] + [900]
+    case = Sight(dt, [new] * 71, past, 8, 4, 64, 16, families=[(70, 2048), (1, 0)])
+    case.keys, case.values = case.keys.nan_to_num(), case.values.nan_to_num()
+    got = case.run_attention(hints=None, window=window, sinks=sinks)
+    case.check_attention(got, window=window, sinks=sinks)

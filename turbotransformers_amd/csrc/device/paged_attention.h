@@ -275,6 +275,27 @@ __device__ __forceinline__ void come_to(const PagedView& view, PageCursor& c, in
   if (past >= 2 * kWave) fetch_pages<ROW_BYTES>(view, c, kv_head, key);
   else hold_pages<ROW_BYTES>(view, c, kv_head, c.first + kWave, c.ahead);
 }
+// SIGHT: behind a gap lie pages that are known from the start, so their numbers are asked for with the first ones and not when the gap is reached (which costs a workgroup a trip to memory).
+struct GapCursor : PageCursor {
+  int next;  // number of the first page that `ahead` is of
+};
+template <int ROW_BYTES>
+__device__ __forceinline__ void fetch_pages(const PagedView& view, GapCursor& c, int kv_head, int key, int behind) {
+  fetch_pages<ROW_BYTES>(view, c, kv_head, key);
+  c.next = c.first + kWave;
+  if (behind > key) {
+    c.next = behind >> view.page_shift;
+    c.ahead = c.table[min(c.next + (int)(threadIdx.x % kWave), c.last)];
+  }
+}
+template <int ROW_BYTES>
+__device__ __forceinline__ void come_to(const PagedView& view, GapCursor& c, int kv_head, int key) {
+  const int page = key >> view.page_shift;
+  if (__builtin_expect(page - c.first < kWave, 1)) return;
+  if ((unsigned)(page - c.next) < (unsigned)kWave) hold_pages<ROW_BYTES>(view, c, kv_head, c.next, c.ahead);
+  else fetch_pages<ROW_BYTES>(view, static_cast<PageCursor&>(c), kv_head, key);
+  c.next = c.first + kWave;
+}
 // Byte of the cache at which the row of `key`, uniform and a multiple of 16, begins; the rows of its group follow.
 template <int ROW_BYTES>
 __device__ __forceinline__ int64_t group_at(const PagedView& view, const PageCursor& c, int key) {

@@ -108,6 +108,18 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
   return p;
 }
 
+// Whether reading a family's keys once is worth a second launch, which joins what they give with what the sequences' own keys do: from about so many bytes less on (of which the caches would take
+// most).  us, families / none, one token each behind common keys and 50 of its own: bf16, 32 and 8 heads of 128, 4 sequences behind 4000 (49 MB less) 17.6 / 17.2, 8 behind 2000 (57) 18.9 / 19.0, 32
+// behind 1000 (127) 21.8 / 21.3, 16 behind 4000 (246) 21.9 / 30.6, 64 behind 8000 (2064) 40 / 147; fp16, 12 heads of 64, 4 behind 4000 (37) 15.8 / 15.8, 16 behind 1000 (46) 13.7 / 8.9, 32 behind
+// 2000 (190) 15.9 / 25.5; fp32, 12 heads of 64, 8 behind 2000 (86) 21.6 / 21.1, 64 behind 512 (198) 20.3 / 23.4, 8 behind 8000 (344) 35 / 45.  Where nothing is known they are taken as they come.
+constexpr int64_t kSharedBytes = 80 << 20;
+bool sharing_pays(const PagedView& view, const ttmi_paged_sight& sight, int dtype) {
+  if (sight.families == nullptr) return false;
+  if (sight.family_count == 0 || sight.max_shared == 0) return true;
+  const int64_t held = view.table_pitch << view.page_shift, shared = std::min(sight.max_shared, held);
+  return std::max<int64_t>(0, view.batch - sight.family_count) * shared >= kSharedBytes / (2 * view.kv_heads * view.head_dim * (int64_t)dtype_size(dtype));
+}
+
 int check_sight(const ttmi_paged_sight* sight) {
   TTMI_REQUIRE(sight != nullptr, "sight is null");
   TTMI_REQUIRE(sight->window >= 0 && sight->sinks >= 0 && sight->family_count >= 0 && sight->max_shared >= 0,
@@ -187,13 +199,15 @@ int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int64_t out_
 int ttmi_paged_attention_sight_workspace(const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, int64_t heads, int64_t max_tokens, int64_t max_length,
                                          const ttmi_paged_sight* sight, int dtype, int64_t* bytes) {
   if (int rc = check_sight(sight)) return rc;
-  if (sight->families == nullptr && (sight->sinks == 0 || sight->window == 0))
-    return ttmi_paged_attention_workspace(cache, batch, heads, max_tokens, max_length, sight->window, dtype, bytes);
   PagedView view;
   TTMI_REQUIRE(bytes != nullptr, "bytes is null");
   if (int rc = paged_view(cache, batch, heads, &view)) return rc;
+  ttmi_paged_sight used = *sight;
+  if (!sharing_pays(view, used, dtype)) used.families = nullptr;
+  if (used.families == nullptr && (used.sinks == 0 || used.window == 0))
+    return ttmi_paged_attention_workspace(cache, batch, heads, max_tokens, max_length, used.window, dtype, bytes);
   TTMI_REQUIRE(max_tokens >= 0 && max_length >= 0, "max_tokens and max_length must not be negative");
-  *bytes = batch->tokens == 0 || batch->batch == 0 ? 0 : plan_sight(view, heads, max_tokens, max_length, *sight, dtype).floats * 4;
+  *bytes = batch->tokens == 0 || batch->batch == 0 ? 0 : plan_sight(view, heads, max_tokens, max_length, used, dtype).floats * 4;
   return 0;
 }
 
@@ -201,17 +215,19 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
                                const ttmi_paged_batch* batch, int64_t max_tokens, int64_t max_length, float scale, int causal, const ttmi_paged_sight* sight,
                                void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
   if (int rc = check_sight(sight)) return rc;
-  if (sight->families == nullptr && (sight->sinks == 0 || sight->window == 0))
-    return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, sight->window, workspace, workspace_bytes,
-                                dtype, stream);
   SightLaunch l;
   PagedArgs& a = l.all;
   if (int rc = attention_args(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, sight->window, dtype, &a)) return rc;
   if (batch->tokens == 0 || batch->batch == 0) return 0;
-  const SightPlan p = plan_sight(a.view, heads, max_tokens, max_length, *sight, dtype);
+  ttmi_paged_sight used = *sight;
+  if (!sharing_pays(a.view, used, dtype)) used.families = nullptr;
+  if (used.families == nullptr && (used.sinks == 0 || used.window == 0))
+    return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, used.window, workspace, workspace_bytes,
+                                dtype, stream);
+  const SightPlan p = plan_sight(a.view, heads, max_tokens, max_length, used, dtype);
   TTMI_REQUIRE(p.floats == 0 || (workspace != nullptr && workspace_bytes >= p.floats * 4 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                "the workspace is too small or not 16-byte aligned");
-  a.sinks = (int)std::min(sight->sinks, kWidest), a.families = sight->families;
+  a.sinks = (int)std::min(used.sinks, kWidest), a.families = used.families;
   a.partial = static_cast<float*>(workspace);
   a.every = !p.own.few, a.chunk = p.own.tile_chunk, a.splits = p.own.tile_splits, a.ordered = 1;
   a.shares = p.shares, a.family_splits = p.family_splits, a.family_least = p.family_least;

@@ -232,7 +232,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
     const int rows_all = seq.tokens * a.group;
     if (rows_all <= 0 || (rows_all > a.few && !(SIGHT ? a.few_every : a.every))) return;  // (a workgroup of its own)
     if (round0 == 0 && kv_head == 0 && tid == 0 && view.lengths[b] > seq.length) page_error(view);
-    PageCursor cursor;
+    typename std::conditional<SIGHT, GapCursor, PageCursor>::type cursor;
     cursor.table = view.table + (int64_t)b * view.table_pitch;
     cursor.first = 0, cursor.ahead = 0, cursor.at = 0;
 
@@ -419,7 +419,9 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
       };
       int place = lo + wave * S::kKeys;
       if (place < hi) {
-        if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, key_at(place));
+        // (a wavefront's tiles lie kStep apart: behind the gap it begins anywhere in one of its steps, aligned as its tiles are)
+        if constexpr (!SMALL && SIGHT) fetch_pages<S::kRowBytes>(view, cursor, kv_head, key_at(place), span.skip > 0 && place < span.seam ? span.seam + span.skip : 0);
+        else if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, place);
         load_values(key_at(place));
         load_keys(key_at(place));
         for (; place + kStep < hi; place += kStep) work_on(place, std::true_type{});

@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
   if (!a.run_few || (rows > kFewRows && !a.few_every)) {
     const Reach mine = seq.own_reach(a, row - seq.start);
     const int row0 = r / kTileRows * kTileRows, last = min(rows, row0 + kTileRows) - 1;
-    const Span span = span_of<kSpanTiles>(sight_of(seq.own_reach(a, row0 / a.group), seq.own_reach(a, last / a.group)), seq.base);
+    const Span span = span_of<kSpanTiles<T>>(sight_of(seq.own_reach(a, row0 / a.group), seq.own_reach(a, last / a.group)), seq.base);
     parts = own_parts(mine, span, seq.base, seq.span_chunk(a));
     place = a.own_at + at * a.splits, second = place + 1, step = 1;
   } else if (a.families == nullptr) {

@@ -25,7 +25,8 @@ namespace ttmi {
 namespace {
 
 constexpr int kTileRows = 128;  // of a workgroup
-constexpr int kSpanTiles = 64;  // a tile or two
+template <typename T>
+constexpr int kSpanTiles = sizeof(T) == 2 ? 64 : 32;
 // Parts that a row's own keys lie in (1 where it sees none of them).
 __device__ __forceinline__ int own_parts(const Reach& r, const Span& span, int base, int chunk) {
   return r.end > base ? (span.place_of(r.end - 1) - span.lo) / chunk + 1 : 1;
@@ -33,7 +34,7 @@ __device__ __forceinline__ int own_parts(const Reach& r, const Span& span, int b
 
 template <typename T, int D>
 struct Tiles {
-  static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // (a part of kSpanTiles)
+  static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // (as in kSpanTiles)
   static constexpr int kSubs = kKeys / 32;
   static constexpr int kElems = 16 / (int)sizeof(T);
   static constexpr int kRowBytes = D * (int)sizeof(T);
@@ -237,7 +238,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
       }
     } else {
       chunk = seq.span_chunk(a);
-      span = span_of<kSpanTiles>(sight, seq.base);
+      span = span_of<kSpanTiles<T>>(sight, seq.base);
       lo = (int)min(span.lo + part * (int64_t)chunk, (int64_t)span.hi), hi = (int)min(span.lo + (part + 1) * (int64_t)chunk, (int64_t)span.hi);
       if (lo >= hi && part != 0) return;
     }
@@ -260,7 +261,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
     for (int e = 0; e < 16; ++e) ot[t][e] = 0.f;
   float top = -INFINITY, sum = 0.f;
 
-  PageCursor cursor;
+  typename std::conditional<SIGHT, GapCursor, PageCursor>::type cursor;
   cursor.table = view.table + (int64_t)b * view.table_pitch;
   cursor.last = max(0, (sight.end - 1) >> view.page_shift);
   cursor.first = 0, cursor.ahead = 0, cursor.at = 0;
@@ -302,7 +303,8 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
   if (lo < hi) {
     // (Loads past the last tile fetch that once more, out of L2: a load that may or may not have been sent would make the compiler wait for all of them.)
     const int last = lo + (hi - 1 - lo) / S::kKeys * S::kKeys;
-    if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, key_at(lo));
+    if constexpr (!SMALL && SIGHT) fetch_pages<S::kRowBytes>(view, cursor, kv_head, key_at(lo), span.skip > 0 && lo < span.seam ? span.seam + span.skip : 0);
+    else if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, lo);
 #pragma unroll
     for (int i = 0; i < S::kPieces; ++i) load_piece(i, key_at(lo), 0);
     if (tid == 0) wild = 0;
