@@ -8,6 +8,7 @@
 #include "paged_attention.h"
 
 #include <limits>
+#include <cstdlib>
 
 namespace ttmi {
 namespace {
@@ -204,7 +205,7 @@ int ttmi_paged_attention_sight_workspace(const ttmi_paged_cache* cache, const tt
   if (int rc = paged_view(cache, batch, heads, &view)) return rc;
   ttmi_paged_sight used = *sight;
   if (!sharing_pays(view, used, dtype)) used.families = nullptr;
-  if (used.families == nullptr && (used.sinks == 0 || used.window == 0))
+  if (used.families == nullptr && (used.sinks == 0 || used.window == 0) && !getenv("FORCE"))
     return ttmi_paged_attention_workspace(cache, batch, heads, max_tokens, max_length, used.window, dtype, bytes);
   TTMI_REQUIRE(max_tokens >= 0 && max_length >= 0, "max_tokens and max_length must not be negative");
   *bytes = batch->tokens == 0 || batch->batch == 0 ? 0 : plan_sight(view, heads, max_tokens, max_length, used, dtype).floats * 4;
@@ -221,7 +222,7 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   ttmi_paged_sight used = *sight;
   if (!sharing_pays(a.view, used, dtype)) used.families = nullptr;
-  if (used.families == nullptr && (used.sinks == 0 || used.window == 0))
+  if (used.families == nullptr && (used.sinks == 0 || used.window == 0) && !getenv("FORCE"))
     return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, used.window, workspace, workspace_bytes,
                                 dtype, stream);
   const SightPlan p = plan_sight(a.view, heads, max_tokens, max_length, used, dtype);

@@ -101,24 +101,31 @@ __device__ __forceinline__ bool find_family_job(const PagedArgs& a, const Shares
   }
   return false;
 }
-// The share of a workgroup in the families' keys (`lanes`: the first 64 sequences, where there are no more), or in blocks of sequences with many rows, over their own keys.  More
-// blocks than was said are taken in turns.
+// The share of a workgroup in the families' keys (`lanes`: the first 64 sequences, where there are no more), taken in turns where there are more than workgroups; or a part of a block of a sequence
+// with many rows, over its own keys.
 template <typename T, int D, bool SMALL, bool FAMILIES>
 __device__ __forceinline__ void sight_tiles(const PagedArgs& a, bool families, const Shares& s, int group, LaneSequences lanes, TilesShared<T, D>& shared) {
-  const int kv_heads = a.view.kv_heads, kv_head = group % kv_heads, own_part = group / kv_heads % a.splits;
-  families = FAMILIES && families;
-  const int step = families ? s.family_groups : a.own_blocks;
+  const int kv_heads = a.view.kv_heads, kv_head = group % kv_heads;
+  if constexpr (!FAMILIES) {
+    int b, block;
+    if (!find_block(a, group / kv_heads / a.splits, &b, &block)) return;
+    tiles<T, D, SMALL, true, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, group / kv_heads % a.splits, shared);
+    return;
+  }
+  const int step = families ? s.family_groups : 1, stop = families ? s.items : 1;
   bool there = a.view.batch <= kWave;
-  for (int item = group / kv_heads / (families ? 1 : a.splits), stop = families ? s.items : INT32_MAX; item < stop; item += step) {
+  for (int item = families ? group / kv_heads : 0; item < stop; item += step) {
     Job job;
     if (families) {
       if (!find_family_job(a, s, item, there, lanes, &job)) return;
     } else {
-      if (!find_block<true>(a, item, &lanes, &job.b, &job.block, &stop)) return;
-      job.part = own_part, job.chunk = 0, job.seq = lanes.sequence(job.b - lanes.base), job.family = Family{};
+      if (!find_block(a, group / kv_heads / a.splits, &job.b, &job.block)) return;
+      lanes = lane_sequences(a, job.b & ~(kWave - 1));
+      job.part = group / kv_heads % a.splits, job.chunk = 0, job.seq = lanes.sequence(job.b % kWave), job.family = Family{};
     }
     there = false;  // (they are not kept where the registers are needed)
     tiles<T, D, SMALL, true, FAMILIES>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, kv_head, job.part, shared);
+    if (item + step >= stop) break;  // (without waiting for what was stored)
     __syncthreads();
   }
 }

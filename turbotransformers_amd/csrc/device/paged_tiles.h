@@ -94,19 +94,11 @@ __device__ __forceinline__ void store_part(const PagedArgs& a, int64_t at, int64
 // The `want`-th block of rows of all sequences -> its sequence and number in it (false: there are fewer).  Every lane looks at a sequence of 64.
 // Where there are more workgroups than the chip takes at a time, those with the most keys come first: sequences by their keys (64 of them at a time), and in a sequence the
 // last rows, which have the most keys before them.
-// SIGHT: *upto: a number from which on there are none.
-template <bool SIGHT>
-__device__ __forceinline__ bool find_block(const PagedArgs& a, int want, LaneSequences* lanes, int* b, int* block, int* upto) {
+__device__ __forceinline__ bool find_block(const PagedArgs& a, int want, int* b, int* block) {
   const int lane = (int)(threadIdx.x % kWave);
-  int passed = 0;
   for (int base = 0; base < a.view.batch; base += kWave) {
     int blocks = 0, reach = 0;
-    if constexpr (SIGHT) {
-      *lanes = lane_sequences(a, base);
-      const int rows = lanes->tokens * a.group;
-      if (rows > kFewRows || a.every) blocks = (rows + kTileRows - 1) / kTileRows;
-      reach = a.window > 0 ? min(lanes->length, a.window + lanes->tokens) : lanes->length;
-    } else if (base + lane < a.view.batch) {
+    if (base + lane < a.view.batch) {
       const Sequence seq = sequence(a, base + lane);
       const int rows = seq.tokens * a.group;
       if (rows > kFewRows || a.every) blocks = (rows + kTileRows - 1) / kTileRows;
@@ -133,10 +125,9 @@ __device__ __forceinline__ bool find_block(const PagedArgs& a, int want, LaneSeq
       const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(want >= before && want < before + blocks)) - 1);
       *b = base + found;
       *block = __builtin_amdgcn_readlane(before + blocks, found) - 1 - want;
-      if constexpr (SIGHT) *upto = base + kWave < a.view.batch ? INT32_MAX : passed + all;
       return true;
     }
-    want -= all, passed += all;
+    want -= all;
   }
   return false;
 }
@@ -363,13 +354,24 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
 #pragma unroll
       for (int i = 0; i < S::kPieces; ++i) load_piece(i, after, set);
       if (__builtin_expect(!all_see<SIGHT>(wave_sight, key, S::kKeys), 0)) {
-        const int from = mine.begin - key - 4 * lhalf, low = mine.low - key - 4 * lhalf;
-        const uint32_t span = (uint32_t)(mine.end - mine.begin);
+        // (a tile below `low` may have a hole behind what is seen of the first keys: then what is seen in it ends with the rest, and the hole is taken out)
+        const bool holed = SIGHT && key < wave_sight.low;
+        const int begin = holed ? min(mine.begin, key) : mine.begin, from = begin - key - 4 * lhalf;
+        const uint32_t span = (uint32_t)(mine.end - begin);
 #pragma unroll
         for (int u = 0; u < S::kSubs; ++u)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if ((uint32_t)(32 * u + 8 * (e / 4) + e % 4 - from) >= span && (!SIGHT || 32 * u + 8 * (e / 4) + e % 4 >= low)) st[u][e] = -INFINITY;
+            if ((uint32_t)(32 * u + 8 * (e / 4) + e % 4 - from) >= span) st[u][e] = -INFINITY;
+        if (holed) {
+          const int hole = mine.low - key - 4 * lhalf;
+          const uint32_t keys = (uint32_t)max(0, mine.begin - mine.low);
+#pragma unroll
+          for (int u = 0; u < S::kSubs; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if ((uint32_t)(32 * u + 8 * (e / 4) + e % 4 - hole) < keys) st[u][e] = -INFINITY;
+        }
       }
       float m;
       {
@@ -507,8 +509,8 @@ template <typename T, int D, bool SMALL>
 __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   __shared__ TilesShared<T, D> shared;
   const int kv_head = blockIdx.x % a.view.kv_heads;
-  int b, block, upto;
-  if (!find_block<false>(a, blockIdx.x / a.view.kv_heads, nullptr, &b, &block, &upto)) return;
+  int b, block;
+  if (!find_block(a, blockIdx.x / a.view.kv_heads, &b, &block)) return;
   tiles<T, D, SMALL, false, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, blockIdx.z, shared);
 }
 
