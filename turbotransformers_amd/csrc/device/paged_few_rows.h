@@ -182,6 +182,11 @@ __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t 
   p.kv_head = rest / p.rounds, p.round = rest - p.kv_head * p.rounds;
   return p;
 }
+// a / b of numbers that are not negative: a division of 64 bits takes longer than a trip to L2, and they are seldom needed.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (__builtin_expect((((uint64_t)a | (uint64_t)b) >> 32) == 0, 1)) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
 // Workgroups that share the work.  At least kFewest rounds each, so that a wavefront has more than its first tile's wait.  us, 1 / 2 / 4 of them, 8 key heads of 128: 1 sequence
 // of 1500 keys 11.6 / 12.5 / 15.6, of 8000 16.4 / 14.1 / 15.6, 8 of 1000 19.0 / 16.7 / 17.7, 8 of 2000 21.2 / 21.4 / 25.8.
 constexpr int kFewest = 2;
@@ -211,7 +216,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
   if (splits > 0) {
     const int64_t units = SIGHT && all_units >= 0 ? all_units : count_units<SIGHT>(a, walk), workgroups = sharers(splits, units);
     if (workgroup >= workgroups) return;
-    unit = units * workgroup / workgroups, stop = units * (workgroup + 1) / workgroups;
+    if constexpr (SIGHT) unit = quotient(units * workgroup, workgroups), stop = quotient(units * (workgroup + 1), workgroups);
+    else unit = units * workgroup / workgroups, stop = units * (workgroup + 1) / workgroups;
   }
   while (unit < stop) {
     Place place;
@@ -493,7 +499,7 @@ __device__ __forceinline__ Sharers sharers_of(const PagedArgs& a, Walk& walk, in
   while (walk.base + kWave <= b) walk_on<SIGHT>(a, walk);
   const int lane = b - walk.base, rounds = __builtin_amdgcn_readlane(walk.rounds, lane);
   const int64_t unit = walk.before + lane_of(walk.upto, lane) - (int64_t)rounds * (a.view.kv_heads - kv_head);
-  return {((unit + kStart + 1) * workgroups - 1) / units, ((unit + rounds) * workgroups - 1) / units};
+  return {quotient((unit + kStart + 1) * workgroups - 1, units), quotient((unit + rounds) * workgroups - 1, units)};
 }
 
 // Pairs that were several workgroups': their rows' partial results are joined, in 5 to 7 us, nearly all of them the launch and three trips to memory.  A workgroup per pair and row, or per pair where there are many of them: then a wavefront

@@ -61,9 +61,10 @@ __device__ __forceinline__ Shares shares_of(const PagedArgs& a, Walk& walk, int6
       longest = __builtin_amdgcn_readlane(w.steps, __ffsll((unsigned long long)more) - 1);
   }
   Shares s;
-  const int64_t family_cost = steps * kStepCost<T, D>, cost = family_cost + *units / kv_heads * kRoundCost<T, D>;
-  const int groups = max(kv_heads, (int)(cost > 0 ? (uint64_t)(a.shares * family_cost) / (uint64_t)cost : 0));
-  s.steps = max(max(a.family_least, (longest + a.family_splits - 1) / a.family_splits), (int)min((steps * kv_heads + groups - 1) / groups, (int64_t)INT32_MAX));
+  // (in floats: every workgroup finds the same, and those that follow are told)
+  const float family_cost = (float)(steps * kv_heads) * kStepCost<T, D>, cost = family_cost + (float)*units * kRoundCost<T, D>;
+  const float groups = fmaxf((float)kv_heads, cost > 0.f ? a.shares * (family_cost / cost) : 0.f);
+  s.steps = max(max(a.family_least, (longest + a.family_splits - 1) / a.family_splits), (int)fminf(__builtin_ceilf((float)(steps * kv_heads) / groups), 0x1p30f));
   s.items = 0;
   for (int base = 0; base < a.view.batch; base += kWave) {
     const FamilyWork w = family_work(a, single ? walk.lanes : lane_sequences(a, base));
