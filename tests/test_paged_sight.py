@@ -217,5 +217,5 @@ def test_families_are_taken_where_they_save_reads(lib):
     alone = [room(lib, n, n, most=1, longest=longest, families=None) for n, longest in ((8, 600), (64, 600))]
     assert alone == [0, 0]  # (short contexts are not cut)
     call = lambda n, shared, count=1: room(lib, n, n, most=1, longest=600, count=count, shared=shared)
-    assert call(8, 512) == call(64, 64) == call(64, 512, 60) == 0
-    assert call(64, 512) > 0 and call(8, 8192) > 0 and call(8, 0) > 0 and call(8, 512, 0) > 0
+    assert call(8, 512) == call(64, 64) == call(64, 256) == call(64, 512, 60) == 0
+    assert call(64, 4096) > 0 and call(8, 16384) > 0 and call(8, 0) > 0 and call(8, 512, 0) > 0

@@ -184,18 +184,26 @@ struct LaneSequences {
     return s;
   }
 };
-__device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int base) {
-  const PagedView& view = a.view;
-  const int lane = (int)(threadIdx.x % kWave), b = base + lane, at = min(b, view.batch - 1);
-  LaneSequences s;
-  s.base = base;
-  s.starts = view.starts[at], s.ends = view.starts[at + 1];
-  const int length = view.lengths[at];
-  int row[3] = {-1, 0, 0};
+struct LaneNumbers {  // as they are given
+  int starts, ends, length, row[3];
+};
+__device__ __forceinline__ LaneNumbers lane_numbers(const PagedArgs& a, int base) {
+  const int at = min(base + (int)(threadIdx.x % kWave), a.view.batch - 1);
+  LaneNumbers n = {a.view.starts[at], a.view.starts[at + 1], a.view.lengths[at], {-1, 0, 0}};
   if (a.families != nullptr) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) row[i] = a.families[3 * (int64_t)at + i];
+    for (int i = 0; i < 3; ++i) n.row[i] = a.families[3 * (int64_t)at + i];
   }
+  return n;
+}
+__device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int base, const LaneNumbers& numbers) {
+  const PagedView& view = a.view;
+  const int lane = (int)(threadIdx.x % kWave), b = base + lane;
+  LaneSequences s;
+  s.base = base;
+  s.starts = numbers.starts, s.ends = numbers.ends;
+  const int length = numbers.length;
+  const int(&row)[3] = numbers.row;
   const int held = (int)min((int64_t)length, view.table_pitch << view.page_shift);
   s.start = max(0, s.starts), s.tokens = b < view.batch ? max(0, min(s.ends, view.tokens) - s.start) : 0;
   s.length = max(0, held), s.first = length - s.tokens;
@@ -216,6 +224,7 @@ __device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int 
   if (b < end) s.own = keys;
   return s;
 }
+__device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int base) { return lane_sequences(a, base, lane_numbers(a, base)); }
 // The sequence of a family that a row of q belongs to, each lane's own, and what of the family's keys the row sees; *member: whether that sequence says that it is of the family.  Where each
 // sequence has one new token and they lie among the 64, no trip to memory.
 __device__ __forceinline__ Reach family_reach(const PagedArgs& a, const LaneSequences& s, const Family& f, int start, int row, bool* member) {

@@ -7,6 +7,7 @@
 // paged_tiles.hip.  This file cuts the work: keys of a sequence into parts, where there are few rows and heads, whose results a small kernel joins.
 #include "paged_attention.h"
 
+#include <cmath>
 #include <limits>
 #include <cstdlib>
 
@@ -76,9 +77,41 @@ PagedPlan plan(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t
   return p;
 }
 
+// Blocks of 128 rows over `steps` steps of 64 keys, cut into how many parts, and about how long they take (us): workgroups of one part, two on a CU, in as many rounds as there are (a last one that
+// leaves each CU at most one takes about half as long, but not where they wait for keys), and what writing and joining the parts costs.
+struct Cut {
+  int64_t parts;
+  double us;
+};
+Cut best_cut(double blocks, int64_t steps, double step, bool single, int64_t tokens, int64_t heads, int64_t head_dim) {
+  const double cus = compute_units(), join = (double)tokens * heads * (head_dim + 2) * 8 / 4.5e6;
+  Cut best = {1, 1e30};
+  for (int64_t parts = 1; parts <= 64 && parts <= steps; ++parts) {
+    const double groups = blocks * parts, rounds = std::floor(groups / (2 * cus)), rest = groups - rounds * 2 * cus;
+    const double us = (rounds + (rest <= 0 ? 0 : rest <= cus && !single ? 0.55 : 1)) * (double)ceil_div(steps, parts) * step + parts * join;
+    if (us < best.us) best = {parts, us};
+  }
+  return best;
+}
+// us a step where two workgroups are on a CU: bound by products, or (single tokens, few of whose rows are alive) by the wait for keys
+double step_us(int dtype, int64_t head_dim, bool single) {
+  if (dtype == TTMI_F32) return head_dim == 128 ? 27 : single ? 11 : 8;
+  return head_dim == 128 ? (single ? 4 : 2.3) : (single ? 2.2 : 1.35);
+}
+bool single_tokens(const PagedView& view, int64_t heads) { return view.tokens * (heads / view.kv_heads) <= kFewRows * (int64_t)view.batch; }
+struct FamilyGuess {
+  double blocks;  // of rows
+  int64_t steps;  // of the longest
+};
+FamilyGuess guess_families(const PagedView& view, int64_t heads, const ttmi_paged_sight& sight) {
+  const int64_t held = view.table_pitch << view.page_shift, shared = sight.max_shared > 0 ? std::min(sight.max_shared, held) : held;
+  const int64_t count = std::max<int64_t>(1, std::min<int64_t>(sight.family_count, view.batch / 2));
+  return {(double)std::max(count, ceil_div(view.tokens * (heads / view.kv_heads), 128)), std::max<int64_t>(1, shared / 64)};
+}
+
 // With first keys that stay visible and with families.  The sequences' own keys are cut as ever (their number is guessed from max_length: a sequence on its own may be that long).  A family's are
-// cut on the device, which knows how many there are; here it is said how many workgroups there will be, two a CU or, where each would have more than 32 steps of 64 keys, four times as many
-// (16 questions about 20000 tokens, 32 and 8 heads of 128: 1 / 2 / 3 / 5 / 8 parts 650 / 570 / 498 / 475 / 487 us).
+// cut on the device, which knows how many there are; here it is said into how many parts at most, and how many workgroups there will be: one for each part, or two a CU where sequences
+// with few rows take a share of them (16 questions about 20000 tokens, 32 and 8 heads of 128: 1 / 2 / 3 / 5 / 8 parts 650 / 570 / 498 / 475 / 487 us).
 struct SightPlan {
   PagedPlan own;
   int shares, family_splits, family_least, own_blocks;
@@ -93,32 +126,44 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
   p.shares = p.family_splits = p.family_least = 0, p.family_rows = p.whole_rows = 0;
   const bool families = sight.families != nullptr;
   if (families) {
-    const int64_t held = view.table_pitch << view.page_shift, shared = std::max<int64_t>(1, sight.max_shared > 0 ? std::min(sight.max_shared, held) : held);
-    const int64_t count = std::max<int64_t>(1, std::min<int64_t>(sight.family_count, view.batch / 2)), cus = compute_units();
-    const int64_t steps = ceil_div(shared, 64), all = std::max(count, ceil_div(tokens * group, 128)) * steps * view.kv_heads;
-    p.shares = (int)std::max(all > 64 * cus ? 8 * cus : 2 * cus, 2 * (int64_t)view.kv_heads);  // (each head has one, and leaves as many)
+    const FamilyGuess guess = guess_families(view, heads, sight);
+    const bool single = single_tokens(view, heads);
+    const int64_t two = 2 * compute_units(), pairs = (int64_t)guess.blocks * view.kv_heads;
     p.family_least = dtype == TTMI_F32 ? 1 : 2;
-    // (where the sequences' own keys have a share too, parts are longer and so fewer)
-    p.family_splits = (int)ceil_div(steps, std::max<int64_t>(p.family_least, all / p.shares)) + 1;
+    // (single tokens: as many as the device may find best for all workgroups there are)
+    const int64_t parts = single ? ceil_div(guess.steps, std::max<int64_t>(p.family_least, pairs * guess.steps / two)) + 1
+                                 : best_cut((double)pairs, guess.steps, step_us(dtype, d, single), single, tokens, heads, d).parts;
+    p.family_splits = (int)parts;
+    // (not more than there is room for at a time, where these are all; each head has one, and leaves as many)
+    const bool with_few = p.own.few && p.own.few_splits > 0;
+    p.shares = (int)std::max<int64_t>(single ? two : with_few ? std::max(two, pairs * parts * 5 / 4) : pairs * parts, 2 * (int64_t)view.kv_heads);
     p.family_rows = tokens * heads * p.family_splits;
     p.whole_rows = p.own.few ? tokens * heads : 0;
   }
   p.few_rows = p.own.few ? 2ll * p.own.few_splits * kFewRows : 0;
   p.own_rows = p.own.tiles && (families || p.own.tile_splits > 1) ? tokens * heads * p.own.tile_splits : 0;
-  p.floats = (p.few_rows + p.own_rows + p.family_rows + p.whole_rows) * (d + 2) + (families ? 4 : 0);
+  p.floats = (p.few_rows + p.own_rows + p.family_rows + p.whole_rows) * (d + 2) + (families ? 4 + 2 * (int64_t)view.batch : 0);
   return p;
 }
 
-// Whether reading a family's keys once is worth a second launch, which joins what they give with what the sequences' own keys do: from about so many bytes less on (of which the caches would take
-// most).  us, families / none, one token each behind common keys and 50 of its own: bf16, 32 and 8 heads of 128, 4 sequences behind 4000 (49 MB less) 17.6 / 17.2, 8 behind 2000 (57) 18.9 / 19.0, 32
-// behind 1000 (127) 21.8 / 21.3, 16 behind 4000 (246) 21.9 / 30.6, 64 behind 8000 (2064) 40 / 147; fp16, 12 heads of 64, 4 behind 4000 (37) 15.8 / 15.8, 16 behind 1000 (46) 13.7 / 8.9, 32 behind
-// 2000 (190) 15.9 / 25.5; fp32, 12 heads of 64, 8 behind 2000 (86) 21.6 / 21.1, 64 behind 512 (198) 20.3 / 23.4, 8 behind 8000 (344) 35 / 45.  Where nothing is known they are taken as they come.
-constexpr int64_t kSharedBytes = 80 << 20;
-bool sharing_pays(const PagedView& view, const ttmi_paged_sight& sight, int dtype) {
+// Whether reading a family's keys once is worth it: a second launch, which joins what they give with what the sequences' own keys do, and blocks of 128 rows that may be mostly empty, for reads
+// that the caches would take most of.  us, families / none, one token each and 50 keys of its own:
+//   bf16, 32 and 8 heads of 128: 4 sequences behind 4000 keys 17.6 / 17.2, 8 behind 2000 18.9 / 19.0, 64 behind 512 20.9 / 15.2, 64 behind 1000 25.9 / 28.4, 64 behind 8000 40 / 147;
+//                                8 families of 2 behind 4000 37 / 33, 4 of 8 29.7 / 51.0, 16 of 4 behind 1000 32.2 / 29.9, 16 of 4 behind 4000 75 / 89, 8 of 8 behind 16000 153 / 322
+//   fp16, 12 heads of 64:        16 behind 1000 13.7 / 8.9, 16 behind 2000 14.2 / 18.0, 8 behind 4000 15.5 / 18.6; 32 and 8 heads: 4 of 16 behind 1000 20.3 / 14.1, 8 of 8 behind 4000 38.8 / 45.7
+//   fp32, 32 and 8 heads of 128: 32 behind 1000 46 / 38, 32 behind 4000 58 / 101, 8 of 8 behind 16000 819 / 687; of 64: 32 behind 4000 30.2 / 57.3, 8 of 8 behind 16000 316 / 368
+// Where nothing is known they are taken as they come.
+bool sharing_pays(const PagedView& view, int64_t heads, const ttmi_paged_sight& sight, int dtype) {
   if (sight.families == nullptr) return false;
   if (sight.family_count == 0 || sight.max_shared == 0) return true;
-  const int64_t held = view.table_pitch << view.page_shift, shared = std::min(sight.max_shared, held);
-  return std::max<int64_t>(0, view.batch - sight.family_count) * shared >= kSharedBytes / (2 * view.kv_heads * view.head_dim * (int64_t)dtype_size(dtype));
+  const FamilyGuess guess = guess_families(view, heads, sight);
+  const bool f32 = dtype == TTMI_F32, wide = view.head_dim == 128, single = single_tokens(view, heads);
+  const double step = step_us(dtype, view.head_dim, single), rows = (double)view.tokens * (double)(heads / view.kv_heads);
+  const auto tiles = [&](double blocks) { return best_cut(blocks * view.kv_heads, guess.steps, step, single, view.tokens, heads, view.head_dim).us; };
+  const double shared = (f32 ? (wide ? 30 : 12) : (wide ? 12 : 10)) + (f32 ? 0.15 : 0.1) * view.batch + tiles(guess.blocks);
+  const double reads = (double)view.batch * guess.steps * 64 * (2 * view.kv_heads * view.head_dim * (double)dtype_size(dtype)) / 13e6;
+  // (sequences with many rows have blocks of their own, half a one empty each)
+  return shared < 7 + (single ? reads : std::max(reads, tiles(rows / 128 + view.batch / 2.0)));
 }
 
 int check_sight(const ttmi_paged_sight* sight) {
@@ -204,7 +249,7 @@ int ttmi_paged_attention_sight_workspace(const ttmi_paged_cache* cache, const tt
   TTMI_REQUIRE(bytes != nullptr, "bytes is null");
   if (int rc = paged_view(cache, batch, heads, &view)) return rc;
   ttmi_paged_sight used = *sight;
-  if (!sharing_pays(view, used, dtype)) used.families = nullptr;
+  if (!sharing_pays(view, heads, used, dtype)) used.families = nullptr;
   if (used.families == nullptr && (used.sinks == 0 || used.window == 0) && !getenv("FORCE"))
     return ttmi_paged_attention_workspace(cache, batch, heads, max_tokens, max_length, used.window, dtype, bytes);
   TTMI_REQUIRE(max_tokens >= 0 && max_length >= 0, "max_tokens and max_length must not be negative");
@@ -221,7 +266,7 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
   if (int rc = attention_args(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, sight->window, dtype, &a)) return rc;
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   ttmi_paged_sight used = *sight;
-  if (!sharing_pays(a.view, used, dtype)) used.families = nullptr;
+  if (!sharing_pays(a.view, heads, used, dtype)) used.families = nullptr;
   if (used.families == nullptr && (used.sinks == 0 || used.window == 0) && !getenv("FORCE"))
     return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, used.window, workspace, workspace_bytes,
                                 dtype, stream);

@@ -92,7 +92,8 @@ struct Walk {  // 64 sequences, a lane each
   LaneSequences lanes;    // SIGHT
   int base, rounds;       // number of the first; rounds of this lane's, for one head
   int64_t before, upto;   // units of all sequences before these; of these up to this lane's, it included
-  int64_t groups;         // of batches of more than 64 sequences: units of this lane's 64th of them and of those before it
+  int64_t groups;         // of batches of more than 64 sequences: units of this lane's 64th of them and of those before it (SIGHT: or `ahead`: not counted, the walk only goes on)
+  bool ahead;
 };
 constexpr int kSpanTile = 32;  // a tile or two
 template <bool SIGHT>
@@ -171,7 +172,7 @@ struct Place {
 };
 template <bool SIGHT>
 __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t unit) {
-  if (a.view.batch > kWave && (unit < w.before || unit >= w.before + lane_of(w.upto, kWave - 1)))
+  if (a.view.batch > kWave && !(SIGHT && w.ahead) && (unit < w.before || unit >= w.before + lane_of(w.upto, kWave - 1)))
     walk_to_group<SIGHT>(a, w, __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(w.groups > unit)) - 1));
   while (w.before + lane_of(w.upto, kWave - 1) <= unit) walk_on<SIGHT>(a, w);
   const int64_t at = unit - w.before;
@@ -493,12 +494,8 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedAr
 struct Sharers {
   int64_t first, last;
 };
-template <bool SIGHT>
-__device__ __forceinline__ Sharers sharers_of(const PagedArgs& a, Walk& walk, int64_t units, int64_t workgroups, int b, int kv_head) {
-  if (a.view.batch > kWave) walk_to_group<SIGHT>(a, walk, b / group_size(a));
-  while (walk.base + kWave <= b) walk_on<SIGHT>(a, walk);
-  const int lane = b - walk.base, rounds = __builtin_amdgcn_readlane(walk.rounds, lane);
-  const int64_t unit = walk.before + lane_of(walk.upto, lane) - (int64_t)rounds * (a.view.kv_heads - kv_head);
+// `unit`: the first of the pair.
+__device__ __forceinline__ Sharers sharers_of(int64_t unit, int rounds, int64_t units, int64_t workgroups) {
   return {quotient((unit + kStart + 1) * workgroups - 1, units), quotient((unit + rounds) * workgroups - 1, units)};
 }
 
@@ -516,7 +513,10 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a, b
   if (rows > a.few || (int)blockIdx.y >= rows) return;
   Walk walk{};
   const int64_t units = count_units<SIGHT>(a, walk), workgroups = sharers(a.splits, units);
-  const Sharers shared = sharers_of<SIGHT>(a, walk, units, workgroups, b, kv_head);
+  if (view.batch > kWave) walk_to_group<SIGHT>(a, walk, b / group_size(a));
+  while (walk.base + kWave <= b) walk_on<SIGHT>(a, walk);
+  const int lane = b - walk.base, rounds = __builtin_amdgcn_readlane(walk.rounds, lane);
+  const Sharers shared = sharers_of(walk.before + lane_of(walk.upto, lane) - (int64_t)rounds * (view.kv_heads - kv_head), rounds, units, workgroups);
   const int64_t first = shared.first, last = shared.last;
   if (first == last) return;
   const int parts = (int)(last - first) + 1;

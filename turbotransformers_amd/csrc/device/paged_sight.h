@@ -33,7 +33,7 @@ __device__ __forceinline__ FamilyWork family_work(const PagedArgs& a, const Lane
   return {(int)(((int64_t)lanes.family_tokens * a.group + kTileRows - 1) / kTileRows), lanes.family_keys / 64};
 }
 __device__ __forceinline__ int family_parts(int steps, int most) { return (steps + most - 1) / most; }
-// For kernels that follow, behind the partial results.
+// For the kernel that follows, behind the partial results: the units of the few-rows kernel, how they are shared out, and how many come before each sequence.
 struct ShareNote {
   int steps, few_groups;
   int64_t units;
@@ -42,93 +42,124 @@ template <int D>
 __device__ __forceinline__ ShareNote* share_note(const PagedArgs& a) {
   return reinterpret_cast<ShareNote*>(a.partial + a.rows * (D + 2));
 }
-// walk, *units: those of the few-rows kernel (and the first 64 sequences, where there are no more).
-template <typename T, int D>
-__device__ __forceinline__ Shares shares_of(const PagedArgs& a, Walk& walk, int64_t* units) {
-  const int kv_heads = a.view.kv_heads;
-  const bool few = a.run_few && a.few_splits > 0, single = a.view.batch <= kWave;
-  *units = 0;
-  if (few) *units = count_units<true>(a, walk);
-  else if (single) walk.lanes = lane_sequences(a, 0);
-  // (sums of 64 numbers that are capped for the balance alone)
-  constexpr int kCap = 1 << 24;
-  int64_t steps = 0;
-  int longest = 0;
-  for (int base = 0; base < a.view.batch; base += kWave) {
-    const FamilyWork w = family_work(a, single ? walk.lanes : lane_sequences(a, base));
-    steps += sum_of_lanes((int)min((int64_t)w.blocks * w.steps, (int64_t)kCap));
-    for (uint64_t more = __ballot(w.steps > longest); more != 0; more = __ballot(w.steps > longest))
-      longest = __builtin_amdgcn_readlane(w.steps, __ffsll((unsigned long long)more) - 1);
-  }
-  Shares s;
-  // (in floats: every workgroup finds the same, and those that follow are told)
-  const float family_cost = (float)(steps * kv_heads) * kStepCost<T, D>, cost = family_cost + (float)*units * kRoundCost<T, D>;
-  const float groups = fmaxf((float)kv_heads, cost > 0.f ? a.shares * (family_cost / cost) : 0.f);
-  s.steps = max(max(a.family_least, (longest + a.family_splits - 1) / a.family_splits), (int)fminf(__builtin_ceilf((float)(steps * kv_heads) / groups), 0x1p30f));
-  s.items = 0;
-  for (int base = 0; base < a.view.batch; base += kWave) {
-    const FamilyWork w = family_work(a, single ? walk.lanes : lane_sequences(a, base));
-    s.items += sum_of_lanes(w.blocks * family_parts(w.steps, s.steps));
-  }
-  // (at least an eighth is left for the others)
-  s.family_groups = min(s.items, max(1, (few ? a.shares - a.shares / 8 : a.shares) / kv_heads));
-  s.few_groups = max(1, min(a.few_splits, a.shares - s.family_groups * kv_heads));
-  return s;
+template <int D>
+__device__ __forceinline__ int64_t* units_before(const PagedArgs& a) {
+  return reinterpret_cast<int64_t*>(share_note<D>(a) + 1);
 }
-
-// The item-th part of a block of a family's rows -> whether there is one.
+// A part of a block of a family's rows, or of a sequence's with many.
 struct Job {
   int b, block, part, chunk;
   Sequence seq;
   Family family;
 };
-__device__ __forceinline__ bool find_family_job(const PagedArgs& a, const Shares& s, int item, bool there, LaneSequences& lanes, Job* job) {
-  int passed = 0;
-  for (int base = 0; base < a.view.batch; base += kWave) {
-    if (!there) lanes = lane_sequences(a, base);
-    const FamilyWork w = family_work(a, lanes);
-    const int mine = w.blocks * family_parts(w.steps, s.steps), upto = passed + sum_up_to_here(mine), all = __builtin_amdgcn_readlane(upto, kWave - 1);
-    if (item >= all) {
-      passed = all;
-      continue;
-    }
-    const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(item < upto)) - 1);
-    const int at = item - __builtin_amdgcn_readlane(upto - mine, found), blocks = __builtin_amdgcn_readlane(w.blocks, found);
-    const int steps = __builtin_amdgcn_readlane(w.steps, found), parts = family_parts(steps, s.steps);
-    // (workgroups beside each other have the same keys of a head, on one XCD where there are eight heads)
-    job->b = base + found, job->part = at / blocks, job->block = at - job->part * blocks, job->chunk = (steps + parts - 1) / parts * 64;
-    job->seq = lanes.family_sequence(found), job->family = lanes.family(found);
-    return true;
-  }
-  return false;
+// The item-th of all, in parts of `steps` at most, which is among the 64 sequences from `base` on, `passed` items being those of others before -> its lanes.
+__device__ __forceinline__ LaneSequences family_job(const PagedArgs& a, int steps, int item, int base, int passed, Job* job) {
+  const LaneSequences lanes = lane_sequences(a, base);
+  const FamilyWork w = family_work(a, lanes);
+  const int mine = w.blocks * family_parts(w.steps, steps), upto = passed + sum_up_to_here(mine);
+  const int lane = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(item < upto)) - 1);
+  const int at = item - __builtin_amdgcn_readlane(upto - mine, lane), blocks = __builtin_amdgcn_readlane(w.blocks, lane);
+  const int all = __builtin_amdgcn_readlane(w.steps, lane), parts = family_parts(all, steps);
+  // (workgroups beside each other have the same keys of a head, on one XCD where there are eight heads)
+  job->b = base + lane, job->part = at / blocks, job->block = at - job->part * blocks, job->chunk = (all + parts - 1) / parts * 64;
+  job->seq = lanes.family_sequence(lane), job->family = lanes.family(lane);
+  return lanes;
 }
-// The share of a workgroup in the families' keys (`lanes`: the first 64 sequences, where there are no more), taken in turns where there are more than workgroups; or a part of a block of a sequence
-// with many rows, over its own keys.
-template <typename T, int D, bool SMALL, bool FAMILIES>
-__device__ __forceinline__ void sight_tiles(const PagedArgs& a, bool families, const Shares& s, int group, LaneSequences lanes, TilesShared<T, D>& shared) {
-  const int kv_heads = a.view.kv_heads, kv_head = group % kv_heads;
-  if constexpr (!FAMILIES) {
-    int b, block;
-    if (!find_block(a, group / kv_heads / a.splits, &b, &block)) return;
-    tiles<T, D, SMALL, true, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, group / kv_heads % a.splits, shared);
-    return;
+// Up to kSeen times 64 sequences are asked for at once, and what is needed of them stays in registers until the workgroup knows its share; more are read again for each number.
+constexpr int kSeen = 4;
+// What a workgroup of a.shares finds out.
+template <typename T, int D>
+struct Scan {
+  FamilyWork work[kSeen];
+  int rounds[kSeen];
+  Shares s;
+  int64_t units;
+};
+__device__ __forceinline__ bool seen_at_once(const PagedArgs& a) { return a.view.batch <= kSeen * kWave; }
+__device__ __forceinline__ bool few_shared(const PagedArgs& a) { return a.run_few && a.few_splits > 0; }
+// f(number of the first, work of this lane's family) for 64 sequences after the other
+template <typename T, int D, typename F>
+__device__ __forceinline__ void each_family(const PagedArgs& a, const Scan<T, D>& scan, F f) {
+  if (seen_at_once(a)) {
+#pragma unroll
+    for (int g = 0; g < kSeen; ++g)
+      if (g * kWave < a.view.batch) f(g * kWave, scan.work[g]);
+  } else {
+    for (int base = 0; base < a.view.batch; base += kWave) f(base, family_work(a, lane_sequences(a, base)));
   }
-  const int step = families ? s.family_groups : 1, stop = families ? s.items : 1;
-  bool there = a.view.batch <= kWave;
-  for (int item = families ? group / kv_heads : 0; item < stop; item += step) {
-    Job job;
-    if (families) {
-      if (!find_family_job(a, s, item, there, lanes, &job)) return;
-    } else {
-      if (!find_block(a, group / kv_heads / a.splits, &job.b, &job.block)) return;
-      lanes = lane_sequences(a, job.b & ~(kWave - 1));
-      job.part = group / kv_heads % a.splits, job.chunk = 0, job.seq = lanes.sequence(job.b % kWave), job.family = Family{};
+}
+template <typename T, int D>
+__device__ __forceinline__ Scan<T, D> scan_of(const PagedArgs& a, Walk& walk) {
+  const int kv_heads = a.view.kv_heads;
+  Scan<T, D> scan;
+  scan.units = 0;
+  if (seen_at_once(a)) {
+    LaneNumbers numbers[kSeen];
+#pragma unroll
+    for (int g = 0; g < kSeen; ++g)
+      if (g * kWave < a.view.batch) numbers[g] = lane_numbers(a, g * kWave);
+#pragma unroll
+    for (int g = 0; g < kSeen; ++g) {
+      scan.rounds[g] = 0, scan.work[g] = {0, 0};
+      if (g * kWave < a.view.batch) {
+        const LaneSequences lanes = lane_sequences(a, g * kWave, numbers[g]);
+        scan.work[g] = family_work(a, lanes);
+        if (few_shared(a)) {
+          scan.rounds[g] = rounds_of<true>(a, own_sequence(lanes));
+          scan.units += (int64_t)sum_of_lanes(scan.rounds[g]) * kv_heads;
+        }
+      }
     }
-    there = false;  // (they are not kept where the registers are needed)
-    tiles<T, D, SMALL, true, FAMILIES>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, kv_head, job.part, shared);
-    if (item + step >= stop) break;  // (without waiting for what was stored)
-    __syncthreads();
+  } else if (few_shared(a)) scan.units = count_units<true>(a, walk);
+  // (sums of 64 numbers that are capped for the balance alone)
+  constexpr int kCap = 1 << 24;
+  int64_t steps = 0;
+  int longest = 0;
+  each_family(a, scan, [&](int, const FamilyWork& w) {
+    steps += sum_of_lanes((int)min((int64_t)w.blocks * w.steps, (int64_t)kCap));
+    for (uint64_t more = __ballot(w.steps > longest); more != 0; more = __ballot(w.steps > longest))
+      longest = __builtin_amdgcn_readlane(w.steps, __ffsll((unsigned long long)more) - 1);
+  });
+  // (in floats: every workgroup finds the same, and the kernel that follows is told)
+  Shares& s = scan.s;
+  const float family_cost = (float)(steps * kv_heads) * kStepCost<T, D>, cost = family_cost + (float)scan.units * kRoundCost<T, D>;
+  const float groups = fmaxf((float)kv_heads, cost > 0.f ? a.shares * (family_cost / cost) : 0.f);
+  s.steps = max(max(a.family_least, (longest + a.family_splits - 1) / a.family_splits), (int)fminf(__builtin_ceilf((float)(steps * kv_heads) / groups), 0x1p30f));
+  s.items = 0;
+  each_family(a, scan, [&](int, const FamilyWork& w) { s.items += sum_of_lanes(w.blocks * family_parts(w.steps, s.steps)); });
+  // (at least an eighth is left for the others)
+  s.family_groups = min(s.items, max(1, (few_shared(a) ? a.shares - a.shares / 8 : a.shares) / kv_heads));
+  s.few_groups = max(1, min(a.few_splits, a.shares - s.family_groups * kv_heads));
+  return scan;
+}
+// One workgroup does, before it turns to its share.
+template <typename T, int D>
+__device__ __forceinline__ void tell(const PagedArgs& a, const Scan<T, D>& scan) {
+  const int lane = (int)threadIdx.x;
+  if (lane >= kWave) return;
+  if (lane == 0) *share_note<D>(a) = {scan.s.steps, scan.s.few_groups, scan.units};
+  int64_t before = 0;
+  for (int base = 0; few_shared(a) && base < a.view.batch; base += kWave) {
+    const int mine = rounds_of<true>(a, own_sequence(lane_sequences(a, base))), upto = sum_up_to_here(mine);
+    if (base + lane < a.view.batch) units_before<D>(a)[base + lane] = before + (int64_t)(upto - mine) * a.view.kv_heads;
+    before += (int64_t)__builtin_amdgcn_readlane(upto, kWave - 1) * a.view.kv_heads;
   }
+}
+// The walk of the few-rows kernel where its workgroup begins.
+template <typename T, int D>
+__device__ __forceinline__ void begin_walk(const PagedArgs& a, const Scan<T, D>& scan, int workgroup, Walk& walk) {
+  if (!seen_at_once(a)) return;
+  const int64_t unit = quotient(scan.units * workgroup, sharers(scan.s.few_groups, scan.units));
+  int64_t from = 0, before = 0;
+  int base = 0, mine = scan.rounds[0];
+#pragma unroll
+  for (int g = 0; g < kSeen; ++g)
+    if (g * kWave < a.view.batch) {
+      if (before <= unit) base = g * kWave, from = before, mine = scan.rounds[g];
+      before += (int64_t)sum_of_lanes(scan.rounds[g]) * a.view.kv_heads;
+    }
+  walk.ahead = true, walk.base = base, walk.before = from, walk.rounds = mine, walk.upto = (int64_t)sum_up_to_here(mine) * a.view.kv_heads;
+  walk.lanes = lane_sequences(a, base);
 }
 
 // One launch: a.shares workgroups (FAMILIES) for families and for sequences with few rows, a.tile_groups for those with many, the rest, if any, for few rows (FEW).  So a
@@ -141,25 +172,70 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
     TilesShared<T, D> tiles;
     FewRowsShared<T, D, 4> few;
   } shared;
-  int group = blockIdx.x, few_groups = a.few_splits;
-  Walk walk{};
-  Shares s{};
-  int64_t units = -1;
-  const int shares = FAMILIES ? a.shares : 0;
-  bool families = false, own = !FEW;
-  if (FAMILIES && group < shares) {
-    s = shares_of<T, D>(a, walk, &units);
-    if (group == 0 && threadIdx.x == 0) *share_note<D>(a) = {s.steps, s.few_groups, units};
-    families = group < s.family_groups * a.view.kv_heads;
-    if (!families) group -= s.family_groups * a.view.kv_heads, few_groups = s.few_groups;
-    if (!families && (!FEW || units == 0 || group >= few_groups)) return;
+  const int kv_heads = a.view.kv_heads;
+  int group = blockIdx.x;
+  if constexpr (!FAMILIES) {
+    if (!FEW || group < a.tile_groups) {
+      int b, block;
+      if (!find_block(a, group / kv_heads / a.splits, &b, &block)) return;
+      tiles<T, D, SMALL, true, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, group % kv_heads, group / kv_heads % a.splits, shared.tiles);
+    } else if constexpr (FEW) {
+      Walk walk{};
+      few_rows<T, D, 4, false, true>(a, group - a.tile_groups, a.few_splits, walk, -1, shared.few);
+    }
   } else {
-    group -= shares;
-    own = !FEW || group < a.tile_groups;
-    if (!own) group -= a.tile_groups;
+    Job job;
+    LaneSequences lanes;
+    int item = 0, step = 1, stop = 1, steps = 1;  // parts of families are taken in turns where there are more than workgroups
+    int few_groups = -1;
+    Walk walk{};
+    int64_t units = -1;
+    int base = 0, passed = 0;
+    bool own = false;
+    if (group < a.shares) {
+      const Scan<T, D> scan = scan_of<T, D>(a, walk);
+      if (group == 0) tell(a, scan);
+      const int family_groups = scan.s.family_groups * kv_heads;
+      if (group < family_groups) {
+        item = group / kv_heads, step = scan.s.family_groups, stop = scan.s.items, steps = scan.s.steps;
+        int upto = 0;
+        each_family(a, scan, [&](int from, const FamilyWork& w) {
+          if (upto <= item) base = from, passed = upto;
+          upto += sum_of_lanes(w.blocks * family_parts(w.steps, steps));
+        });
+      } else {
+        group -= family_groups, few_groups = scan.s.few_groups, units = scan.units;
+        if (!FEW || units == 0 || group >= few_groups) return;
+        begin_walk(a, scan, group, walk);
+      }
+    } else {
+      group -= a.shares;
+      own = group < a.tile_groups;
+      if (!own) group -= a.tile_groups, few_groups = 0;
+    }
+    if (few_groups >= 0) {
+      if constexpr (FEW) few_rows<T, D, 4, false, true>(a, group, few_groups, walk, units, shared.few);
+      return;
+    }
+    for (;;) {
+      if (own) {
+        if (!find_block(a, group / kv_heads / a.splits, &job.b, &job.block)) return;
+        lanes = lane_sequences(a, job.b & ~(kWave - 1));
+        job.part = group / kv_heads % a.splits, job.chunk = 0, job.seq = lanes.sequence(job.b % kWave), job.family = Family{};
+      } else lanes = family_job(a, steps, item, base, passed, &job);
+      tiles<T, D, SMALL, true, true>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, group % kv_heads, job.part, shared.tiles);
+      item += step;
+      if (item >= stop) break;
+      __syncthreads();
+      // on to the 64 sequences that have it
+      for (;;) {
+        const FamilyWork w = family_work(a, lane_sequences(a, base));
+        const int upto = passed + sum_of_lanes(w.blocks * family_parts(w.steps, steps));
+        if (item < upto) break;
+        passed = upto, base += kWave;
+      }
+    }
   }
-  if (families || own) sight_tiles<T, D, SMALL, FAMILIES>(a, families, s, group, walk.lanes, shared.tiles);
-  else if constexpr (FEW) few_rows<T, D, 4, false, true>(a, group, few_groups, walk, units, shared.few);
 }
 
 // A wavefront a row and head.
@@ -171,17 +247,21 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
   ShareNote note{};
   if (a.families != nullptr) note = *share_note<D>(a);
   // the row's sequence: the first that ends behind it
-  Walk walk{};
+  const int lane = (int)(threadIdx.x % kWave);
+  LaneSequences lanes;
   int b = -1;
+  int64_t before = 0;
   for (int base = 0; base < view.batch; base += kWave) {
-    walk.lanes = lane_sequences(a, base);
-    const int before = __popcll(__ballot(base + (int)(threadIdx.x % kWave) < view.batch && walk.lanes.ends <= row));
-    if (before == kWave) continue;
-    b = base + before;
+    if (a.families != nullptr && a.run_few && a.few_splits > 0) before = units_before<D>(a)[min(base + lane, view.batch - 1)];
+    lanes = lane_sequences(a, base);
+    const int ended = __popcll(__ballot(base + lane < view.batch && lanes.ends <= row));
+    if (ended == kWave) continue;
+    b = base + ended;
     break;
   }
   if (b < 0 || b >= view.batch) return;
-  const Sequence seq = walk.lanes.sequence(b - walk.lanes.base);
+  const Sequence seq = lanes.sequence(b - lanes.base);
+  before = lane_of(before, b - lanes.base);
   if (row < seq.start || row >= seq.start + seq.tokens) return;
   const int kv_head = head / a.group, r = (row - seq.start) * a.group + head % a.group, rows = seq.tokens * a.group;
   const int64_t at = (int64_t)row * a.heads + head;
@@ -202,11 +282,8 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
   } else if (a.families == nullptr) {
     return;
   } else if (a.few_splits > 0) {
-    int64_t units = note.units;
-    if (view.batch <= kWave) walk.base = 0, walk.before = 0, walk.rounds = rounds_of<true>(a, own_sequence(walk.lanes)),
-                             walk.upto = (int64_t)sum_up_to_here(walk.rounds) * view.kv_heads;
-    else units = count_units<true>(a, walk);
-    const Sharers shared = sharers_of<true>(a, walk, units, sharers(view.page_shift >= 4 ? note.few_groups : a.few_splits, units), b, kv_head);
+    const int rounds = rounds_of<true>(a, seq);
+    const Sharers shared = sharers_of(before + (int64_t)rounds * kv_head, rounds, note.units, sharers(view.page_shift >= 4 ? note.few_groups : a.few_splits, note.units));
     if (shared.last > shared.first) {
       parts = (int)(shared.last - shared.first) + 1;
       place = (2 * shared.first + 1) * kFewRows + r, second = 2 * (shared.first + 1) * kFewRows + r, step = 2 * kFewRows;
@@ -228,7 +305,7 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
   }
   // up to 64 parts: each lane has what one weighs, and the sums, four columns a lane and a few parts at a time, are asked for without waiting for that
   constexpr int kThreads = D / 4, kBeside = kWave / kThreads, kAsked = 8;
-  const int lane = (int)(threadIdx.x % kWave), d0 = lane % kThreads * 4, share = lane / kThreads;
+  const int d0 = lane % kThreads * 4, share = lane / kThreads;
   const int64_t mine = place_of(min(lane, all - 1));
   const floatx2 met = *reinterpret_cast<const floatx2*>(ml + 2 * mine);
   floatx4 sum = {0.f, 0.f, 0.f, 0.f};
