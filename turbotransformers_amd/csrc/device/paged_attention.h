@@ -32,7 +32,8 @@ struct PagedArgs {
   const int32_t* families;  // null: none
   // shares: workgroups that the families' keys, in at most family_splits parts of at least family_least steps of 64, and the sequences with few rows take among them;
   // few_splits, few_every: splits and every of the few-rows kernel, where it runs (run_few); own_blocks: blocks of 128 rows of sequences' own keys, tile_groups workgroups.
-  int shares, family_splits, family_least, run_few, few_splits, few_every, own_blocks, tile_groups;
+  // family_few: rows of a family up to which it is the few-rows kernel's, in blocks of kFewRows, where that is among those workgroups.
+  int shares, family_splits, family_least, family_few, run_few, few_splits, few_every, own_blocks, tile_groups;
   // With families `partial` holds the rows of all results that are joined: those of the few-rows kernel (2 splits kFewRows), and from these on, for each row of q and head:
   int64_t own_at, family_at, whole_at, rows;  // of a sequence's own keys in parts, of its family's in parts, of its own where one workgroup had them all; the end
 };
@@ -225,6 +226,24 @@ __device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int 
   return s;
 }
 __device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int base) { return lane_sequences(a, base, lane_numbers(a, base)); }
+// Blocks of kFewRows rows of a lane's family, where the few-rows kernel takes it, and its rows of 128, where that of many rows does.
+struct FamilyBlocks {
+  int few, many;
+};
+__device__ __forceinline__ FamilyBlocks family_blocks(const PagedArgs& a, const LaneSequences& lanes) {
+  const int64_t rows = (int64_t)lanes.family_tokens * a.group;
+  const bool few = rows <= a.family_few;
+  return {few ? (int)(rows + kFewRows - 1) / kFewRows : 0, few ? 0 : (int)((rows + 127) / 128)};
+}
+// The keys of a part that some row of a family's block sees: from lo to hi, shortened (both stay multiples of TILE, or the end of what is seen).  With a window these are the first keys that stay
+// visible, the windows' or, from the one to the other, both.
+template <int TILE>
+__device__ __forceinline__ void seen_of_part(const Sight& s, int* lo, int* hi) {
+  if (*lo >= s.low) *lo = max(*lo, min(*hi, s.first & ~(TILE - 1)));
+  *hi = min(*hi, s.end);
+  if (*hi <= s.first) *hi = min(*hi, s.low);
+  *hi = max(*lo, *hi);
+}
 // The sequence of a family that a row of q belongs to, each lane's own, and what of the family's keys the row sees; *member: whether that sequence says that it is of the family.  Where each
 // sequence has one new token and they lie among the 64, no trip to memory.
 __device__ __forceinline__ Reach family_reach(const PagedArgs& a, const LaneSequences& s, const Family& f, int start, int row, bool* member) {

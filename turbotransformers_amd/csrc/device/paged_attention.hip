@@ -99,6 +99,11 @@ double step_us(int dtype, int64_t head_dim, bool single) {
   return head_dim == 128 ? (single ? 4 : 2.3) : (single ? 2.2 : 1.35);
 }
 bool single_tokens(const PagedView& view, int64_t heads) { return view.tokens * (heads / view.kv_heads) <= kFewRows * (int64_t)view.batch; }
+// Rows of a family up to which the few-rows kernel takes its keys, 16 rows at a time, from memory or again from L2: the other reads them once for up to 128, but one wavefront of it computes 32 of
+// them alone, which takes fp32 sixteen times as long.  us, one token each, 12 heads of 64 / 32 and 8 of 128, that kernel / this one: fp16, 16 families of 4 behind 8000 keys 105 / 84, 8 of 8 63 / 47; bf16, 4 rows
+// a sequence, 16 of 4 161 / 115, 8 of 8 (32 rows) 72 / 92; fp32 16 of 4 412 / 156, 8 of 8 253 / 90, 64 (64 rows) behind 1000 39.5 / 29.0; 4 rows a sequence, 16 of 4 828 / 213, 16 (64 rows) behind
+// 8000 81 / 58.
+int family_few_rows(int dtype) { return dtype == TTMI_F32 ? 64 : 16; }
 struct FamilyGuess {
   double blocks;  // of rows
   int64_t steps;  // of the longest
@@ -114,7 +119,7 @@ FamilyGuess guess_families(const PagedView& view, int64_t heads, const ttmi_page
 // with few rows take a share of them (16 questions about 20000 tokens, 32 and 8 heads of 128: 1 / 2 / 3 / 5 / 8 parts 650 / 570 / 498 / 475 / 487 us).
 struct SightPlan {
   PagedPlan own;
-  int shares, family_splits, family_least, own_blocks;
+  int shares, family_splits, family_least, family_few, own_blocks;
   int64_t few_rows, own_rows, family_rows, whole_rows, floats;  // of the workspace
 };
 SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, const ttmi_paged_sight& sight, int dtype) {
@@ -123,13 +128,14 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
   p.own = plan(view, heads, max_tokens, max_length, window, dtype);
   const int64_t group = heads / view.kv_heads, tokens = view.tokens, d = view.head_dim;
   p.own_blocks = p.own.tiles ? (int)(tokens * group / 128 + std::min<int64_t>(view.batch, tokens)) : 0;
-  p.shares = p.family_splits = p.family_least = 0, p.family_rows = p.whole_rows = 0;
+  p.shares = p.family_splits = p.family_least = p.family_few = 0, p.family_rows = p.whole_rows = 0;
   const bool families = sight.families != nullptr;
   if (families) {
     const FamilyGuess guess = guess_families(view, heads, sight);
     const bool single = single_tokens(view, heads);
     const int64_t two = 2 * compute_units(), pairs = (int64_t)guess.blocks * view.kv_heads;
     p.family_least = dtype == TTMI_F32 ? 1 : 2;
+    if (p.own.few) p.own.few_splits = 2 * compute_units(), p.family_few = family_few_rows(dtype);
     // (single tokens: as many as the device may find best for all workgroups there are)
     const int64_t parts = single ? ceil_div(guess.steps, std::max<int64_t>(p.family_least, pairs * guess.steps / two)) + 1
                                  : best_cut((double)pairs, guess.steps, step_us(dtype, d, single), single, tokens, heads, d).parts;
@@ -160,8 +166,10 @@ bool sharing_pays(const PagedView& view, int64_t heads, const ttmi_paged_sight& 
   const bool f32 = dtype == TTMI_F32, wide = view.head_dim == 128, single = single_tokens(view, heads);
   const double step = step_us(dtype, view.head_dim, single), rows = (double)view.tokens * (double)(heads / view.kv_heads);
   const auto tiles = [&](double blocks) { return best_cut(blocks * view.kv_heads, guess.steps, step, single, view.tokens, heads, view.head_dim).us; };
-  const double shared = (f32 ? (wide ? 30 : 12) : (wide ? 12 : 10)) + (f32 ? 0.15 : 0.1) * view.batch + tiles(guess.blocks);
-  const double reads = (double)view.batch * guess.steps * 64 * (2 * view.kv_heads * view.head_dim * (double)dtype_size(dtype)) / 13e6;
+  const double bytes = guess.steps * 64.0 * (2 * view.kv_heads * view.head_dim * (double)dtype_size(dtype)), reads = view.batch * bytes / (f32 ? 11e6 : 13e6);
+  const double count = (double)std::min<int64_t>(sight.family_count, std::max(1, view.batch / 2)), most = std::ceil(rows / count);
+  const double shared = single && most <= family_few_rows(dtype) ? (wide && !f32 ? 12 : 10) + (f32 ? 0.15 : 0.1) * view.batch + count * std::ceil(most / kFewRows) * bytes / 5.3e6
+                                                                 : (f32 ? (wide ? 30 : 12) : (wide ? 12 : 10)) + (f32 ? 0.15 : 0.1) * view.batch + tiles(guess.blocks);
   // (sequences with many rows have blocks of their own, half a one empty each)
   return shared < 7 + (single ? reads : std::max(reads, tiles(rows / 128 + view.batch / 2.0)));
 }
@@ -276,7 +284,7 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
   a.sinks = (int)std::min(used.sinks, kWidest), a.families = used.families;
   a.partial = static_cast<float*>(workspace);
   a.every = !p.own.few, a.chunk = p.own.tile_chunk, a.splits = p.own.tile_splits, a.ordered = 1;
-  a.shares = p.shares, a.family_splits = p.family_splits, a.family_least = p.family_least;
+  a.shares = p.shares, a.family_splits = p.family_splits, a.family_least = p.family_least, a.family_few = p.family_few;
   a.own_at = p.few_rows, a.family_at = a.own_at + p.own_rows, a.whole_at = a.family_at + p.family_rows, a.rows = a.whole_at + p.whole_rows;
   l.run_tiles = p.own.tiles || p.shares > 0;
   a.run_few = p.own.few, a.few = p.own.few_rows, a.few_splits = p.own.few_splits, a.few_every = !p.own.tiles;

@@ -91,6 +91,7 @@ __device__ __forceinline__ Sequence own_sequence(const LaneSequences& lanes) {
 struct Walk {  // 64 sequences, a lane each
   LaneSequences lanes;    // SIGHT
   int base, rounds;       // number of the first; rounds of this lane's, for one head
+  int family_rounds, family_blocks;  // SIGHT: the same of the family that it leads, for one head and block of rows, and those blocks: they come first
   int64_t before, upto;   // units of all sequences before these; of these up to this lane's, it included
   int64_t groups;         // of batches of more than 64 sequences: units of this lane's 64th of them and of those before it (SIGHT: or `ahead`: not counted, the walk only goes on)
   bool ahead;
@@ -121,13 +122,23 @@ __device__ __forceinline__ int64_t sum_up_to_lane(int64_t v) {
   }
   return v;
 }
+// Rounds of a lane's family, for one head and block of kFewRows rows (0: none here), and of all there are for one head.
+__device__ __forceinline__ int family_rounds_of(const LaneSequences& lanes, int blocks) { return blocks > 0 ? kStart + lanes.family_keys / kRound : 0; }
+__device__ __forceinline__ int all_rounds_of(const PagedArgs& a, const LaneSequences& lanes) {
+  const int blocks = a.families != nullptr ? family_blocks(a, lanes).few : 0;
+  return rounds_of<true>(a, own_sequence(lanes)) + blocks * family_rounds_of(lanes, blocks);
+}
+__device__ __forceinline__ void take_lanes(const PagedArgs& a, Walk& w) {
+  w.rounds = rounds_of<true>(a, own_sequence(w.lanes));
+  w.family_blocks = a.families != nullptr ? family_blocks(a, w.lanes).few : 0, w.family_rounds = family_rounds_of(w.lanes, w.family_blocks);
+  w.upto = (int64_t)sum_up_to_here(w.rounds + w.family_blocks * w.family_rounds) * a.view.kv_heads;
+}
 template <bool SIGHT>
 __device__ __forceinline__ void walk_to(const PagedArgs& a, Walk& w, int base, int64_t before) {
   w.base = base, w.before = before;
   if constexpr (SIGHT) {
     w.lanes = lane_sequences(a, base);
-    w.rounds = rounds_of<true>(a, own_sequence(w.lanes));
-    w.upto = (int64_t)sum_up_to_here(w.rounds) * a.view.kv_heads;
+    take_lanes(a, w);
   } else {
     const int lane = (int)(threadIdx.x % kWave);
     w.rounds = base + lane < a.view.batch ? rounds_of<false>(a, sequence(a, base + lane)) : 0;
@@ -154,7 +165,7 @@ __device__ __forceinline__ int64_t count_units(const PagedArgs& a, Walk& w) {
   if constexpr (SIGHT) {
     // 64 sequences at a time; what each group of `size` has is kept by its lane
     for (int base = 0; base < a.view.batch; base += kWave) {
-      const int upto = sum_up_to_here(rounds_of<true>(a, own_sequence(lane_sequences(a, base))));
+      const int upto = sum_up_to_here(all_rounds_of(a, lane_sequences(a, base)));
       const int from = min(max(first - base, 0), kWave), to = min(max(first + size - base, 0), kWave);
       const int low = __shfl(upto, max(from - 1, 0), kWave), high = __shfl(upto, max(to - 1, 0), kWave);
       mine += (to > 0 ? high : 0) - (from > 0 ? low : 0);
@@ -169,6 +180,7 @@ __device__ __forceinline__ int64_t count_units(const PagedArgs& a, Walk& w) {
 }
 struct Place {
   int b, kv_head, round, rounds;  // round: of this head's `rounds`
+  int block = -1;                 // SIGHT: of the rows of the family that b leads
 };
 template <bool SIGHT>
 __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t unit) {
@@ -179,8 +191,22 @@ __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t 
   const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(w.upto > at)) - 1);
   Place p;
   p.b = w.base + found, p.rounds = __builtin_amdgcn_readlane(w.rounds, found);
-  const int rest = (int)(at - (lane_of(w.upto, found) - (int64_t)p.rounds * a.view.kv_heads));
-  p.kv_head = rest / p.rounds, p.round = rest - p.kv_head * p.rounds;
+  if constexpr (SIGHT) {
+    const int blocks = __builtin_amdgcn_readlane(w.family_blocks, found), family_rounds = __builtin_amdgcn_readlane(w.family_rounds, found);
+    int rest = (int)(at - (lane_of(w.upto, found) - (int64_t)(p.rounds + blocks * family_rounds) * a.view.kv_heads));
+    const int of_family = blocks * family_rounds * a.view.kv_heads;
+    if (rest < of_family) {
+      p.rounds = family_rounds;
+      const int pair = rest / family_rounds;
+      p.round = rest - pair * family_rounds, p.block = pair / a.view.kv_heads, p.kv_head = pair - p.block * a.view.kv_heads;
+    } else {
+      rest -= of_family;
+      p.kv_head = rest / p.rounds, p.round = rest - p.kv_head * p.rounds;
+    }
+  } else {
+    const int rest = (int)(at - (lane_of(w.upto, found) - (int64_t)p.rounds * a.view.kv_heads));
+    p.kv_head = rest / p.rounds, p.round = rest - p.kv_head * p.rounds;
+  }
   return p;
 }
 // a / b of numbers that are not negative: a division of 64 bits takes longer than a trip to L2, and they are seldom needed.
@@ -197,6 +223,7 @@ template <typename T, int D, int NW>
 struct FewRowsShared {
   __align__(16) char tiles[FewRows<T, D, NW>::kLds];
   float met[NW][kFewRows][2];
+  int theirs[kFewRows];  // SIGHT: of a family's rows, whether they are
 };
 
 // The share of one of `splits` workgroups (0: of a pair); SIGHT: units and walk as count_units gives them, if units >= 0.  SMALL: pages of fewer than 16 slots
@@ -232,26 +259,53 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
     unit = ends;
     if (round1 <= round0) continue;
     Sequence seq;
+    Family family{};
     if constexpr (SIGHT) {
       if (splits == 0) walk.lanes = lane_sequences(a, b & ~(kWave - 1));
       seq = walk.lanes.sequence(b - walk.lanes.base);
+      if (place.block >= 0) family = walk.lanes.family(b - walk.lanes.base), seq = walk.lanes.family_sequence(b - walk.lanes.base);
     } else seq = sequence(a, b);
-    const int rows_all = seq.tokens * a.group;
-    if (rows_all <= 0 || (rows_all > a.few && !(SIGHT ? a.few_every : a.every))) return;  // (a workgroup of its own)
-    if (round0 == 0 && kv_head == 0 && tid == 0 && view.lengths[b] > seq.length) page_error(view);
+    const bool of_family = SIGHT && place.block >= 0;
+    const int rows_all = of_family ? min(seq.tokens * a.group, (place.block + 1) * kFewRows) : seq.tokens * a.group;
+    if (!of_family && (rows_all <= 0 || (rows_all > a.few && !(SIGHT ? a.few_every : a.every)))) return;  // (a workgroup of its own)
+    if (round0 == 0 && kv_head == 0 && tid == 0 && !of_family && view.lengths[b] > seq.length) page_error(view);
     typename std::conditional<SIGHT, GapCursor, PageCursor>::type cursor;
     cursor.table = view.table + (int64_t)b * view.table_pitch;
     cursor.first = 0, cursor.ahead = 0, cursor.at = 0;
 
-    for (int row0 = 0; row0 < rows_all; row0 += kFewRows) {
+    for (int row0 = of_family ? place.block * kFewRows : 0; row0 < rows_all; row0 += kFewRows) {
       const int rows = min(kFewRows, rows_all - row0);
       const int token0 = row0 / a.group, token1 = (row0 + rows - 1) / a.group;
       const int token = row < rows ? (row0 + row) / a.group : token0, head = kv_head * a.group + (row < rows ? row0 + row - token * a.group : 0);
-      const Reach mine = seq.reach_of<SIGHT>(a, token);
-      const Sight sight = sight_of(seq.reach_of<SIGHT>(a, token0), seq.reach_of<SIGHT>(a, token1));
+      Reach mine;
+      Sight sight;
       Span span;
       int lo, hi;  // SIGHT: places
-      if constexpr (SIGHT) {
+      if (of_family) {
+        bool member;
+        mine = family_reach(a, walk.lanes, family, seq.start, seq.start + token, &member);
+        if (wave == 0 && quarter == 0) shared.theirs[row] = member;
+        sight = {0, family.keys, 0, family.keys, 0, 0};
+        if (!__all(mine.begin == 0 && mine.end == family.keys && mine.low == 0)) {  // (lanes without a row have the first one's)
+          sight = {mine.begin, mine.end, mine.begin, mine.end, mine.low, mine.low};
+#pragma unroll 1
+          for (int d = 1; d < kFewRows; d *= 2) {
+            sight.first = min(sight.first, __shfl_xor(sight.first, d, kWave)), sight.end = max(sight.end, __shfl_xor(sight.end, d, kWave));
+            sight.sure_first = max(sight.sure_first, __shfl_xor(sight.sure_first, d, kWave)), sight.sure_end = min(sight.sure_end, __shfl_xor(sight.sure_end, d, kWave));
+            sight.low = max(sight.low, __shfl_xor(sight.low, d, kWave)), sight.sure_low = min(sight.sure_low, __shfl_xor(sight.sure_low, d, kWave));
+          }
+          sight = {__builtin_amdgcn_readfirstlane(sight.first), __builtin_amdgcn_readfirstlane(sight.end), __builtin_amdgcn_readfirstlane(sight.sure_first),
+                   __builtin_amdgcn_readfirstlane(sight.sure_end), __builtin_amdgcn_readfirstlane(sight.low), __builtin_amdgcn_readfirstlane(sight.sure_low)};
+        }
+        span = {0, 0, 0, 0};
+        lo = round0 * kRound, hi = complete ? family.keys : min(family.keys, round1 * kRound);
+        if (a.window > 0) seen_of_part<kSpanTile>(sight, &lo, &hi);
+      } else {
+        mine = seq.reach_of<SIGHT>(a, token);
+        sight = sight_of(seq.reach_of<SIGHT>(a, token0), seq.reach_of<SIGHT>(a, token1));
+      }
+      if (of_family) {
+      } else if constexpr (SIGHT) {
         span = span_of<kSpanTile>(sight, seq.base);
         lo = span.lo, hi = span.hi;
         if (!complete) {
@@ -461,7 +515,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
             for (int c = 0; c < kWide; ++c) o[c] += stage[(w * kFewRows + r) * S::kPitch + d0 + c] * weight;
           }
           const int t = (row0 + r) / a.group, h = kv_head * a.group + row0 + r - t * a.group;
-          if (complete && (!SIGHT || seq.base == 0)) {
+          if (complete && (!SIGHT || (seq.base == 0 && !of_family))) {
             const float inv = inverse_sum(total, seq.reach(a, t).end > 0);
             T* to = static_cast<T*>(a.out) + (seq.start + t) * a.out_pitch + (int64_t)h * D + d0;
             Vec<T, kWide> x;
@@ -469,12 +523,17 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
             for (int c = 0; c < kWide; ++c) x.v[c] = from_float<T>(o[c] * inv);
             store_vec<T, kWide>(to, x);
           } else {
-            const bool whole = SIGHT && complete;  // (of a family's: what it has of its own)
-            const int64_t at = whole ? a.whole_at + (seq.start + t) * (int64_t)a.heads + h : (2 * (int64_t)workgroup + (round0 == 0 ? 1 : 0)) * kFewRows + r;
-            float* const ml = a.partial + (SIGHT ? a.rows : 2 * (int64_t)splits * kFewRows) * D + at * 2;
+            int64_t at = (2 * (int64_t)workgroup + (round0 == 0 ? 1 : 0)) * kFewRows + r;
+            if (SIGHT && complete) {  // (of a family's: what it has in common, or of its own)
+              const int64_t row_at = (seq.start + t) * (int64_t)a.heads + h;
+              at = of_family ? a.family_at + row_at * a.family_splits : a.whole_at + row_at;
+            }
+            if (!of_family || shared.theirs[r]) {
+              float* const ml = a.partial + (SIGHT ? a.rows : 2 * (int64_t)splits * kFewRows) * D + at * 2;
   #pragma unroll
-            for (int c = 0; c < kWide; ++c) a.partial[at * D + d0 + c] = o[c];
-            if (d0 == 0) ml[0] = best, ml[1] = total;
+              for (int c = 0; c < kWide; ++c) a.partial[at * D + d0 + c] = o[c];
+              if (d0 == 0) ml[0] = best, ml[1] = total;
+            }
           }
         }
       }

@@ -30,7 +30,8 @@ struct FamilyWork {  // of a lane's family
   int blocks, steps;
 };
 __device__ __forceinline__ FamilyWork family_work(const PagedArgs& a, const LaneSequences& lanes) {
-  return {(int)(((int64_t)lanes.family_tokens * a.group + kTileRows - 1) / kTileRows), lanes.family_keys / 64};
+  const int blocks = family_blocks(a, lanes).many;
+  return {blocks, blocks > 0 ? lanes.family_keys / 64 : 0};
 }
 __device__ __forceinline__ int family_parts(int steps, int most) { return (steps + most - 1) / most; }
 // For the kernel that follows, behind the partial results: the units of the few-rows kernel, how they are shared out, and how many come before each sequence.
@@ -105,7 +106,7 @@ __device__ __forceinline__ Scan<T, D> scan_of(const PagedArgs& a, Walk& walk) {
         const LaneSequences lanes = lane_sequences(a, g * kWave, numbers[g]);
         scan.work[g] = family_work(a, lanes);
         if (few_shared(a)) {
-          scan.rounds[g] = rounds_of<true>(a, own_sequence(lanes));
+          scan.rounds[g] = all_rounds_of(a, lanes);
           scan.units += (int64_t)sum_of_lanes(scan.rounds[g]) * kv_heads;
         }
       }
@@ -140,7 +141,7 @@ __device__ __forceinline__ void tell(const PagedArgs& a, const Scan<T, D>& scan)
   if (lane == 0) *share_note<D>(a) = {scan.s.steps, scan.s.few_groups, scan.units};
   int64_t before = 0;
   for (int base = 0; few_shared(a) && base < a.view.batch; base += kWave) {
-    const int mine = rounds_of<true>(a, own_sequence(lane_sequences(a, base))), upto = sum_up_to_here(mine);
+    const int mine = all_rounds_of(a, lane_sequences(a, base)), upto = sum_up_to_here(mine);
     if (base + lane < a.view.batch) units_before<D>(a)[base + lane] = before + (int64_t)(upto - mine) * a.view.kv_heads;
     before += (int64_t)__builtin_amdgcn_readlane(upto, kWave - 1) * a.view.kv_heads;
   }
@@ -151,15 +152,15 @@ __device__ __forceinline__ void begin_walk(const PagedArgs& a, const Scan<T, D>&
   if (!seen_at_once(a)) return;
   const int64_t unit = quotient(scan.units * workgroup, sharers(scan.s.few_groups, scan.units));
   int64_t from = 0, before = 0;
-  int base = 0, mine = scan.rounds[0];
+  int base = 0;
 #pragma unroll
   for (int g = 0; g < kSeen; ++g)
     if (g * kWave < a.view.batch) {
-      if (before <= unit) base = g * kWave, from = before, mine = scan.rounds[g];
+      if (before <= unit) base = g * kWave, from = before;
       before += (int64_t)sum_of_lanes(scan.rounds[g]) * a.view.kv_heads;
     }
-  walk.ahead = true, walk.base = base, walk.before = from, walk.rounds = mine, walk.upto = (int64_t)sum_up_to_here(mine) * a.view.kv_heads;
-  walk.lanes = lane_sequences(a, base);
+  walk.ahead = true, walk.base = base, walk.before = from, walk.lanes = lane_sequences(a, base);
+  take_lanes(a, walk);
 }
 
 // One launch: a.shares workgroups (FAMILIES) for families and for sequences with few rows, a.tile_groups for those with many, the rest, if any, for few rows (FEW).  So a
@@ -261,14 +262,39 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
   }
   if (b < 0 || b >= view.batch) return;
   const Sequence seq = lanes.sequence(b - lanes.base);
+  const int64_t before_all = before;
+  // (the family that it leads comes first)
   before = lane_of(before, b - lanes.base);
+  if (a.families != nullptr) {
+    const int blocks = family_blocks(a, lanes).few;
+    before += (int64_t)__builtin_amdgcn_readlane(blocks * family_rounds_of(lanes, blocks), b - lanes.base) * view.kv_heads;
+  }
   if (row < seq.start || row >= seq.start + seq.tokens) return;
   const int kv_head = head / a.group, r = (row - seq.start) * a.group + head % a.group, rows = seq.tokens * a.group;
   const int64_t at = (int64_t)row * a.heads + head;
+  // parts of what it has in common with its family, and of its own: where the first is, and how far the others lie apart behind the second
   int of_family = 0;
-  if (seq.base > 0) {  // (as many parts as there are chunks, which are equal but for the last)
-    const int steps = seq.base / 64, parts = family_parts(steps, note.steps), chunk = (steps + parts - 1) / parts;
-    of_family = (steps + chunk - 1) / chunk;
+  int64_t family_place = 0, family_second = 0, family_step = 0;
+  if (seq.base > 0) {
+    const int leader = __builtin_amdgcn_readlane(lanes.leader, b - lanes.base);
+    LaneSequences theirs = lanes;
+    if (leader < lanes.base) theirs = lane_sequences(a, leader & ~(kWave - 1));
+    const int blocks = __builtin_amdgcn_readlane(family_blocks(a, theirs).few, leader - theirs.base);
+    of_family = 1, family_place = a.family_at + at * a.family_splits;
+    if (blocks == 0) {  // (as many parts as there are chunks, which are equal but for the last)
+      const int steps = seq.base / 64, most = family_parts(steps, note.steps), chunk = (steps + most - 1) / most;
+      of_family = (steps + chunk - 1) / chunk, family_second = family_place + 1, family_step = 1;
+    } else {
+      const int of_rows = (row - __builtin_amdgcn_readlane(theirs.start, leader - theirs.base)) * a.group + head % a.group, block = of_rows / kFewRows;
+      const int rounds = kStart + seq.base / kRound;
+      const int64_t unit = (leader < lanes.base ? units_before<D>(a)[leader] : lane_of(before_all, leader - lanes.base)) + (int64_t)(block * view.kv_heads + kv_head) * rounds;
+      const Sharers shared = sharers_of(unit, rounds, note.units, sharers(view.page_shift >= 4 ? note.few_groups : a.few_splits, note.units));
+      if (shared.last > shared.first) {
+        of_family = (int)(shared.last - shared.first) + 1;
+        family_place = (2 * shared.first + 1) * kFewRows + of_rows % kFewRows;
+        family_second = 2 * (shared.first + 1) * kFewRows + of_rows % kFewRows, family_step = 2 * kFewRows;
+      }
+    }
   }
   int parts = 1;                    // of the sequence's own keys
   int64_t place = a.whole_at + at;  // of them, and how far they lie apart
@@ -290,14 +316,14 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
     }
   }
   if (of_family == 0 && parts == 1) return;  // (there already)
-  const int64_t family_place = a.family_at + at * a.family_splits;
   const int all = of_family + parts;
   const bool sees = seq.reach(a, row - seq.start).end > 0;
   T* const out = static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)head * D;
   const float* const ml = a.partial + a.rows * D;
   auto place_of = [&](int p) {
     const int own = p - of_family;
-    return own < 0 ? family_place + p : own == 0 ? place : second + (own - 1) * step;
+    if (own < 0) return p == 0 ? family_place : family_second + (p - 1) * family_step;
+    return own == 0 ? place : second + (own - 1) * step;
   };
   if (all > kWave) {
     join_parts_by_wavefront<T, D>(a.partial, ml, all, sees, place_of, out);

@@ -221,12 +221,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
       span = {0, 0, 0, 0};
       if (z * (int64_t)chunk >= seq.length) return;
       lo = z * chunk, hi = (int)min((z + 1) * (int64_t)chunk, (int64_t)seq.length);
-      if (a.window > 0) {  // of this part: the first keys that stay visible, the windows' or, from the one to the other, both
-        if (lo >= sight.low) lo = max(lo, min(hi, sight.first & ~(S::kKeys - 1)));
-        hi = min(hi, sight.end);
-        if (hi <= sight.first) hi = min(hi, sight.low);
-        hi = max(lo, hi);
-      }
+      if (a.window > 0) seen_of_part<S::kKeys>(sight, &lo, &hi);
     } else {
       chunk = seq.span_chunk(a);
       span = span_of<kSpanTiles<T>>(sight, seq.base);
