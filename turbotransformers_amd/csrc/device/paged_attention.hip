@@ -9,7 +9,6 @@
 
 #include <cmath>
 #include <limits>
-#include <cstdlib>
 
 namespace ttmi {
 namespace {
@@ -258,7 +257,7 @@ int ttmi_paged_attention_sight_workspace(const ttmi_paged_cache* cache, const tt
   if (int rc = paged_view(cache, batch, heads, &view)) return rc;
   ttmi_paged_sight used = *sight;
   if (!sharing_pays(view, heads, used, dtype)) used.families = nullptr;
-  if (used.families == nullptr && (used.sinks == 0 || used.window == 0) && !getenv("FORCE"))
+  if (used.families == nullptr && (used.sinks == 0 || used.window == 0))
     return ttmi_paged_attention_workspace(cache, batch, heads, max_tokens, max_length, used.window, dtype, bytes);
   TTMI_REQUIRE(max_tokens >= 0 && max_length >= 0, "max_tokens and max_length must not be negative");
   *bytes = batch->tokens == 0 || batch->batch == 0 ? 0 : plan_sight(view, heads, max_tokens, max_length, used, dtype).floats * 4;
@@ -275,7 +274,7 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   ttmi_paged_sight used = *sight;
   if (!sharing_pays(a.view, heads, used, dtype)) used.families = nullptr;
-  if (used.families == nullptr && (used.sinks == 0 || used.window == 0) && !getenv("FORCE"))
+  if (used.families == nullptr && (used.sinks == 0 || used.window == 0))
     return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, used.window, workspace, workspace_bytes,
                                 dtype, stream);
   const SightPlan p = plan_sight(a.view, heads, max_tokens, max_length, used, dtype);
