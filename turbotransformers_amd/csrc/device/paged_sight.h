@@ -14,10 +14,12 @@ namespace ttmi {
 
 namespace {
 
-// How a.shares workgroups are divided.  Work on a family is counted in steps of 64 keys of a block of 128 rows, that on the others in rounds of the few-rows kernel.  What a step costs a workgroup, in
-// sixteenths of a microsecond with two workgroups on a CU, and what a round does where all of them read: its bytes at 9.8 GB/s.
+// How a.shares workgroups are divided.  Work on a family's blocks of 128 rows is counted in steps of 64 keys of one, all other in rounds of the few-rows kernel.  What a round costs a workgroup, in
+// sixteenths of a microsecond, where all of them read: its bytes at 9.8 GB/s.  What a step does beside them is measured (a tile is asked for one ahead, and comes late): us for 64 sequences behind
+// 6000 common keys, bf16, 32 and 8 heads of 128, up to 1500 of their own, at 20 / 40 / 60 / 88 / 120 / 160: 67.5 / 48.9 / 43.8 / 43.5 / 44.8 / 49.4; fp16 of 64, 1000: 31.2 / 28.8 / 30.5 / 32.3 / 35.6 /
+// 35.4; fp32 of 64, 600: 125 / 76.6 / 67.0 / 59.3 / 57.1 / 54.9; fp32 of 128, behind 4000, 300, at 120 / 220 / 300: 105 / 87.8 / 82.3.
 template <typename T, int D>
-constexpr int kStepCost = sizeof(T) == 4 ? (D == 128 ? 200 : 120) : (D == 128 ? 88 : 64);
+constexpr int kStepCost = sizeof(T) == 4 ? (D == 128 ? 320 : 140) : (D == 128 ? 72 : 48);
 template <typename T, int D>
 constexpr int kRoundCost = 16 * kRound * 2 * D * (int)sizeof(T) / 9800;
 struct Shares {
