@@ -55,18 +55,16 @@ struct Job {
   Sequence seq;
   Family family;
 };
-// The item-th of all, in parts of `steps` at most, which is among the 64 sequences from `base` on, `passed` items being those of others before -> its lanes.
-__device__ __forceinline__ LaneSequences family_job(const PagedArgs& a, int steps, int item, int base, int passed, Job* job) {
-  const LaneSequences lanes = lane_sequences(a, base);
+// The item-th of all, in parts of `steps` at most, which is among 64 sequences, `passed` items being those of others before.
+__device__ __forceinline__ void family_job(const PagedArgs& a, const LaneSequences& lanes, int steps, int item, int passed, Job* job) {
   const FamilyWork w = family_work(a, lanes);
   const int mine = w.blocks * family_parts(w.steps, steps), upto = passed + sum_up_to_here(mine);
   const int lane = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(item < upto)) - 1);
   const int at = item - __builtin_amdgcn_readlane(upto - mine, lane), blocks = __builtin_amdgcn_readlane(w.blocks, lane);
   const int all = __builtin_amdgcn_readlane(w.steps, lane), parts = family_parts(all, steps);
   // (workgroups beside each other have the same keys of a head, on one XCD where there are eight heads)
-  job->b = base + lane, job->part = at / blocks, job->block = at - job->part * blocks, job->chunk = (all + parts - 1) / parts * 64;
+  job->b = lanes.base + lane, job->part = at / blocks, job->block = at - job->part * blocks, job->chunk = (all + parts - 1) / parts * 64;
   job->seq = lanes.family_sequence(lane), job->family = lanes.family(lane);
-  return lanes;
 }
 // Up to kSeen times 64 sequences are asked for at once, and what is needed of them stays in registers until the workgroup knows its share; more are read again for each number.
 constexpr int kSeen = 4;
@@ -107,6 +105,7 @@ __device__ __forceinline__ Scan<T, D> scan_of(const PagedArgs& a, Walk& walk) {
       if (g * kWave < a.view.batch) {
         const LaneSequences lanes = lane_sequences(a, g * kWave, numbers[g]);
         scan.work[g] = family_work(a, lanes);
+        if (g == 0) walk.lanes = lanes;
         if (few_shared(a)) {
           scan.rounds[g] = all_rounds_of(a, lanes);
           scan.units += (int64_t)sum_of_lanes(scan.rounds[g]) * kv_heads;
@@ -161,7 +160,8 @@ __device__ __forceinline__ void begin_walk(const PagedArgs& a, const Scan<T, D>&
       if (before <= unit) base = g * kWave, from = before;
       before += (int64_t)sum_of_lanes(scan.rounds[g]) * a.view.kv_heads;
     }
-  walk.ahead = true, walk.base = base, walk.before = from, walk.lanes = lane_sequences(a, base);
+  walk.ahead = true, walk.base = base, walk.before = from;
+  if (base > 0) walk.lanes = lane_sequences(a, base);
   take_lanes(a, walk);
 }
 
@@ -206,6 +206,8 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
           if (upto <= item) base = from, passed = upto;
           upto += sum_of_lanes(w.blocks * family_parts(w.steps, steps));
         });
+        lanes = walk.lanes;
+        if (base > 0 || !seen_at_once(a)) lanes = lane_sequences(a, base);
       } else {
         group -= family_groups, few_groups = scan.s.few_groups, units = scan.units;
         if (!FEW || units == 0 || group >= few_groups) return;
@@ -225,14 +227,15 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
         if (!find_block(a, group / kv_heads / a.splits, &job.b, &job.block)) return;
         lanes = lane_sequences(a, job.b & ~(kWave - 1));
         job.part = group / kv_heads % a.splits, job.chunk = 0, job.seq = lanes.sequence(job.b % kWave), job.family = Family{};
-      } else lanes = family_job(a, steps, item, base, passed, &job);
+      } else family_job(a, lanes, steps, item, passed, &job);
       tiles<T, D, SMALL, true, true>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, group % kv_heads, job.part, shared.tiles);
       item += step;
       if (item >= stop) break;
       __syncthreads();
       // on to the 64 sequences that have it
       for (;;) {
-        const FamilyWork w = family_work(a, lane_sequences(a, base));
+        lanes = lane_sequences(a, base);  // (not kept meanwhile: the registers are needed)
+        const FamilyWork w = family_work(a, lanes);
         const int upto = passed + sum_of_lanes(w.blocks * family_parts(w.steps, steps));
         if (item < upto) break;
         passed = upto, base += kWave;
