@@ -612,7 +612,7 @@ TTMI_API int ttmi_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out,
 
 /* The same with queries and keys normed head by head before they are turned: x becomes x / sqrt(sum_i x_i^2 / head_dim + eps) * w.  q_norm, k_norm: the
  * weights w on the device, float32 (norm_dtype TTMI_F32) or of the tensors' type, [head_dim] for all heads (norm pitches 0) or one row a head, *_norm_pitch
- * elements apart; null: those heads are not normed.  Weights are aligned to their elements.  Sums are held in fp32 (a sum of squares must stay below 2^128), the result is rounded once, after the
+ * elements apart; null: those heads are not normed.  Weights are aligned to their elements (to two of them where pairs are interleaved) and lie in nothing that is written.  Sums are held in fp32 (a sum of squares must stay below 2^128), the result is rounded once, after the
  * turn.  eps is not negative.  No counterpart in the reference. */
 TTMI_API int ttmi_rotary_append_normed(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t q_pitch, int64_t heads,
                                        const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, const double* inv_freq,
@@ -645,8 +645,10 @@ TTMI_API int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int
  *   families        DEVICE int32 [batch, 3], or null.  Sequences that begin with the same keys in the same pages may be a family: they follow one another in the
  *                   batch, and the row of each is (number of the first of them, number behind the last, keys they have in common).  Those keys
  *                   are read once for all of them, where the first one's row of the table says.  A sequence whose row does not agree with that of
- *                   the first it names, or whose row says 0 keys, is on its own.  The result is that without families but for roundings.
- *   family_count, max_shared   how many families there are and the most keys of one, or 0 if unknown: hints like max_tokens. */
+ *                   the first it names, or whose row says 0 keys, is on its own.  Keys are shared in steps of 128.  The result is that without families but for
+ *                   roundings.
+ *   family_count, max_shared   how many families there are and the most keys of one, or 0 if unknown: hints like max_tokens.  Where they say that
+ *                   there is nothing to gain, each sequence reads its keys itself. */
 typedef struct ttmi_paged_sight {
   int64_t window;
   int64_t sinks;
@@ -656,7 +658,7 @@ typedef struct ttmi_paged_sight {
 } ttmi_paged_sight;
 
 /* ttmi_paged_attention with a window and first tokens that stay visible, and with keys that sequences share read once.  Arguments, types and limits
- * are those of ttmi_paged_attention; 2 * batch * kv_heads is less than 2^23 with families.  No counterpart in the reference. */
+ * are those of ttmi_paged_attention.  No counterpart in the reference. */
 TTMI_API int ttmi_paged_attention_sight_workspace(const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, int64_t heads, int64_t max_tokens,
                                                   int64_t max_length, const ttmi_paged_sight* sight, int dtype, int64_t* bytes);
 TTMI_API int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_t out_pitch, int64_t heads,

@@ -51,10 +51,14 @@ def test_tokens_of_the_step_are_not_shared(monkeypatch):
 def test_a_family_takes_a_further_member_where_that_saves_keys():
     """Three texts that begin alike: rows of pages 0..99 in common by 100, 100, then 20 pages.  Two members more of the short prefix are worth it, one is not."""
     def rows(*common):  # common[i]: pages of 8 slots that i and i + 1 begin with
-        table = np.arange(100 * (len(common) + 1), dtype=np.int32).reshape(-1, 100)
-        for i, n in enumerate(common):
-            table[i + 1, :n] = table[i, :n]
-        return paged._families(table, [800] * len(table), 8)
+        pool = tt.cxx.PagePool(1000, 8)
+        names = [pool.add()]
+        pool.extend(names, [800])
+        for n in common:
+            names.append(pool.fork(names[-1]))
+            pool.truncate(names[-1], 8 * n)
+            pool.extend(names[-1:], [800 - 8 * n])
+        return pool.families(names, [800] * len(names), 128)
     got, count, most = rows(100, 100, 20)
     assert got.tolist() == [[0, 3, 800]] * 3 + [[3, 4, 0]] and (count, most) == (1, 800)
     got, count, most = rows(30, 20)  # 2 * 160 > 240
@@ -94,6 +98,19 @@ def test_families_are_runs_with_the_same_pages(seed, monkeypatch):
             assert table[b][:n // size] == table[first][:n // size]
         seen += step.family_count
     assert seen > 20
+
+
+def test_families_refuse():
+    pool = tt.cxx.PagePool(10, 4)
+    a = pool.add()
+    for call in (lambda: pool.families([a], [], 1), lambda: pool.families([a + 1], [1], 1)):
+        with pytest.raises(tt.cxx.EnforceNotMet):
+            call()
+    pool.extend([a], [8])
+    b = pool.fork(a)
+    # (never more than a sequence has, whatever is said)
+    assert pool.families([a, b], [100, -5], 1)[1:] == (0, 0) and pool.families([a, b], [100, 100], 1)[0].tolist() == [[0, 2, 8]] * 2
+    assert pool.families([], [], 1)[0].shape == (0, 3)
 
 
 def test_a_step_without_sequences_or_tokens():
@@ -194,7 +211,8 @@ def test_workspace_does_not_grow_with_keys_that_a_window_hides(lib, dtype):
 
 def test_launches_that_are_too_large_are_refused(lib):
     assert attend(lib, cache(kv_heads=1), batch(tokens=1 << 20), heads=1 << 10, q_pitch=1 << 16, out_pitch=1 << 16) == -1
-    assert attend(lib, cache(), batch(batch=1 << 21)) == -1
+    assert attend(lib, cache(), batch(batch=1 << 22)) == -1
+    assert b"than one launch takes" in lib.ttmi_last_error()
 
 
 def test_python_calls_that_are_refused():

@@ -244,7 +244,7 @@ def test_common_keys_end_where_the_first_sequence_does(dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("batch", [63, 64, 65, 200])
+@pytest.mark.parametrize("batch", [63, 64, 65, 200, 300])
 def test_many_families(dt, batch):
     """More sequences than a wavefront has lanes, families across that border, some sequences without new tokens and some long ones."""
     rng = random.Random(batch)
@@ -260,11 +260,40 @@ def test_many_families(dt, batch):
     check(dt, new, past, 4, 2, 64, 16, families=families)
 
 
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("pairs,page", [(40, 16), (330, 16), (40, 4)])
+def test_more_parts_of_families_than_workgroups(dt, pairs, page):
+    """Families of two sequences with up to 72 rows a key/value head, of other lengths each, said to be one short family: workgroups take several of their parts."""
+    rng = random.Random(pairs)
+    families = [(2, rng.choice([128, 130, 300])) for _ in range(pairs)]
+    past = [keys + rng.choice([0, 5]) for members, keys in families for _ in range(members)]
+    case = Sight(dt, [1] * len(past), past, 72, 2, 64, page, families=families)
+    want, tol = case.attention()
+    for hints in ((0, 0), (0, 64)):
+        got = case.run_attention(hints=hints).cpu().double()
+        assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [700, 650, 600]), ([30, 1, 20], [700, 650, 600])])
+def test_queries_that_are_not_finite_spoil_their_own_row(dt, new, past):
+    case = Sight(dt, new, past, 8, 2, 64, 16, families=[(3, 592)])
+    clean = case.run_attention().cpu()
+    case.check_attention(clean)
+    spoiled = torch.zeros(clean.shape, dtype=torch.bool)
+    for b, head in ((0, 1), (2, 5)):
+        case.q[int(case.starts[b]), head, 3] = math.nan
+        spoiled[int(case.starts[b]), head] = True
+    got = case.run_attention().cpu()
+    assert torch.equal(torch.isnan(got), spoiled) and torch.equal(got[~spoiled], clean[~spoiled])
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
-def test_what_is_not_finite_in_common_keys(dt, bad):
+@pytest.mark.parametrize("new,past", [([1, 30, 1, 1], [700, 300, 400, 500]), ([1, 3, 1, 1], [700, 316, 400, 500])])
+def test_what_is_not_finite_in_common_keys(dt, bad, new, past):
     """A value of a common key reaches every token that sees it, in its column alone; one behind every token's position, or in front of some tokens' windows, only those who see it."""
-    new, past, window = [1, 30, 1, 1], [700, 300, 400, 500], 330
+    window = 330
     case = Sight(dt, new, past, 4, 2, 64, 16, families=[(4, 320)])  # (tokens 300 to 319 of the second sequence are common keys)
     for w in (0, window):
         clean = case.run_attention(window=w).cpu()
@@ -327,8 +356,9 @@ def test_offsets_beyond_32_bits(dt):
     tt.cxx.synchronize()
 
 
-def test_pages_outside_the_cache_are_reported():
-    case = Sight("f16", [1, 30, 1, 1], [400, 307, 290, 100], 4, 2, 64, 16, families=[(3, 256), (1, 0)])
+@pytest.mark.parametrize("new", [[1, 30, 1, 1], [1, 1, 1, 1]])
+def test_pages_outside_the_cache_are_reported(new):
+    case = Sight("f16", new, [400, 307, 290, 100], 4, 2, 64, 16, families=[(3, 256), (1, 0)])
     case.keys, case.values = case.keys.nan_to_num(), case.values.nan_to_num()
     for kw in (dict(families=torch.from_numpy(case.rows).cuda()), dict(window=200, sinks=20), dict(families=torch.from_numpy(case.rows).cuda(), window=200, sinks=20)):
         for bad in (-1, 1 << 20):

@@ -11,7 +11,6 @@
 #include "paged_tiles.h"
 
 namespace ttmi {
-
 namespace {
 
 // How a.shares workgroups are divided.  Work on a family's blocks of 128 rows is counted in steps of 64 keys of one, all other in rounds of the few-rows kernel.  What a round costs a workgroup, in
@@ -234,6 +233,7 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
       __syncthreads();
       // on to the 64 sequences that have it
       for (;;) {
+        if (base >= a.view.batch) return;
         lanes = lane_sequences(a, base);  // (not kept meanwhile: the registers are needed)
         const FamilyWork w = family_work(a, lanes);
         const int upto = passed + sum_of_lanes(w.blocks * family_parts(w.steps, steps));

@@ -143,5 +143,38 @@ PagePool::Copies PagePool::Compact() {
   return moves;
 }
 
+PagePool::FamilyRows PagePool::Families(const std::vector<int64_t>& sequences, const std::vector<int64_t>& held, int64_t least) const {
+  TT_ENFORCE_EQ(sequences.size(), held.size(), "one number of tokens for each sequence");
+  const int64_t n = (int64_t)sequences.size();
+  FamilyRows out;
+  out.rows.reserve((size_t)n * 3);
+  auto add = [&](int64_t first, int64_t end, int64_t tokens) {
+    for (int64_t b = first; b < end; ++b)
+      out.rows.insert(out.rows.end(), {(int32_t)first, (int32_t)end, (int32_t)tokens});
+    if (end - first > 1) ++out.count, out.most = std::max(out.most, tokens);
+  };
+  const Sequence* last = nullptr;
+  int64_t first = 0, common = 0;  // sequences first .. b - 1 have `common` tokens in common (one alone: all)
+  for (int64_t b = 0; b < n; ++b) {
+    const Sequence& s = Of(sequences[(size_t)b]);
+    if (last != nullptr) {
+      const int64_t full = std::min({held[(size_t)b], held[(size_t)b - 1], s.length, last->length}) / page_size_;
+      const auto end = s.pages.begin() + std::max<int64_t>(0, full);
+      const int64_t link = (std::mismatch(s.pages.begin(), end, last->pages.begin()).first - s.pages.begin()) * page_size_, members = b - first;
+      const int64_t with = members == 1 ? link : std::min(common, link);
+      // one more member, if that saves more tokens than the shorter prefix loses for the others
+      if (link >= least && link > 0 && (members == 1 || members * with >= (members - 1) * common)) {
+        common = with;
+      } else {
+        add(first, b, members > 1 ? common : 0);
+        first = b;
+      }
+    }
+    last = &s;
+  }
+  if (n > 0) add(first, n, n - first > 1 ? common : 0);
+  return out;
+}
+
 }  // namespace core
 }  // namespace turbo_transformers

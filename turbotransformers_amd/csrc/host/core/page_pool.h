@@ -30,6 +30,14 @@ class PagePool {
   Copies Compact();  // live pages move to the lowest numbers; the moves have to be made before anything else reads or writes the cache
   Copies MovesOf() const;  // what Compact would return, with nothing changed: moves to free pages as well
 
+  // Neighbours among `sequences` that begin with the same pages, full with their first held[i] tokens: rows [sequences][3] of (number of a family's first, number behind its last, tokens they have in
+  // common), (own number, next, 0) for a sequence that is on its own.  A link of fewer than `least` tokens is none.
+  struct FamilyRows {
+    std::vector<int32_t> rows;
+    int64_t count = 0, most = 0;  // families; the most tokens of one
+  };
+  FamilyRows Families(const std::vector<int64_t>& sequences, const std::vector<int64_t>& held, int64_t least) const;
+
   int64_t Length(int64_t sequence) const { return Of(sequence).length; }
   const std::vector<int32_t>& Pages(int64_t sequence) const { return Of(sequence).pages; }
   int32_t References(int64_t page) const;

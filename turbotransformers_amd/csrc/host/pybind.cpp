@@ -528,6 +528,15 @@ PYBIND11_MODULE(turbo_transformers_cxx, m) {
              return out;
            },
            py::arg("sequences"), py::arg("width"))
+      .def(
+          "families",
+          [](const core::PagePool& pool, const std::vector<int64_t>& sequences, const std::vector<int64_t>& held, int64_t least) {
+            const core::PagePool::FamilyRows families = pool.Families(sequences, held, least);
+            py::array_t<int32_t> rows({(py::ssize_t)sequences.size(), (py::ssize_t)3});
+            std::copy(families.rows.begin(), families.rows.end(), rows.mutable_data());
+            return py::make_tuple(rows, families.count, families.most);
+          },
+          py::arg("sequences"), py::arg("held"), py::arg("least"))
       .def_property_readonly("free_pages", &core::PagePool::free_pages)
       .def_property_readonly("pages", &core::PagePool::pages)
       .def_property_readonly("page_size", &core::PagePool::page_size)

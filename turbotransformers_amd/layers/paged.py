@@ -13,7 +13,6 @@ replayed with other contents of all tensors.  A page outside the cache, or a tok
 import math
 from typing import Optional, Sequence
 
-import numpy as np
 import torch
 
 from .. import cxx
@@ -120,35 +119,6 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, stretch: float = 
     return inv_freq.to(device if device is not None else 'cuda')
 
 
-def _families(table: np.ndarray, before: Sequence[int], page_size: int):
-    """Families of neighbours whose first pages are the same ones, full before this step -> rows [batch, 3], how many families, the most keys of one."""
-    n = len(before)
-    rows = np.stack([np.arange(n), np.arange(1, n + 1), np.zeros(n, np.int64)], axis=1).astype(np.int32)
-    if n < 2:
-        return rows, 0, 0
-    full = np.asarray(before, np.int64) // page_size
-    differs = table[1:] != table[:-1]
-    common = np.where(differs.any(axis=1), differs.argmax(axis=1), table.shape[1]) if table.shape[1] else np.zeros(n - 1, np.int64)
-    links = np.minimum(common, np.minimum(full[1:], full[:-1])) * page_size
-    links[links < _LEAST_SHARED] = 0
-    count = most = first = 0
-    keys = int(links[0])  # what sequences first .. b - 1 have in common with b - 1's next
-    for b in range(1, n + 1):
-        link = int(links[b - 1]) if b < n else 0
-        members = b - first
-        if members == 1:
-            keys = link
-        # one more member, if that saves more keys than the shorter prefix loses for the others
-        if link and (members == 1 or members * min(keys, link) >= (members - 1) * keys):
-            keys = min(keys, link)
-            continue
-        if members > 1:
-            rows[first:b] = (first, b, keys)
-            count, most = count + 1, max(most, keys)
-        first = b
-    return rows, count, most
-
-
 class PagedBatch:
     """The sequences of one step as the operators take them; all layers of the step share it."""
 
@@ -221,7 +191,7 @@ class PagedCache:
         for n in tokens:
             starts.append(starts[-1] + n)
         table = self.pool.table(sequences, max(1, -(-longest // self.pool.page_size)))
-        rows, family_count, max_shared = _families(table, before, self.pool.page_size) if before is not None else (None, 0, 0)
+        rows, family_count, max_shared = self.pool.families(sequences, before, _LEAST_SHARED) if before is not None else (None, 0, 0)
         # one copy to the device: [table | starts | lengths | families]
         parts = [torch.from_numpy(table).flatten(), torch.tensor(starts + lengths, dtype=torch.int32)]
         if family_count:
