@@ -123,8 +123,9 @@ static void launch_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out
 }
 
 // ---- the same with norms of heads -----------------------------------------------------------------------------------------
-// x -> x / sqrt(sum x^2 / d + eps) * w of each head of queries and keys, then the turn.  A head's row is what LANES neighbouring lanes hold, N items each (as above: W elements,
-// or the two halves' W elements of W pairs), so the sum of its squares is a few exchanges within a wavefront, and each row is read once.
+// x -> x / sqrt(sum x^2 / d + eps) * w of each head of queries and keys, then the turn.  A head's row is what `lanes` neighbouring lanes hold, N items each (as above: W elements,
+// or the two halves' W elements of W pairs), so the sum of its squares is a few exchanges within a wavefront, and each row is read once; rows and weights are on their way while the angles are computed.
+// Bytes bound it: the 6 chunks above from HBM 41 us, 4.7 TB/s (without norms, which has a workgroup for each 256 items, 43); a token of each of 8 sequences 4.0.
 struct NormView {
   const void *q, *k;  // weights; null: not normed
   int64_t q_pitch, k_pitch;
@@ -141,60 +142,79 @@ __global__ __launch_bounds__(256) void rotary_append_normed_kernel(const T* qkv,
   const int start = view.starts[b];
   if (token < start) return;
   const int position = view.lengths[b] - view.starts[b + 1] + token;
+
+  const int d = view.head_dim, hk = view.kv_heads;
+  bool stored = position >= 0 && (position >> view.page_shift) < view.table_pitch;
+  int page = 0;
+  if (stored) page = view.table[(int64_t)b * view.table_pitch + (position >> view.page_shift)];
+
+  const int pairs = INTERLEAVED ? 0 : half / W;
+  const int items = d / W - pairs, plain = d / W;
+  const T* const in = qkv + (int64_t)token * qkv_pitch;
+  const int lane = (int)threadIdx.x % lanes, all = heads + 2 * hk, per = (int)blockDim.x / lanes;
+  // What a lane has of a head of queries or keys and its weights: asked for before anything that has to be waited for.  (Values are copied.)
+  Vec<T, W> lo[N], hi[N];
+  Vec<WT, W> wlo[N], whi[N];
+  const WT* weights;
+  auto load = [&](int head) __attribute__((always_inline)) {
+    const bool query = head < heads;
+    const WT* const w = static_cast<const WT*>(query ? norm.q : norm.k);
+    weights = w != nullptr ? w + (query ? (int64_t)head * norm.q_pitch : (int64_t)(head - heads) * norm.k_pitch) : nullptr;
+    const T* const x = in + (int64_t)head * d;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int item = lane + n * lanes;
+      if (head >= heads + hk || item >= items) continue;
+      const bool pair = !INTERLEAVED && item < pairs;
+      const int at = (INTERLEAVED || pair ? item : item + pairs) * W;
+      lo[n] = load_vec<T, W>(x + at);
+      if (pair) hi[n] = load_vec<T, W>(x + half + at);
+      if (weights != nullptr) {
+        wlo[n] = load_vec<WT, W>(weights + at);
+        if (pair) whi[n] = load_vec<WT, W>(weights + half + at);
+      }
+    }
+  };
+  int base = blockIdx.y * per;
+  load(base + (int)threadIdx.x / lanes);
+
   __shared__ float2 turn[128];
   for (int i = threadIdx.x; i < half; i += blockDim.x) {
     const float2 u = unit_turn((double)position * inv_freq[i]);
     turn[i] = make_float2(u.x * amplitude, u.y * amplitude);
   }
   __syncthreads();
-
-  const int d = view.head_dim, hk = view.kv_heads;
-  bool stored = position >= 0 && (position >> view.page_shift) < view.table_pitch;
-  int page = 0;
-  if (stored) {
-    page = view.table[(int64_t)b * view.table_pitch + (position >> view.page_shift)];
-    stored = (unsigned)page < (unsigned)view.pages;
-  }
+  stored = stored && (unsigned)page < (unsigned)view.pages;
   if (!stored && threadIdx.x == 0) page_error(view);
   const int slot = position & ((1 << view.page_shift) - 1);
   const int64_t row0 = (((int64_t)page * hk) << view.page_shift) + slot;
 
-  const int pairs = INTERLEAVED ? 0 : half / W;
-  const int items = d / W - pairs, plain = d / W;
-  const T* const in = qkv + (int64_t)token * qkv_pitch;
-  const int lane = (int)threadIdx.x % lanes, all = heads + 2 * hk;
   // (a wavefront's lanes go round together: those whose head does not exist take part in the exchanges)
-  const int per = (int)blockDim.x / lanes;
-  for (int base = blockIdx.y * per; base < all; base += gridDim.y * per) {
+  while (base < all) {
     const int head = base + (int)threadIdx.x / lanes;
     const bool query = head < heads, value = head >= heads + hk, there = head < all && (query || stored);
-    const T* const x = in + (int64_t)(head < all ? head : 0) * d;
     T* const y = query ? q_out + (int64_t)token * q_pitch + (int64_t)head * d
                        : (value ? values : keys) + (row0 + ((int64_t)(value ? head - heads - hk : head - heads) << view.page_shift)) * d;
     if (there && value) {
+      const T* const x = in + (int64_t)head * d;
       for (int i = lane; i < plain; i += lanes) store_vec<T, W>(y + i * W, load_vec<T, W>(x + i * W));
     }
-    const bool turned = there && !value;
-    const WT* const w = static_cast<const WT*>(query ? norm.q : norm.k);
-    const bool normed = turned && w != nullptr;
-    const WT* const weights = normed ? w + (query ? (int64_t)head * norm.q_pitch : (int64_t)(head - heads) * norm.k_pitch) : nullptr;
-    Vec<T, W> lo[N], hi[N];
+    const bool turned = !value, normed = turned && weights != nullptr;
     float sum = 0.f;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int item = lane + n * lanes;
       if (!turned || item >= items) continue;
-      const bool pair = !INTERLEAVED && item < pairs;
-      lo[n] = load_vec<T, W>(x + (INTERLEAVED || pair ? item : item + pairs) * W);
-      if (pair) hi[n] = load_vec<T, W>(x + half + item * W);
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         const float a = to_float(lo[n].v[e]);
         sum = __builtin_fmaf(a, a, sum);
-        if (pair) {
-          const float c = to_float(hi[n].v[e]);
-          sum = __builtin_fmaf(c, c, sum);
-        }
+      }
+      if (INTERLEAVED || item >= pairs) continue;
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float c = to_float(hi[n].v[e]);
+        sum = __builtin_fmaf(c, c, sum);
       }
     }
     for (int step = lanes / 2; step > 0; step /= 2) sum += __shfl_xor(sum, step, kWave);
@@ -202,24 +222,22 @@ __global__ __launch_bounds__(256) void rotary_append_normed_kernel(const T* qkv,
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int item = lane + n * lanes;
-      if (!turned || item >= items) continue;
+      if (!turned || !there || item >= items) continue;
       const bool pair = !INTERLEAVED && item < pairs;
       const int at = (INTERLEAVED || pair ? item : item + pairs) * W;
       float a[W], c[W];
 #pragma unroll
       for (int e = 0; e < W; ++e) a[e] = to_float(lo[n].v[e]) * factor;
       if (normed) {
-        const Vec<WT, W> u = load_vec<WT, W>(weights + at);
 #pragma unroll
-        for (int e = 0; e < W; ++e) a[e] *= to_float(u.v[e]);
+        for (int e = 0; e < W; ++e) a[e] *= to_float(wlo[n].v[e]);
       }
       if (pair) {
 #pragma unroll
         for (int e = 0; e < W; ++e) c[e] = to_float(hi[n].v[e]) * factor;
         if (normed) {
-          const Vec<WT, W> u = load_vec<WT, W>(weights + half + at);
 #pragma unroll
-          for (int e = 0; e < W; ++e) c[e] *= to_float(u.v[e]);
+          for (int e = 0; e < W; ++e) c[e] *= to_float(whi[n].v[e]);
         }
 #pragma unroll
         for (int e = 0; e < W; ++e) {
@@ -241,6 +259,8 @@ __global__ __launch_bounds__(256) void rotary_append_normed_kernel(const T* qkv,
       }
       store_vec<T, W>(y + at, lo[n]);
     }
+    base += gridDim.y * per;
+    if (base < all) load(base + (int)threadIdx.x / lanes);
   }
 }
 
@@ -250,8 +270,12 @@ static void launch_rotary_append_normed(const void* qkv, int64_t qkv_pitch, void
   const int items = view.head_dim / W - (INTERLEAVED ? 0 : half / W);
   int lanes = 1;
   while (lanes < items && lanes < kWave) lanes *= 2;
-  const int parts = (int)std::min<int64_t>(ceil_div((int64_t)(heads + 2 * view.kv_heads) * lanes, 256), 64);
-  hipLaunchKernelGGL((rotary_append_normed_kernel<T, WT, W, N, INTERLEAVED>), dim3(view.tokens, parts), dim3(256), 0, stream, static_cast<const T*>(qkv), qkv_pitch,
+  const int64_t wanted = (int64_t)(heads + 2 * view.kv_heads) * lanes;
+  const int threads = (int)std::min<int64_t>(ceil_div(wanted, kWave) * kWave, 256);
+  // One workgroup for all heads of a token where there are eight tokens for each CU: what it finds out before its rows counts once then.  us, one / one for each 256 lanes, 32 + 8 + 8 heads of 128,
+  // bf16: 1024 tokens 9.7 / 8.7, 2167 13.6 / 14.2, 7798 40.9 / 49.1.
+  const int parts = view.tokens >= 8 * compute_units() ? 1 : (int)std::min<int64_t>(ceil_div(wanted, threads), 64);
+  hipLaunchKernelGGL((rotary_append_normed_kernel<T, WT, W, N, INTERLEAVED>), dim3(view.tokens, parts), dim3(threads), 0, stream, static_cast<const T*>(qkv), qkv_pitch,
                      static_cast<T*>(q_out), q_pitch, heads, static_cast<T*>(cache->keys), static_cast<T*>(cache->values), view, inv_freq, half, amplitude, norm,
                      lanes);
 }
