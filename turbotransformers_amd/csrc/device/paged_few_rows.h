@@ -16,7 +16,7 @@
 // 4 sequences of 60000 to 131071 keys, fp16, 264 and 7 (6.0 TB/s, part of it out of the last-level cache).  One sequence of 387 keys, 12 heads of 64, fp16: 6.7, of which
 // most is the trips to memory that follow one another: length, pages, keys.
 //
-// SIGHT: rows that see the first keys of their sequence besides a window, and sequences whose first keys are their family's (another kernel's).  The keys that a pair's rows see are laid
+// kSinks, kFamilies: rows that see the first keys of their sequence besides a window, and sequences whose first keys are their family's (another kernel's).  The keys that a pair's rows see are laid
 // behind each other in whole tiles (Span), so that rounds and tiles go over them without the gap.
 #pragma once
 
@@ -88,12 +88,13 @@ __device__ __forceinline__ Sequence own_sequence(const LaneSequences& lanes) {
   s.start = lanes.start, s.tokens = lanes.tokens, s.length = lanes.length, s.first = lanes.first, s.base = lanes.own;
   return s;
 }
+constexpr int kWindow = 0, kSinks = 1, kFamilies = 2;  // what a kernel knows of: windows alone; first keys that stay visible; families, too
 struct Walk {  // 64 sequences, a lane each
-  LaneSequences lanes;    // SIGHT
+  LaneSequences lanes;    // kFamilies
   int base, rounds;       // number of the first; rounds of this lane's, for one head
-  int family_rounds, family_blocks;  // SIGHT: the same of the family that it leads, for one head and block of rows, and those blocks: they come first
+  int family_rounds, family_blocks;  // kFamilies: the same of the family that it leads, for one head and block of rows, and those blocks: they come first
   int64_t before, upto;   // units of all sequences before these; of these up to this lane's, it included
-  int64_t groups;         // of batches of more than 64 sequences: units of this lane's 64th of them and of those before it (SIGHT: or `ahead`: not counted, the walk only goes on)
+  int64_t groups;         // of batches of more than 64 sequences: units of this lane's 64th of them and of those before it (kFamilies: or `ahead`: not counted, the walk only goes on)
   bool ahead;
 };
 constexpr int kSpanTile = 32;  // a tile or two
@@ -133,36 +134,36 @@ __device__ __forceinline__ void take_lanes(const PagedArgs& a, Walk& w) {
   w.family_blocks = a.families != nullptr ? family_blocks(a, w.lanes).few : 0, w.family_rounds = family_rounds_of(w.lanes, w.family_blocks);
   w.upto = (int64_t)sum_up_to_here(w.rounds + w.family_blocks * w.family_rounds) * a.view.kv_heads;
 }
-template <bool SIGHT>
+template <int SEES>
 __device__ __forceinline__ void walk_to(const PagedArgs& a, Walk& w, int base, int64_t before) {
   w.base = base, w.before = before;
-  if constexpr (SIGHT) {
+  if constexpr (SEES == kFamilies) {
     w.lanes = lane_sequences(a, base);
     take_lanes(a, w);
   } else {
     const int lane = (int)(threadIdx.x % kWave);
-    w.rounds = base + lane < a.view.batch ? rounds_of<false>(a, sequence(a, base + lane)) : 0;
+    w.rounds = base + lane < a.view.batch ? rounds_of<SEES == kSinks>(a, sequence(a, base + lane)) : 0;
     w.upto = sum_up_to_lane((int64_t)w.rounds * a.view.kv_heads);
   }
 }
-template <bool SIGHT>
-__device__ __forceinline__ void walk_on(const PagedArgs& a, Walk& w) { walk_to<SIGHT>(a, w, w.base + kWave, w.before + lane_of(w.upto, kWave - 1)); }
+template <int SEES>
+__device__ __forceinline__ void walk_on(const PagedArgs& a, Walk& w) { walk_to<SEES>(a, w, w.base + kWave, w.before + lane_of(w.upto, kWave - 1)); }
 __device__ __forceinline__ int group_size(const PagedArgs& a) { return (a.view.batch + kWave - 1) / kWave; }
-template <bool SIGHT>
+template <int SEES>
 __device__ __forceinline__ void walk_to_group(const PagedArgs& a, Walk& w, int group) {
-  walk_to<SIGHT>(a, w, group * group_size(a), group > 0 ? lane_of(w.groups, group - 1) : 0);
+  walk_to<SEES>(a, w, group * group_size(a), group > 0 ? lane_of(w.groups, group - 1) : 0);
 }
 // -> all units
-template <bool SIGHT>
+template <int SEES>
 __device__ __forceinline__ int64_t count_units(const PagedArgs& a, Walk& w) {
   w.groups = 0;
   if (a.view.batch <= kWave) {
-    walk_to<SIGHT>(a, w, 0, 0);
+    walk_to<SEES>(a, w, 0, 0);
     return lane_of(w.upto, kWave - 1);
   }
   const int size = group_size(a), first = (int)(threadIdx.x % kWave) * size;
   int64_t mine = 0;
-  if constexpr (SIGHT) {
+  if constexpr (SEES == kFamilies) {
     // 64 sequences at a time; what each group of `size` has is kept by its lane
     for (int base = 0; base < a.view.batch; base += kWave) {
       const int upto = sum_up_to_here(all_rounds_of(a, lane_sequences(a, base)));
@@ -172,7 +173,7 @@ __device__ __forceinline__ int64_t count_units(const PagedArgs& a, Walk& w) {
     }
   } else {
 #pragma unroll 4
-    for (int i = 0; i < size; ++i) mine += first + i < a.view.batch ? rounds_of<false>(a, sequence(a, first + i)) : 0;
+    for (int i = 0; i < size; ++i) mine += first + i < a.view.batch ? rounds_of<SEES == kSinks>(a, sequence(a, first + i)) : 0;
   }
   w.groups = sum_up_to_lane(mine * a.view.kv_heads);
   w.base = 0, w.rounds = 0, w.before = w.upto = 0;
@@ -180,18 +181,18 @@ __device__ __forceinline__ int64_t count_units(const PagedArgs& a, Walk& w) {
 }
 struct Place {
   int b, kv_head, round, rounds;  // round: of this head's `rounds`
-  int block = -1;                 // SIGHT: of the rows of the family that b leads
+  int block = -1;                 // kFamilies: of the rows of the family that b leads
 };
-template <bool SIGHT>
+template <int SEES>
 __device__ __forceinline__ Place find_unit(const PagedArgs& a, Walk& w, int64_t unit) {
-  if (a.view.batch > kWave && !(SIGHT && w.ahead) && (unit < w.before || unit >= w.before + lane_of(w.upto, kWave - 1)))
-    walk_to_group<SIGHT>(a, w, __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(w.groups > unit)) - 1));
-  while (w.before + lane_of(w.upto, kWave - 1) <= unit) walk_on<SIGHT>(a, w);
+  if (a.view.batch > kWave && !(SEES == kFamilies && w.ahead) && (unit < w.before || unit >= w.before + lane_of(w.upto, kWave - 1)))
+    walk_to_group<SEES>(a, w, __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(w.groups > unit)) - 1));
+  while (w.before + lane_of(w.upto, kWave - 1) <= unit) walk_on<SEES>(a, w);
   const int64_t at = unit - w.before;
   const int found = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(w.upto > at)) - 1);
   Place p;
   p.b = w.base + found, p.rounds = __builtin_amdgcn_readlane(w.rounds, found);
-  if constexpr (SIGHT) {
+  if constexpr (SEES == kFamilies) {
     const int blocks = __builtin_amdgcn_readlane(w.family_blocks, found), family_rounds = __builtin_amdgcn_readlane(w.family_rounds, found);
     int rest = (int)(at - (lane_of(w.upto, found) - (int64_t)(p.rounds + blocks * family_rounds) * a.view.kv_heads));
     const int of_family = blocks * family_rounds * a.view.kv_heads;
@@ -223,13 +224,14 @@ template <typename T, int D, int NW>
 struct FewRowsShared {
   __align__(16) char tiles[FewRows<T, D, NW>::kLds];
   float met[NW][kFewRows][2];
-  int theirs[kFewRows];  // SIGHT: of a family's rows, whether they are
+  int theirs[kFewRows];  // kFamilies: of a family's rows, whether they are
 };
 
-// The share of one of `splits` workgroups (0: of a pair); SIGHT: units and walk as count_units gives them, if units >= 0.  SMALL: pages of fewer than 16 slots
-template <typename T, int D, int NW, bool SMALL, bool SIGHT>
+// The share of one of `splits` workgroups (0: of a pair); kFamilies: units and walk as count_units gives them, if units >= 0.  SMALL: pages of fewer than 16 slots
+template <typename T, int D, int NW, bool SMALL, int SEES>
 __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int splits, Walk& walk, int64_t all_units, FewRowsShared<T, D, NW>& shared) {
   using S = FewRows<T, D, NW>;
+  constexpr bool SIGHT = SEES != kWindow, FAMILIES = SEES == kFamilies;
   char* const smem = shared.tiles;
   auto& met = shared.met;
   const PagedView& view = a.view;
@@ -242,14 +244,14 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
   // splits 0: a workgroup for each pair
   int64_t unit = workgroup, stop = unit + 1;
   if (splits > 0) {
-    const int64_t units = SIGHT && all_units >= 0 ? all_units : count_units<SIGHT>(a, walk), workgroups = sharers(splits, units);
+    const int64_t units = FAMILIES && all_units >= 0 ? all_units : count_units<SEES>(a, walk), workgroups = sharers(splits, units);
     if (workgroup >= workgroups) return;
     if constexpr (SIGHT) unit = quotient(units * workgroup, workgroups), stop = quotient(units * (workgroup + 1), workgroups);
     else unit = units * workgroup / workgroups, stop = units * (workgroup + 1) / workgroups;
   }
   while (unit < stop) {
     Place place;
-    if (splits > 0) place = find_unit<SIGHT>(a, walk, unit);
+    if (splits > 0) place = find_unit<SEES>(a, walk, unit);
     else place.b = (int)(unit / view.kv_heads), place.kv_head = (int)(unit % view.kv_heads), place.round = 0, place.rounds = INT32_MAX;
     const int b = place.b, kv_head = place.kv_head;
     const int64_t ends = splits > 0 ? min(stop, unit + place.rounds - place.round) : stop;
@@ -260,12 +262,12 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
     if (round1 <= round0) continue;
     Sequence seq;
     Family family{};
-    if constexpr (SIGHT) {
+    if constexpr (FAMILIES) {
       if (splits == 0) walk.lanes = lane_sequences(a, b & ~(kWave - 1));
       seq = walk.lanes.sequence(b - walk.lanes.base);
       if (place.block >= 0) family = walk.lanes.family(b - walk.lanes.base), seq = walk.lanes.family_sequence(b - walk.lanes.base);
     } else seq = sequence(a, b);
-    const bool of_family = SIGHT && place.block >= 0;
+    const bool of_family = FAMILIES && place.block >= 0;
     const int rows_all = of_family ? min(seq.tokens * a.group, (place.block + 1) * kFewRows) : seq.tokens * a.group;
     if (!of_family && (rows_all <= 0 || (rows_all > a.few && !(SIGHT ? a.few_every : a.every)))) return;  // (a workgroup of its own)
     if (round0 == 0 && kv_head == 0 && tid == 0 && !of_family && view.lengths[b] > seq.length) page_error(view);
@@ -542,11 +544,11 @@ __device__ __forceinline__ void few_rows(const PagedArgs& a, int workgroup, int 
   }
 }
 
-template <typename T, int D, int NW, bool SMALL, bool SIGHT>
+template <typename T, int D, int NW, bool SMALL, int SEES>
 __global__ __launch_bounds__(NW * 64, 8 / NW) void few_rows_kernel(const PagedArgs a) {
   __shared__ FewRowsShared<T, D, NW> shared;
   Walk walk{};
-  few_rows<T, D, NW, SMALL, SIGHT>(a, blockIdx.x, a.splits, walk, -1, shared);
+  few_rows<T, D, NW, SMALL, SEES>(a, blockIdx.x, a.splits, walk, -1, shared);
 }
 
 // Which workgroups had a part of a pair: from first to last.
@@ -563,7 +565,7 @@ __device__ __forceinline__ Sharers sharers_of(int64_t unit, int rounds, int64_t 
 // us, a workgroup per row / per pair, 32 query and 8 key heads of 128: 1 sequence of 3000 keys 12.8 / 14.2, 8 (64 pairs) 24.9 / 25.4, 64 of 1500 (512) 75.4 / 73.8, 200 (1600)
 // 241 / 228; 16 query heads of one key head, one sequence of 100000 keys beside 63 of 500, whose pair has most of the parts, 45.7 / 145.
 constexpr int kManyPairs = 512;
-template <typename T, int D, bool SIGHT>
+template <typename T, int D, int SEES>
 __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a, bool by_pair) {
   const PagedView& view = a.view;
   const int kv_head = blockIdx.x % view.kv_heads, b = blockIdx.x / view.kv_heads;
@@ -571,15 +573,15 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a, b
   const int rows = seq.tokens * a.group;
   if (rows > a.few || (int)blockIdx.y >= rows) return;
   Walk walk{};
-  const int64_t units = count_units<SIGHT>(a, walk), workgroups = sharers(a.splits, units);
-  if (view.batch > kWave) walk_to_group<SIGHT>(a, walk, b / group_size(a));
-  while (walk.base + kWave <= b) walk_on<SIGHT>(a, walk);
+  const int64_t units = count_units<SEES>(a, walk), workgroups = sharers(a.splits, units);
+  if (view.batch > kWave) walk_to_group<SEES>(a, walk, b / group_size(a));
+  while (walk.base + kWave <= b) walk_on<SEES>(a, walk);
   const int lane = b - walk.base, rounds = __builtin_amdgcn_readlane(walk.rounds, lane);
   const Sharers shared = sharers_of(walk.before + lane_of(walk.upto, lane) - (int64_t)rounds * (view.kv_heads - kv_head), rounds, units, workgroups);
   const int64_t first = shared.first, last = shared.last;
   if (first == last) return;
   const int parts = (int)(last - first) + 1;
-  const float* const ml = a.partial + (SIGHT ? a.rows : 2 * (int64_t)a.splits * kFewRows) * D;
+  const float* const ml = a.partial + (SEES != kWindow ? a.rows : 2 * (int64_t)a.splits * kFewRows) * D;
   auto sees = [&](int r) { return seq.reach(a, r / a.group).end > 0; };
   auto place = [&](int r) {
     const int t = r / a.group, h = kv_head * a.group + r - t * a.group;
@@ -596,26 +598,28 @@ __global__ __launch_bounds__(256) void join_few_rows_kernel(const PagedArgs a, b
       a.partial, ml, parts, sees(r), [&](int p) { return (2 * (first + p) + (p == 0 ? 1 : 0)) * kFewRows + r; }, place(r));
 }
 
-template <typename T, int D, bool SIGHT>
+template <typename T, int D, int SEES>
 void start_join_few_rows(const PagedArgs& a, hipStream_t stream) {
-  if (a.splits == 0 || a.families != nullptr) return;
+  if (a.splits == 0) return;
   const unsigned pairs = (unsigned)((int64_t)a.view.batch * a.view.kv_heads);
   const bool by_pair = pairs >= kManyPairs;
-  hipLaunchKernelGGL((join_few_rows_kernel<T, D, SIGHT>), dim3(pairs, by_pair ? 1u : (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0,
+  hipLaunchKernelGGL((join_few_rows_kernel<T, D, SEES>), dim3(pairs, by_pair ? 1u : (unsigned)std::min<int64_t>(a.few, (int64_t)a.view.tokens * a.group)), dim3(256), 0,
                      stream, a, by_pair);
 }
-template <typename T, bool SIGHT>
+template <typename T, int SEES>
 void start_few_rows(const PagedArgs& a, int64_t head_dim, hipStream_t stream) {
   const unsigned pairs = (unsigned)((int64_t)a.view.batch * a.view.kv_heads);
   const bool small = a.view.page_shift < 4;
   auto sized = [&](auto d) {
     constexpr int D = decltype(d)::value;
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.splits > 0 ? (unsigned)a.splits : pairs), dim3(a.waves * 64), 0, stream, a); };
-    if (small && a.waves == 4) launch(few_rows_kernel<T, D, 4, true, SIGHT>);
-    else if (small) launch(few_rows_kernel<T, D, 8, true, SIGHT>);
-    else if (a.waves == 4) launch(few_rows_kernel<T, D, 4, false, SIGHT>);
-    else launch(few_rows_kernel<T, D, 8, false, SIGHT>);
-    start_join_few_rows<T, D, SIGHT>(a, stream);
+    if (small && a.waves == 4) launch(few_rows_kernel<T, D, 4, true, SEES>);
+    else if (small) launch(few_rows_kernel<T, D, 8, true, SEES>);
+    if constexpr (SEES != kFamilies) {  // (which are another launch's, but for small pages)
+      if (!small && a.waves == 4) launch(few_rows_kernel<T, D, 4, false, SEES>);
+      else if (!small) launch(few_rows_kernel<T, D, 8, false, SEES>);
+      start_join_few_rows<T, D, SEES>(a, stream);
+    }
   };
   if (head_dim == 64) sized(std::integral_constant<int, 64>{});
   else sized(std::integral_constant<int, 128>{});

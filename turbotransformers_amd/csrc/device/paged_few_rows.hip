@@ -4,7 +4,7 @@
 namespace ttmi {
 
 int launch_few_rows(const PagedArgs& a, int dtype, int64_t head_dim, hipStream_t stream) {
-  TTMI_DISPATCH_FLOAT(dtype, T, { (start_few_rows<T, false>(a, head_dim, stream)); });
+  TTMI_DISPATCH_FLOAT(dtype, T, { (start_few_rows<T, kWindow>(a, head_dim, stream)); });
   return launch_status("paged_attention");
 }
 

@@ -111,7 +111,7 @@ __device__ __forceinline__ Scan<T, D> scan_of(const PagedArgs& a, Walk& walk) {
         }
       }
     }
-  } else if (few_shared(a)) scan.units = count_units<true>(a, walk);
+  } else if (few_shared(a)) scan.units = count_units<kFamilies>(a, walk);
   // (sums of 64 numbers that are capped for the balance alone)
   constexpr int kCap = 1 << 24;
   int64_t steps = 0;
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
       tiles<T, D, SMALL, true, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, group % kv_heads, group / kv_heads % a.splits, shared.tiles);
     } else if constexpr (FEW) {
       Walk walk{};
-      few_rows<T, D, 4, false, true>(a, group - a.tile_groups, a.few_splits, walk, -1, shared.few);
+      few_rows<T, D, 4, false, kSinks>(a, group - a.tile_groups, a.few_splits, walk, -1, shared.few);
     }
   } else {
     Job job;
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
       if (!own) group -= a.tile_groups, few_groups = 0;
     }
     if (few_groups >= 0) {
-      if constexpr (FEW) few_rows<T, D, 4, false, true>(a, group, few_groups, walk, units, shared.few);
+      if constexpr (FEW) few_rows<T, D, 4, false, kFamilies>(a, group, few_groups, walk, units, shared.few);
       return;
     }
     for (;;) {
@@ -382,17 +382,18 @@ void start_sight(const SightLaunch& l, int64_t head_dim, hipStream_t stream) {
     // (where sequences with few rows are shared out among all workgroups, those are a.shares)
     const int few_groups = a.few_splits == 0 ? a.view.batch * a.view.kv_heads : shares > 0 ? 0 : a.few_splits;
     auto launch = [&](auto kernel, int groups) { hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), 0, stream, a); };
-    if (!l.run_tiles) start_few_rows<T, true>(l.few, head_dim, stream);
+    if (!l.run_tiles) start_few_rows<T, kSinks>(l.few, head_dim, stream);
     else if (!small && a.run_few) {
       if (shares > 0) launch(sight_kernel<T, D, false, true, true>, shares + a.tile_groups + few_groups);
       else launch(sight_kernel<T, D, false, false, true>, a.tile_groups + few_groups);
-      start_join_few_rows<T, D, true>(l.few, stream);
+      if (shares == 0) start_join_few_rows<T, D, kSinks>(l.few, stream);
     } else {
       if (small && shares > 0) launch(sight_kernel<T, D, true, true, false>, shares + a.tile_groups);
       else if (small) launch(sight_kernel<T, D, true, false, false>, a.tile_groups);
       else if (shares > 0) launch(sight_kernel<T, D, false, true, false>, shares + a.tile_groups);
       else launch(sight_kernel<T, D, false, false, false>, a.tile_groups);
-      if (a.run_few) start_few_rows<T, true>(l.few, head_dim, stream);
+      if (a.run_few && shares > 0) start_few_rows<T, kFamilies>(l.few, head_dim, stream);
+      else if (a.run_few) start_few_rows<T, kSinks>(l.few, head_dim, stream);
     }
     if (a.families != nullptr || (l.run_tiles && a.splits > 1))
       hipLaunchKernelGGL((join_sight_kernel<T, D>), dim3(a.view.tokens, (unsigned)ceil_div(a.heads, 4)), dim3(256), 0, stream, a);
