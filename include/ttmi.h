@@ -612,8 +612,9 @@ TTMI_API int ttmi_rotary_append(const void* qkv, int64_t qkv_pitch, void* q_out,
 
 /* The same with queries and keys normed head by head before they are turned: x becomes x / sqrt(sum_i x_i^2 / head_dim + eps) * w.  q_norm, k_norm: the
  * weights w on the device, float32 (norm_dtype TTMI_F32) or of the tensors' type, [head_dim] for all heads (norm pitches 0) or one row a head, *_norm_pitch
- * elements apart; null: those heads are not normed.  Weights are aligned to their elements (to two of them where pairs are interleaved) and lie in nothing that is written.  Sums are held in fp32 (a sum of squares must stay below 2^128), the result is rounded once, after the
- * turn.  eps is not negative.  No counterpart in the reference. */
+ * elements apart; null: those heads are not normed.  Weights are aligned to their elements (to two of them where pairs are
+ * interleaved) and lie in nothing that is written.  Sums are held in fp32 (a sum of squares must stay below 2^128), the result is rounded once, after
+ * the turn.  eps is not negative.  No counterpart in the reference. */
 TTMI_API int ttmi_rotary_append_normed(const void* qkv, int64_t qkv_pitch, void* q_out, int64_t q_pitch, int64_t heads,
                                        const ttmi_paged_cache* cache, const ttmi_paged_batch* batch, const double* inv_freq,
                                        int64_t rotary_dim, int interleaved, float amplitude, const void* q_norm, int64_t q_norm_pitch,

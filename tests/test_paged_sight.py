@@ -213,6 +213,9 @@ def test_launches_that_are_too_large_are_refused(lib):
     assert attend(lib, cache(kv_heads=1), batch(tokens=1 << 20), heads=1 << 10, q_pitch=1 << 16, out_pitch=1 << 16) == -1
     assert attend(lib, cache(), batch(batch=1 << 22)) == -1
     assert b"than one launch takes" in lib.ttmi_last_error()
+    # rows that the sequences' own keys and the families' fill a launch with between them
+    assert attend(lib, cache(kv_heads=128), batch(batch=4, tokens=(1 << 23) - 1), heads=128, q_pitch=1 << 13, out_pitch=1 << 13) == -1
+    assert b"than one launch takes" in lib.ttmi_last_error()
 
 
 def test_python_calls_that_are_refused():

@@ -91,7 +91,6 @@ __device__ __forceinline__ Sequence sequence(const PagedArgs& a, int b) {
   return s;
 }
 
-
 // Keys that a block of rows sees: those from first to end, of which all rows see those from sure_first to sure_end; SIGHT: and those below low, of which all see those below
 // sure_low.
 struct Sight {

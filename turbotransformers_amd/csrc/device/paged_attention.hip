@@ -152,11 +152,11 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
 }
 
 // Whether reading a family's keys once is worth it: a second launch, which joins what they give with what the sequences' own keys do, and blocks of 128 rows that may be mostly empty, for reads
-// that the caches would take most of.  us, families / none, one token each and 50 keys of its own:
-//   bf16, 32 and 8 heads of 128: 4 sequences behind 4000 keys 17.6 / 17.2, 8 behind 2000 18.9 / 19.0, 64 behind 512 20.9 / 15.2, 64 behind 1000 25.9 / 28.4, 64 behind 8000 40 / 147;
-//                                8 families of 2 behind 4000 37 / 33, 4 of 8 29.7 / 51.0, 16 of 4 behind 1000 32.2 / 29.9, 16 of 4 behind 4000 75 / 89, 8 of 8 behind 16000 153 / 322
-//   fp16, 12 heads of 64:        16 behind 1000 13.7 / 8.9, 16 behind 2000 14.2 / 18.0, 8 behind 4000 15.5 / 18.6; 32 and 8 heads: 4 of 16 behind 1000 20.3 / 14.1, 8 of 8 behind 4000 38.8 / 45.7
-//   fp32, 32 and 8 heads of 128: 32 behind 1000 46 / 38, 32 behind 4000 58 / 101, 8 of 8 behind 16000 819 / 687; of 64: 32 behind 4000 30.2 / 57.3, 8 of 8 behind 16000 316 / 368
+// that the caches would take most of.  us, families / none, one token each and 50 keys of its own, behind 1000, 2000, 4000, 8000 keys (where both are level the answer is no):
+//   bf16, 32 and 8 heads of 128: 8 sequences 15.8 / 15.4, 17.4 / 17.2, 22.4 / 21.5, 27.4 / 30.3; 64 28.7 / 28.7, 30.0 / 46.4, 29.7 / 79.8, 40.7 / 147; 256 63.8 / 96.7 .. 95.3 / 572;
+//                                8 families of 2 17.7 / 17.6 .. 54.7 / 53.8; 4 of 8 21.4 / 21.5, 26.6 / 31.3, 30.2 / 49.7, 40.8 / 82.9; 16 of 4 29.7 / 29.3, 37.9 / 47.9, 55.5 / 90.6, 115 / 181
+//   fp16, 12 heads of 64:        16 sequences 9.2 / 8.9, 15.2 / 18.7, 16.0 / 25.5, 19.3 / 39.2; 16 families of 4 20.7 / 20.5, 32.6 / 41.8, 45.6 / 67.8, 84.0 / 141
+//   fp32, the same heads:        4 sequences 13.3 / 13.0, 15.8 / 15.7, 16.6 / 22.2, 22.1 / 28.9; 64 27.7 / 47.5 .. 48.1 / 264; 32 and 8 heads of 128, 64: 54.2 / 53.9, 62.5 / 93.6 .. 141 / 321
 // Where nothing is known they are taken as they come.
 bool sharing_pays(const PagedView& view, int64_t heads, const ttmi_paged_sight& sight, int dtype) {
   if (sight.families == nullptr) return false;
@@ -278,6 +278,8 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
     return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, used.window, workspace, workspace_bytes,
                                 dtype, stream);
   const SightPlan p = plan_sight(a.view, heads, max_tokens, max_length, used, dtype);
+  const int64_t kv_heads = cache->kv_heads, tile_groups = p.own_blocks * kv_heads * p.own.tile_splits, few_groups = p.own.few_splits > 0 ? p.own.few_splits : batch->batch * kv_heads;
+  TTMI_REQUIRE(p.shares + tile_groups + (p.own.few ? few_groups : 0) < 1 << 24, "more rows or sequences than one launch takes");
   TTMI_REQUIRE(p.floats == 0 || (workspace != nullptr && workspace_bytes >= p.floats * 4 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                "the workspace is too small or not 16-byte aligned");
   a.sinks = (int)std::min(used.sinks, kWidest), a.families = used.families;
@@ -287,7 +289,7 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
   a.own_at = p.few_rows, a.family_at = a.own_at + p.own_rows, a.whole_at = a.family_at + p.family_rows, a.rows = a.whole_at + p.whole_rows;
   l.run_tiles = p.own.tiles || p.shares > 0;
   a.run_few = p.own.few, a.few = p.own.few_rows, a.few_splits = p.own.few_splits, a.few_every = !p.own.tiles;
-  a.own_blocks = p.own_blocks, a.tile_groups = (int)(p.own_blocks * a.view.kv_heads * p.own.tile_splits);
+  a.own_blocks = p.own_blocks, a.tile_groups = (int)tile_groups;
   l.few = a;
   l.few.splits = p.own.few_splits;
   l.few.waves = l.run_tiles && a.view.page_shift >= 4 ? 4 : p.own.few_waves;  // (4 in one launch with the others)

@@ -1,5 +1,5 @@
 // Attention over pages where tokens see the first keys of their sequence besides a window, and where sequences share keys: the kernels of paged_few_rows.h and paged_tiles.h
-// with SIGHT, and what joins the results of a row.
+// that know of both, in one launch, and what joins the results of a row.
 //
 // With families a row's softmax is one over two lists of keys, its family's [0, P) and its sequence's own [P, length):
 //     o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i,   m = max m_i,
