@@ -157,6 +157,47 @@ def test_what_is_not_finite_reaches_only_the_tokens_that_see_it(dt, bad, new, pa
         assert torch.equal(got[~spoiled], clean[~spoiled])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("what", ["keys", "queries"])
+def test_numbers_near_the_largest(d, what):
+    """fp32 products are taken apart into those of narrower numbers, which the largest ones are not: scores of moderate size from a factor beyond 2^127 and one that makes up for it."""
+    case = Sight("f32", [140, 30, 3], [0, 90, 300], 4, 2, d, 16)
+    case.check_attention(case.run_attention(window=50, sinks=7), window=50, sinks=7)
+    small = 2.0 ** -125 * (1 + torch.rand(case.q.shape[:2], generator=torch.Generator().manual_seed(3)))  # (2^127.99 times 2^-124 at most, times the scale)
+    if what == "keys":
+        case.q[..., 5] = small
+        for b, position in ((0, 2), (0, 77), (0, 130), (1, 100), (2, 301)):
+            case.keys[case.table[b, position // 16], :, position % 16, 5] = 3.4e38 if position % 2 else -2.0 ** 127
+    else:
+        case.keys[..., 5] = torch.where(torch.isnan(case.keys[..., 5]), case.keys[..., 5], torch.full_like(case.keys[..., 5], 2.0 ** -125))
+        for row in (0, 31, 64, 139, 150, 171):
+            case.q[row, 1, 5], case.q[row, 2, 5] = 3.4028234e38, -1.9e38
+    case.check_attention(case.run_attention(window=50, sinks=7), window=50, sinks=7)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_near_the_largest_in_common(d):
+    case = Sight("f32", [40, 30, 20, 1, 1], [300, 256, 270, 400, 300], 4, 2, d, 16, families=[(3, 256), (2, 288)])
+    case.q[..., 5] = 2.0 ** -125
+    for b, position in ((0, 2), (0, 77), (0, 255), (1, 280), (3, 5), (3, 288)):
+        case.keys[case.table[b, position // 16], :, position % 16, 5] = 3.4e38 if position % 2 else -2.0 ** 127
+    case.check_attention(case.run_attention())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_of_minus_infinity(d):
+    """A key with a score of minus infinity weighs nothing, whether it comes from an infinity or from numbers near it: the bits are those of a score that is merely low."""
+    case = Sight("f32", [140, 30], [0, 90], 4, 2, d, 16)
+    case.q[..., 5] = -1.0
+    outs = []
+    for low in (3000.0, 3.4e38, math.inf):
+        for b, position in ((0, 2), (0, 77), (1, 100)):
+            case.keys[case.table[b, position // 16], :, position % 16, 5] = low
+        outs.append(case.run_attention(window=50, sinks=7).cpu())
+    assert torch.isfinite(outs[0]).all()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
 # ------------------------------------------------------------------------------------------------------- families ------
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("d", [64, 128])

@@ -167,11 +167,14 @@ __device__ __forceinline__ void begin_walk(const PagedArgs& a, const Scan<T, D>&
 // One launch: a.shares workgroups (FAMILIES) for families and for sequences with few rows, a.tile_groups for those with many, the rest, if any, for few rows (FEW).  So a
 // CU has workgroups that multiply beside others that read.  (Families take registers and FEW does not cost any, but instructions: a prompt of 8192 tokens in a window of 1024, 32 and 8
 // heads of 128, 206 us with both, 195 without.)
+// Heads of 128 in three parts each take the registers of two workgroups, which families and sequences with few rows cannot spare.
+template <typename T, int D, bool FAMILIES, bool FEW>
+constexpr bool kThirds = sizeof(T) == 4 && (D == 64 || (!FAMILIES && !FEW));
 template <typename T, int D, bool SMALL, bool FAMILIES, bool FEW>
-__global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(256, (D == 128 && kThirds<T, D, FAMILIES, FEW> ? 1 : 2)) void sight_kernel(const PagedArgs a) {
   static_assert(!FEW || !SMALL, "with small pages sequences with few rows have a launch of their own");
   __shared__ union {
-    TilesShared<T, D> tiles;
+    TilesShared<T, D, kThirds<T, D, FAMILIES, FEW>> tiles;
     FewRowsShared<T, D, 4> few;
   } shared;
   const int kv_heads = a.view.kv_heads;
@@ -180,7 +183,7 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
     if (!FEW || group < a.tile_groups) {
       int b, block;
       if (!find_block(a, group / kv_heads / a.splits, &b, &block)) return;
-      tiles<T, D, SMALL, true, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, group % kv_heads, group / kv_heads % a.splits, shared.tiles);
+      tiles<T, D, SMALL, true, false, kThirds<T, D, FAMILIES, FEW>>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, group % kv_heads, group / kv_heads % a.splits, shared.tiles);
     } else if constexpr (FEW) {
       Walk walk{};
       few_rows<T, D, 4, false, kSinks>(a, group - a.tile_groups, a.few_splits, walk, -1, shared.few);
@@ -227,7 +230,7 @@ __global__ __launch_bounds__(256, 2) void sight_kernel(const PagedArgs a) {
         lanes = lane_sequences(a, job.b & ~(kWave - 1));
         job.part = group / kv_heads % a.splits, job.chunk = 0, job.seq = lanes.sequence(job.b % kWave), job.family = Family{};
       } else family_job(a, lanes, steps, item, passed, &job);
-      tiles<T, D, SMALL, true, true>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, group % kv_heads, job.part, shared.tiles);
+      tiles<T, D, SMALL, true, true, kThirds<T, D, FAMILIES, FEW>>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, group % kv_heads, job.part, shared.tiles);
       item += step;
       if (item >= stop) break;
       __syncthreads();

@@ -15,6 +15,12 @@
 // fp32 with heads of 128 has no registers left (256 and 96 bytes of scratch a lane): a prompt of 1000 tokens 153 us.
 // What was built and taken out: 256 rows a workgroup with the products of 32 keys beside the exponentials of the 32 before, level to 3 % faster for heads of 128, 2 % slower for those of 64.
 //
+// THIRDS (fp32 with SIGHT): the fp32 instruction takes sixteen times as long as the bf16 one, so a number is a sum of three bf16, x = h + m + l to its last place, and a product six of theirs,
+//     x y = h h' + (h m' + m h') + (m m' + h l' + l h'), up to 2^-23 of it left out (m is at most 2^-8, l 2^-16 of x);
+// keys and values are taken apart on their way to LDS, queries once, probabilities as they come; sums are fp32 as ever.  Numbers from 2^127 on, whose h may be an infinity, have their scores
+// computed one by one.  us, that instruction / this, 12 heads of 64: 8 prompts of 33 to 900 tokens, window 200 41.5 / 34.7, one of 4000, window 1000 171 / 112, 8 questions of 40 to 100 tokens behind 4000 common
+// keys 94 / 70; 32 and 8 heads of 128: a prompt of 1000, window 300 125 / 73, 20 chunks of up to 300 behind up to 3000 keys 214 / 120.  Against 64 bits the error goes from 2.5e-7 to 1.8e-7.
+//
 // SIGHT: rows that see the first keys of their sequence besides a window (the keys that a block sees lie behind each other in whole tiles, Span), sequences whose first keys are their family's,
 // and families: the rows of all sequences of one over the keys that they have in common, each of which sees what its own position lets it see.
 #pragma once
@@ -132,10 +138,38 @@ __device__ __forceinline__ bool find_block(const PagedArgs& a, int want, int* b,
   return false;
 }
 
-template <typename T, int D>
+// Four floats as sums of three bf16 each, whose products the bf16 instructions add up 16 keys at a time.
+struct Thirds {
+  u32x2 part[3];
+};
+__device__ __forceinline__ Thirds thirds(const u32x4& raw) {
+  const floatx4 x = __builtin_bit_cast(floatx4, raw);
+  Thirds t;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint32_t both = pack2<bf16>(a, b);
+      t.part[p][i] = both;
+      a -= __builtin_bit_cast(float, both << 16), b -= __builtin_bit_cast(float, both & 0xffff0000u);
+    }
+  }
+  return t;
+}
+// Numbers that this cannot take apart: their bf16 may be an infinity, times which the other parts would be NaN.
+constexpr float kTooLarge = 0x1p127f;
+__device__ __forceinline__ bool too_large(const u32x4& raw) {
+  const floatx4 x = __builtin_bit_cast(floatx4, raw);
+  return fmaxf(fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1])), fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3]))) >= kTooLarge;
+}
+
+template <typename T, int D, bool THIRDS>
 struct TilesShared {
-  __align__(16) char tiles[4 * Tiles<T, D>::kBytes];
+  static constexpr int kBytes = THIRDS ? Tiles<T, D>::kBytes * 3 / 2 : Tiles<T, D>::kBytes;  // of a tile of keys, or of values
+  __align__(16) char tiles[4 * kBytes];
   int wild;  // whether values that only some rows see hold infinities or NaNs
+  int large;  // THIRDS: whether a key was too large
   int sights[4][6];  // of a family's rows, wavefront by wavefront
 };
 
@@ -174,10 +208,12 @@ __device__ __forceinline__ void family_sights(const Family& f, const Reach& mine
 
 // Part `z` of a block of rows of sequence b; SIGHT: of the sequence's own keys, or (family.keys > 0) of the family's that it leads, in parts of family_chunk keys.
 // SMALL: pages of fewer than 16 slots
-template <typename T, int D, bool SMALL, bool SIGHT, bool FAMILIES>
+// THIRDS: fp32 by the bf16 instructions
+template <typename T, int D, bool SMALL, bool SIGHT, bool FAMILIES, bool THIRDS>
 __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, const Sequence& seq, const LaneSequences& lanes, const Family& family, int family_chunk,
-                                      int kv_head, int z, TilesShared<T, D>& shared) {
+                                      int kv_head, int z, TilesShared<T, D, THIRDS>& shared) {
   using S = Tiles<T, D>;
+  constexpr int kTileBytes = TilesShared<T, D, THIRDS>::kBytes, kPlane = kTileBytes / 3;  // (THIRDS: of a third of the tile)
   char* const smem = shared.tiles;
   int& wild = shared.wild;
   const PagedView& view = a.view;
@@ -234,11 +270,28 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
     else return place;
   };
 
-  u32x4 qf[S::kSteps];
+  const T* const query = static_cast<const T*>(a.q) + (seq.start + token) * a.q_pitch + (int64_t)head * D;
+  u32x4 qf[THIRDS ? 1 : S::kSteps], qt[THIRDS ? 3 : 1][D / 16];
+  bool large_query = false;
+  if constexpr (!THIRDS) {
 #pragma unroll
-  for (int i = 0; i < S::kSteps; ++i) {
-    qf[i] = u32x4{0u, 0u, 0u, 0u};
-    if (live) qf[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + (seq.start + token) * a.q_pitch + (int64_t)head * D + (2 * i + lhalf) * S::kElems);
+    for (int i = 0; i < S::kSteps; ++i) {
+      qf[i] = u32x4{0u, 0u, 0u, 0u};
+      if (live) qf[i] = *reinterpret_cast<const u32x4*>(query + (2 * i + lhalf) * S::kElems);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (live) x = *reinterpret_cast<const u32x4*>(query + 16 * i + 8 * lhalf + 4 * j);
+        large_query = large_query || too_large(x);
+        const Thirds t = thirds(x);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) qt[p][i][2 * j] = t.part[p][0], qt[p][i][2 * j + 1] = t.part[p][1];
+      }
+    large_query = __shfl_xor((int)large_query, 32, kWave) != 0 || large_query;  // (the row's other half)
   }
   floatx16 ot[S::kOut];
 #pragma unroll
@@ -267,10 +320,20 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
       vr[set][i] = *reinterpret_cast<const u32x4*>(values + from);
     }
   };
-  auto key_stage = [&](int s) __attribute__((always_inline)) { return smem + s * 2 * S::kBytes; };
-  auto value_stage = [&](int s) __attribute__((always_inline)) { return smem + s * 2 * S::kBytes + S::kBytes; };
+  auto key_stage = [&](int s) __attribute__((always_inline)) { return smem + s * 2 * kTileBytes; };
+  auto value_stage = [&](int s) __attribute__((always_inline)) { return smem + s * 2 * kTileBytes + kTileBytes; };
   auto store_piece = [&](int i, int s, int set) __attribute__((always_inline)) {
     const int at = i * 4096 + tid * 16, r = at / S::kRowBytes, c = at % S::kRowBytes / 16;
+    if constexpr (THIRDS) {
+      if (__builtin_expect(too_large(kr[set][i]), 0)) shared.large = 1;
+      const Thirds k = thirds(kr[set][i]), v = thirds(vr[set][i]);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        *reinterpret_cast<u32x2*>(key_stage(s) + p * kPlane + r * 2 * D + key_piece<bf16, D>(r, c / 2) * 16 + c % 2 * 8) = k.part[p];
+        *reinterpret_cast<u32x2*>(value_stage(s) + p * kPlane + r * 2 * D + tile_value_piece<bf16, D>(r, c / 2) * 16 + c % 2 * 8) = v.part[p];
+      }
+      return;
+    }
     *reinterpret_cast<u32x4*>(key_stage(s) + r * S::kRowBytes + key_piece<T, D>(r, c) * 16) = kr[set][i];
     *reinterpret_cast<u32x4*>(value_stage(s) + r * S::kRowBytes + tile_value_piece<T, D>(r, c) * 16) = vr[set][i];
   };
@@ -293,7 +356,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
     else if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, lo);
 #pragma unroll
     for (int i = 0; i < S::kPieces; ++i) load_piece(i, key_at(lo), 0);
-    if (tid == 0) wild = 0;
+    if (tid == 0) wild = 0, shared.large = 0;
     __syncthreads();
     if (partly_seen(key_at(lo))) clean_values(key_at(lo), 0);
 #pragma unroll
@@ -330,21 +393,65 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
       for (int u = 0; u < S::kSubs; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) st[u][e] = 0.f;
-      auto read_keys = [&](int n) __attribute__((always_inline)) {  // the operand of the n-th matrix instruction of St
-        const int r = 32 * (n % S::kSubs) + lrow;
-        return *reinterpret_cast<const u32x4*>(kt + r * S::kRowBytes + key_piece<T, D>(r, 2 * (n / S::kSubs) + lhalf) * 16);
-      };
       // Reads run kAhead instructions before their use.  The fences keep that order: left to itself the compiler waits for each read in front of its use.
-      constexpr int kAhead = 4, kScores = S::kSubs * S::kSteps;
+      constexpr int kAhead = 4;
       u32x4 f[kAhead];
+      if constexpr (!THIRDS) {
+        auto read_keys = [&](int n) __attribute__((always_inline)) {  // the operand of the n-th matrix instruction of St
+          const int r = 32 * (n % S::kSubs) + lrow;
+          return *reinterpret_cast<const u32x4*>(kt + r * S::kRowBytes + key_piece<T, D>(r, 2 * (n / S::kSubs) + lhalf) * 16);
+        };
+        constexpr int kScores = S::kSubs * S::kSteps;
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) f[n] = read_keys(n);
+        for (int n = 0; n < kAhead; ++n) f[n] = read_keys(n);
 #pragma unroll
-      for (int n = 0; n < kScores; ++n) {
-        st[n % S::kSubs] = mma32<T>(f[n % kAhead], qf[n / S::kSubs], st[n % S::kSubs]);
-        if (n + kAhead < kScores) f[n % kAhead] = read_keys(n + kAhead);
-        if (n < S::kPieces) store_piece(n, s ^ 1, set);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int n = 0; n < kScores; ++n) {
+          st[n % S::kSubs] = mma32<T>(f[n % kAhead], qf[n / S::kSubs], st[n % S::kSubs]);
+          if (n + kAhead < kScores) f[n % kAhead] = read_keys(n + kAhead);
+          if (n < S::kPieces) store_piece(n, s ^ 1, set);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        // products of the parts, the small ones in a sum of their own (those of the smallest with each other and with the middle ones are less than what fp32 rounds)
+        floatx16 small = st[0];
+        u32x4 k[2][3];
+        auto read_keys = [&](int i, int p) __attribute__((always_inline)) {
+          return *reinterpret_cast<const u32x4*>(kt + p * kPlane + lrow * 2 * D + key_piece<bf16, D>(lrow, 2 * i + lhalf) * 16);
+        };
+#pragma unroll
+        for (int p = 0; p < 3; ++p) k[0][p] = read_keys(0, p);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          if (i + 1 < D / 16) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) k[(i + 1) % 2][p] = read_keys(i + 1, p);
+          }
+          const u32x4(&x)[3] = k[i % 2];
+          small = mma32<bf16>(x[2], qt[0][i], small);
+          st[0] = mma32<bf16>(x[1], qt[0][i], st[0]);
+          small = mma32<bf16>(x[0], qt[2][i], small);
+          st[0] = mma32<bf16>(x[0], qt[1][i], st[0]);
+          small = mma32<bf16>(x[1], qt[1][i], small);
+          st[0] = mma32<bf16>(x[0], qt[0][i], st[0]);
+          if (i < S::kPieces) store_piece(i, s ^ 1, set);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        st[0] += small;
+        // (scores of too large numbers, and no others, element by element)
+        if (__builtin_expect(__any(large_query) || shared.large, 0)) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const T* const row = keys + row_offset<D>(view, cursor, kv_head, key + 8 * (e / 4) + 4 * lhalf + e % 4);
+            float score = 0.f;
+            bool large = large_query;
+            if (live) {
+#pragma unroll 1
+              for (int d = 0; d < D; ++d) score = __builtin_fmaf(row[d], query[d], score), large = large || __builtin_fabsf(row[d]) >= kTooLarge;
+            }
+            st[0][e] = large ? score : st[0][e];
+            __builtin_amdgcn_sched_barrier(0);  // (few registers: this path is cold)
+          }
+        }
       }
 #pragma unroll
       for (int i = 0; i < S::kPieces; ++i) load_piece(i, after, set);
@@ -431,6 +538,53 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+      } else if constexpr (THIRDS) {
+        u32x4 pt[3][2];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          floatx4 p;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][4 * g + j], a.scale_log2e, -zero));
+            sum += p[j];
+          }
+          const Thirds t = thirds(__builtin_bit_cast(u32x4, p));
+#pragma unroll
+          for (int n = 0; n < 3; ++n) pt[n][g / 2][g % 2 * 2] = t.part[n][0], pt[n][g / 2][g % 2 * 2 + 1] = t.part[n][1];
+        }
+        auto read_values = [&](int n, int p) __attribute__((always_inline)) {  // kOut operands for each 16 keys
+          const int r0 = 16 * (n / S::kOut) + 4 * lhalf + ((lane >> 2) & 3), t = n % S::kOut;
+          u32x4 v;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int r = r0 + 8 * g;
+            const u32x2 half =
+                read_transposed(vt + p * kPlane + r * 2 * D + tile_value_piece<bf16, D>(r, 4 * t + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8);
+            v[2 * g] = half[0], v[2 * g + 1] = half[1];
+          }
+          return v;
+        };
+        u32x4 v[2][3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) v[0][p] = read_values(0, p);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < 2 * S::kOut; ++n) {
+          if (n + 1 < 2 * S::kOut) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) v[(n + 1) % 2][p] = read_values(n + 1, p);
+          }
+          const u32x4(&x)[3] = v[n % 2];
+          floatx16& to = ot[n % S::kOut];
+          const int g = n / S::kOut;
+          to = mma32<bf16>(x[2], pt[0][g], to);
+          to = mma32<bf16>(x[0], pt[2][g], to);
+          to = mma32<bf16>(x[1], pt[1][g], to);
+          to = mma32<bf16>(x[1], pt[0][g], to);
+          to = mma32<bf16>(x[0], pt[1][g], to);
+          to = mma32<bf16>(x[0], pt[0][g], to);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       } else {
         static_assert(sizeof(T) == 2 || S::kSubs == 1, "32 keys");
 #pragma unroll
@@ -502,11 +656,11 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
 
 template <typename T, int D, bool SMALL>
 __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
-  __shared__ TilesShared<T, D> shared;
+  __shared__ TilesShared<T, D, false> shared;
   const int kv_head = blockIdx.x % a.view.kv_heads;
   int b, block;
   if (!find_block(a, blockIdx.x / a.view.kv_heads, &b, &block)) return;
-  tiles<T, D, SMALL, false, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, blockIdx.z, shared);
+  tiles<T, D, SMALL, false, false, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, blockIdx.z, shared);
 }
 
 }  // namespace
