@@ -82,19 +82,22 @@ struct Cut {
   int64_t parts;
   double us;
 };
+double rounds_of(double groups, bool single) {
+  const double cus = compute_units(), rounds = std::floor(groups / (2 * cus)), rest = groups - rounds * 2 * cus;
+  return rounds + (rest <= 0 ? 0 : rest <= cus && !single ? 0.55 : 1);
+}
 Cut best_cut(double blocks, int64_t steps, double step, bool single, int64_t tokens, int64_t heads, int64_t head_dim) {
-  const double cus = compute_units(), join = (double)tokens * heads * (head_dim + 2) * 8 / 4.5e6;
+  const double join = (double)tokens * heads * (head_dim + 2) * 8 / (single ? 9e6 : 4.5e6);
   Cut best = {1, 1e30};
   for (int64_t parts = 1; parts <= 64 && parts <= steps; ++parts) {
-    const double groups = blocks * parts, rounds = std::floor(groups / (2 * cus)), rest = groups - rounds * 2 * cus;
-    const double us = (rounds + (rest <= 0 ? 0 : rest <= cus && !single ? 0.55 : 1)) * (double)ceil_div(steps, parts) * step + parts * join;
+    const double us = rounds_of(blocks * parts, single) * (double)ceil_div(steps, parts) * step + parts * join;
     if (us < best.us) best = {parts, us};
   }
   return best;
 }
 // us a step where two workgroups are on a CU: bound by products, or (single tokens, few of whose rows are alive) by the wait for keys
 double step_us(int dtype, int64_t head_dim, bool single) {
-  if (dtype == TTMI_F32) return head_dim == 128 ? 27 : single ? 11 : 8;
+  if (dtype == TTMI_F32) return head_dim == 128 ? (single ? 20 : 27) : single ? 8 : 5.5;
   return head_dim == 128 ? (single ? 4 : 2.3) : (single ? 2.2 : 1.35);
 }
 bool single_tokens(const PagedView& view, int64_t heads) { return view.tokens * (heads / view.kv_heads) <= kFewRows * (int64_t)view.batch; }
@@ -121,10 +124,13 @@ struct SightPlan {
   int shares, family_splits, family_least, family_few, own_blocks;
   int64_t few_rows, own_rows, family_rows, whole_rows, floats;  // of the workspace
 };
+PagedPlan plan_own(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, const ttmi_paged_sight& sight, int dtype) {
+  const int64_t sinks = std::min(sight.sinks, kWidest), window = sight.window > 0 ? std::min(std::min(sight.window, kWidest) + sinks + 128, kWidest) : 0;
+  return plan(view, heads, max_tokens, max_length, window, dtype);
+}
 SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, const ttmi_paged_sight& sight, int dtype) {
   SightPlan p;
-  const int64_t sinks = std::min(sight.sinks, kWidest), window = sight.window > 0 ? std::min(std::min(sight.window, kWidest) + sinks + 128, kWidest) : 0;
-  p.own = plan(view, heads, max_tokens, max_length, window, dtype);
+  p.own = plan_own(view, heads, max_tokens, max_length, sight, dtype);
   const int64_t group = heads / view.kv_heads, tokens = view.tokens, d = view.head_dim;
   p.own_blocks = p.own.tiles ? (int)(tokens * group / 128 + std::min<int64_t>(view.batch, tokens)) : 0;
   p.shares = p.family_splits = p.family_least = p.family_few = 0, p.family_rows = p.whole_rows = 0;
@@ -152,25 +158,40 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
 }
 
 // Whether reading a family's keys once is worth it: a second launch, which joins what they give with what the sequences' own keys do, and blocks of 128 rows that may be mostly empty, for reads
-// that the caches would take most of.  us, families / none, one token each and 50 keys of its own, behind 1000, 2000, 4000, 8000 keys (where both are level the answer is no):
-//   bf16, 32 and 8 heads of 128: 8 sequences 15.8 / 15.4, 17.4 / 17.2, 22.4 / 21.5, 27.4 / 30.3; 64 28.7 / 28.7, 30.0 / 46.4, 29.7 / 79.8, 40.7 / 147; 256 63.8 / 96.7 .. 95.3 / 572;
-//                                8 families of 2 17.7 / 17.6 .. 54.7 / 53.8; 4 of 8 21.4 / 21.5, 26.6 / 31.3, 30.2 / 49.7, 40.8 / 82.9; 16 of 4 29.7 / 29.3, 37.9 / 47.9, 55.5 / 90.6, 115 / 181
-//   fp16, 12 heads of 64:        16 sequences 9.2 / 8.9, 15.2 / 18.7, 16.0 / 25.5, 19.3 / 39.2; 16 families of 4 20.7 / 20.5, 32.6 / 41.8, 45.6 / 67.8, 84.0 / 141
-//   fp32, the same heads:        4 sequences 13.3 / 13.0, 15.8 / 15.7, 16.6 / 22.2, 22.1 / 28.9; 64 27.7 / 47.5 .. 48.1 / 264; 32 and 8 heads of 128, 64: 54.2 / 53.9, 62.5 / 93.6 .. 141 / 321
+// that the caches would take most of.  Both are estimated, with what fits the measured; us, families / none, one token each and 50 keys of its own, behind 1000, 2000, 4000, 8000 keys (where both are
+// level the answer is no):
+//   bf16, 32 and 8 heads of 128: 8 sequences 15.3 / 14.7, 17.0 / 17.9, 20.9 / 21.9, 26.2 / 30.1; 64 27.9 / 28.7, 30.4 / 48.0, 30.5 / 80.8, 41.8 / 148; 256 63.0 / 96.9 .. 95.6 / 573;
+//                                8 families of 2 17.6 / 17.9 .. 54.8 / 54.2; 4 of 8 22.4 / 21.5, 26.9 / 31.1, 30.4 / 49.8, 40.1 / 83.3; 16 of 4 31.5 / 29.3, 38.4 / 48.8, 55.6 / 90.3, 115 / 181
+//   fp16, 12 heads of 64:        16 sequences 9.6 / 9.3, 15.5 / 19.1, 15.4 / 24.8, 20.4 / 39.0; 16 families of 4 21.0 / 20.7, 32.7 / 41.9, 46.2 / 68.7, 84.3 / 140
+//   fp32, the same heads:        4 sequences 15.9 / 13.4, 16.2 / 16.8, 16.7 / 21.3, 22.6 / 28.7; 64 28.8 / 48.0 .. 49.5 / 268; 32 and 8 heads of 128, 64: 54.8 / 54.4, 64.3 / 95.3 .. 142 / 321
+// and of more tokens: 4 sequences of up to 12, 24 and 12 heads of 64, fp32, behind 1400 keys 20.8 / 44.6; 9 of 5 to 9, 32 and 4 heads of 128, fp32, behind up to 4200 120 / 144; 8 of up to 69, 6 and 2 heads of
+// 128, bf16, behind 7500 56 / 43 (no).  Over 128 random batches what it takes is 1.6 % slower on average than the better of the two; none alone 20 %.
 // Where nothing is known they are taken as they come.
-bool sharing_pays(const PagedView& view, int64_t heads, const ttmi_paged_sight& sight, int dtype) {
+bool sharing_pays(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, const ttmi_paged_sight& sight, int dtype) {
   if (sight.families == nullptr) return false;
   if (sight.family_count == 0 || sight.max_shared == 0) return true;
-  const FamilyGuess guess = guess_families(view, heads, sight);
+  FamilyGuess guess = guess_families(view, heads, sight);
+  if (sight.window > 0) guess.steps = std::min(guess.steps, ceil_div(std::min(sight.window, kWidest) + std::min(sight.sinks, kWidest), 64) + 1);  // (seen of the common keys)
+  const PagedPlan own = plan_own(view, heads, max_tokens, max_length, sight, dtype);
   const bool f32 = dtype == TTMI_F32, wide = view.head_dim == 128, single = single_tokens(view, heads);
-  const double step = step_us(dtype, view.head_dim, single), rows = (double)view.tokens * (double)(heads / view.kv_heads);
-  const auto tiles = [&](double blocks) { return best_cut(blocks * view.kv_heads, guess.steps, step, single, view.tokens, heads, view.head_dim).us; };
-  const double bytes = guess.steps * 64.0 * (2 * view.kv_heads * view.head_dim * (double)dtype_size(dtype)), reads = view.batch * bytes / (f32 ? 11e6 : 13e6);
+  const double step = step_us(dtype, view.head_dim, single), rows = (double)view.tokens * (double)(heads / view.kv_heads), batch = view.batch;
+  const double bytes = guess.steps * 64.0 * (2 * view.kv_heads * view.head_dim * (double)dtype_size(dtype));
+  // each by itself: the common keys again and again, out of the caches, and a launch that joins, or (many rows) the walk over a part of them
+  double alone = (own.few && own.few_splits == 0 ? 7 : f32 ? 14 : 12) + batch * bytes / (f32 ? 12.5e6 : 14e6);
+  if (single && own.tiles) alone += 5;
+  if (!single) {
+    // (half a block of each sequence is empty, and each has one)
+    const double groups = std::max(rows / 128 + batch / 2, batch) * (double)view.kv_heads * own.tile_splits, steps = (double)ceil_div(std::min<int64_t>(own.tile_chunk, guess.steps * 64), 64);
+    alone = std::max(alone, 7 + rounds_of(groups, false) * steps * step);
+  }
+  if (alone <= 11) return false;  // (what a second launch and the rest of it take at least)
+  // shared: as many bytes as families read, or blocks of their rows over parts of the keys
   const double count = (double)std::min<int64_t>(sight.family_count, std::max(1, view.batch / 2)), most = std::ceil(rows / count);
-  const double shared = single && most <= family_few_rows(dtype) ? (wide && !f32 ? 12 : 10) + (f32 ? 0.15 : 0.1) * view.batch + count * std::ceil(most / kFewRows) * bytes / 5.3e6
-                                                                 : (f32 ? (wide ? 30 : 12) : (wide ? 12 : 10)) + (f32 ? 0.15 : 0.1) * view.batch + tiles(guess.blocks);
-  // (sequences with many rows have blocks of their own, half a one empty each)
-  return shared < 7 + (single ? reads : std::max(reads, tiles(rows / 128 + view.batch / 2.0)));
+  double shared;
+  if (single && most <= family_few_rows(dtype)) shared = (f32 ? (wide ? 16 : 14.5) : 13) + 0.05 * batch + count * std::ceil(most / kFewRows) * bytes / 6e6;
+  else shared = (f32 ? (wide ? 22 : 12) : (wide ? 12 : 11)) + (f32 ? 0.15 : 0.1) * batch + (!single && own.few ? 8 : 0) +
+                best_cut(guess.blocks * (double)view.kv_heads, guess.steps, step, single, view.tokens, heads, view.head_dim).us;
+  return shared < alone;
 }
 
 int check_sight(const ttmi_paged_sight* sight) {
@@ -256,7 +277,7 @@ int ttmi_paged_attention_sight_workspace(const ttmi_paged_cache* cache, const tt
   TTMI_REQUIRE(bytes != nullptr, "bytes is null");
   if (int rc = paged_view(cache, batch, heads, &view)) return rc;
   ttmi_paged_sight used = *sight;
-  if (!sharing_pays(view, heads, used, dtype)) used.families = nullptr;
+  if (!sharing_pays(view, heads, max_tokens, max_length, used, dtype)) used.families = nullptr;
   if (used.families == nullptr && (used.sinks == 0 || used.window == 0))
     return ttmi_paged_attention_workspace(cache, batch, heads, max_tokens, max_length, used.window, dtype, bytes);
   TTMI_REQUIRE(max_tokens >= 0 && max_length >= 0, "max_tokens and max_length must not be negative");
@@ -273,7 +294,7 @@ int ttmi_paged_attention_sight(const void* q, int64_t q_pitch, void* out, int64_
   if (int rc = attention_args(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, sight->window, dtype, &a)) return rc;
   if (batch->tokens == 0 || batch->batch == 0) return 0;
   ttmi_paged_sight used = *sight;
-  if (!sharing_pays(a.view, heads, used, dtype)) used.families = nullptr;
+  if (!sharing_pays(a.view, heads, max_tokens, max_length, used, dtype)) used.families = nullptr;
   if (used.families == nullptr && (used.sinks == 0 || used.window == 0))
     return ttmi_paged_attention(q, q_pitch, out, out_pitch, heads, cache, batch, max_tokens, max_length, scale, causal, used.window, workspace, workspace_bytes,
                                 dtype, stream);
