@@ -185,6 +185,19 @@ def test_keys_near_the_largest_in_common(d):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [3.4e38, math.inf, 0.0])
+def test_what_lies_behind_the_last_key_and_under_the_gap(d, bad):
+    """Slots that no token sees may hold anything (NaN otherwise, here); the bits are the same."""
+    case = Sight("f32", [140, 30, 2], [400, 90, 37], 4, 2, d, 16)
+    outs = []
+    for fill in (math.nan, bad):
+        case.keys, case.values = (torch.where(torch.isnan(x), torch.full_like(x, fill), x) for x in (case.keys, case.values))
+        case.keys[case.table[0, 10:20]], case.values[case.table[0, 10:20]] = fill, fill  # (positions 160 to 319; the first new token's window begins at 351)
+        outs.append(case.run_attention(window=50, sinks=7).cpu()[:172])
+    assert torch.equal(outs[0], outs[1]) and torch.isfinite(outs[0]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_scores_of_minus_infinity(d):
     """A key with a score of minus infinity weighs nothing, whether it comes from an infinity or from numbers near it: the bits are those of a score that is merely low."""
     case = Sight("f32", [140, 30], [0, 90], 4, 2, d, 16)

@@ -344,7 +344,9 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
 #pragma unroll
     for (int i = 0; i < S::kPieces; ++i) {
       const int k = key + (i * 4096 + tid * 16) / S::kRowBytes;
-      if (!some_see<SIGHT>(sight, k)) vr[set][i] = u32x4{0u, 0u, 0u, 0u};
+      const bool seen = some_see<SIGHT>(sight, k);
+      if (!seen) vr[set][i] = u32x4{0u, 0u, 0u, 0u};
+      if (THIRDS && !seen) kr[set][i] = u32x4{0u, 0u, 0u, 0u};  // (or one that is too large would have its tile's scores looked at one by one)
       if (not_finite<T>(vr[set][i])) wild = 1;
       vr[set][i] = finite_part<T>(vr[set][i]);
     }
