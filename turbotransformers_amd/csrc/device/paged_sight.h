@@ -254,28 +254,32 @@ __global__ __launch_bounds__(256, (D == 128 && kThirds<T, D, FAMILIES, FEW> ? 1 
   }
 }
 
-// A wavefront a row and head.
-template <typename T, int D>
+// A wavefront a row and head, or (MANY) several heads.
+template <typename T, int D, bool MANY>
 __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
   const PagedView& view = a.view;
-  const int row = blockIdx.x, head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (head >= a.heads) return;
+  const int row = blockIdx.x, first_head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (first_head >= a.heads) return;
   ShareNote note{};
   if (a.families != nullptr) note = *share_note<D>(a);
   // the row's sequence: the first that ends behind it
   const int lane = (int)(threadIdx.x % kWave);
   LaneSequences lanes;
-  int b = -1;
+  int b = 0;
   int64_t before = 0;
-  for (int base = 0; base < view.batch; base += kWave) {
-    if (a.families != nullptr && a.run_few && a.few_splits > 0) before = units_before<D>(a)[min(base + lane, view.batch - 1)];
-    lanes = lane_sequences(a, base);
-    const int ended = __popcll(__ballot(base + lane < view.batch && lanes.ends <= row));
-    if (ended == kWave) continue;
-    b = base + ended;
-    break;
-  }
-  if (b < 0 || b >= view.batch) return;
+  // (among the last 64 of which the first begins up to it: two trips to memory.  256 sequences, one token each, 32 heads of 128: 15.4 us for one after the other, 13.0 so, 11.6 with more heads a wavefront.)
+  int base = 0;
+  if (view.batch > kWave)
+    for (int from = 0; from < view.batch; from += kWave * kWave) {
+      const int at = from + lane * kWave;
+      const int begun = __popcll(__ballot(at < view.batch && view.starts[min(at, view.batch - 1)] <= row));
+      if (begun == 0) break;
+      base = from + (begun - 1) * kWave;
+    }
+  if (a.families != nullptr && a.run_few && a.few_splits > 0) before = units_before<D>(a)[min(base + lane, view.batch - 1)];
+  lanes = lane_sequences(a, base);
+  b = base + __popcll(__ballot(base + lane < view.batch && lanes.ends <= row));
+  if (b >= min(view.batch, base + kWave)) return;
   const Sequence seq = lanes.sequence(b - lanes.base);
   const int64_t before_all = before;
   // (the family that it leads comes first)
@@ -285,101 +289,111 @@ __global__ __launch_bounds__(256) void join_sight_kernel(const PagedArgs a) {
     before += (int64_t)__builtin_amdgcn_readlane(blocks * family_rounds_of(lanes, blocks), b - lanes.base) * view.kv_heads;
   }
   if (row < seq.start || row >= seq.start + seq.tokens) return;
-  const int kv_head = head / a.group, r = (row - seq.start) * a.group + head % a.group, rows = seq.tokens * a.group;
-  const int64_t at = (int64_t)row * a.heads + head;
-  // parts of what it has in common with its family, and of its own: where the first is, and how far the others lie apart behind the second
-  int of_family = 0;
-  int64_t family_place = 0, family_second = 0, family_step = 0;
+  // its family's parts: how many, or where they begin
+  const int rows = seq.tokens * a.group;
+  int family_parts_all = 0, family_start = 0;
+  int64_t family_before = 0;
   if (seq.base > 0) {
     const int leader = __builtin_amdgcn_readlane(lanes.leader, b - lanes.base);
     LaneSequences theirs = lanes;
     if (leader < lanes.base) theirs = lane_sequences(a, leader & ~(kWave - 1));
-    const int blocks = __builtin_amdgcn_readlane(family_blocks(a, theirs).few, leader - theirs.base);
-    of_family = 1, family_place = a.family_at + at * a.family_splits;
-    if (blocks == 0) {  // (as many parts as there are chunks, which are equal but for the last)
+    if (__builtin_amdgcn_readlane(family_blocks(a, theirs).few, leader - theirs.base) == 0) {  // (as many parts as there are chunks, which are equal but for the last)
       const int steps = seq.base / 64, most = family_parts(steps, note.steps), chunk = (steps + most - 1) / most;
-      of_family = (steps + chunk - 1) / chunk, family_second = family_place + 1, family_step = 1;
+      family_parts_all = (steps + chunk - 1) / chunk;
     } else {
-      const int of_rows = (row - __builtin_amdgcn_readlane(theirs.start, leader - theirs.base)) * a.group + head % a.group, block = of_rows / kFewRows;
-      const int rounds = kStart + seq.base / kRound;
-      const int64_t unit = (leader < lanes.base ? units_before<D>(a)[leader] : lane_of(before_all, leader - lanes.base)) + (int64_t)(block * view.kv_heads + kv_head) * rounds;
-      const Sharers shared = sharers_of(unit, rounds, note.units, sharers(view.page_shift >= 4 ? note.few_groups : a.few_splits, note.units));
-      if (shared.last > shared.first) {
-        of_family = (int)(shared.last - shared.first) + 1;
-        family_place = (2 * shared.first + 1) * kFewRows + of_rows % kFewRows;
-        family_second = 2 * (shared.first + 1) * kFewRows + of_rows % kFewRows, family_step = 2 * kFewRows;
+      family_start = __builtin_amdgcn_readlane(theirs.start, leader - theirs.base);
+      family_before = leader < lanes.base ? units_before<D>(a)[leader] : lane_of(before_all, leader - lanes.base);
+    }
+  }
+  const bool by_tiles = !a.run_few || (rows > kFewRows && !a.few_every), sees = seq.reach(a, row - seq.start).end > 0;
+  if (!by_tiles && a.families == nullptr) return;
+  const int rounds = !by_tiles && a.few_splits > 0 ? rounds_of<true>(a, seq) : 0;
+  const int64_t workgroups = a.families != nullptr ? sharers(view.page_shift >= 4 ? note.few_groups : a.few_splits, note.units) : 0;
+  const float* const ml = a.partial + a.rows * D;
+  for (int head = first_head; head < (MANY ? a.heads : first_head + 1); head += MANY ? 4 * gridDim.y : 1) {
+    const int kv_head = head / a.group, r = (row - seq.start) * a.group + head % a.group;
+    const int64_t at = (int64_t)row * a.heads + head;
+    // parts of what it has in common with its family, and of its own: where the first is, and how far the others lie apart behind the second
+    int of_family = 0;
+    int64_t family_place = a.family_at + at * a.family_splits, family_second = family_place + 1, family_step = 1;
+    if (seq.base > 0) {
+      of_family = max(1, family_parts_all);
+      if (family_parts_all == 0) {
+        const int of_rows = (row - family_start) * a.group + head % a.group, block = of_rows / kFewRows, family_rounds = kStart + seq.base / kRound;
+        const Sharers shared = sharers_of(family_before + (int64_t)(block * view.kv_heads + kv_head) * family_rounds, family_rounds, note.units, workgroups);
+        if (shared.last > shared.first) {
+          of_family = (int)(shared.last - shared.first) + 1;
+          family_place = (2 * shared.first + 1) * kFewRows + of_rows % kFewRows;
+          family_second = 2 * (shared.first + 1) * kFewRows + of_rows % kFewRows, family_step = 2 * kFewRows;
+        }
       }
     }
-  }
-  int parts = 1;                    // of the sequence's own keys
-  int64_t place = a.whole_at + at;  // of them, and how far they lie apart
-  int64_t second = 0, step = 0;
-  if (!a.run_few || (rows > kFewRows && !a.few_every)) {
-    const Reach mine = seq.own_reach(a, row - seq.start);
-    const int row0 = r / kTileRows * kTileRows, last = min(rows, row0 + kTileRows) - 1;
-    const Span span = span_of<kSpanTiles<T>>(sight_of(seq.own_reach(a, row0 / a.group), seq.own_reach(a, last / a.group)), seq.base);
-    parts = own_parts(mine, span, seq.base, seq.span_chunk(a));
-    place = a.own_at + at * a.splits, second = place + 1, step = 1;
-  } else if (a.families == nullptr) {
-    return;
-  } else if (a.few_splits > 0) {
-    const int rounds = rounds_of<true>(a, seq);
-    const Sharers shared = sharers_of(before + (int64_t)rounds * kv_head, rounds, note.units, sharers(view.page_shift >= 4 ? note.few_groups : a.few_splits, note.units));
-    if (shared.last > shared.first) {
-      parts = (int)(shared.last - shared.first) + 1;
-      place = (2 * shared.first + 1) * kFewRows + r, second = 2 * (shared.first + 1) * kFewRows + r, step = 2 * kFewRows;
+    int parts = 1;                    // of the sequence's own keys
+    int64_t place = a.whole_at + at;  // of them, and how far they lie apart
+    int64_t second = 0, step = 0;
+    if (by_tiles) {
+      const Reach mine = seq.own_reach(a, row - seq.start);
+      const int row0 = r / kTileRows * kTileRows, last = min(rows, row0 + kTileRows) - 1;
+      const Span span = span_of<kSpanTiles<T>>(sight_of(seq.own_reach(a, row0 / a.group), seq.own_reach(a, last / a.group)), seq.base);
+      parts = own_parts(mine, span, seq.base, seq.span_chunk(a));
+      place = a.own_at + at * a.splits, second = place + 1, step = 1;
+    } else if (a.few_splits > 0) {
+      const Sharers shared = sharers_of(before + (int64_t)rounds * kv_head, rounds, note.units, workgroups);
+      if (shared.last > shared.first) {
+        parts = (int)(shared.last - shared.first) + 1;
+        place = (2 * shared.first + 1) * kFewRows + r, second = 2 * (shared.first + 1) * kFewRows + r, step = 2 * kFewRows;
+      }
+    }
+    if (of_family == 0 && parts == 1) continue;  // (there already)
+    const int all = of_family + parts;
+    T* const out = static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)head * D;
+    auto place_of = [&](int p) {
+      const int own = p - of_family;
+      if (own < 0) return p == 0 ? family_place : family_second + (p - 1) * family_step;
+      return own == 0 ? place : second + (own - 1) * step;
+    };
+    if (all > kWave) {
+      join_parts_by_wavefront<T, D>(a.partial, ml, all, sees, place_of, out);
+      continue;
+    }
+    // up to 64 parts: each lane has what one weighs, and the sums, four columns a lane and a few parts at a time, are asked for without waiting for that
+    constexpr int kThreads = D / 4, kBeside = kWave / kThreads, kAsked = 8;
+    const int d0 = lane % kThreads * 4, share = lane / kThreads;
+    const int64_t mine = place_of(min(lane, all - 1));
+    const floatx2 met = *reinterpret_cast<const floatx2*>(ml + 2 * mine);
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    float weight = 0.f, total = 0.f;
+    for (int first = 0; first < all; first += kAsked * kBeside) {
+      floatx4 x[kAsked];
+#pragma unroll
+      for (int i = 0; i < kAsked; ++i) {
+        const int p = min(first + i * kBeside + share, all - 1);
+        x[i] = *reinterpret_cast<const floatx4*>(a.partial + place_of(p) * D + d0);
+      }
+      if (first == 0) {
+        const float best = group_max<kWave>(lane < all ? met[0] : -INFINITY);
+        weight = lane < all ? __builtin_amdgcn_exp2f(met[0] - (best == -INFINITY ? 0.f : best)) : 0.f;
+        total = group_sum<kWave>(lane < all ? met[1] * weight : 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < kAsked; ++i) {
+        const int p = first + i * kBeside + share;
+        const float w = __shfl(weight, min(p, kWave - 1), kWave);
+        if (p < all) sum += x[i] * w;
+      }
+    }
+#pragma unroll
+    for (int d = kThreads; d < kWave; d *= 2)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], d, kWave);
+    if (share == 0) {
+      const float inv = inverse_sum(total, sees);
+      Vec<T, 4> y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) y.v[c] = from_float<T>(sum[c] * inv);
+      store_vec<T, 4>(out + d0, y);
     }
   }
-  if (of_family == 0 && parts == 1) return;  // (there already)
-  const int all = of_family + parts;
-  const bool sees = seq.reach(a, row - seq.start).end > 0;
-  T* const out = static_cast<T*>(a.out) + (int64_t)row * a.out_pitch + (int64_t)head * D;
-  const float* const ml = a.partial + a.rows * D;
-  auto place_of = [&](int p) {
-    const int own = p - of_family;
-    if (own < 0) return p == 0 ? family_place : family_second + (p - 1) * family_step;
-    return own == 0 ? place : second + (own - 1) * step;
-  };
-  if (all > kWave) {
-    join_parts_by_wavefront<T, D>(a.partial, ml, all, sees, place_of, out);
-    return;
-  }
-  // up to 64 parts: each lane has what one weighs, and the sums, four columns a lane and a few parts at a time, are asked for without waiting for that
-  constexpr int kThreads = D / 4, kBeside = kWave / kThreads, kAsked = 8;
-  const int d0 = lane % kThreads * 4, share = lane / kThreads;
-  const int64_t mine = place_of(min(lane, all - 1));
-  const floatx2 met = *reinterpret_cast<const floatx2*>(ml + 2 * mine);
-  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-  float weight = 0.f, total = 0.f;
-  for (int first = 0; first < all; first += kAsked * kBeside) {
-    floatx4 x[kAsked];
-#pragma unroll
-    for (int i = 0; i < kAsked; ++i) {
-      const int p = min(first + i * kBeside + share, all - 1);
-      x[i] = *reinterpret_cast<const floatx4*>(a.partial + place_of(p) * D + d0);
-    }
-    if (first == 0) {
-      const float best = group_max<kWave>(lane < all ? met[0] : -INFINITY);
-      weight = lane < all ? __builtin_amdgcn_exp2f(met[0] - (best == -INFINITY ? 0.f : best)) : 0.f;
-      total = group_sum<kWave>(lane < all ? met[1] * weight : 0.f);
-    }
-#pragma unroll
-    for (int i = 0; i < kAsked; ++i) {
-      const int p = first + i * kBeside + share;
-      const float w = __shfl(weight, min(p, kWave - 1), kWave);
-      if (p < all) sum += x[i] * w;
-    }
-  }
-#pragma unroll
-  for (int d = kThreads; d < kWave; d *= 2)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], d, kWave);
-  if (share != 0) return;
-  const float inv = inverse_sum(total, sees);
-  Vec<T, 4> y;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) y.v[c] = from_float<T>(sum[c] * inv);
-  store_vec<T, 4>(out + d0, y);
 }
 
 template <typename T>
@@ -405,8 +419,13 @@ void start_sight(const SightLaunch& l, int64_t head_dim, hipStream_t stream) {
       if (a.run_few && shares > 0) start_few_rows<T, kFamilies>(l.few, head_dim, stream);
       else if (a.run_few) start_few_rows<T, kSinks>(l.few, head_dim, stream);
     }
-    if (a.families != nullptr || (l.run_tiles && a.splits > 1))
-      hipLaunchKernelGGL((join_sight_kernel<T, D>), dim3(a.view.tokens, (unsigned)ceil_div(a.heads, 4)), dim3(256), 0, stream, a);
+    // (as many heads a wavefront as leave four workgroups a CU: each finds out first what its row's sequence is)
+    const int64_t fours = ceil_div(a.heads, 4), per = std::max<int64_t>(1, std::min<int64_t>(fours, (int64_t)a.view.tokens * fours / (4 * compute_units())));
+    auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.view.tokens, (unsigned)ceil_div(fours, per)), dim3(256), 0, stream, a); };
+    if (a.families != nullptr || (l.run_tiles && a.splits > 1)) {
+      if (per > 1) join(join_sight_kernel<T, D, true>);
+      else join(join_sight_kernel<T, D, false>);
+    }
   };
   if (head_dim == 64) sized(std::integral_constant<int, 64>{});
   else sized(std::integral_constant<int, 128>{});
