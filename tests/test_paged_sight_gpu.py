@@ -297,6 +297,19 @@ def test_common_keys_end_where_the_first_sequence_does(dt):
     case.check_attention(case.run_attention(families=[[0, 3, 640]] * 3))
 
 
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads", [(20, 4), (32, 8)])
+def test_many_rows_of_many_heads_are_joined(dt, heads, kv_heads):
+    """280 sequences, so many rows and heads that a wavefront joins several of them; families of 2 to 70, over the bounds of 64 sequences, some sequences with chunks."""
+    rng = random.Random(7)
+    families, left = [], 280
+    while left:
+        members = min(left, rng.choice([1, 2, 3, 9, 40, 70]))
+        families.append((members, rng.choice([128, 144]) if members > 1 else 0))
+        left -= members
+    check(dt, [rng.choice([1, 1, 1, 1, 7]) for _ in range(280)], [rng.randint(144, 160) for _ in range(280)], heads, kv_heads, 64, 16, families=families)
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("batch", [63, 64, 65, 200, 300])
 def test_many_families(dt, batch):
