@@ -645,9 +645,9 @@ TTMI_API int ttmi_paged_attention(const void* q, int64_t q_pitch, void* out, int
  *                   window 0: all of them (sinks says nothing then)
  *   families        DEVICE int32 [batch, 3], or null.  Sequences that begin with the same keys in the same pages may be a family: they follow one another in the
  *                   batch, and the row of each is (number of the first of them, number behind the last, keys they have in common).  Those keys
- *                   are read once for all of them, where the first one's row of the table says.  A sequence whose row does not agree with that of
- *                   the first it names, or whose row says 0 keys, is on its own.  Keys are shared in steps of 128.  The result is that without families but for
- *                   roundings.
+ *                   are read once for all of them, where the first one's row of the table says.  A sequence whose row is not, number by number, that of
+ *                   the first it names, or whose row says 0 keys, is on its own and reads its own pages.  Keys are shared in steps of 128.  The result is that
+ *                   without families but for roundings.
  *   family_count, max_shared   how many families there are and the most keys of one, or 0 if unknown: hints like max_tokens.  Where they say that
  *                   there is nothing to gain, each sequence reads its keys itself. */
 typedef struct ttmi_paged_sight {

@@ -290,6 +290,87 @@ def test_rows_of_families_that_disagree_are_sequences_on_their_own():
     tt.cxx.synchronize()
 
 
+class Apart(Sight):
+    """A family of the sequences `first` to `end`, all behind the same `keys` tokens but for those of `others`, {sequence: (its row, tokens that it has in common)}.  What
+    would have been the pages of common tokens holds NaN."""
+
+    def __init__(self, dt, new, past, heads, kv_heads, d, page, first, end, keys, others, **kw):
+        super().__init__(dt, new, past, heads, kv_heads, d, page, **kw)
+        for b in range(first, end):
+            row, common = others.get(b, ((first, end, keys), keys))
+            n = common // page if b > first else 0
+            own = self.table[b, :n].tolist()
+            self.keys[own], self.values[own] = math.nan, math.nan
+            self.table[b, :n] = self.table[first, :n]
+            self.rows[b] = row
+        self.families = True
+
+
+ROWS_THAT_DIFFER = [((0, 6, 0), 0), ((0, 6, 128), 128), ((0, 6, 128), 0), ((0, 6, 256), 128), ((0, 6, 511), 0), ((0, 6, 640), 0), ((0, 6, -512), 0), ((0, 5, 512), 0),
+                    ((0, 7, 512), 256), ((0, 2, 512), 0), ((0, 1 << 30, 512), 0), ((1, 6, 512), 0)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("new", [[1] * 6, [1, 20, 130, 1, 1, 5]])
+@pytest.mark.parametrize("heads,page", [(4, 16), (8, 16), (8, 4)])
+def test_a_sequence_whose_row_differs_from_the_firsts_reads_its_own_pages(dt, new, heads, page):
+    """Sequences that name the first of a family and say another end or another number of keys, none among them, hold other pages: each its own tokens' attention, in the
+    kernels for few and for many rows, in the middle of a family's rows and at their end."""
+    for row, common in ROWS_THAT_DIFFER:
+        for window, sinks in ((0, 0), (300, 140)):
+            case = Apart(dt, new, [600, 530, 700, 512, 650, 590], heads, 2, 64, page, 0, 6, 512, {2: (row, common), 5: (row, common)})
+            case.check_attention(case.run_attention(window=window, sinks=sinks), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("batch", [80, 300])
+@pytest.mark.parametrize("chunks", [False, True])
+def test_rows_that_differ_across_the_bounds_of_64_sequences(dt, batch, chunks):
+    """A family whose first sequence is among other 64 than some that name it, with and without a row like its."""
+    first, end = batch - 25, batch
+    others = {b: ((first, end, says), 0) for b, says in ((first + 2, 0), (first + 3, 256), (end - 6, 0), (end - 5, 256), (end - 1, 0))}
+    new = [3 if chunks and b % 5 == 0 else 1 for b in range(batch)]
+    case = Apart(dt, new, [3] * first + [130 + b % 3 for b in range(25)], 32, 2, 64, 16, first, end, 128, others)
+    case.check_attention(case.run_attention())
+    case = Apart(dt, new, [3] * 60 + [130 + b % 3 for b in range(20)] + [3] * (batch - 80), 32, 2, 64, 16, 60, 80, 128,
+                 {b: ((60, 80, says), 0) for b, says in ((62, 0), (65, 256), (70, 0), (79, 64))})
+    case.check_attention(case.run_attention())
+
+
+def test_a_sequence_leaves_its_family_between_replays():
+    """A recorded step whose second sequence is switched off in the tensor of families, gets another text's pages, and comes back."""
+    case = Sight("bf16", [1, 1, 1], [700, 690, 650], 8, 2, 64, 16, families=[(3, 640)])
+    other = Case("bf16", [1], [690], 8, 2, 64, 16, seed=5)
+    pages = case.keys.shape[0]
+    keys, values = torch.cat((case.keys, other.keys)).nan_to_num().cuda(), torch.cat((case.values, other.values)).nan_to_num().cuda()
+    table, starts, lengths = case.device_args()
+    table.clamp_(0, pages - 1)
+    rows = torch.from_numpy(case.rows).cuda()
+    q = case.q.cuda()
+    call = lambda: tt.paged_attention(q, keys, values, table, starts, lengths, max_tokens=1, max_length=701, families=rows)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    kept = table[1].clone()
+    other.q = case.q[1:2]
+    for away in (False, True, True, False):
+        table[1] = kept
+        rows[1, 2] = 0 if away else 640
+        if away:
+            table[1, :44] = torch.from_numpy(other.table[0, :44]).cuda() + pages
+        graph.replay()
+        torch.randn(1 << 16, device="cuda").sum()
+        torch.cuda.synchronize()
+        want, tol = case.attention()
+        if away:
+            want[1:2], tol[1:2] = other.attention()
+        assert ((out.cpu().double() - want).abs() <= tol).all(), away
+        out.fill_(math.nan)
+    tt.cxx.synchronize()
+
+
 @pytest.mark.parametrize("dt", ["f16", "f32"])
 def test_common_keys_end_where_the_first_sequence_does(dt):
     """A row that promises more keys than the first sequence of the family has: what it has not is each sequence's own."""

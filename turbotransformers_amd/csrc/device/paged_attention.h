@@ -144,19 +144,18 @@ __device__ __forceinline__ int sum_up_to_here(int v) {
 }
 __device__ __forceinline__ int sum_of_lanes(int v) { return __builtin_amdgcn_readlane(sum_up_to_here(v), kWave - 1); }
 
-// A family: sequences that follow one another and begin with the same keys.  What the rows of `families` say counts where the first sequence of a family and
-// another one agree on it, so that no key is left out or read twice whatever they hold.
+// A family: sequences that follow one another and begin with the same keys.  A sequence is of a family where its row of `families` is, number by number, that of the first sequence that it
+// names: any other is on its own, whatever either says, so that no key is left out, read twice or taken from another text.  Decided in lane_sequences and, for rows of sequences that are
+// not among the 64 at hand, in family_reach.
 struct Family {
   int first, end, keys;  // sequences; keys in common, a multiple of kShareStep, 0: no family
 };
-__device__ __forceinline__ Family family_led_by(const PagedArgs& a, int b) {
+// Keys that a sequence whose row is `row` has in common with the first one that it names, which is before the 64 at hand.
+__device__ __forceinline__ int keys_in_common(const PagedArgs& a, const int (&row)[3]) {
   const PagedView& view = a.view;
-  const int32_t* const row = a.families + 3 * (int64_t)b;
-  Family f;
-  f.first = b, f.end = min(row[1], view.batch);
-  const int held = (int)min((int64_t)view.lengths[b], view.table_pitch << view.page_shift);
-  f.keys = row[0] == b && f.end > b + 1 ? max(0, min(row[2], held)) & ~(kShareStep - 1) : 0;
-  return f;
+  const int32_t* const its = a.families + 3 * (int64_t)row[0];
+  const int held = (int)min((int64_t)view.lengths[row[0]], view.table_pitch << view.page_shift);
+  return its[0] == row[0] && its[1] == row[1] && its[2] == row[2] ? max(0, min(row[2], held)) & ~(kShareStep - 1) : 0;
 }
 
 // 64 sequences, a lane each, with one trip to memory: what they are, the families that they lead and whose keys are not their own.
@@ -164,7 +163,7 @@ struct LaneSequences {
   int base;                            // number of the first
   int starts, ends;                    // of the packed rows, as they are given
   int start, tokens, length, first, own;  // as in Sequence (own: its base)
-  int leader;                          // the first of its family, as its row says
+  int leader;                          // the first of its family; -1: it is on its own
   int family_end, family_keys, family_tokens;  // of the family that it leads; keys 0: none
 
   __device__ __forceinline__ Sequence sequence(int lane) const {
@@ -207,7 +206,7 @@ __device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int 
   const int held = (int)min((int64_t)length, view.table_pitch << view.page_shift);
   s.start = max(0, s.starts), s.tokens = b < view.batch ? max(0, min(s.ends, view.tokens) - s.start) : 0;
   s.length = max(0, held), s.first = length - s.tokens;
-  s.own = 0, s.leader = row[0], s.family_end = min(row[1], view.batch), s.family_keys = s.family_tokens = 0;
+  s.own = 0, s.leader = -1, s.family_end = min(row[1], view.batch), s.family_keys = s.family_tokens = 0;
   if (a.families == nullptr) return s;
   if (b < view.batch && row[0] == b && s.family_end > b + 1) s.family_keys = max(0, min(row[2], held)) & ~(kShareStep - 1);
   const int last = s.family_end - 1 - base;
@@ -215,13 +214,12 @@ __device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int 
   if (s.family_keys > 0 && last >= kWave) rows_end = view.starts[s.family_end];
   if (s.family_keys > 0) s.family_tokens = max(0, min(rows_end, view.tokens) - s.start);
   const int from = row[0] - base, there = max(0, min(from, kWave - 1));
-  int keys = __shfl(s.family_keys, there, kWave), end = __shfl(s.family_end, there, kWave);
+  int keys = __shfl(s.family_keys, there, kWave);
+  const int its_end = __shfl(row[1], there, kWave), its_keys = __shfl(row[2], there, kWave);
+  if (its_end != row[1] || its_keys != row[2] || b >= s.family_end) keys = 0;
   if ((unsigned)row[0] > (unsigned)b) keys = 0;
-  else if (from < 0) {
-    const Family f = family_led_by(a, row[0]);
-    keys = f.keys, end = f.end;
-  }
-  if (b < end) s.own = keys;
+  else if (from < 0) keys = b < s.family_end ? keys_in_common(a, row) : 0;
+  if (keys > 0) s.own = keys, s.leader = row[0];
   return s;
 }
 __device__ __forceinline__ LaneSequences lane_sequences(const PagedArgs& a, int base) { return lane_sequences(a, base, lane_numbers(a, base)); }
@@ -243,12 +241,12 @@ __device__ __forceinline__ void seen_of_part(const Sight& s, int* lo, int* hi) {
   if (*hi <= s.first) *hi = min(*hi, s.low);
   *hi = max(*lo, *hi);
 }
-// The sequence of a family that a row of q belongs to, each lane's own, and what of the family's keys the row sees; *member: whether that sequence says that it is of the family.  Where each
+// The sequence of a family that a row of q belongs to, each lane's own, and what of the family's keys the row sees; *member: whether that sequence is of the family.  Where each
 // sequence has one new token and they lie among the 64, no trip to memory.
 __device__ __forceinline__ Reach family_reach(const PagedArgs& a, const LaneSequences& s, const Family& f, int start, int row, bool* member) {
   const PagedView& view = a.view;
   const int guess = min(f.first + row - start, f.end - 1), at = min(guess - s.base, kWave - 1);
-  int leader = __shfl(s.leader, at, kWave);
+  *member = __shfl(s.leader, at, kWave) == f.first;
   Sequence q;
   q.start = __shfl(s.start, at, kWave), q.tokens = __shfl(s.tokens, at, kWave), q.length = __shfl(s.length, at, kWave), q.first = __shfl(s.first, at, kWave);
   if (!(guess - s.base < kWave && q.start <= row && row < q.start + q.tokens)) {
@@ -259,9 +257,9 @@ __device__ __forceinline__ Reach family_reach(const PagedArgs& a, const LaneSequ
       else hi = mid;
     }
     q = sequence(a, lo);
-    leader = a.families[3 * (int64_t)lo];
+    const int32_t *const its = a.families + 3 * (int64_t)lo, *const firsts = a.families + 3 * (int64_t)f.first;
+    *member = its[0] == f.first && its[1] == firsts[1] && its[2] == firsts[2];
   }
-  *member = leader == f.first;
   Reach r = q.reach(a, row - q.start);
   r.low = min(f.keys, a.window > 0 ? min(a.sinks, r.end) : 0);
   r.end = min(f.keys, r.end);

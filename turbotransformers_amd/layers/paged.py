@@ -77,7 +77,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     max_tokens, max_length: the most new tokens and keys of a sequence, where known: they choose how the work is cut, not what is computed.
     families: int32 [batch, 3] on the GPU: neighbouring sequences whose first keys lie in the same pages may be a family, whose common keys are read once for all of them.
     The row of each of its sequences is (number of the first of them, number behind the last, keys they have in common); of one that is on its own (its own number, the next,
-    0).  The common keys are read where the first one's row of the table says, in steps of 128 (fewer are not shared).  The result is that without families but for roundings.
+    0); one whose row is not that of the first it names is on its own as well.  The common keys are read where the first one's row of the table says, in steps of 128 (fewer are not
+    shared).  The result is that without families but for roundings.
     family_count, max_shared: how many families there are and the most keys of one, where known: hints as well.  `PagedCache.extend(..., share=True)` fills in all three.
     -> like q: `out` if given."""
     if out is None:
