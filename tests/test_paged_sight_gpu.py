@@ -198,6 +198,58 @@ def test_what_lies_behind_the_last_key_and_under_the_gap(d, bad):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("what", ["keys", "queries", "values", "a column of keys", "a column of queries", "one value of each sequence", "scale"])
+@pytest.mark.parametrize("e", [97, 101, 112, 120, 125])
+def test_numbers_far_from_one(d, what, e):
+    """Numbers whose parts would fall below those that bf16 has, with factors that make up for it: the tolerance of fp32 as ever, in the kernels with and without first tokens, chunks,
+    families and single tokens.  (Results below the normal numbers: each product and each of their sums is off by up to 2^-150 besides, against a sum of probabilities of at least 1, and
+    so is the result.)"""
+    new, past = [140, 30, 3, 1], [0, 90, 300, 200]
+    for families, window, sinks in (((), 50, 7), ((), 50, 0), (((2, 0), (2, 192)), 0, 0), (((2, 0), (2, 192)), 60, 5)):
+        case = Sight("f32", new, past, 4, 2, d, 16, families=families)
+        scale = 1 / math.sqrt(d)
+        if what == "keys":
+            case.keys, case.q = case.keys * 2.0 ** -e, case.q * 2.0 ** e
+        elif what == "queries":
+            case.q, case.keys = case.q * 2.0 ** -e, case.keys * 2.0 ** e
+        elif what == "values":
+            case.values = case.values * 2.0 ** -e
+        elif what == "a column of keys":
+            case.keys[..., 5], case.q[..., 5] = case.keys[..., 5] * 2.0 ** -e, case.q[..., 5] * 2.0 ** e
+        elif what == "a column of queries":
+            case.q[..., 5], case.keys[..., 5] = case.q[..., 5] * 2.0 ** -e, case.keys[..., 5] * 2.0 ** e
+        elif what == "one value of each sequence":  # that stands alone in its column
+            case.values[..., 7] = torch.where(torch.isnan(case.values[..., 7]), case.values[..., 7], torch.zeros_like(case.values[..., 7]))
+            for b, n in enumerate(case.lengths):
+                case.values[case.table[b, (n - 2) // 16], :, (n - 2) % 16, 7] = 1.2345678 * 2.0 ** -e
+        else:
+            case.q, case.keys, scale = case.q * 2.0 ** -(e // 2), case.keys * 2.0 ** -(e // 2), scale * 2.0 ** (2 * (e // 2))
+        got = case.run_attention(window=window, sinks=sinks, scale=scale).cpu().double()
+        want, tol = case.attention(window=window, sinks=sinks, scale=scale)
+        assert ((got - want).abs() <= tol + (2 * max(case.lengths) + 1) * 2.0 ** -150).all(), (families, window, sinks)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,past,window,sinks,families", [([140, 30, 2], [400, 90, 37], 50, 7, ()), ([40], [5000], 1000, 7, ()), ([150], [0], 1000, 20, ()), ([20, 30, 1], [300, 290, 270], 0, 0, ((3, 256),)),
+                                                            ([20, 30, 1], [1300, 1290, 1270], 100, 9, ((3, 1256),))])
+def test_small_numbers_that_no_token_sees(d, new, past, window, sinks, families):
+    """Behind a sequence's last key and in the gap of its window they change no bit, as others do not."""
+    case = Sight("f32", new, past, 4, 2, d, 16, families=families)
+    outs = []
+    for fill in (math.nan, 2.0 ** -120):
+        case.keys, case.values = (torch.where(torch.isnan(x), torch.full_like(x, fill), x) for x in (case.keys, case.values))
+        for b, p in enumerate(past):  # (whole pages that lie under the gap of the first new token and so of all: in a family, of its sequence with the fewest)
+            p = min(past) if families else p
+            if window and p - window > sinks:
+                pages = case.table[b, -(-sinks // 16):(p + 1 - window) // 16]
+                case.keys[pages], case.values[pages] = fill, fill
+        outs.append(case.run_attention(window=window, sinks=sinks).cpu()[:sum(new)])
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
+    case.keys, case.values = torch.zeros_like(case.keys), torch.zeros_like(case.values)
+    assert (case.run_attention(window=window, sinks=sinks)[:sum(new)] == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_scores_of_minus_infinity(d):
     """A key with a score of minus infinity weighs nothing, whether it comes from an infinity or from numbers near it: the bits are those of a score that is merely low."""
     case = Sight("f32", [140, 30], [0, 90], 4, 2, d, 16)

@@ -177,20 +177,37 @@ __device__ __forceinline__ int part_of(const PagedArgs& a, int n) {
 // Heads of 128 in three parts each take the registers of two workgroups, which families and sequences with few rows cannot spare.
 template <typename T, int D, bool FAMILIES, bool FEW>
 constexpr bool kThirds = sizeof(T) == 4 && (D == 64 || (!FAMILIES && !FEW));
+// A part of a block of rows, in three parts a number if they hold it.
+template <typename T, int D, bool SMALL, bool FAMILIES, bool THIRDS, typename Shared>
+__device__ __forceinline__ void part_of_block(const PagedArgs& a, const Job& job, LaneSequences lanes, int kv_head, Shared& shared) {
+  int thread = threadIdx.x;
+  if constexpr (THIRDS) {
+    if (__builtin_expect(tiles<T, D, SMALL, true, FAMILIES, true>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, kv_head, job.part, thread, shared.tiles), 1)) return;
+    __syncthreads();
+    // (what both ways find out alike must not stay in registers meanwhile: the compiler is not to know that it is alike)
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(thread));
+#endif
+    if constexpr (FAMILIES) lanes = lane_sequences(a, __builtin_amdgcn_readfirstlane(lanes.base));
+  }
+  tiles<T, D, SMALL, true, FAMILIES, false>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, kv_head, job.part, thread, shared.whole);
+}
 template <typename T, int D, bool SMALL, bool FAMILIES, bool FEW>
 __global__ __launch_bounds__(256, (D == 128 && kThirds<T, D, FAMILIES, FEW> ? 1 : 2)) void sight_kernel(const PagedArgs a) {
   static_assert(!FEW || !SMALL, "with small pages sequences with few rows have a launch of their own");
   __shared__ union {
     TilesShared<T, D, kThirds<T, D, FAMILIES, FEW>> tiles;
+    TilesShared<T, D, false> whole;
     FewRowsShared<T, D, 4> few;
   } shared;
   const int kv_heads = a.view.kv_heads;
   int group = blockIdx.x;
   if constexpr (!FAMILIES) {
     if (!FEW || group < a.tile_groups) {
-      int b, block;
-      if (!find_block(a, group / kv_heads / a.splits, &b, &block)) return;
-      tiles<T, D, SMALL, true, false, kThirds<T, D, FAMILIES, FEW>>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, group % kv_heads, part_of(a, group / kv_heads), shared.tiles);
+      Job job{};
+      if (!find_block(a, group / kv_heads / a.splits, &job.b, &job.block)) return;
+      job.part = part_of(a, group / kv_heads), job.seq = sequence(a, job.b);
+      part_of_block<T, D, SMALL, false, kThirds<T, D, FAMILIES, FEW>>(a, job, LaneSequences{}, group % kv_heads, shared);
     } else if constexpr (FEW) {
       Walk walk{};
       few_rows<T, D, 4, false, kSinks>(a, group - a.tile_groups, a.few_splits, walk, -1, shared.few);
@@ -237,7 +254,7 @@ __global__ __launch_bounds__(256, (D == 128 && kThirds<T, D, FAMILIES, FEW> ? 1 
         lanes = lane_sequences(a, job.b & ~(kWave - 1));
         job.part = part_of(a, group / kv_heads), job.chunk = 0, job.seq = lanes.sequence(job.b % kWave), job.family = Family{};
       } else family_job(a, lanes, steps, item, passed, &job);
-      tiles<T, D, SMALL, true, true, kThirds<T, D, FAMILIES, FEW>>(a, job.b, job.block, job.seq, lanes, job.family, job.chunk, group % kv_heads, job.part, shared.tiles);
+      part_of_block<T, D, SMALL, true, kThirds<T, D, FAMILIES, FEW>>(a, job, lanes, group % kv_heads, shared);
       item += step;
       if (item >= stop) break;
       __syncthreads();

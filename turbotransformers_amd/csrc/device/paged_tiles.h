@@ -18,8 +18,10 @@
 // THIRDS (fp32 with SIGHT): the fp32 instruction takes sixteen times as long as the bf16 one, so a number is a sum of three bf16, x = h + m + l to its last place, and a product six of theirs,
 //     x y = h h' + (h m' + m h') + (m m' + h l' + l h'), up to 2^-23 of it left out (m is at most 2^-8, l 2^-16 of x);
 // keys and values are taken apart on their way to LDS, queries once, probabilities as they come; sums are fp32 as ever.  Numbers from 2^127 on, whose h may be an infinity, have their scores
-// computed one by one.  us, that instruction / this, 12 heads of 64: 8 prompts of 33 to 900 tokens, window 200 41.5 / 34.7, one of 4000, window 1000 171 / 112, 8 questions of 40 to 100 tokens behind 4000 common
-// keys 94 / 70; 32 and 8 heads of 128: a prompt of 1000, window 300 125 / 73, 20 chunks of up to 300 behind up to 3000 keys 214 / 120.  Against 64 bits the error goes from 2.5e-7 to 1.8e-7.
+// computed one by one.  Where one that is not zero lies below 2^-100, whose l may be lost, the workgroup finds out while it takes them apart, and begins anew with the fp32 instruction (without the
+// look for them: 8 prompts 33.5 us, one of 4000 104).  us, that instruction / this, 12 heads of 64: 8 prompts of 33 to 900 tokens, window 200 41.5 / 35.2, one of 4000, window 1000 171 / 109, 8 questions of
+// 40 to 100 tokens behind 4000 common keys 94 / 70; 32 and 8 heads of 128: a prompt of 1000, window 300 125 / 74, 20 chunks of up to 300 behind up to 3000 keys 214 / 127.  Against 64 bits the error goes
+// from 2.5e-7 to 1.8e-7.
 //
 // SIGHT: rows that see the first keys of their sequence besides a window (the keys that a block sees lie behind each other in whole tiles, Span), sequences whose first keys are their family's,
 // and families: the rows of all sequences of one over the keys that they have in common, each of which sees what its own position lets it see.
@@ -164,12 +166,22 @@ __device__ __forceinline__ bool too_large(const u32x4& raw) {
   return fmaxf(fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1])), fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3]))) >= kTooLarge;
 }
 
+// And those whose last part lies below bf16's normal numbers (2^-126 for a last place of 2^-123), zero apart.  least: the least of what was looked at so far, as a magnitude's bits
+// twice and less one.
+constexpr uint32_t kTooSmall = 2 * 0x0d800000u - 1;  // 2^-100
+__device__ __forceinline__ uint32_t least_of(uint32_t least, const u32x4& raw) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) least = min(least, (raw[i] << 1) - 1u);
+  return least;
+}
+
 template <typename T, int D, bool THIRDS>
 struct TilesShared {
   static constexpr int kBytes = THIRDS ? Tiles<T, D>::kBytes * 3 / 2 : Tiles<T, D>::kBytes;  // of a tile of keys, or of values
   __align__(16) char tiles[4 * kBytes];
   int wild;  // whether values that only some rows see hold infinities or NaNs
   int large;  // THIRDS: whether a key was too large
+  int small;  // THIRDS: whether a number was too small
   int sights[4][6];  // of a family's rows, wavefront by wavefront
 };
 
@@ -208,10 +220,10 @@ __device__ __forceinline__ void family_sights(const Family& f, const Reach& mine
 
 // Part `z` of a block of rows of sequence b; SIGHT: of the sequence's own keys, or (family.keys > 0) of the family's that it leads, in parts of family_chunk keys.
 // SMALL: pages of fewer than 16 slots
-// THIRDS: fp32 by the bf16 instructions
+// THIRDS: fp32 by the bf16 instructions.  -> false where a number was too small for that: nothing is stored then, and the part is one for the fp32 instruction
 template <typename T, int D, bool SMALL, bool SIGHT, bool FAMILIES, bool THIRDS>
-__device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, const Sequence& seq, const LaneSequences& lanes, const Family& family, int family_chunk,
-                                      int kv_head, int z, TilesShared<T, D, THIRDS>& shared) {
+__device__ __forceinline__ bool tiles(const PagedArgs& a, int b, int block, const Sequence& seq, const LaneSequences& lanes, const Family& family, int family_chunk,
+                                      int kv_head, int z, int tid, TilesShared<T, D, THIRDS>& shared) {
   using S = Tiles<T, D>;
   constexpr int kTileBytes = TilesShared<T, D, THIRDS>::kBytes, kPlane = kTileBytes / 3;  // (THIRDS: of a third of the tile)
   char* const smem = shared.tiles;
@@ -219,9 +231,9 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
   const PagedView& view = a.view;
   const bool families = FAMILIES && family.keys > 0;
   const int row0 = block * kTileRows, rows = min(kTileRows, seq.tokens * a.group - row0);
-  if (z == 0 && kv_head == 0 && block == 0 && threadIdx.x == 0 && !families && seq.first + seq.tokens > seq.length) page_error(view);
+  if (z == 0 && kv_head == 0 && block == 0 && tid == 0 && !families && seq.first + seq.tokens > seq.length) page_error(view);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lrow = lane & 31, lhalf = lane >> 5;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lrow = lane & 31, lhalf = lane >> 5;
   const T* const keys = static_cast<const T*>(a.keys);
   const T* const values = static_cast<const T*>(a.values);
   const int wave_rows = max(0, min(32, rows - wave * 32));
@@ -249,20 +261,20 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
     chunk = seq.chunk(a);
     part0 = sight.first / chunk, part = part0 + z;
     lo = (int)max(part * (int64_t)chunk, (int64_t)(sight.first & ~(S::kKeys - 1))), hi = (int)min((part + 1) * (int64_t)chunk, (int64_t)sight.end);
-    if (lo >= hi && part != part0) return;
+    if (lo >= hi && part != part0) return true;
   } else {
     part0 = 0, part = z;
     if (families) {  // all rows of a family have the same parts, and write them
       chunk = family_chunk;
       span = {0, 0, 0, 0};
-      if (z * (int64_t)chunk >= seq.length) return;
+      if (z * (int64_t)chunk >= seq.length) return true;
       lo = z * chunk, hi = (int)min((z + 1) * (int64_t)chunk, (int64_t)seq.length);
       if (a.window > 0) seen_of_part<S::kKeys>(sight, &lo, &hi);
     } else {
       chunk = seq.span_chunk(a);
       span = span_of<kSpanTiles<T>>(sight, seq.base);
       lo = (int)min(span.lo + part * (int64_t)chunk, (int64_t)span.hi), hi = (int)min(span.lo + (part + 1) * (int64_t)chunk, (int64_t)span.hi);
-      if (lo >= hi && part != 0) return;
+      if (lo >= hi && part != 0) return true;
     }
   }
   auto key_at = [&](int place) __attribute__((always_inline)) {
@@ -273,6 +285,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
   const T* const query = static_cast<const T*>(a.q) + (seq.start + token) * a.q_pitch + (int64_t)head * D;
   u32x4 qf[THIRDS ? 1 : S::kSteps], qt[THIRDS ? 3 : 1][D / 16];
   bool large_query = false;
+  uint32_t least = UINT32_MAX;  // THIRDS: of this lane's share of what the workgroup reads and some row sees
   if constexpr (!THIRDS) {
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i) {
@@ -286,7 +299,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
       for (int j = 0; j < 2; ++j) {
         u32x4 x = {0u, 0u, 0u, 0u};
         if (live) x = *reinterpret_cast<const u32x4*>(query + 16 * i + 8 * lhalf + 4 * j);
-        large_query = large_query || too_large(x);
+        large_query = large_query || too_large(x), least = least_of(least, x);
         const Thirds t = thirds(x);
 #pragma unroll
         for (int p = 0; p < 3; ++p) qt[p][i][2 * j] = t.part[p][0], qt[p][i][2 * j + 1] = t.part[p][1];
@@ -326,6 +339,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
     const int at = i * 4096 + tid * 16, r = at / S::kRowBytes, c = at % S::kRowBytes / 16;
     if constexpr (THIRDS) {
       if (__builtin_expect(too_large(kr[set][i]), 0)) shared.large = 1;
+      least = least_of(least_of(least, kr[set][i]), vr[set][i]);
       const Thirds k = thirds(kr[set][i]), v = thirds(vr[set][i]);
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
@@ -358,7 +372,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
     else if constexpr (!SMALL) fetch_pages<S::kRowBytes>(view, cursor, kv_head, lo);
 #pragma unroll
     for (int i = 0; i < S::kPieces; ++i) load_piece(i, key_at(lo), 0);
-    if (tid == 0) wild = 0, shared.large = 0;
+    if (tid == 0) wild = 0, shared.large = shared.small = 0;
     __syncthreads();
     if (partly_seen(key_at(lo))) clean_values(key_at(lo), 0);
 #pragma unroll
@@ -629,9 +643,20 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
       }
       __syncthreads();
     };
+    // (the last one stores that which was fetched once more, which nothing is asked about)
+    auto count = [&](int place, auto stage) __attribute__((always_inline)) {
+      const uint32_t before = least;
+      work_on(place, stage);
+      if constexpr (THIRDS) least = place + S::kKeys < hi ? least : before;
+    };
     for (int place = lo; place < hi; place += 2 * S::kKeys) {
-      work_on(place, std::integral_constant<int, 0>{});
-      if (place + S::kKeys < hi) work_on(place + S::kKeys, std::integral_constant<int, 1>{});
+      count(place, std::integral_constant<int, 0>{});
+      if (place + S::kKeys < hi) count(place + S::kKeys, std::integral_constant<int, 1>{});
+    }
+    if constexpr (THIRDS) {
+      if (__builtin_expect(least < kTooSmall, 0)) shared.small = 1;
+      __syncthreads();
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(shared.small), 0)) return false;
     }
   }
 
@@ -639,7 +664,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
     const LanePair both = swap_halves(sum);
     sum = both.a + both.b;
   }
-  if (!live) return;
+  if (!live) return true;
   const int64_t at_token = seq.start + token;
   if constexpr (!SIGHT) {
     const bool sees_some = mine.end > 0;
@@ -654,6 +679,7 @@ __device__ __forceinline__ void tiles(const PagedArgs& a, int b, int block, cons
       if (part == 0) store_out<T, D>(a, at_token, head, mine.end > 0, lhalf, ot, sum);
     } else if (part <= last_part) store_part<D>(a, a.own_at + (at_token * a.heads + head) * a.splits + part, a.rows, lhalf, ot, top, sum);
   }
+  return true;
 }
 
 template <typename T, int D, bool SMALL>
@@ -662,7 +688,7 @@ __global__ __launch_bounds__(256, 2) void tiles_kernel(const PagedArgs a) {
   const int kv_head = blockIdx.x % a.view.kv_heads;
   int b, block;
   if (!find_block(a, blockIdx.x / a.view.kv_heads, &b, &block)) return;
-  tiles<T, D, SMALL, false, false, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, blockIdx.z, shared);
+  tiles<T, D, SMALL, false, false, false>(a, b, block, sequence(a, b), LaneSequences{}, Family{}, 0, kv_head, blockIdx.z, threadIdx.x, shared);
 }
 
 }  // namespace
