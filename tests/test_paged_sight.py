@@ -197,6 +197,21 @@ def test_workspace_refuses(lib):
     assert room(lib, 2, 0) == 0
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,families,shared,faster", [
+    (capi.BF16, 32, 8, 128, (4, 4), 1000, False), (capi.BF16, 32, 8, 128, (4, 8), 1000, False), (capi.BF16, 32, 8, 128, (1, 16), 1000, False), (capi.F32, 12, 12, 64, (1, 4), 1000, False),
+    (capi.F16, 12, 12, 64, (8, 8), 1000, False), (capi.BF16, 32, 8, 128, (8, 2), 1000, False), (capi.BF16, 32, 8, 128, (4, 8), 2000, True), (capi.BF16, 32, 8, 128, (1, 256), 1000, True),
+    (capi.BF16, 32, 8, 128, (16, 4), 2000, True), (capi.BF16, 32, 8, 128, (2, 4), 3000, True), (capi.F16, 12, 12, 64, (1, 64), 1500, True), (capi.F16, 12, 12, 64, (8, 8), 1500, True),
+    (capi.F32, 12, 12, 64, (1, 4), 3000, True), (capi.F32, 12, 12, 64, (1, 64), 1000, True), (capi.F32, 32, 8, 128, (1, 64), 1500, True), (capi.F32, 32, 8, 128, (1, 64), 1000, False)])
+def test_families_are_shared_where_that_was_measured_to_be_faster(lib, dtype, heads, kv_heads, d, families, shared, faster):
+    """(families, sequences of each), a token and 50 keys of its own each: as the times say where the two differ, and that nothing is shared where they are level (4 families of 8
+    behind 1000 keys 21.9 / 21.5 us).  What a call asks for as its workspace tells which way it goes."""
+    count, members = families
+    n, held = count * members, shared // 16 * 16
+    asked = dict(heads=heads, kv_heads=kv_heads, d=d, most=1, longest=shared + 51, dtype=dtype, pitch=-(-(shared + 51) // 16))
+    assert (room(lib, n, n, count=count, shared=held, **asked) != room(lib, n, n, families=None, **asked)) == faster
+    assert room(lib, n, n, **asked) != room(lib, n, n, families=None, **asked)  # unknown: as they come
+
+
 @pytest.mark.parametrize("dtype", [capi.F32, capi.F16])
 def test_workspace_does_not_grow_with_keys_that_a_window_hides(lib, dtype):
     """300 tokens that see their last 500 keys and the first 20: as much room with a table for 2^24 positions as with one for 2^12, and with the largest numbers as with

@@ -158,14 +158,15 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
 }
 
 // Whether reading a family's keys once is worth it: a second launch, which joins what they give with what the sequences' own keys do, and blocks of 128 rows that may be mostly empty, for reads
-// that the caches would take most of.  Both are estimated, with what fits the measured; us, families / none, one token each and 50 keys of its own, behind 1000, 2000, 4000, 8000 keys (where both are
-// level the answer is no):
-//   bf16, 32 and 8 heads of 128: 8 sequences 15.3 / 14.7, 17.0 / 17.9, 20.9 / 21.9, 26.2 / 30.1; 64 27.9 / 28.7, 30.4 / 48.0, 30.5 / 80.8, 41.8 / 148; 256 63.0 / 96.9 .. 95.6 / 573;
-//                                8 families of 2 17.6 / 17.9 .. 54.8 / 54.2; 4 of 8 22.4 / 21.5, 26.9 / 31.1, 30.4 / 49.8, 40.1 / 83.3; 16 of 4 31.5 / 29.3, 38.4 / 48.8, 55.6 / 90.3, 115 / 181
-//   fp16, 12 heads of 64:        16 sequences 9.6 / 9.3, 15.5 / 19.1, 15.4 / 24.8, 20.4 / 39.0; 16 families of 4 21.0 / 20.7, 32.7 / 41.9, 46.2 / 68.7, 84.3 / 140
-//   fp32, the same heads:        4 sequences 15.9 / 13.4, 16.2 / 16.8, 16.7 / 21.3, 22.6 / 28.7; 64 28.8 / 48.0 .. 49.5 / 268; 32 and 8 heads of 128, 64: 54.8 / 54.4, 64.3 / 95.3 .. 142 / 321
+// that the caches would take most of.  Both are estimated, with what fits the measured; us, families / none, one token each and 50 keys of its own, behind 1000, 2000, 4000, 8000 keys:
+//   bf16, 32 and 8 heads of 128: 8 sequences 17.4 / 14.8, 18.6 / 16.6, 20.3 / 21.4, 25.3 / 29.5; 64 26.7 / 28.0, 30.0 / 45.1, 32.2 / 78.6, 40.7 / 147; 256 59.6 / 95.1 .. 68.9 / 297 (4000);
+//                                8 families of 2 20.4 / 17.5 .. 51.6 / 53.9; 4 of 8 21.9 / 21.5, 26.6 / 31.1, 30.0 / 48.7, 39.8 / 82.3; 16 of 4 30.7 / 29.3, 37.7 / 47.5, 54.8 / 88.7, 115 / 180
+//   fp16, 12 heads of 64:        16 sequences 15.0 / 9.0, 15.0 / 18.5, 14.6 / 25.0, 18.3 / 36.6; 16 families of 4 26.3 / 20.4, 31.7 / 40.6, 45.1 / 65.9, 81.8 / 137
+//   fp32, the same heads:        4 sequences 15.8 / 12.8, 15.9 / 15.7, 16.1 / 21.3, 22.3 / 27.5; 64 28.1 / 46.8 .. 49.3 / 262; 32 and 8 heads of 128, 64: 59.7 / 55.5, 63.3 / 92.0 .. 141 / 319
 // and of more tokens: 4 sequences of up to 12, 24 and 12 heads of 64, fp32, behind 1400 keys 20.8 / 44.6; 9 of 5 to 9, 32 and 4 heads of 128, fp32, behind up to 4200 120 / 144; 8 of up to 69, 6 and 2 heads of
-// 128, bf16, behind 7500 56 / 43 (no).  Over 128 random batches what it takes is 1.6 % slower on average than the better of the two; none alone 20 %.
+// 128, bf16, behind 7500 56 / 43 (no).
+// Where the two are within some per cent of each other it may take the slower one: over 195 such batches what it takes is 0.3 % slower on average than the better of the two, at most 8 % where it shares
+// (8 families of 8 behind 512 keys, fp32 25.7 / 23.9) and 16 where it does not (2 sequences behind 4000, fp32 16.1 / 18.7), none alone 46 %.
 // Where nothing is known they are taken as they come.
 bool sharing_pays(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, const ttmi_paged_sight& sight, int dtype) {
   if (sight.families == nullptr) return false;
@@ -177,7 +178,7 @@ bool sharing_pays(const PagedView& view, int64_t heads, int64_t max_tokens, int6
   const double step = step_us(dtype, view.head_dim, single), rows = (double)view.tokens * (double)(heads / view.kv_heads), batch = view.batch;
   const double bytes = guess.steps * 64.0 * (2 * view.kv_heads * view.head_dim * (double)dtype_size(dtype));
   // each by itself: the common keys again and again, out of the caches, and a launch that joins, or (many rows) the walk over a part of them
-  double alone = (own.few && own.few_splits == 0 ? 7 : f32 ? 14 : 12) + batch * bytes / (f32 ? 12.5e6 : 14e6);
+  double alone = (own.few && own.few_splits == 0 ? 7 : f32 ? (wide ? 14 : 13.5) : 12) + batch * bytes / (f32 ? 12.5e6 : 15e6);
   if (single && own.tiles) alone += 5;
   if (!single) {
     // (half a block of each sequence is empty, and each has one)
