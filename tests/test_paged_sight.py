@@ -212,6 +212,20 @@ def test_families_are_shared_where_that_was_measured_to_be_faster(lib, dtype, he
     assert room(lib, n, n, **asked) != room(lib, n, n, families=None, **asked)  # unknown: as they come
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,families,tokens,shared,faster", [
+    (capi.BF16, 32, 8, 128, (1, 32), 20, 1000, False), (capi.BF16, 32, 8, 128, (8, 4), 20, 1000, False), (capi.BF16, 32, 8, 128, (8, 4), 50, 2000, False),
+    (capi.BF16, 32, 8, 128, (1, 16), 50, 2000, False), (capi.BF16, 8, 4, 64, (4, 2), 150, 5000, False), (capi.F32, 32, 8, 128, (8, 4), 50, 700, False),
+    (capi.F32, 16, 2, 128, (4, 2), 50, 2000, False), (capi.BF16, 32, 8, 128, (1, 100), 6, 4000, True), (capi.F32, 12, 12, 64, (1, 48), 20, 700, True),
+    (capi.F32, 12, 12, 64, (1, 4), 50, 2000, True), (capi.BF16, 32, 8, 128, (1, 16), 100, 20000, True)])
+def test_families_with_chunks_are_shared_where_that_was_measured_to_be_faster(lib, dtype, heads, kv_heads, d, families, tokens, shared, faster):
+    """The same of sequences with several new tokens each, where either way took up to twice as long as the other."""
+    count, members = families
+    n, held = count * members, shared // 16 * 16
+    longest = shared + 50 + tokens
+    asked = dict(heads=heads, kv_heads=kv_heads, d=d, most=tokens, longest=longest, dtype=dtype, pitch=-(-longest // 16))
+    assert (room(lib, n, n * tokens, count=count, shared=held, **asked) != room(lib, n, n * tokens, families=None, **asked)) == faster
+
+
 @pytest.mark.parametrize("dtype", [capi.F32, capi.F16])
 def test_workspace_does_not_grow_with_keys_that_a_window_hides(lib, dtype):
     """300 tokens that see their last 500 keys and the first 20: as much room with a table for 2^24 positions as with one for 2^12, and with the largest numbers as with

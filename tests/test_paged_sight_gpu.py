@@ -929,3 +929,36 @@ def test_families_that_are_worth_it(dt, new, window, sinks):
     case.keys, case.values = case.keys.nan_to_num(), case.values.nan_to_num()
     got = case.run_attention(hints=None, window=window, sinks=sinks)
     case.check_attention(got, window=window, sinks=sinks)
+
+
+def workspace(case, hints, window=0, sinks=0, families=True):
+    """What the call of `case` asks for as its workspace: with the families shared it is another one than without."""
+    lib = capi.load()
+    count, most = hints
+    cache = capi.PagedCache(16, 32, *case.keys.shape)  # (addresses that are not looked at)
+    batch = capi.PagedBatch(16, case.table.shape[1], 16, 16, len(case.new), case.tokens)
+    sight = capi.PagedSight(window, sinks, 16 if families else None, count, most)
+    n = ctypes.c_int64(-1)
+    dtype = {"f32": capi.F32, "f16": capi.F16, "bf16": capi.BF16}[case.dt]
+    capi.check(lib.ttmi_paged_attention_sight_workspace(ctypes.byref(cache), ctypes.byref(batch), case.heads, max(case.new), max(case.lengths), ctypes.byref(sight), dtype,
+                                                        ctypes.byref(n)))
+    return n.value
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("new,keys,window,sinks", [(1, 2048, 0, 0), (1, 2048, 2000, 40), (20, 4096, 0, 0)])
+def test_shared_and_not_shared_by_the_hints(dt, new, keys, window, sinks):
+    """A batch whose hints let its families be shared, and one that they do not, by the workspace that the call asks for: both, and the calls without hints, which share, and without
+    families give every sequence the formula's results; what is not shared has the bits of a call without families."""
+    rng = random.Random(new)
+    many = Sight(dt, [new] * 71, [keys + rng.choice([1, 20, 300]) for _ in range(70)] + [900], 8, 4, 64, 16, families=[(70, keys), (1, 0)])
+    few = Sight(dt, [new] * 5, [150 + 9 * i for i in range(4)] + [200], 8, 4, 64, 16, families=[(4, 144), (1, 0)])
+    for case, hints, shared in ((many, (1, keys), True), (few, (1, 144), False)):
+        kw = dict(window=window, sinks=sinks)
+        assert (workspace(case, hints, **kw) != workspace(case, hints, families=False, **kw)) == shared
+        assert workspace(case, (0, 0), **kw) != workspace(case, (0, 0), families=False, **kw)
+        hinted, unknown, none = case.run_attention(hints=None, **kw), case.run_attention(**kw), Case.run_attention(case, **kw)
+        want, tol = case.attention(**kw)
+        for got in (hinted, unknown, none):
+            assert ((got.cpu().double() - want).abs() <= tol).all()
+        assert shared or torch.equal(hinted, none)

@@ -107,13 +107,13 @@ bool single_tokens(const PagedView& view, int64_t heads) { return view.tokens * 
 // 8000 81 / 58.
 int family_few_rows(int dtype) { return dtype == TTMI_F32 ? 64 : 16; }
 struct FamilyGuess {
-  double blocks;  // of rows
+  double count, blocks;  // of them, and of rows
   int64_t steps;  // of the longest
 };
 FamilyGuess guess_families(const PagedView& view, int64_t heads, const ttmi_paged_sight& sight) {
   const int64_t held = view.table_pitch << view.page_shift, shared = sight.max_shared > 0 ? std::min(sight.max_shared, held) : held;
   const int64_t count = std::max<int64_t>(1, std::min<int64_t>(sight.family_count, view.batch / 2));
-  return {(double)std::max(count, ceil_div(view.tokens * (heads / view.kv_heads), 128)), std::max<int64_t>(1, shared / 64)};
+  return {(double)count, (double)std::max(count, ceil_div(view.tokens * (heads / view.kv_heads), 128)), std::max<int64_t>(1, shared / 64)};
 }
 
 // With first keys that stay visible and with families.  The sequences' own keys are cut as ever (their number is guessed from max_length: a sequence on its own may be that long).  A family's are
@@ -163,10 +163,37 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
 //                                8 families of 2 20.4 / 17.5 .. 51.6 / 53.9; 4 of 8 21.9 / 21.5, 26.6 / 31.1, 30.0 / 48.7, 39.8 / 82.3; 16 of 4 30.7 / 29.3, 37.7 / 47.5, 54.8 / 88.7, 115 / 180
 //   fp16, 12 heads of 64:        16 sequences 15.0 / 9.0, 15.0 / 18.5, 14.6 / 25.0, 18.3 / 36.6; 16 families of 4 26.3 / 20.4, 31.7 / 40.6, 45.1 / 65.9, 81.8 / 137
 //   fp32, the same heads:        4 sequences 15.8 / 12.8, 15.9 / 15.7, 16.1 / 21.3, 22.3 / 27.5; 64 28.1 / 46.8 .. 49.3 / 262; 32 and 8 heads of 128, 64: 59.7 / 55.5, 63.3 / 92.0 .. 141 / 319
-// and of more tokens: 4 sequences of up to 12, 24 and 12 heads of 64, fp32, behind 1400 keys 20.8 / 44.6; 9 of 5 to 9, 32 and 4 heads of 128, fp32, behind up to 4200 120 / 144; 8 of up to 69, 6 and 2 heads of
-// 128, bf16, behind 7500 56 / 43 (no).
 // Where the two are within some per cent of each other it may take the slower one: over 195 such batches what it takes is 0.3 % slower on average than the better of the two, at most 8 % where it shares
 // (8 families of 8 behind 512 keys, fp32 25.7 / 23.9) and 16 where it does not (2 sequences behind 4000, fp32 16.1 / 18.7), none alone 46 %.
+//
+// Of more tokens a sequence (more than 16 rows a key/value head on average) all blocks are the kernel's for many rows: what counts is the longest part of one (`step` for each of its steps of 64 keys),
+// what all blocks do (`work` for as many steps of a full block as there are workgroups at a time, of which each 32 rows take most), partial results written and joined (`join`, for 10^6 bytes of them both
+// ways), and with families a second set of blocks, for the sequences' own keys (`block`, for as many as there are at a time).  us, families / none, bf16, 32 and 8 heads of 128:
+//   32 sequences of 20 tokens behind 1000, 2000, 4000 keys 57 / 30, 71 / 49, 89 / 88; 8 families of 4 79 / 31, 74 / 50, 104 / 88; 16 of 50 behind 2000, 5000 83 / 52, 124 / 112; 100 of 6 behind 2000, 4000 99 / 117 (no), 114 / 194
+//   fp32: 8 families of 4 with 50 tokens behind 700, 2000 347 / 226, 657 / 553 (yes); heads of 64, 12 of them: 4 of 50 behind 2000 41 / 56, 48 of 20 behind 700 81 / 138
+// Over 714 batches of 5 to 150 tokens a sequence what it takes is 1.1 % slower on average than the better of the two, at most 31 % (16 of 150 behind 2000, fp32 843 / 1101, no), none alone 19 %; over 122 random batches of all kinds 0.3 and 19 %.
+struct ManyTokens {
+  double once, step, work, join, block;  // us
+};
+bool many_tokens_share(const PagedView& view, int64_t heads, int64_t max_length, const ttmi_paged_sight& sight, int dtype, const PagedPlan& own, const FamilyGuess& guess) {
+  const bool f32 = dtype == TTMI_F32, wide = view.head_dim == 128;
+  const ManyTokens a = f32 ? (wide ? ManyTokens{17, 4.9, 16.5, 0.17, 0} : ManyTokens{15.5, 0.8, 13, 0, 0}) : wide ? ManyTokens{14.5, 0.55, 2.1, 0.16, 0} : ManyTokens{12, 0.4, 1.5, 0.2, 0};
+  const ManyTokens s = f32 ? (wide ? ManyTokens{27, 4.5, 14.7, 0.6, 38} : ManyTokens{20, 1.1, 5.3, 0.45, 35}) : wide ? ManyTokens{17.5, 0.45, 1.8, 0.35, 22} : ManyTokens{13, 0.4, 1.1, 0.55, 18};
+  const int64_t held = view.table_pitch << view.page_shift, longest = max_length > 0 ? std::min(max_length, held) : held, shared = std::min(sight.max_shared, held);
+  const double rows = (double)view.tokens * (double)(heads / view.kv_heads), batch = view.batch, at_a_time = 2.0 * compute_units() / (double)view.kv_heads;
+  const double own_steps = sight.window > 0 ? 1.0 : std::max(1.0, (double)(longest - shared) / 64);
+  // (half a block, or half of 32 rows, of each sequence is empty, and each has one)
+  const double blocks = std::max(batch, rows / 128 + batch / 2), full = 0.7 * std::max(batch, rows / 32 + batch / 2) / 4 + 0.3 * blocks;
+  const double family_full = 0.7 * std::max(guess.count, std::ceil(rows / 32)) / 4 + 0.3 * guess.blocks;
+  const double join = (double)view.tokens * (double)heads * (double)(view.head_dim + 2) * 8e-6, steps = (double)guess.steps;
+  const int64_t parts = best_cut(guess.blocks * (double)view.kv_heads, guess.steps, step_us(dtype, view.head_dim, false), false, view.tokens, heads, view.head_dim).parts;
+  const double alone = a.once + a.step * std::min((double)ceil_div(own.tile_chunk, 64), steps + own_steps) + a.work * full * (steps + own_steps) / at_a_time +
+                       (own.tile_splits > 1 ? a.join * join * own.tile_splits : 0);
+  const double together = s.once + s.step * (double)ceil_div(guess.steps, parts) + s.work * (family_full * steps + full * own_steps) / at_a_time + s.join * join * (double)(parts + 1) +
+                          s.block * blocks / at_a_time;
+  return together < alone;
+}
+
 // Where nothing is known they are taken as they come.
 bool sharing_pays(const PagedView& view, int64_t heads, int64_t max_tokens, int64_t max_length, const ttmi_paged_sight& sight, int dtype) {
   if (sight.families == nullptr) return false;
@@ -177,20 +204,16 @@ bool sharing_pays(const PagedView& view, int64_t heads, int64_t max_tokens, int6
   const bool f32 = dtype == TTMI_F32, wide = view.head_dim == 128, single = single_tokens(view, heads);
   const double step = step_us(dtype, view.head_dim, single), rows = (double)view.tokens * (double)(heads / view.kv_heads), batch = view.batch;
   const double bytes = guess.steps * 64.0 * (2 * view.kv_heads * view.head_dim * (double)dtype_size(dtype));
-  // each by itself: the common keys again and again, out of the caches, and a launch that joins, or (many rows) the walk over a part of them
+  if (!single) return many_tokens_share(view, heads, max_length, sight, dtype, own, guess);
+  // each by itself: the common keys again and again, out of the caches, and a launch that joins
   double alone = (own.few && own.few_splits == 0 ? 7 : f32 ? (wide ? 14 : 13.5) : 12) + batch * bytes / (f32 ? 12.5e6 : 15e6);
-  if (single && own.tiles) alone += 5;
-  if (!single) {
-    // (half a block of each sequence is empty, and each has one)
-    const double groups = std::max(rows / 128 + batch / 2, batch) * (double)view.kv_heads * own.tile_splits, steps = (double)ceil_div(std::min<int64_t>(own.tile_chunk, guess.steps * 64), 64);
-    alone = std::max(alone, 7 + rounds_of(groups, false) * steps * step);
-  }
+  if (own.tiles) alone += 5;
   if (alone <= 11) return false;  // (what a second launch and the rest of it take at least)
   // shared: as many bytes as families read, or blocks of their rows over parts of the keys
   const double count = (double)std::min<int64_t>(sight.family_count, std::max(1, view.batch / 2)), most = std::ceil(rows / count);
   double shared;
-  if (single && most <= family_few_rows(dtype)) shared = (f32 ? (wide ? 16 : 14.5) : 13) + 0.05 * batch + count * std::ceil(most / kFewRows) * bytes / 6e6;
-  else shared = (f32 ? (wide ? 22 : 12) : (wide ? 12 : 11)) + (f32 ? 0.15 : 0.1) * batch + (!single && own.few ? 8 : 0) +
+  if (most <= family_few_rows(dtype)) shared = (f32 ? (wide ? 16 : 14.5) : 13) + 0.05 * batch + count * std::ceil(most / kFewRows) * bytes / 6e6;
+  else shared = (f32 ? (wide ? 22 : 12) : (wide ? 12 : 11)) + (f32 ? 0.15 : 0.1) * batch +
                 best_cut(guess.blocks * (double)view.kv_heads, guess.steps, step, single, view.tokens, heads, view.head_dim).us;
   return shared < alone;
 }
