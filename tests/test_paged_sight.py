@@ -226,6 +226,19 @@ def test_families_with_chunks_are_shared_where_that_was_measured_to_be_faster(li
     assert (room(lib, n, n * tokens, count=count, shared=held, **asked) != room(lib, n, n * tokens, families=None, **asked)) == faster
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,families,tokens,shared,window,sinks,faster", [
+    (capi.BF16, 32, 8, 128, (16, 4), 1, 8000, 1500, 4, False), (capi.BF16, 12, 12, 64, (8, 4), 1, 8000, 1500, 4, False), (capi.F32, 32, 8, 128, (16, 4), 1, 8000, 500, 4, False),
+    (capi.F32, 32, 8, 128, (1, 16), 1, 8000, 500, 4, False), (capi.F32, 32, 8, 128, (8, 4), 20, 2000, 1500, 4, False), (capi.BF16, 32, 8, 128, (8, 4), 20, 8000, 4000, 4, False),
+    (capi.BF16, 32, 8, 128, (1, 64), 1, 8000, 4000, 4, True), (capi.BF16, 32, 8, 128, (1, 64), 1, 8000, 1500, 9000, True), (capi.F32, 32, 8, 128, (1, 64), 1, 8000, 4000, 4, True)])
+def test_families_behind_windows_are_shared_where_that_was_measured_to_be_faster(lib, dtype, heads, kv_heads, d, families, tokens, shared, window, sinks, faster):
+    """Common keys that a window hides cost those who share them some of what they would if they were seen, and the others nothing."""
+    count, members = families
+    n, held = count * members, shared // 16 * 16
+    longest = shared + 50 + tokens
+    asked = dict(heads=heads, kv_heads=kv_heads, d=d, most=tokens, longest=longest, dtype=dtype, pitch=-(-longest // 16), window=window, sinks=sinks)
+    assert (room(lib, n, n * tokens, count=count, shared=held, **asked) != room(lib, n, n * tokens, families=None, **asked)) == faster
+
+
 @pytest.mark.parametrize("dtype", [capi.F32, capi.F16])
 def test_workspace_does_not_grow_with_keys_that_a_window_hides(lib, dtype):
     """300 tokens that see their last 500 keys and the first 20: as much room with a table for 2^24 positions as with one for 2^12, and with the largest numbers as with

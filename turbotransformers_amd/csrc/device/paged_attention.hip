@@ -172,24 +172,31 @@ SightPlan plan_sight(const PagedView& view, int64_t heads, int64_t max_tokens, i
 //   32 sequences of 20 tokens behind 1000, 2000, 4000 keys 57 / 30, 71 / 49, 89 / 88; 8 families of 4 79 / 31, 74 / 50, 104 / 88; 16 of 50 behind 2000, 5000 83 / 52, 124 / 112; 100 of 6 behind 2000, 4000 99 / 117 (no), 114 / 194
 //   fp32: 8 families of 4 with 50 tokens behind 700, 2000 347 / 226, 657 / 553 (yes); heads of 64, 12 of them: 4 of 50 behind 2000 41 / 56, 48 of 20 behind 700 81 / 138
 // Over 714 batches of 5 to 150 tokens a sequence what it takes is 1.1 % slower on average than the better of the two, at most 31 % (16 of 150 behind 2000, fp32 843 / 1101, no), none alone 19 %; over 122 random batches of all kinds 0.3 and 19 %.
+//
+// Windows: common keys that they hide are estimated as half of seen ones (many tokens: a quarter).  us, families / none, behind 8000 keys, windows of 500, 1500 and 4000 with 4 first tokens: bf16, 32 and 8
+// heads of 128, 64 sequences 34.7 / 16.3, 36.6 / 38.5, 37.9 / 79.4; 16 families of 4 58.5 / 17.4, 60.2 / 39.8, 71.7 / 89.6; 64 with 20 tokens each 108 / 47.6, 123 / 69.6, 175 / 145; fp32, 16 families of 4
+// 99.2 / 38.3, 107 / 81.4, 159 / 193.  Over 400 such batches what it takes is 1.7 % slower on average than the better of the two, at most 57 % (16 of 20 tokens, fp32, window 4000, 270 / 424, no), none alone
+// 29 %.
 struct ManyTokens {
   double once, step, work, join, block;  // us
 };
-bool many_tokens_share(const PagedView& view, int64_t heads, int64_t max_length, const ttmi_paged_sight& sight, int dtype, const PagedPlan& own, const FamilyGuess& guess) {
+bool many_tokens_share(const PagedView& view, int64_t heads, int64_t max_length, const ttmi_paged_sight& sight, int dtype, const PagedPlan& own, const FamilyGuess& guess, int64_t walked) {
   const bool f32 = dtype == TTMI_F32, wide = view.head_dim == 128;
-  const ManyTokens a = f32 ? (wide ? ManyTokens{17, 4.9, 16.5, 0.17, 0} : ManyTokens{15.5, 0.8, 13, 0, 0}) : wide ? ManyTokens{14.5, 0.55, 2.1, 0.16, 0} : ManyTokens{12, 0.4, 1.5, 0.2, 0};
+  ManyTokens a = f32 ? (wide ? ManyTokens{17, 4.9, 16.5, 0.17, 0} : ManyTokens{15.5, 0.8, 13, 0, 0}) : wide ? ManyTokens{14.5, 0.55, 2.1, 0.16, 0} : ManyTokens{12, 0.4, 1.5, 0.2, 0};
   const ManyTokens s = f32 ? (wide ? ManyTokens{27, 4.5, 14.7, 0.6, 38} : ManyTokens{20, 1.1, 5.3, 0.45, 35}) : wide ? ManyTokens{17.5, 0.45, 1.8, 0.35, 22} : ManyTokens{13, 0.4, 1.1, 0.55, 18};
+  // (behind a gap fp32 by three parts a number, which heads of 128 have without families and sequences of few rows)
+  if (f32 && sight.window > 0 && sight.sinks > 0 && !(wide && own.few)) a.step *= 0.65, a.work *= 0.65;
   const int64_t held = view.table_pitch << view.page_shift, longest = max_length > 0 ? std::min(max_length, held) : held, shared = std::min(sight.max_shared, held);
   const double rows = (double)view.tokens * (double)(heads / view.kv_heads), batch = view.batch, at_a_time = 2.0 * compute_units() / (double)view.kv_heads;
-  const double own_steps = sight.window > 0 ? 1.0 : std::max(1.0, (double)(longest - shared) / 64);
+  const double own_steps = std::max(1.0, (double)std::min(longest - shared, sight.window > 0 ? sight.window : kWidest) / 64);
   // (half a block, or half of 32 rows, of each sequence is empty, and each has one)
   const double blocks = std::max(batch, rows / 128 + batch / 2), full = 0.7 * std::max(batch, rows / 32 + batch / 2) / 4 + 0.3 * blocks;
   const double family_full = 0.7 * std::max(guess.count, std::ceil(rows / 32)) / 4 + 0.3 * guess.blocks;
   const double join = (double)view.tokens * (double)heads * (double)(view.head_dim + 2) * 8e-6, steps = (double)guess.steps;
-  const int64_t parts = best_cut(guess.blocks * (double)view.kv_heads, guess.steps, step_us(dtype, view.head_dim, false), false, view.tokens, heads, view.head_dim).parts;
+  const int64_t parts = best_cut(guess.blocks * (double)view.kv_heads, walked, step_us(dtype, view.head_dim, false), false, view.tokens, heads, view.head_dim).parts;
   const double alone = a.once + a.step * std::min((double)ceil_div(own.tile_chunk, 64), steps + own_steps) + a.work * full * (steps + own_steps) / at_a_time +
                        (own.tile_splits > 1 ? a.join * join * own.tile_splits : 0);
-  const double together = s.once + s.step * (double)ceil_div(guess.steps, parts) + s.work * (family_full * steps + full * own_steps) / at_a_time + s.join * join * (double)(parts + 1) +
+  const double together = s.once + s.step * (double)ceil_div(walked, parts) + s.work * (family_full * (double)walked + full * own_steps) / at_a_time + s.join * join * (double)(parts + 1) +
                           s.block * blocks / at_a_time;
   return together < alone;
 }
@@ -199,12 +206,15 @@ bool sharing_pays(const PagedView& view, int64_t heads, int64_t max_tokens, int6
   if (sight.families == nullptr) return false;
   if (sight.family_count == 0 || sight.max_shared == 0) return true;
   FamilyGuess guess = guess_families(view, heads, sight);
-  if (sight.window > 0) guess.steps = std::min(guess.steps, ceil_div(std::min(sight.window, kWidest) + std::min(sight.sinks, kWidest), 64) + 1);  // (seen of the common keys)
+  const int64_t all = guess.steps;
+  if (sight.window > 0) guess.steps = std::min(all, ceil_div(std::min(sight.window, kWidest) + std::min(sight.sinks, kWidest), 64) + 1);  // (seen of the common keys)
   const PagedPlan own = plan_own(view, heads, max_tokens, max_length, sight, dtype);
   const bool f32 = dtype == TTMI_F32, wide = view.head_dim == 128, single = single_tokens(view, heads);
   const double step = step_us(dtype, view.head_dim, single), rows = (double)view.tokens * (double)(heads / view.kv_heads), batch = view.batch;
   const double bytes = guess.steps * 64.0 * (2 * view.kv_heads * view.head_dim * (double)dtype_size(dtype));
-  if (!single) return many_tokens_share(view, heads, max_length, sight, dtype, own, guess);
+  // Common keys that a window hides: they are cut into parts with the others, of which the ends alone are trimmed, so they cost those who share some of what they would if they were seen.
+  const int64_t walked = guess.steps + (all - guess.steps) / (single ? 2 : 4);
+  if (!single) return many_tokens_share(view, heads, max_length, sight, dtype, own, guess, walked);
   // each by itself: the common keys again and again, out of the caches, and a launch that joins
   double alone = (own.few && own.few_splits == 0 ? 7 : f32 ? (wide ? 14 : 13.5) : 12) + batch * bytes / (f32 ? 12.5e6 : 15e6);
   if (own.tiles) alone += 5;
@@ -212,9 +222,9 @@ bool sharing_pays(const PagedView& view, int64_t heads, int64_t max_tokens, int6
   // shared: as many bytes as families read, or blocks of their rows over parts of the keys
   const double count = (double)std::min<int64_t>(sight.family_count, std::max(1, view.batch / 2)), most = std::ceil(rows / count);
   double shared;
-  if (most <= family_few_rows(dtype)) shared = (f32 ? (wide ? 16 : 14.5) : 13) + 0.05 * batch + count * std::ceil(most / kFewRows) * bytes / 6e6;
+  if (most <= family_few_rows(dtype)) shared = (f32 ? (wide ? 16 : 14.5) : 13) + 0.05 * batch + count * std::ceil(most / kFewRows) * bytes * ((double)walked / (double)guess.steps) / 6e6;
   else shared = (f32 ? (wide ? 22 : 12) : (wide ? 12 : 11)) + (f32 ? 0.15 : 0.1) * batch +
-                best_cut(guess.blocks * (double)view.kv_heads, guess.steps, step, single, view.tokens, heads, view.head_dim).us;
+                best_cut(guess.blocks * (double)view.kv_heads, walked, step, single, view.tokens, heads, view.head_dim).us;
   return shared < alone;
 }
 
